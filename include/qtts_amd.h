@@ -78,7 +78,8 @@ typedef enum {
     QTTS_OP_INT8_LINEAR = 4,
     QTTS_OP_FP8W = 5,
     QTTS_OP_W8A16_SILU = 6,
-    QTTS_OP_W8A16_FUSED = 7
+    QTTS_OP_W8A16_FUSED = 7,
+    QTTS_OP_LORA = 8 /* n: rows of one adapter's A (partitions * rank) */
 } qtts_op;
 
 /* What qtts_w8a16_fused_gemm_strips applies to its activations before the GEMM. */
@@ -421,6 +422,61 @@ int qtts_int8_linear_strips(const void* x, int x_dtype, int64_t m, int64_t k, in
 int qtts_fp8w_gemm_strips(const void* x, int x_dtype, int64_t m, int64_t k, int64_t ldx,
                           const uint8_t* qs, int64_t n, const float* scale, const void* bias,
                           void* y, int64_t ldy, int algo, void* ws, int64_t ws_bytes, void* stream);
+
+/* --- 8-bit activations from their producers --------------------------------------- */
+
+/* RMSNorm of a residual sum, straight to the per-token codes of a W8A8 linear:
+ *   h = x_dtype(x + residual)             (residual NULL: h = x)
+ *   v[r, c] = h[r, c] * inv * f32(weight[c]),  inv = 1 / sqrt(sum_c h[r, c]^2 / k + eps)
+ *   sx[r] = max(max_c |v[r, c]|, 1e-6) / L,    L = 448 (QTTS_CODE_E4M3) or 127 (QTTS_CODE_INT8)
+ *   qx[r, c] = code(v[r, c] / sx[r])           (nearest, ties to even)
+ * in one pass, with v in fp32 up to its code.  No counterpart in the reference, which adds
+ * (qtts/models/talker.py:270-271), normalizes (qtts/layers/norm.py:50-76) and quantizes
+ * (qtts/quant/fp8.py:77-78, qtts/quant/int8.py:146-149) in separate kernels and rounds to
+ * x_dtype between them; there the 1e-6 and, for int8, the scale are in x_dtype too.
+ * A NaN among a row's v makes its scale NaN (its e4m3 codes are NaN, its int8 codes 0).
+ * x, residual: [m, k] of x_dtype (bf16, fp16, fp32), row strides ldx, ldr.  weight: [k] of
+ * x_dtype.  qx: [m, k] codes, row stride k.  sx: [m] fp32.  hidden: [m, k], receives h, row
+ * stride ldh, or NULL; it may be x or the residual itself (same pointer and stride).
+ * normed: [m, k], receives x_dtype(v), row stride ldn, or NULL (for readers of 16-bit rows,
+ * such as qtts_lora_add).  No two other arrays may share a byte. */
+int qtts_rms_norm_quant(const void* x, int x_dtype, int64_t m, int64_t k, int64_t ldx, const void* residual,
+                        int64_t ldr, const void* weight, float eps, int codes, void* qx, float* sx, void* hidden,
+                        int64_t ldh, void* normed, int64_t ldn, void* stream);
+
+/* GatedMLP's activation (qtts/layers/activation.py:142-147), straight to the per-token codes
+ * of a W8A8 down projection: v[r, c] = silu(g) * u in fp32, g = gate_up[r, c],
+ * u = gate_up[r, k + c]; sx and qx of v as in qtts_rms_norm_quant.  No counterpart in the
+ * reference, which rounds silu(g), the product and the quantizer's steps to x_dtype in turn.
+ * gate_up: [m, 2k] of x_dtype, row stride ld_gate_up.  act: [m, k], receives x_dtype(v), row
+ * stride ldact, or NULL. */
+int qtts_silu_mul_quant(const void* gate_up, int x_dtype, int64_t m, int64_t k, int64_t ld_gate_up, int codes,
+                        void* qx, float* sx, void* act, int64_t ldact, void* stream);
+
+/* --- low-rank adapters of many requests -------------------------------------------- */
+
+#define QTTS_LORA_MAX_PARTS 8
+#define QTTS_LORA_MAX_RANK 128
+
+/* Each row's own low-rank adapter, added to the output of a projection that all rows share:
+ *   s = index[r];  t[r, i] = sum_c x[r, c] * a[s, p * rank + i, c]
+ *   out[r, j] = x_dtype(base[r, j] + scaling[s] * sum_{i < ranks[s]} t[r, i] * b[s, j, i])
+ * for the output partition p of column j (part_ends: [parts] ascending column ends on the
+ * host, the last n; a merged qkv or gate_up has an A block per partition).  Rows whose index
+ * is outside [0, slots) have out = base.  Sums in fp32 (t is carried to the second product as
+ * two 16-bit halves, 16 bits or more of it).  No counterpart in the reference.
+ * x: [m, k] of x_dtype (bf16 or fp16), row stride ldx.  index: [m] int32, on the device.
+ * a: [slots, parts * rank, k], b: [slots, n, rank], contiguous, of x_dtype.  ranks: [slots]
+ * int32 or NULL (all `rank`); entries of a and b past a slot's rank are not used.  scaling:
+ * [slots] fp32.  base, out: [m, n] of x_dtype, row strides ldb, ldo; out may be base itself
+ * and shares no byte with x.  rank <= QTTS_LORA_MAX_RANK, parts <= QTTS_LORA_MAX_PARTS.
+ * plan: what qtts_lora_plan made of the same index and slots, or NULL; with it, rows of one
+ * adapter are read together wherever they stand.  Workspace: qtts_workspace_bytes(QTTS_OP_LORA,
+ * m, parts * rank, k, 0). */
+int qtts_lora_add(const void* x, int x_dtype, int64_t m, int64_t k, int64_t ldx, const int32_t* index,
+                  const int32_t* plan, int64_t slots, const void* a, const void* b, int64_t rank, const int32_t* ranks,
+                  const float* scaling, const int64_t* part_ends, int64_t parts, const void* base, int64_t ldb,
+                  void* out, int64_t n, int64_t ldo, void* ws, int64_t ws_bytes, void* stream);
 
 /* Kernel timer.  No counterpart in the reference: benchmark instrumentation.
  * Between qtts_kernel_timer_begin and qtts_kernel_timer_end, each kernel the

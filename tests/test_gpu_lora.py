@@ -1,0 +1,231 @@
+"""Low-rank adapters of many requests beside a shared projection (ops.lora_batch, ops.lora_add) against 64 bits.
+
+Tolerance of an output element, from the arithmetic (u = 2^-24): half a step of the output's type relative to the
+result (eps / 2), plus the fp32 sums: K + R products each off by at most u of the sum of their magnitudes, twice
+(rounding of the product's addition, and the order), and the first product's result carried to the second as two 16-bit
+halves (2^-16 of it in bf16, the coarser of the two types)."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from qtts_amd import ops as _ops
+    assert _ops.device_supported(), "GPU is not a gfx950"
+    _ops.reserve_workspace(torch.device("cuda"), 64 << 20)
+    return _ops
+
+
+def _rand(shape, dtype, seed, scale=1.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return (torch.randn(shape, generator=g, device="cuda") * scale).to(dtype)
+
+
+def _case(m, k, parts, slots, rank, dtype, seed, index=None, mixed=True):
+    n = sum(parts)
+    g = torch.Generator().manual_seed(seed)
+    if index is None:
+        index = torch.randint(-1, slots, (m,), generator=g, dtype=torch.int32)
+    ranks = torch.randint(0, rank + 1, (slots,), generator=g, dtype=torch.int32) if mixed else None
+    if ranks is not None and slots > 1:
+        ranks[0] = rank
+    return {"base": _rand((m, n), dtype, seed), "x": _rand((m, k), dtype, seed + 1), "index": index.cuda(),
+            "a": _rand((slots, len(parts) * rank, k), dtype, seed + 2, max(k, 1) ** -0.5),
+            "b": _rand((slots, n, rank), dtype, seed + 3, 0.2), "scaling": _rand((slots,), torch.float32, seed + 4) + 2,
+            "ranks": None if ranks is None else ranks.cuda(), "parts": parts, "slots": slots, "rank": rank}
+
+
+def _exact(c):
+    """(result, error bound without the output's rounding), in 64 bits on the CPU."""
+    y = c["base"].double().cpu()
+    bound = y.abs() * U
+    x, index, rank = c["x"].double().cpu(), c["index"].cpu(), c["rank"]
+    lo = 0
+    for p, width in enumerate(c["parts"]):
+        for s in range(c["slots"]):
+            rows = (index == s).nonzero().flatten()
+            r = rank if c["ranks"] is None else int(c["ranks"][s].clamp(0, rank))
+            if not len(rows) or not r:
+                continue
+            a = c["a"][s, p * rank:p * rank + r].double().cpu()
+            b = c["b"][s, lo:lo + width, :r].double().cpu()
+            scale = float(c["scaling"][s])
+            y[rows, lo:lo + width] += scale * (x[rows] @ a.t() @ b.t())
+            mags = abs(scale) * (x[rows].abs() @ a.abs().t() @ b.abs().t())
+            carried = abs(scale) * ((x[rows] @ a.t()).abs() @ b.abs().t())
+            bound[rows, lo:lo + width] += 2 * (x.shape[1] + r + 8) * U * mags + 2.0 ** -16 * carried
+        lo += width
+    return y, bound
+
+
+def _check(out, c, what=""):
+    y, bound = _exact(c)
+    tiny = torch.finfo(out.dtype).smallest_normal * torch.finfo(out.dtype).eps / 2
+    err = (out.double().cpu() - y).abs()
+    ok = err <= bound + torch.finfo(out.dtype).eps / 2 * (y.abs() + bound) + tiny
+    assert ok.all(), f"{what}: {int((~ok).sum())} of {ok.numel()} off, first at {(~ok).nonzero()[0].tolist()}"
+    none = ((c["index"] < 0) | (c["index"] >= c["slots"])).nonzero().flatten()
+    assert torch.equal(out[none], c["base"][none]), f"{what}: a row without an adapter changed"
+
+
+def _run(ops, c, out=None):
+    return ops.lora_add(c["base"], c["x"], ops.lora_batch(c["index"], c["slots"]), c["a"], c["b"], c["scaling"], c["ranks"],
+                        c["parts"], out=out)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("m,k,parts,slots,rank", [
+    (1, 2048, [2048], 4, 16), (1, 64, [64], 1, 8), (2, 1024, [2048, 1024, 1024], 3, 16), (16, 256, [512], 1, 16),
+    (17, 256, [520], 1, 32), (27, 2048, [2048, 1024, 1024], 9, 16), (33, 128, [64, 72], 40, 24), (64, 512, [640], 32, 64),
+    (65, 512, [640], 3, 16), (130, 256, [256, 256], 7, 128), (200, 96, [136], 150, 8), (1003, 64, [48], 5, 16),
+    (64, 64, [64], 1, 128), (300, 2048, [80], 2, 40)])
+def test_lora(ops, m, k, parts, slots, rank, dtype):
+    for mixed in (True, False):
+        c = _case(m, k, parts, slots, rank, dtype, seed=m + k + rank, mixed=mixed)
+        _check(_run(ops, c), c, f"{m}x{k} parts {parts} slots {slots} rank {rank} {dtype}")
+
+
+@pytest.mark.parametrize("m", [1, 5, 40, 100])
+@pytest.mark.parametrize("k,parts,rank", [(33, [17], 3), (65, [40, 1, 23], 4), (100, [13, 64], 12), (8, [8], 1),
+                                          (2047, [31], 16), (64, [100], 17), (24, [7], 127), (16, [0, 24, 0], 8)])
+def test_odd_sizes(ops, m, k, parts, rank):
+    c = _case(m, k, parts, 3, rank, torch.bfloat16, seed=m + k)
+    _check(_run(ops, c), c, f"{m}x{k} parts {parts} rank {rank}")
+
+
+@pytest.mark.parametrize("m", [6, 70])
+def test_strides_offsets_and_in_place(ops, m):
+    """Rows of wider buffers, starts off 16 bytes, out the base itself, rows of another buffer left alone."""
+    k, n = 128, 96
+    for off in (0, 8, 1):
+        c = _case(m, k, [64, 32], 4, 16, torch.bfloat16, seed=5 + off)
+        wide_x = torch.zeros(m, k + 40, dtype=torch.bfloat16, device="cuda")
+        wide_b = torch.full((m + 2, n + 48), 7.0, dtype=torch.bfloat16, device="cuda")
+        wide_x[:, off:off + k] = c["x"]
+        wide_b[1:m + 1, off:off + n] = c["base"]
+        view = wide_b[1:m + 1, off:off + n]
+        batch = ops.lora_batch(c["index"], 4)
+        out = ops.lora_add(view, wide_x[:, off:off + k], batch, c["a"], c["b"], c["scaling"], c["ranks"], c["parts"])
+        _check(out, c, f"offset {off}")
+        got = ops.lora_add(view, wide_x[:, off:off + k], batch, c["a"], c["b"], c["scaling"], c["ranks"], c["parts"], out=view)
+        assert got.data_ptr() == view.data_ptr()
+        assert torch.equal(view, out), "in place"
+        wide_b[1:m + 1, off:off + n] = 7.0
+        assert (wide_b == 7.0).all(), "written outside its rows or columns"
+    x3, b3 = c["x"].view(2, m // 2, k), c["base"].view(2, m // 2, n)
+    y3 = ops.lora_add(b3, x3, batch, c["a"], c["b"], c["scaling"], c["ranks"], c["parts"])
+    assert y3.shape == b3.shape and torch.equal(y3.view(m, n), out)
+
+
+@pytest.mark.parametrize("m", [3, 64, 90])
+def test_routing_edges(ops, m):
+    """No row with an adapter, every row with one, one adapter a row, indices out of range, no slots at all."""
+    for name, index in {"none": torch.full((m,), -1), "one": torch.full((m,), 2), "each": torch.arange(m) % 7,
+                        "range": torch.arange(m) * 1000 - 5, "extremes": torch.tensor([2 ** 31 - 1, -2 ** 31, 0] * 30)[:m],
+                        "last": torch.tensor([-1] * (m - 1) + [6])}.items():
+        c = _case(m, 64, [48], 7, 16, torch.bfloat16, seed=3, index=index.to(torch.int32))
+        _check(_run(ops, c), c, f"{name} {m}")
+    e = torch.empty
+    kw = dict(dtype=torch.bfloat16, device="cuda")
+    out = ops.lora_add(c["base"], c["x"], ops.lora_batch(c["index"], 0), e(0, 16, 64, **kw), e(0, 48, 16, **kw),
+                       e(0, device="cuda"))
+    assert torch.equal(out, c["base"])
+
+
+@pytest.mark.parametrize("m", [4, 80])
+def test_ranks_hide_what_is_past_them(ops, m):
+    """Entries past a slot's rank may hold anything, NaN and infinities among it; so may slots that no row takes,
+    and rows without an adapter."""
+    c = _case(m, 64, [32, 40], 5, 24, torch.float16, seed=9, mixed=False)
+    c["index"] = (torch.arange(m) % 4 - 1).to(torch.int32).cuda()
+    c["ranks"] = torch.tensor([5, 0, 24, 3, 9], dtype=torch.int32).cuda()
+    want = _run(ops, c)
+    _check(want, c)
+    for s, r in enumerate(c["ranks"].tolist()):
+        c["b"][s, :, r:] = float("nan")
+        c["a"][s].view(2, 24, 64)[:, r:] = float("inf")
+    c["a"][3:] = float("nan")
+    c["b"][3:] = float("inf")
+    c["scaling"][3:] = float("nan")
+    c["x"][c["index"] < 0] = float("nan")
+    got = _run(ops, c)
+    assert torch.equal(got, want)
+    c["ranks"] = torch.tensor([5, -3, 99, 3, 9], dtype=torch.int32).cuda()  # taken into 0..rank
+    assert torch.isfinite(_run(ops, c)).all()
+
+
+@pytest.mark.parametrize("m", [6, 100])
+def test_values_stay_in_their_rows(ops, m):
+    """NaN and infinity in one row's activations reach that row alone."""
+    c = _case(m, 128, [64], 3, 16, torch.bfloat16, seed=21, index=torch.zeros(m, dtype=torch.int32), mixed=False)
+    want = _run(ops, c)
+    c["x"][2, 5] = float("nan")
+    c["x"][4, 0] = float("inf")
+    got = _run(ops, c)
+    rest = [r for r in range(m) if r not in (2, 4)]
+    assert torch.equal(got[rest], want[rest]) and torch.isnan(got[2]).all() and not torch.isfinite(got[4]).any()
+
+
+def test_fp16_range(ops):
+    """The first product's sums may pass fp16's range (65504): they are kept in fp32 or scaled."""
+    c = _case(5, 512, [64], 2, 16, torch.float16, seed=23, mixed=False, index=torch.tensor([0, 1, 0, -1, 1], dtype=torch.int32))
+    c["x"] *= 1000
+    c["a"] *= 500
+    c["b"] *= 1e-5
+    _check(_run(ops, c), c)
+    c["x"] *= 1e-6  # and far below its smallest normal
+    c["a"] *= 1e-5
+    c["b"] = (c["b"].float() * 1e5).half()
+    _check(_run(ops, c), c)
+
+
+@pytest.mark.parametrize("m", [1, 48, 100])
+def test_graph_follows_the_index(ops, m):
+    """A captured call reads index, activations and adapters anew on every replay, whatever ran in between."""
+    c = _case(m, 256, [128, 64], 6, 16, torch.bfloat16, seed=31)
+    other = _case(70, 256, [512], 2, 32, torch.bfloat16, seed=32)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        _run(ops, c)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        batch = ops.lora_batch(c["index"], 6)
+        out = ops.lora_add(c["base"], c["x"], batch, c["a"], c["b"], c["scaling"], c["ranks"], c["parts"])
+        again = ops.lora_add(out, c["x"], batch, c["a"], c["b"], c["scaling"], c["ranks"], c["parts"])
+    for i in range(3):
+        fresh = _case(m, 256, [128, 64], 6, 16, torch.bfloat16, seed=40 + i)
+        for key in ("index", "x", "base", "a", "ranks"):
+            c[key].copy_(fresh[key])
+        graph.replay()
+        _check(_run(ops, other), other, "eager between")
+        torch.cuda.synchronize()
+        want = _run(ops, c)
+        assert torch.equal(out, want), f"replay {i}"
+        assert torch.equal(again, _run(ops, dict(c, base=want))), f"replay {i}"
+        _check(out, c, f"replay {i}")
+
+
+def test_repeats_give_the_same_bits(ops):
+    for m in (30, 500):
+        c = _case(m, 1024, [512], 8, 16, torch.bfloat16, seed=51)
+        first = _run(ops, c)
+        for _ in range(3):
+            assert torch.equal(_run(ops, c), first)
+
+
+def test_a_row_does_not_depend_on_its_batch(ops):
+    """Within one kernel's range, a row's result is the same bits alone among others or in another order."""
+    c = _case(40, 512, [256], 5, 16, torch.bfloat16, seed=53)
+    want = _run(ops, c)
+    perm = torch.randperm(40, generator=torch.Generator().manual_seed(1)).cuda()
+    d = dict(c, x=c["x"][perm], base=c["base"][perm], index=c["index"][perm])
+    assert torch.equal(_run(ops, d), want[perm])

@@ -1,0 +1,265 @@
+"""RMSNorm with the residual's addition and GatedMLP's activation, straight to 8-bit codes and their scales
+(ops.rms_norm_quant, ops.silu_mul_quant), against 64-bit evaluations.
+
+Tolerances, from the arithmetic (u = 2^-24, one fp32 rounding):
+
+* the row's scale and its values v: the sum of squares adds up to K / 64 squares a lane and then 64 lanes and at most
+  16 waves, each addition off by u, halved by the square root; a handful of roundings follow (the root, its
+  reciprocal, the products, silu's exponential and quotient: 16 u covers them, and an exponential's argument g
+  carries |g| u more, |g| <= 64 before the result vanishes).  REL(k) below;
+* a code: half a step of its grid about v / scale (e4m3: relative 2^-4, absolute 2^-10 under 2^-6; int8: 1/2), plus
+  v's own error;
+* 16-bit outputs: half a step of the type, eps / 2 relative, plus v's own error.
+"""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+DTYPES = [torch.bfloat16, torch.float16, torch.float32]
+LIMIT = {0: 127.0, 1: 448.0}
+
+
+def rel(k: int) -> float:
+    return (k / 128 + 48 + 64 + 16) * U
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from qtts_amd import ops as _ops
+    assert _ops.device_supported(), "GPU is not a gfx950"
+    return _ops
+
+
+def _rand(shape, dtype, seed, scale=1.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return (torch.randn(shape, generator=g, device="cuda") * scale).to(dtype)
+
+
+def _check_codes(q, s, v, codes, tol, what):
+    """q and s against the 64-bit rows v."""
+    amax = v.abs().amax(1).clamp_min(1e-6) if v.shape[1] else torch.full((v.shape[0],), 1e-6, dtype=torch.float64)
+    want = amax / LIMIT[codes]
+    assert s.dtype == torch.float32 and s.shape == want.shape
+    s = s.double().cpu()
+    # 1e-6 itself is rounded to fp32
+    assert ((s - want).abs() <= (tol + U) * want).all(), f"{what}: scale off by {((s - want).abs() / want).max()}"
+    x, got = v / want[:, None], q.cpu().double()
+    half = torch.full_like(x, 0.5) if codes == 0 else torch.maximum(x.abs() * 2.0 ** -4, torch.tensor(2.0 ** -10).double())
+    err = (got - x).abs()
+    assert (err <= half * (1 + 4 * tol) + 2 * tol * x.abs()).all(), f"{what}: code off by {(err / half).max()} half steps"
+    assert got.abs().max() <= LIMIT[codes] if got.numel() else True
+
+
+def _check_16bit(y, v, tol, what):
+    """y against v: one rounding to y's type (fp32: none beyond v's own error)."""
+    step = torch.finfo(y.dtype).eps / 2 if y.dtype != torch.float32 else 0.0
+    tiny = torch.finfo(y.dtype).smallest_normal * torch.finfo(y.dtype).eps / 2
+    err = (y.double().cpu() - v).abs()
+    assert (err <= (step + 2 * tol) * v.abs() + tiny).all(), f"{what}: off by {(err / v.abs().clamp_min(1e-30)).max()}"
+
+
+def _norm64(h, w, eps):
+    h, w = h.double().cpu(), w.double().cpu()
+    return h / (h.pow(2).mean(1, keepdim=True) + eps).sqrt() * w
+
+
+def _silu64(gu):
+    g, u = gu.double().cpu().chunk(2, 1)
+    return g * torch.sigmoid(g) * u
+
+
+SHAPES = [(1, 8), (1, 2048), (3, 100), (5, 1003), (17, 1024), (9, 520), (2, 6144), (3, 7), (70, 1), (4, 8192), (2, 9001),
+          (2, 12296), (1, 33000), (2000, 72)]
+
+
+@pytest.mark.parametrize("codes", [1, 0], ids=["e4m3", "int8"])
+@pytest.mark.parametrize("dtype", DTYPES, ids=["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("m,k", SHAPES)
+def test_norm(ops, m, k, dtype, codes):
+    w = 1 + _rand((k,), torch.float32, 1, 0.1)
+    w = w.to(dtype)
+    x = _rand((m, k), dtype, 2)
+    for residual in (None, _rand((m, k), dtype, 3, 2.0)):
+        for want in (False, True):
+            q, s, hidden, normed = ops.rms_norm_quant(x, w, 1e-6, residual, codes, want_normed=want)
+            what = f"{m}x{k} {dtype} codes {codes} residual {residual is not None}"
+            h = x if residual is None else x + residual
+            if residual is None:
+                assert hidden is None
+            else:
+                assert torch.equal(hidden, h), what
+            v = _norm64(h, w, 1e-6)
+            _check_codes(q, s, v, codes, rel(k), what)
+            assert (normed is not None) == want
+            if want:
+                _check_16bit(normed, v, rel(k), what)
+
+
+@pytest.mark.parametrize("codes", [1, 0], ids=["e4m3", "int8"])
+@pytest.mark.parametrize("dtype", DTYPES, ids=["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("m,k", SHAPES)
+def test_silu(ops, m, k, dtype, codes):
+    gu = _rand((m, 2 * k), dtype, 5, 3.0)
+    for want in (False, True):
+        q, s, act = ops.silu_mul_quant(gu, codes, want_act=want)
+        v = _silu64(gu)
+        _check_codes(q, s, v, codes, rel(0), f"{m}x{k} {dtype} {codes}")
+        assert (act is not None) == want
+        if want:
+            _check_16bit(act, v, rel(0), f"{m}x{k} {dtype} {codes}")
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=["bf16", "fp16", "fp32"])
+def test_strided_and_shaped(ops, dtype):
+    """Rows of a wider buffer, rows that start off 16 bytes, and leading dimensions."""
+    k, m = 264, 6
+    wide = _rand((m, 3 * k + 9), dtype, 7)
+    w = (1 + _rand((k,), torch.float32, 8, 0.1)).to(dtype)
+    for off in (0, 8, 1, 3):
+        x, r = wide[:, off:off + k], wide[:, off + k + 1:off + 2 * k + 1]
+        q, s, hidden, normed = ops.rms_norm_quant(x, w, 1e-5, r, want_normed=True)
+        qc, sc, hc, nc = ops.rms_norm_quant(x.contiguous(), w, 1e-5, r.contiguous(), want_normed=True)
+        assert torch.equal(hidden, x + r) and torch.equal(hc, hidden)
+        v = _norm64(x + r, w, 1e-5)
+        for a, b in ((q, s), (qc, sc)):
+            _check_codes(a, b, v, 1, rel(k), f"offset {off}")
+        _check_16bit(normed, v, rel(k), f"offset {off}")
+        gu = wide[:, off:off + 2 * k]
+        q, s, act = ops.silu_mul_quant(gu, 0, want_act=True)
+        _check_codes(q, s, _silu64(gu), 0, rel(0), f"offset {off}")
+    x3 = _rand((2, 3, k), dtype, 9)
+    q, s, hidden, normed = ops.rms_norm_quant(x3, w, 1e-5, x3, want_normed=True)
+    assert hidden.shape == normed.shape == x3.shape and q.shape == (6, k) and s.shape == (6,)
+    q, s, act = ops.silu_mul_quant(x3, want_act=True)
+    assert act.shape == (2, 3, k // 2) and q.shape == (6, k // 2)
+
+
+def test_empty(ops):
+    x = torch.empty(0, 64, dtype=torch.bfloat16, device="cuda")
+    w = torch.ones(64, dtype=torch.bfloat16, device="cuda")
+    q, s, hidden, normed = ops.rms_norm_quant(x, w, 1e-6, x, want_normed=True)
+    assert q.shape == (0, 64) and s.shape == (0,) and hidden.shape == normed.shape == (0, 64)
+    q, s, act = ops.silu_mul_quant(x, want_act=True)
+    assert q.shape == (0, 32) and s.shape == (0,) and act.shape == (0, 32)
+    q, s, _, _ = ops.rms_norm_quant(torch.empty(3, 0, device="cuda"), torch.empty(0, device="cuda"))
+    assert q.shape == (3, 0) and torch.allclose(s, torch.full_like(s, 1e-6 / 448), rtol=1e-6)
+    q, s, _ = ops.silu_mul_quant(torch.empty(3, 0, device="cuda"), 0)
+    assert q.shape == (3, 0) and torch.allclose(s, torch.full_like(s, 1e-6 / 127), rtol=1e-6)
+
+
+@pytest.mark.parametrize("codes", [1, 0], ids=["e4m3", "int8"])
+@pytest.mark.parametrize("k", [64, 2048, 2049, 12296])
+def test_odd_rows_leave_the_others_alone(ops, k, codes):
+    """A zero row, a row under the scale's floor, and rows of infinities and NaN among ordinary ones."""
+    x = _rand((9, k), torch.bfloat16, 11)
+    w = (1 + _rand((k,), torch.float32, 12, 0.1)).to(torch.bfloat16)
+    plain = ops.rms_norm_quant(x, w, 1e-6, None, codes)
+    odd = x.clone()
+    odd[1] = 0
+    odd[2, k // 2] = float("nan")
+    odd[4, 3] = float("inf")
+    odd[6, k - 1] = float("-inf")
+    q, s, _, _ = ops.rms_norm_quant(odd, w, 1e-6, None, codes)
+    for r in (0, 3, 5, 7, 8):
+        assert torch.equal(q[r].view(torch.uint8), plain[0][r].view(torch.uint8)) and s[r] == plain[1][r]
+    assert (q[1].float() == 0).all() and abs(s[1].item() / (1e-6 / LIMIT[codes]) - 1) < 4 * U
+    for r in (2, 4, 6):
+        assert torch.isnan(s[r]), "a NaN among the values makes the scale NaN"
+        assert (q[r] == 0).all() if codes == 0 else torch.isnan(q[r].float()).all()
+    gu = torch.cat([x, x.roll(1, 0)], 1)
+    plain = ops.silu_mul_quant(gu, codes)
+    gu[2, k // 2] = float("nan")
+    gu[4, 3] = float("inf")
+    gu[6, k + 2] = 1e-30
+    gu[7] = 0
+    gu[8] = gu[8] * 1e-6
+    q, s, _ = ops.silu_mul_quant(gu, codes)
+    for r in (0, 1, 3, 5):
+        assert torch.equal(q[r].view(torch.uint8), plain[0][r].view(torch.uint8)) and s[r] == plain[1][r]
+    assert torch.isnan(s[2]) and torch.isinf(s[4]) and (q[7].float() == 0).all()
+    _check_codes(q[7:], s[7:], _silu64(gu[7:]), codes, rel(0), "rows under the floor")
+
+
+def test_in_place_hidden(ops):
+    """hidden may be x or the residual (the C entry; the wrapper always returns a fresh one)."""
+    from qtts_amd import _lib
+    L = _lib.load()
+    for k in (2048, 1001, 12296):
+        w = torch.ones(k, dtype=torch.bfloat16, device="cuda")
+        for which in (0, 1):
+            x, r = _rand((5, k), torch.bfloat16, 13), _rand((5, k), torch.bfloat16, 14)
+            want = ops.rms_norm_quant(x, w, 1e-6, r)
+            q, s = torch.empty_like(want[0]), torch.empty_like(want[1])
+            target = (x, r)[which]
+            st = L.qtts_rms_norm_quant(x.data_ptr(), 1, 5, k, k, r.data_ptr(), k, w.data_ptr(), 1e-6, 1, q.data_ptr(),
+                                       s.data_ptr(), target.data_ptr(), k, None, k, torch.cuda.current_stream().cuda_stream)
+            assert st == 0, _lib.last_error()
+            torch.cuda.synchronize()
+            assert torch.equal(target, want[2]) and torch.equal(s, want[1])
+            assert torch.equal(q.view(torch.uint8), want[0].view(torch.uint8))
+
+
+@pytest.mark.parametrize("codes", [1, 0], ids=["e4m3", "int8"])
+def test_feeds_the_w8a8_gemm(ops, codes):
+    """The codes and scales are what the W8A8 GEMMs take: norm, gate_up, activation, down against 64 bits."""
+    m, k, inter = 5, 512, 256
+    x, r = _rand((m, k), torch.bfloat16, 15), _rand((m, k), torch.bfloat16, 16)
+    w = (1 + _rand((k,), torch.float32, 17, 0.1)).to(torch.bfloat16)
+    pack = ops.pack_fp8 if codes else ops.pack_int8
+    gemm = ops.w8a8_fp8_gemm_strips if codes else ops.w8a8_int8_gemm_strips
+    up_q, up_s = pack(_rand((2 * inter, k), torch.float32, 18, 0.05))
+    down_q, down_s = pack(_rand((k, inter), torch.float32, 19, 0.05))
+    q, s, hidden, _ = ops.rms_norm_quant(x, w, 1e-6, r, codes)
+    gu = gemm(q, s, ops.to_strips(up_q), 2 * inter, up_s)
+    ref = (q.double() * s.double()[:, None]) @ (up_q.double() * up_s.double()[:, None]).t()
+    rms = ref.square().mean().sqrt()
+    assert ((gu.double() - ref).abs() <= 2.0 ** -8 * ref.abs() + 1e-3 * rms).all()
+    q, s, _ = ops.silu_mul_quant(gu, codes)
+    y = gemm(q, s, ops.to_strips(down_q), k, down_s)
+    ref = (q.double() * s.double()[:, None]) @ (down_q.double() * down_s.double()[:, None]).t()
+    rms = ref.square().mean().sqrt()
+    assert ((y.double() - ref).abs() <= 2.0 ** -8 * ref.abs() + 1e-3 * rms).all()
+
+
+def test_graph_and_stream(ops):
+    """Captured once and replayed on changing inputs, with eager calls between, and on a stream of its own."""
+    x, r = _rand((6, 2048), torch.bfloat16, 21), _rand((6, 2048), torch.bfloat16, 22)
+    w = (1 + _rand((2048,), torch.float32, 23, 0.1)).to(torch.bfloat16)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        mine = ops.rms_norm_quant(x, w, 1e-6, r, 0, True)
+        mine_act = ops.silu_mul_quant(x, 0, True)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = ops.rms_norm_quant(x, w, 1e-6, r, 0, True)
+        act = ops.silu_mul_quant(out[2], 0, True)
+    for i in range(3):
+        x.copy_(_rand((6, 2048), torch.bfloat16, 21 + 100 * i))
+        graph.replay()
+        want = ops.rms_norm_quant(x, w, 1e-6, r, 0, True)
+        want_act = ops.silu_mul_quant(want[2], 0, True)
+        torch.cuda.synchronize()
+        for a, b in zip((*out, *act), (*want, *want_act)):
+            assert torch.equal(a, b), f"replay {i}"
+        if i == 0:
+            assert all(torch.equal(a, b) for a, b in zip(mine, want))
+            assert torch.equal(mine_act[0], ops.silu_mul_quant(x, 0, True)[0])
+
+
+def test_more_rows_than_workgroups(ops):
+    """Past 2^20 rows a workgroup takes several."""
+    m, k = (1 << 20) + 77, 16
+    x = _rand((m, k), torch.bfloat16, 31)
+    w = torch.ones(k, dtype=torch.bfloat16, device="cuda")
+    q, s, _, _ = ops.rms_norm_quant(x, w, 1e-6, None, 0)
+    pick = torch.tensor([0, 1, 12345, 1 << 19, (1 << 20) - 1, 1 << 20, m - 2, m - 1], device="cuda")
+    _check_codes(q[pick], s[pick], _norm64(x[pick], w, 1e-6), 0, rel(k), "many rows")
+    q, s, _ = ops.silu_mul_quant(x, 1)
+    _check_codes(q[pick], s[pick], _silu64(x[pick]), 1, rel(0), "many rows")

@@ -13,6 +13,7 @@
 
 #include "common.h"
 #include "layout.h"
+#include "lora.h"
 #include "qtts_amd.h"
 
 // Launchers implemented next to their kernels.
@@ -69,6 +70,13 @@ int qtts_int8_fused_ok(int64_t m, int64_t n, int64_t k, int waves);
 int qtts_launch_int8_linear_fused(const void* x, int x_dtype, int64_t m, int64_t k, int64_t ldx, const int8_t* qws,
                                   int64_t n, const float* sw, const void* bias, void* y, int64_t ldy, int div_mode,
                                   int waves, hipStream_t st);
+int qtts_launch_rms_norm_quant(const void* x, int x_dtype, int64_t m, int64_t k, int64_t ldx, const void* res, int64_t ldr,
+                               const void* w, float eps, int codes, void* q, float* sx, void* hidden, int64_t ldh,
+                               void* normed, int64_t ldn, hipStream_t st);
+int qtts_launch_silu_mul_quant(const void* gu, int x_dtype, int64_t m, int64_t k, int64_t ld, int codes, void* q, float* sx,
+                               void* act, int64_t lda, hipStream_t st);
+int64_t qtts_lora_ws_bytes(int64_t m, int64_t rows_a);
+int qtts_launch_lora_add(const qtts::LoraArgs& args, int x_dtype, void* ws, hipStream_t st);
 
 static thread_local char g_last_error[512] = "";
 
@@ -251,6 +259,9 @@ int64_t qtts_workspace_bytes(int op, int64_t m, int64_t n, int64_t k, int algo) 
     case QTTS_OP_FP8W: return qtts_fp8w_ws_bytes(m, n, k, algo);
     case QTTS_OP_W8A16_SILU: return qtts_w8a16_silu_ws_bytes(m, n, k, algo, QTTS_BF16);
     case QTTS_OP_W8A16_FUSED: return qtts_w8a16_fused_ws_bytes(m, n, k, algo, QTTS_BF16);
+    case QTTS_OP_LORA:
+      if (m > (1ll << 58) / n) return qtts_set_error(QTTS_ERR_INVALID_ARGUMENT, "bad workspace query");
+      return qtts_lora_ws_bytes(m, n);
     default: return qtts_set_error(QTTS_ERR_INVALID_ARGUMENT, "unknown op %d", op);
   }
 }
@@ -652,6 +663,102 @@ int qtts_rms_norm(const void* x, int x_dtype, int64_t m, int64_t k, int64_t ldx,
   QTTS_REQUIRE(x && weight && y, "rms_norm: null pointer");
   QTTS_TRY(current_device_check());
   return qtts_launch_rms_norm(x, x_dtype, m, k, ldx, weight, eps, y, ldy, (hipStream_t)stream);
+}
+
+int qtts_rms_norm_quant(const void* x, int x_dtype, int64_t m, int64_t k, int64_t ldx, const void* residual, int64_t ldr,
+                        const void* weight, float eps, int codes, void* qx, float* sx, void* hidden, int64_t ldh,
+                        void* normed, int64_t ldn, void* stream) {
+  QTTS_REQUIRE(m >= 0 && k >= 0, "rms_norm_quant: negative size");
+  QTTS_REQUIRE(m < (1ll << 31) && k < (1ll << 31), "rms_norm_quant: size too large");
+  QTTS_REQUIRE(dtype_ok(x_dtype), "rms_norm_quant: bad dtype code");
+  QTTS_REQUIRE(codes == QTTS_CODE_INT8 || codes == QTTS_CODE_E4M3, "rms_norm_quant: bad code kind %d", codes);
+  QTTS_REQUIRE(ldx >= k && (!residual || ldr >= k) && (!hidden || ldh >= k) && (!normed || ldn >= k),
+               "rms_norm_quant: leading dimension smaller than the row");
+  if (m == 0) return QTTS_OK;
+  QTTS_REQUIRE(sx && (k == 0 || (x && weight && qx)), "rms_norm_quant: null pointer");
+  const int64_t e = dtype_size(x_dtype);
+  QTTS_REQUIRE(!spans_overlap(x, m, ldx, k, e, qx, m, k, k, 1) &&
+                   !(residual && spans_overlap(residual, m, ldr, k, e, qx, m, k, k, 1)),
+               "rms_norm_quant: qx overlaps the activations");
+  QTTS_REQUIRE(!hidden || (hidden == x && ldh == ldx) || !spans_overlap(x, m, ldx, k, e, hidden, m, ldh, k, e),
+               "rms_norm_quant: hidden overlaps x");
+  QTTS_REQUIRE(!hidden || !residual || (hidden == residual && ldh == ldr) ||
+                   !spans_overlap(residual, m, ldr, k, e, hidden, m, ldh, k, e),
+               "rms_norm_quant: hidden overlaps the residual");
+  QTTS_REQUIRE(!normed || (!spans_overlap(x, m, ldx, k, e, normed, m, ldn, k, e) &&
+                           !(residual && spans_overlap(residual, m, ldr, k, e, normed, m, ldn, k, e)) &&
+                           !(hidden && spans_overlap(hidden, m, ldh, k, e, normed, m, ldn, k, e))),
+               "rms_norm_quant: normed overlaps the activations");
+  QTTS_TRY(current_device_check());
+  return qtts_launch_rms_norm_quant(x, x_dtype, m, k, ldx, residual, ldr, weight, eps, codes, qx, sx, hidden, ldh, normed,
+                                    ldn, (hipStream_t)stream);
+}
+
+int qtts_silu_mul_quant(const void* gate_up, int x_dtype, int64_t m, int64_t k, int64_t ld_gate_up, int codes, void* qx,
+                        float* sx, void* act, int64_t ldact, void* stream) {
+  QTTS_REQUIRE(m >= 0 && k >= 0, "silu_mul_quant: negative size");
+  QTTS_REQUIRE(m < (1ll << 31) && k < (1ll << 30), "silu_mul_quant: size too large");
+  QTTS_REQUIRE(dtype_ok(x_dtype), "silu_mul_quant: bad dtype code");
+  QTTS_REQUIRE(codes == QTTS_CODE_INT8 || codes == QTTS_CODE_E4M3, "silu_mul_quant: bad code kind %d", codes);
+  QTTS_REQUIRE(ld_gate_up >= 2 * k && (!act || ldact >= k), "silu_mul_quant: leading dimension smaller than the row");
+  if (m == 0) return QTTS_OK;
+  QTTS_REQUIRE(sx && (k == 0 || (gate_up && qx)), "silu_mul_quant: null pointer");
+  const int64_t e = dtype_size(x_dtype);
+  QTTS_REQUIRE(!spans_overlap(gate_up, m, ld_gate_up, 2 * k, e, qx, m, k, k, 1), "silu_mul_quant: qx overlaps gate_up");
+  QTTS_REQUIRE(!act || !spans_overlap(gate_up, m, ld_gate_up, 2 * k, e, act, m, ldact, k, e),
+               "silu_mul_quant: act overlaps gate_up");
+  QTTS_TRY(current_device_check());
+  return qtts_launch_silu_mul_quant(gate_up, x_dtype, m, k, ld_gate_up, codes, qx, sx, act, ldact, (hipStream_t)stream);
+}
+
+int qtts_lora_add(const void* x, int x_dtype, int64_t m, int64_t k, int64_t ldx, const int32_t* index, const int32_t* plan,
+                  int64_t slots, const void* a, const void* b, int64_t rank, const int32_t* ranks, const float* scaling,
+                  const int64_t* part_ends, int64_t parts, const void* base, int64_t ldb, void* out, int64_t n, int64_t ldo,
+                  void* ws, int64_t ws_bytes, void* stream) {
+  (void)plan;
+  QTTS_REQUIRE(m >= 0 && n >= 0 && k >= 0 && slots >= 0, "lora_add: negative size");
+  QTTS_REQUIRE(m < (1ll << 31) && n < (1ll << 30) && k < (1ll << 30) && slots < (1ll << 30), "lora_add: size too large");
+  QTTS_REQUIRE(x_dtype == QTTS_BF16 || x_dtype == QTTS_F16, "lora_add: activations must be bf16 or fp16");
+  QTTS_REQUIRE(rank >= 1 && rank <= QTTS_LORA_MAX_RANK, "lora_add: rank %lld is not in 1..%d", (long long)rank,
+               QTTS_LORA_MAX_RANK);
+  QTTS_REQUIRE(parts >= 1 && parts <= QTTS_LORA_MAX_PARTS && part_ends, "lora_add: %lld partitions are not in 1..%d",
+               (long long)parts, QTTS_LORA_MAX_PARTS);
+  for (int64_t p = 0; p < parts; ++p)
+    QTTS_REQUIRE(part_ends[p] >= (p ? part_ends[p - 1] : 0), "lora_add: partition ends do not ascend");
+  QTTS_REQUIRE(part_ends[parts - 1] == n, "lora_add: the partitions end at %lld of %lld columns",
+               (long long)part_ends[parts - 1], (long long)n);
+  QTTS_REQUIRE(ldx >= k && ldb >= n && ldo >= n, "lora_add: leading dimension smaller than the row");
+  QTTS_REQUIRE(ws_bytes >= 0, "lora_add: negative workspace size");
+  if (m == 0 || n == 0) return QTTS_OK;
+  QTTS_REQUIRE(base && out && index && (slots == 0 || (scaling && b && (k == 0 || (x && a)))), "lora_add: null pointer");
+  QTTS_REQUIRE((out == base && ldo == ldb) || !spans_overlap(base, m, ldb, n, 2, out, m, ldo, n, 2),
+               "lora_add: out overlaps base");
+  QTTS_REQUIRE(!spans_overlap(x, m, ldx, k, 2, out, m, ldo, n, 2), "lora_add: out overlaps x");
+  const int64_t need = qtts_lora_ws_bytes(m, parts * rank);
+  if (!ws || ws_bytes < need)
+    return qtts_set_error(QTTS_ERR_WORKSPACE, "lora_add: workspace of %lld bytes < %lld needed", (long long)ws_bytes,
+                          (long long)need);
+  QTTS_TRY(current_device_check());
+  qtts::LoraArgs g = {};
+  g.x = x;
+  g.ldx = ldx;
+  g.index = index;
+  g.a = a;
+  g.b = b;
+  g.ranks = ranks;
+  g.scaling = scaling;
+  g.base = base;
+  g.ldb = ldb;
+  g.out = out;
+  g.ldo = ldo;
+  g.m = m;
+  g.k = (int)k;
+  g.n = (int)n;
+  g.slots = (int)slots;
+  g.rank = (int)rank;
+  g.parts.count = (int)parts;
+  for (int64_t p = 0; p < parts; ++p) g.parts.end[p] = (int32_t)part_ends[p];
+  return qtts_launch_lora_add(g, x_dtype, ws, (hipStream_t)stream);
 }
 
 int qtts_w8a16_fused_gemm_strips(const void* x, int x_dtype, int64_t m, int64_t k, int64_t ldx, int prologue,

@@ -60,13 +60,15 @@ ALGO_SKINNY_HALF, ALGO_SKINNY_QUARTER = 3, 4
 #: (for weights read once a step and too large to stay cached between steps); same bits out.
 ALGO_STREAM = 0x80
 # qtts_op
-OP_W8A16, OP_W8A8_FP8, OP_FP8_LINEAR, OP_W8A8_INT8, OP_INT8_LINEAR, OP_FP8W, OP_W8A16_SILU, OP_W8A16_FUSED = range(8)
+OP_W8A16, OP_W8A8_FP8, OP_FP8_LINEAR, OP_W8A8_INT8, OP_INT8_LINEAR, OP_FP8W, OP_W8A16_SILU, OP_W8A16_FUSED, OP_LORA = range(9)
 # qtts_prologue
 PRO_NONE, PRO_SILU_MUL, PRO_RMS_NORM = 0, 1, 2
 # qtts_strip_kind
 STRIP_INT8, STRIP_FP8 = 0, 1
 # qtts_code_kind
 CODE_INT8, CODE_E4M3 = 0, 1
+#: the largest rank and partition count of qtts_lora_add
+LORA_MAX_RANK, LORA_MAX_PARTS = 128, 8
 
 EXPORTS = (
     "qtts_abi_version",
@@ -98,6 +100,9 @@ EXPORTS = (
     "qtts_rms_norm",
     "qtts_w8a16_fused_gemm_strips",
     "qtts_w8a16_gate_up_silu_strips",
+    "qtts_rms_norm_quant",
+    "qtts_silu_mul_quant",
+    "qtts_lora_add",
     "qtts_kernel_timer_begin",
     "qtts_kernel_timer_end",
 )
@@ -192,6 +197,13 @@ def load() -> ctypes.CDLL:
         L.qtts_w8a16_gate_up_silu_strips.restype = i32
         L.qtts_w8a16_gate_up_silu_strips.argtypes = [p, i32, i64, i64, i64, i32, p, ctypes.c_float, p, i64, p, i32,
                                                      p, p, i64, i32, p, i64, p]
+        L.qtts_rms_norm_quant.restype = i32
+        L.qtts_rms_norm_quant.argtypes = [p, i32, i64, i64, i64, p, i64, p, ctypes.c_float, i32, p, p, p, i64, p, i64, p]
+        L.qtts_silu_mul_quant.restype = i32
+        L.qtts_silu_mul_quant.argtypes = [p, i32, i64, i64, i64, i32, p, p, p, i64, p]
+        L.qtts_lora_add.restype = i32
+        L.qtts_lora_add.argtypes = [p, i32, i64, i64, i64, p, p, i64, p, p, i64, p, p, p, i64, p, i64, p, i64, i64, p, i64,
+                                    p]
         L.qtts_kernel_timer_begin.restype = i32
         L.qtts_kernel_timer_begin.argtypes = [i32]
         L.qtts_kernel_timer_end.restype = i32

@@ -8,6 +8,8 @@ CPU or eager-PyTorch fallback: a missing library or an unsupported device raises
 
 from __future__ import annotations
 
+import contextlib
+import ctypes
 import functools
 import threading
 
@@ -15,7 +17,7 @@ import torch
 
 from . import _lib
 from ._lib import (ALGO_AUTO, ALGO_SKINNY_HALF, ALGO_SKINNY_QUARTER, ALGO_STREAM, DIV_DEVICE, DIV_IEEE,  # noqa: F401
-                   OP_FP8_LINEAR, OP_FP8W, OP_INT8_LINEAR, OP_W8A16, OP_W8A16_FUSED, OP_W8A16_SILU, OP_W8A8_FP8, OP_W8A8_INT8, PRO_NONE,
+                   LORA_MAX_PARTS, LORA_MAX_RANK, OP_FP8_LINEAR, OP_FP8W, OP_INT8_LINEAR, OP_LORA, OP_W8A16, OP_W8A16_FUSED, OP_W8A16_SILU, OP_W8A8_FP8, OP_W8A8_INT8, PRO_NONE,
                    PRO_RMS_NORM, PRO_SILU_MUL, STRIP_FP8, STRIP_INT8, CODE_E4M3, CODE_INT8, TILE_READ_AHEAD, TILE_TWO_CHUNKS, algo_code,
                    tile_shape)
 
@@ -822,6 +824,160 @@ def w8a16_gate_up_silu_strips(x: torch.Tensor, qs: torch.Tensor, n: int, scale: 
     return _shaped(act, shape)
 
 
+# ---- 8-bit activations from their producers ------------------------------------------------
+
+_CODE_DTYPES = {CODE_INT8: torch.int8, CODE_E4M3: torch.float8_e4m3fn}
+_NO_GUARD = contextlib.nullcontext()
+
+
+def _on(dev: torch.device):
+    """``dev`` made the current device for a launch on it (nothing to do where it is)."""
+    return _NO_GUARD if dev.index == torch._C._cuda_getDevice() else torch.cuda.device(dev)
+
+
+def _codes_out(rows: int, k: int, codes: int, dev: torch.device) -> tuple[torch.Tensor, torch.Tensor]:
+    dtype = _CODE_DTYPES.get(codes)
+    if dtype is None:
+        raise ValueError(f"codes must be CODE_INT8 or CODE_E4M3, got {codes}")
+    return torch.empty((rows, k), dtype=dtype, device=dev), torch.empty(rows, dtype=torch.float32, device=dev)
+
+
+def rms_norm_quant(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual: torch.Tensor | None = None,
+                   codes: int = CODE_E4M3, want_normed: bool = False):
+    """``RMSNorm(x + residual)`` straight to the per-token codes of a W8A8 linear, in one kernel.
+
+    x ``[..., K]`` bf16 / fp16 / fp32, weight ``[K]``, residual like x or None.  Returns ``(qx [M, K] e4m3 or int8,
+    sx [M] fp32, hidden, normed)``: hidden is ``x + residual`` rounded to x's dtype (None without a residual) and
+    normed the norm's 16-bit value (None unless ``want_normed``), both in x's shape.  The norm's value goes to its
+    code from fp32, ``sx = max(amax, 1e-6) / 448`` (e4m3) or ``/ 127`` (int8); feed ``qx, sx`` to
+    :func:`w8a8_fp8_gemm_strips` / :func:`w8a8_int8_gemm_strips`."""
+    a = _flatten(x)
+    rows, k = a.shape
+    if weight.numel() != k:
+        raise ValueError(f"norm weight has {weight.numel()} entries for rows of {k}")
+    res = None
+    if residual is not None:
+        if residual.shape != x.shape or residual.dtype != x.dtype:
+            raise ValueError(f"residual must be {tuple(x.shape)} {x.dtype}, got {tuple(residual.shape)} {residual.dtype}")
+        res = _flatten(residual)
+    dev = _require_cuda(a, weight, res)
+    dtype = a.dtype
+    w = weight if weight.dtype == dtype and weight.is_contiguous() else weight.to(dtype).contiguous()
+    qx, sx = _codes_out(rows, k, codes, dev)
+    hidden = None if res is None else torch.empty((rows, k), dtype=dtype, device=dev)
+    normed = torch.empty((rows, k), dtype=dtype, device=dev) if want_normed else None
+    with _on(dev):
+        st = _lib.load().qtts_rms_norm_quant(
+            a.data_ptr(), dtype_code(dtype), rows, k, a.stride(0) if rows > 1 else k, _ptr(res),
+            res.stride(0) if res is not None and rows > 1 else k, w.data_ptr(), eps, codes, qx.data_ptr(), sx.data_ptr(),
+            _ptr(hidden), k, _ptr(normed), k, _stream(dev))
+    _lib.check(st, "rms_norm_quant")
+    if x.dim() != 2:
+        hidden = None if hidden is None else hidden.view(x.shape)
+        normed = None if normed is None else normed.view(x.shape)
+    return qx, sx, hidden, normed
+
+
+def silu_mul_quant(gate_up: torch.Tensor, codes: int = CODE_E4M3, want_act: bool = False):
+    """``silu(gate) * up`` of a fused ``[..., 2I]`` gate_up output straight to the per-token codes of a W8A8 down
+    projection, in one kernel: ``(qx [M, I] e4m3 or int8, sx [M] fp32, act)``, act the 16-bit value ``[..., I]`` or
+    None unless ``want_act``.  The value goes to its code from fp32, as in :func:`rms_norm_quant`."""
+    shape = gate_up.shape
+    a = _gate_up_rows(gate_up)
+    rows, k = a.shape[0], a.shape[1] // 2
+    dev = _require_cuda(a)
+    qx, sx = _codes_out(rows, k, codes, dev)
+    act = torch.empty((rows, k), dtype=a.dtype, device=dev) if want_act else None
+    with _on(dev):
+        st = _lib.load().qtts_silu_mul_quant(a.data_ptr(), dtype_code(a.dtype), rows, k,
+                                             a.stride(0) if rows > 1 else 2 * k, codes, qx.data_ptr(), sx.data_ptr(),
+                                             _ptr(act), k, _stream(dev))
+    _lib.check(st, "silu_mul_quant")
+    return qx, sx, act if act is None else _shaped(act, shape)
+
+
+# ---- low-rank adapters of many requests ----------------------------------------------------
+
+class LoraBatch:
+    """Which adapter slot each row of a batch takes: ``index`` ``[M]`` int32 on the GPU (-1, or any value outside
+    ``[0, slots)``: none).  Made once a step by :func:`lora_batch` and shared by every linear of the step.  A captured
+    graph reads the index it was given on every replay."""
+
+    __slots__ = ("index", "slots", "rows")
+
+    def __init__(self, index: torch.Tensor, slots: int) -> None:
+        self.index, self.slots, self.rows = index, slots, index.shape[0]
+
+
+def lora_batch(index: torch.Tensor, slots: int) -> LoraBatch:
+    """The rows' adapter slots, ready for :func:`lora_add`."""
+    if index.dim() != 1 or index.dtype != torch.int32 or not index.is_contiguous():
+        raise ValueError(f"index must be a contiguous 1-D int32 tensor, got {index.dtype} {tuple(index.shape)}")
+    if slots < 0:
+        raise ValueError(f"slots is negative: {slots}")
+    _require_cuda(index)
+    return LoraBatch(index, int(slots))
+
+
+@functools.lru_cache(maxsize=256)
+def _part_ends(partitions: tuple[int, ...]):
+    ends, at = [], 0
+    for size in partitions:
+        if size < 0:
+            raise ValueError(f"partition of {size} columns")
+        at += size
+        ends.append(at)
+    return (ctypes.c_int64 * len(ends))(*ends), at
+
+
+def lora_add(base: torch.Tensor, x: torch.Tensor, batch: LoraBatch, a: torch.Tensor, b: torch.Tensor,
+             scaling: torch.Tensor, ranks: torch.Tensor | None = None, partitions=None,
+             out: torch.Tensor | None = None) -> torch.Tensor:
+    """``base + scaling[s] * (x @ a[s]^T) @ b[s]^T`` with each row's own adapter slot ``s``.
+
+    base ``[..., N]`` is the shared projection's output, x ``[..., K]`` its input (bf16 or fp16).  a ``[S, P * R, K]``
+    and b ``[S, N, R]`` hold S adapters of rank up to R for a linear of P output ``partitions`` (their widths; None:
+    one of N), scaling ``[S]`` fp32, ranks ``[S]`` int32 or None (all R): entries past a slot's rank are not used.
+    Rows without an adapter are base.  Returns a fresh tensor in base's shape, or ``out`` (which may be base)."""
+    xr, br = _flatten(x), _flatten(base)
+    m, k = xr.shape
+    n, dtype = br.shape[1], xr.dtype
+    if br.shape[0] != m or batch.rows != m:
+        raise ValueError(f"x has {m} rows, base {br.shape[0]} and the index {batch.rows}")
+    if br.dtype != dtype or a.dtype != dtype or b.dtype != dtype:
+        raise ValueError(f"x, base, a and b must have one dtype, got {dtype}, {br.dtype}, {a.dtype} and {b.dtype}")
+    if a.dim() != 3 or b.dim() != 3 or not a.is_contiguous() or not b.is_contiguous():
+        raise ValueError("a and b must be contiguous [S, P * R, K] and [S, N, R] tensors")
+    ends, width = _part_ends((n,) if partitions is None else tuple(partitions))
+    rank = b.shape[2]
+    if width != n or a.shape != (batch.slots, len(ends) * rank, k) or b.shape != (batch.slots, n, rank):
+        raise ValueError(f"a {tuple(a.shape)} and b {tuple(b.shape)} do not fit {batch.slots} adapters of a [{n}, {k}] "
+                         f"linear with {len(ends)} partitions of {width} columns in all")
+    if scaling.numel() != batch.slots or scaling.dtype != torch.float32 or not scaling.is_contiguous():
+        raise ValueError(f"scaling must be {batch.slots} contiguous fp32 entries")
+    if ranks is not None and (ranks.numel() != batch.slots or ranks.dtype != torch.int32 or not ranks.is_contiguous()):
+        raise ValueError(f"ranks must be {batch.slots} contiguous int32 entries")
+    dev = _require_cuda(xr, br, a, b, scaling, ranks, batch.index)
+    if out is None:
+        y = torch.empty((m, n), dtype=dtype, device=dev)
+    else:
+        y = _flatten(out)
+        if y.shape != (m, n) or y.dtype != dtype or y.device != dev or y.data_ptr() != out.data_ptr():
+            raise ValueError(f"out must be a [{m}, {n}] {dtype} tensor on {dev}")
+    _ensure_workspace(dev, workspace_bytes(OP_LORA, m, a.shape[1], k), "lora_add")
+    ws, ws_n = _ws_for(dev)
+    with _on(dev):
+        st = _lib.load().qtts_lora_add(
+            xr.data_ptr(), dtype_code(dtype), m, k, xr.stride(0) if m > 1 else k, batch.index.data_ptr(), None,
+            batch.slots, a.data_ptr(), b.data_ptr(), rank, _ptr(ranks), scaling.data_ptr(), ends, len(ends),
+            br.data_ptr(), br.stride(0) if m > 1 else n, y.data_ptr(), n, y.stride(0) if m > 1 else n, ws, ws_n,
+            _stream(dev))
+    _lib.check(st, "lora_add")
+    if out is not None:
+        return out
+    return y if base.dim() == 2 else y.view(base.shape)
+
+
 class KernelTimer:
     """Summed device durations of the kernels this library launches inside the block.
 
@@ -841,7 +997,6 @@ class KernelTimer:
         return self
 
     def __exit__(self, *exc) -> None:
-        import ctypes
         ms, n, u = ctypes.c_double(), ctypes.c_int64(), ctypes.c_int64()
         _lib.check(_lib.load().qtts_kernel_timer_end(ctypes.byref(ms), ctypes.byref(n), ctypes.byref(u)),
                    "kernel_timer_end")
