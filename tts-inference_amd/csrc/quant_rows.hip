@@ -9,7 +9,11 @@
 // kernels (rms_norm or silu_mul, then the activation quantizer) round it to 16 bits in between.  A NaN
 // among a row's v makes its scale NaN, as torch's amax does; e4m3 codes of such a row are NaN, int8
 // codes (which have none) zero.
+#include <algorithm>
+#include <type_traits>
+
 #include "common.h"
+#include "quant_rows_rule.h"
 
 using namespace qtts;
 
@@ -41,11 +45,205 @@ template <bool FP8> __device__ __forceinline__ uint8_t code_of(float v, bool liv
   else return live ? (uint8_t)(int8_t)int8_code_of(v) : 0;
 }
 
-__device__ __forceinline__ float silu_f32(float g) { return g / (1.0f + expf(-g)); }
+// Codes of four values times c, low first.  int8: one fma onto 1.5 * 2^23, whose low byte is then the
+// nearest integer (|v c| <= 127 but for the last bit of c); e4m3: v_cvt_pk_fp8_f32.
+template <bool FP8> __device__ __forceinline__ uint32_t codes4(const float* v, float c, bool fin) {
+  if constexpr (FP8) {
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(v[0] * c, v[1] * c, 0, false);
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(v[2] * c, v[3] * c, w, true);
+  } else {
+    uint32_t t[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) t[i] = __float_as_uint(__builtin_fmaf(v[i], c, 12582912.0f));
+    const uint32_t lo = __builtin_amdgcn_perm(t[1], t[0], 0x0c0c0400u), hi = __builtin_amdgcn_perm(t[3], t[2], 0x0c0c0400u);
+    return fin ? lo | (hi << 16) : 0u;
+  }
+}
 
-// One row a workgroup at a time, element by element, the row read twice.
+// silu(g) = g / (1 + 2^(-g log2 e)), the exponential and the reciprocal by the hardware's (an ulp each; the
+// exponent's own rounding makes it |g| ulps where the result is e^-|g| small).
+__device__ __forceinline__ float silu_f32(float g) {
+  return g * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504f * g));
+}
+
+// ---- eight elements of a row --------------------------------------------------------------
+// VEC: eight neighbours (16-byte aligned, K % 8 == 0), loaded and stored as vectors.  Otherwise element
+// i of vector j is column (8 j + i) T + tid: neighbouring lanes on neighbouring elements, one at a time,
+// for rows that start anywhere; columns past K read the last one and count as zero.
+
+struct Eight { float f[8]; };
+
+template <typename XT, bool VEC, int T> struct RowAccess {
+  int k, tid;
+
+  __device__ __forceinline__ bool live(int j, int i) const {
+    return VEC ? 8 * (tid + T * j) < k : (8 * j + i) * T + tid < k;
+  }
+
+  __device__ __forceinline__ Eight load(const XT* row, int j) const {
+    Eight e;
+    if constexpr (VEC && sizeof(XT) == 2) {
+      const i32x4_t v = *(const i32x4_t*)(row + min(8 * (tid + T * j), k - 8));  // clamped: in the row
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        e.f[2 * i] = to_f32(XT{(uint16_t)v[i]});
+        e.f[2 * i + 1] = to_f32(XT{(uint16_t)((uint32_t)v[i] >> 16)});
+      }
+    } else if constexpr (VEC) {
+      const f32x4_t* v = (const f32x4_t*)(row + min(8 * (tid + T * j), k - 8));
+      const f32x4_t lo = v[0], hi = v[1];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) e.f[i] = lo[i], e.f[4 + i] = hi[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) e.f[i] = to_f32(row[min((8 * j + i) * T + tid, k - 1)]);
+    }
+    return e;
+  }
+
+  __device__ __forceinline__ void store(XT* row, int j, const Eight& e) const {
+    if constexpr (VEC) {
+      if (!live(j, 0)) return;
+      XT* to = row + 8 * (tid + T * j);
+      if constexpr (sizeof(XT) == 2) {
+        i32x4_t v;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = (int)pack2_f32<XT>(e.f[2 * i], e.f[2 * i + 1]);
+        *(i32x4_t*)to = v;
+      } else {
+        ((f32x4_t*)to)[0] = f32x4_t{e.f[0], e.f[1], e.f[2], e.f[3]};
+        ((f32x4_t*)to)[1] = f32x4_t{e.f[4], e.f[5], e.f[6], e.f[7]};
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (live(j, i)) row[(8 * j + i) * T + tid] = from_f32<XT>(e.f[i]);
+    }
+  }
+
+  // The codes of e * c; zeros for a row that is not `live` (int8).
+  template <bool FP8> __device__ __forceinline__ void store_codes(uint8_t* row, int j, const Eight& e, float c, bool fin) const {
+    uint32_t w[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) w[h] = codes4<FP8>(&e.f[4 * h], c, fin);
+    if constexpr (VEC) {
+      if (live(j, 0)) *(uint2*)(row + 8 * (tid + T * j)) = make_uint2(w[0], w[1]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (live(j, i)) row[(8 * j + i) * T + tid] = (uint8_t)(w[i >> 2] >> (8 * (i & 3)));
+    }
+  }
+};
+
+// Sum and largest magnitude over a workgroup of T threads, in every thread.  One LDS exchange for both.
+template <int T> __device__ __forceinline__ void meet(float& ss, uint32_t& mx, float* sum, uint32_t* top) {
+  ss = wave_sum_rows(ss);
+  mx = wave_umax(mx);
+  if constexpr (T > 64) {
+    const int tid = threadIdx.x;
+    if ((tid & 63) == 0) sum[tid >> 6] = ss, top[tid >> 6] = mx;
+    __syncthreads();
+    ss = sum[0], mx = top[0];
+#pragma unroll
+    for (int i = 1; i < T / 64; ++i) ss += sum[i], mx = umax(mx, top[i]);
+  }
+}
+
+// The row in registers (K <= 8 T V): one memory round trip and one exchange a row.  max |h w| is taken in the
+// same pass as the sum of squares, since inv scales every value alike: max |v| = max |h w| inv, and the codes
+// need h w alone, round(h w (inv / scale)).  A product of two 16-bit values is exact in fp32.
+template <typename XT, bool FP8, bool VEC, int T, int V>
+__global__ __launch_bounds__(T) void rms_norm_quant_kernel(
+    const XT* x, int64_t ldx, const XT* res, int64_t ldr, const XT* __restrict__ w, int k, float eps,
+    uint8_t* __restrict__ q, float* __restrict__ sx, XT* hidden, int64_t ldh, XT* __restrict__ normed, int64_t ldn) {
+  __shared__ float sum[T / 64];
+  __shared__ uint32_t top[T / 64];
+  const int64_t row = blockIdx.x;
+  const RowAccess<XT, VEC, T> at{k, (int)threadIdx.x};
+  Eight p[V], wt[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) p[j] = at.load(x + row * ldx, j);
+#pragma unroll
+  for (int j = 0; j < V; ++j) wt[j] = at.load(w, j);
+  if (res) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const Eight r = at.load(res + row * ldr, j);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) p[j].f[i] = round_through<XT>(p[j].f[i] + r.f[i]);
+    }
+  }
+  if (hidden) {  // each element is read and written by one thread: hidden may be x or the residual
+#pragma unroll
+    for (int j = 0; j < V; ++j) at.store(hidden + row * ldh, j, p[j]);
+  }
+  float ss = 0.0f;
+  uint32_t mx = 0;
+#pragma unroll
+  for (int j = 0; j < V; ++j)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float h = at.live(j, i) ? p[j].f[i] : 0.0f;  // a clamped column may hold its hidden already
+      ss = __builtin_fmaf(h, h, ss);
+      p[j].f[i] = h * wt[j].f[i];
+      mx = umax(mx, mag(p[j].f[i]));
+    }
+  meet<T>(ss, mx, sum, top);
+  const float inv = 1.0f / __builtin_sqrtf(ss / (float)k + eps);
+  const float s = row_scale<FP8>(__uint_as_float(mx) * inv), c = inv * (1.0f / s);
+  const bool fin = mag(s) < 0x7f800000u;
+#pragma unroll
+  for (int j = 0; j < V; ++j) at.template store_codes<FP8>(q + row * k, j, p[j], c, fin);
+  if (normed) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) p[j].f[i] *= inv;
+      at.store(normed + row * ldn, j, p[j]);
+    }
+  }
+  if (threadIdx.x == 0) sx[row] = s;
+}
+
+template <typename XT, bool FP8, bool VEC, int T, int V>
+__global__ __launch_bounds__(T) void silu_mul_quant_kernel(const XT* __restrict__ gu, int64_t ld, int k,
+                                                           uint8_t* __restrict__ q, float* __restrict__ sx,
+                                                           XT* __restrict__ act, int64_t lda) {
+  __shared__ float sum[T / 64];
+  __shared__ uint32_t top[T / 64];
+  const int64_t row = blockIdx.x;
+  const RowAccess<XT, VEC, T> at{k, (int)threadIdx.x};
+  const XT* g = gu + row * ld;
+  Eight v[V], u[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) v[j] = at.load(g, j);
+#pragma unroll
+  for (int j = 0; j < V; ++j) u[j] = at.load(g + k, j);
+  float none = 0.0f;
+  uint32_t mx = 0;
+#pragma unroll
+  for (int j = 0; j < V; ++j)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      v[j].f[i] = silu_f32(v[j].f[i]) * u[j].f[i];
+      mx = umax(mx, mag(v[j].f[i]));
+    }
+  meet<T>(none, mx, sum, top);
+  const float s = row_scale<FP8>(__uint_as_float(mx)), rs = 1.0f / s;
+  const bool fin = mag(s) < 0x7f800000u;
+#pragma unroll
+  for (int j = 0; j < V; ++j) at.template store_codes<FP8>(q + row * k, j, v[j], rs, fin);
+  if (act) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) at.store(act + row * lda, j, v[j]);
+  }
+  if (threadIdx.x == 0) sx[row] = s;
+}
+
+// Longer rows, and more rows than a grid has workgroups: element by element, the row read twice.
 template <typename XT, bool FP8>
-__global__ __launch_bounds__(kRowThreads) void rms_norm_quant_kernel(
+__global__ __launch_bounds__(kRowThreads) void rms_norm_quant_long_kernel(
     const XT* x, int64_t ldx, const XT* res, int64_t ldr, const XT* __restrict__ w, int64_t k, float eps,
     uint8_t* __restrict__ q, float* __restrict__ sx, XT* hidden, int64_t ldh, XT* __restrict__ normed, int64_t ldn,
     int64_t m) {
@@ -86,7 +284,7 @@ __global__ __launch_bounds__(kRowThreads) void rms_norm_quant_kernel(
 }
 
 template <typename XT, bool FP8>
-__global__ __launch_bounds__(kRowThreads) void silu_mul_quant_kernel(const XT* __restrict__ gu, int64_t ld, int64_t k,
+__global__ __launch_bounds__(kRowThreads) void silu_mul_quant_long_kernel(const XT* __restrict__ gu, int64_t ld, int64_t k,
                                                                      uint8_t* __restrict__ q, float* __restrict__ sx,
                                                                      XT* __restrict__ act, int64_t lda, int64_t m) {
   __shared__ uint32_t top[kRowThreads / 64];
@@ -115,29 +313,67 @@ __global__ __launch_bounds__(kRowThreads) void silu_mul_quant_kernel(const XT* _
 
 namespace {
 
-constexpr int64_t kMaxRowGrid = 1 << 20;  // workgroups; each takes every gridDim-th row
+constexpr int64_t kMaxRowGrid = 1 << 20;  // workgroups of the long kernels; each takes every gridDim-th row
 
-template <typename XT>
-void norm_by_type(bool fp8, const void* x, int64_t ldx, const void* res, int64_t ldr, const void* w, int64_t k, float eps,
-                  void* q, float* sx, void* hidden, int64_t ldh, void* normed, int64_t ldn, int64_t m, hipStream_t st) {
-  const dim3 grid((unsigned)(m < kMaxRowGrid ? m : kMaxRowGrid)), block(kRowThreads);
-  auto go = [&](auto kernel) {
-    qtts::launch(kernel, grid, block, 0, st, (const XT*)x, ldx, (const XT*)res, ldr, (const XT*)w, k, eps, (uint8_t*)q, sx,
-                 (XT*)hidden, ldh, (XT*)normed, ldn, m);
+bool aligned(const void* p, int64_t ld, int64_t esz) { return !p || ((uintptr_t)p % 16 == 0 && ld * esz % 16 == 0); }
+
+// f(vec, T, V) with the row kernel's shape as compile-time constants; false where the long kernel takes the call.
+template <typename F> bool by_form(bool vec, const RowForm& form, F&& f) {
+  auto shape = [&](auto v) {
+    using std::integral_constant;
+    switch (form.threads * 16 + form.vectors) {
+      case 64 * 16 + 1: f(v, integral_constant<int, 64>{}, integral_constant<int, 1>{}); return true;
+      case 128 * 16 + 1: f(v, integral_constant<int, 128>{}, integral_constant<int, 1>{}); return true;
+      case 256 * 16 + 1: f(v, integral_constant<int, 256>{}, integral_constant<int, 1>{}); return true;
+      case 256 * 16 + 2: f(v, integral_constant<int, 256>{}, integral_constant<int, 2>{}); return true;
+      case 256 * 16 + 3: f(v, integral_constant<int, 256>{}, integral_constant<int, 3>{}); return true;
+      case 256 * 16 + 4: f(v, integral_constant<int, 256>{}, integral_constant<int, 4>{}); return true;
+      default: return false;
+    }
   };
-  if (fp8) go(&rms_norm_quant_kernel<XT, true>);
-  else go(&rms_norm_quant_kernel<XT, false>);
+  return vec ? shape(std::true_type{}) : shape(std::false_type{});
 }
 
-template <typename XT>
-void silu_by_type(bool fp8, const void* gu, int64_t ld, int64_t k, void* q, float* sx, void* act, int64_t lda, int64_t m,
-                  hipStream_t st) {
-  const dim3 grid((unsigned)(m < kMaxRowGrid ? m : kMaxRowGrid)), block(kRowThreads);
-  auto go = [&](auto kernel) {
-    qtts::launch(kernel, grid, block, 0, st, (const XT*)gu, ld, k, (uint8_t*)q, sx, (XT*)act, lda, m);
+template <typename XT, bool FP8>
+void launch_norm(const void* x, int64_t ldx, const void* res, int64_t ldr, const void* w, int64_t k, float eps, void* q,
+                 float* sx, void* hidden, int64_t ldh, void* normed, int64_t ldn, int64_t m, hipStream_t st) {
+  constexpr int64_t e = sizeof(XT);
+  const bool vec = k % 8 == 0 && aligned(x, ldx, e) && aligned(res, ldr, e) && aligned(w, 8, e) && aligned(hidden, ldh, e) &&
+                   aligned(normed, ldn, e) && (uintptr_t)q % 8 == 0;
+  const bool done = by_form(vec, row_form(m, k), [&](auto v, auto t, auto n) {
+    qtts::launch(&rms_norm_quant_kernel<XT, FP8, v.value, t.value, n.value>, dim3((unsigned)m), dim3(t.value), 0, st,
+                 (const XT*)x, ldx, (const XT*)res, ldr, (const XT*)w, k, eps, (uint8_t*)q, sx, (XT*)hidden, ldh,
+                 (XT*)normed, ldn);
+  });
+  if (!done)
+    qtts::launch(&rms_norm_quant_long_kernel<XT, FP8>, dim3((unsigned)std::min(m, kMaxRowGrid)), dim3(kRowThreads), 0, st,
+                 (const XT*)x, ldx, (const XT*)res, ldr, (const XT*)w, k, eps, (uint8_t*)q, sx, (XT*)hidden, ldh,
+                 (XT*)normed, ldn, m);
+}
+
+template <typename XT, bool FP8>
+void launch_silu(const void* gu, int64_t ld, int64_t k, void* q, float* sx, void* act, int64_t lda, int64_t m,
+                 hipStream_t st) {
+  constexpr int64_t e = sizeof(XT);
+  const bool vec = k % 8 == 0 && aligned(gu, ld, e) && aligned(act, lda, e) && (uintptr_t)q % 8 == 0;
+  const bool done = by_form(vec, row_form(m, k), [&](auto v, auto t, auto n) {
+    qtts::launch(&silu_mul_quant_kernel<XT, FP8, v.value, t.value, n.value>, dim3((unsigned)m), dim3(t.value), 0, st,
+                 (const XT*)gu, ld, k, (uint8_t*)q, sx, (XT*)act, lda);
+  });
+  if (!done)
+    qtts::launch(&silu_mul_quant_long_kernel<XT, FP8>, dim3((unsigned)std::min(m, kMaxRowGrid)), dim3(kRowThreads), 0, st,
+                 (const XT*)gu, ld, k, (uint8_t*)q, sx, (XT*)act, lda, m);
+}
+
+// f with the element type and the code kind as types.
+template <typename F> void by_types(int x_dtype, int codes, F&& f) {
+  auto kind = [&](auto xt) {
+    if (codes == QTTS_CODE_E4M3) f(xt, std::true_type{});
+    else f(xt, std::false_type{});
   };
-  if (fp8) go(&silu_mul_quant_kernel<XT, true>);
-  else go(&silu_mul_quant_kernel<XT, false>);
+  if (x_dtype == QTTS_BF16) kind(bf16_t{});
+  else if (x_dtype == QTTS_F16) kind(f16_t{});
+  else kind(float{});
 }
 
 }  // namespace
@@ -145,18 +381,16 @@ void silu_by_type(bool fp8, const void* gu, int64_t ld, int64_t k, void* q, floa
 int qtts_launch_rms_norm_quant(const void* x, int x_dtype, int64_t m, int64_t k, int64_t ldx, const void* res, int64_t ldr,
                                const void* w, float eps, int codes, void* q, float* sx, void* hidden, int64_t ldh,
                                void* normed, int64_t ldn, hipStream_t st) {
-  const bool fp8 = codes == QTTS_CODE_E4M3;
-  if (x_dtype == QTTS_BF16) norm_by_type<bf16_t>(fp8, x, ldx, res, ldr, w, k, eps, q, sx, hidden, ldh, normed, ldn, m, st);
-  else if (x_dtype == QTTS_F16) norm_by_type<f16_t>(fp8, x, ldx, res, ldr, w, k, eps, q, sx, hidden, ldh, normed, ldn, m, st);
-  else norm_by_type<float>(fp8, x, ldx, res, ldr, w, k, eps, q, sx, hidden, ldh, normed, ldn, m, st);
+  by_types(x_dtype, codes, [&](auto xt, auto fp8) {
+    launch_norm<decltype(xt), fp8.value>(x, ldx, res, ldr, w, k, eps, q, sx, hidden, ldh, normed, ldn, m, st);
+  });
   return qtts_check_launch("rms_norm_quant");
 }
 
 int qtts_launch_silu_mul_quant(const void* gu, int x_dtype, int64_t m, int64_t k, int64_t ld, int codes, void* q, float* sx,
                                void* act, int64_t lda, hipStream_t st) {
-  const bool fp8 = codes == QTTS_CODE_E4M3;
-  if (x_dtype == QTTS_BF16) silu_by_type<bf16_t>(fp8, gu, ld, k, q, sx, act, lda, m, st);
-  else if (x_dtype == QTTS_F16) silu_by_type<f16_t>(fp8, gu, ld, k, q, sx, act, lda, m, st);
-  else silu_by_type<float>(fp8, gu, ld, k, q, sx, act, lda, m, st);
+  by_types(x_dtype, codes, [&](auto xt, auto fp8) {
+    launch_silu<decltype(xt), fp8.value>(gu, ld, k, q, sx, act, lda, m, st);
+  });
   return qtts_check_launch("silu_mul_quant");
 }
