@@ -458,6 +458,14 @@ int qtts_silu_mul_quant(const void* gate_up, int x_dtype, int64_t m, int64_t k, 
 #define QTTS_LORA_MAX_PARTS 8
 #define QTTS_LORA_MAX_RANK 128
 
+/* The rows of a batch sorted by adapter, for qtts_lora_add calls of many rows (past 64 it
+ * needs one to read the rows of an adapter together): one kernel, made anew whenever the
+ * index changes (in the same graph where calls are captured), used by every linear of a
+ * step.  index: [m] int32 on the device.  plan: qtts_lora_plan_bytes(m, slots) bytes, 16-byte
+ * aligned; 0 bytes: more slots than a plan takes (768), calls then go without. */
+int64_t qtts_lora_plan_bytes(int64_t m, int64_t slots);
+int qtts_lora_plan(const int32_t* index, int64_t m, int64_t slots, int32_t* plan, int64_t plan_bytes, void* stream);
+
 /* Each row's own low-rank adapter, added to the output of a projection that all rows share:
  *   s = index[r];  t[r, i] = sum_c x[r, c] * a[s, p * rank + i, c]
  *   out[r, j] = x_dtype(base[r, j] + scaling[s] * sum_{i < ranks[s]} t[r, i] * b[s, j, i])
@@ -470,8 +478,8 @@ int qtts_silu_mul_quant(const void* gate_up, int x_dtype, int64_t m, int64_t k, 
  * int32 or NULL (all `rank`); entries of a and b past a slot's rank are not used.  scaling:
  * [slots] fp32.  base, out: [m, n] of x_dtype, row strides ldb, ldo; out may be base itself
  * and shares no byte with x.  rank <= QTTS_LORA_MAX_RANK, parts <= QTTS_LORA_MAX_PARTS.
- * plan: what qtts_lora_plan made of the same index and slots, or NULL; with it, rows of one
- * adapter are read together wherever they stand.  Workspace: qtts_workspace_bytes(QTTS_OP_LORA,
+ * plan: what qtts_lora_plan made of the same index, m and slots, or NULL (rows of one adapter
+ * are then read together within each 64 rows); a plan of another m or slots writes nothing.  Workspace: qtts_workspace_bytes(QTTS_OP_LORA,
  * m, parts * rank, k, 0). */
 int qtts_lora_add(const void* x, int x_dtype, int64_t m, int64_t k, int64_t ldx, const int32_t* index,
                   const int32_t* plan, int64_t slots, const void* a, const void* b, int64_t rank, const int32_t* ranks,

@@ -214,6 +214,44 @@ def test_graph_follows_the_index(ops, m):
         _check(out, c, f"replay {i}")
 
 
+@pytest.mark.parametrize("m,slots", [(65, 1), (100, 3), (1000, 7), (4097, 768), (5000, 40), (70000, 500), (64 * 1024, 1)])
+def test_plan(ops, m, slots):
+    """The plan holds every row once, stably sorted by slot, in tiles of at most 64 rows of one slot."""
+    g = torch.Generator().manual_seed(m)
+    index = torch.randint(-2, slots + 1, (m,), generator=g, dtype=torch.int32)
+    plan = ops.lora_batch(index.cuda(), slots).plan.cpu()
+    slot = torch.where((index < 0) | (index >= slots), slots, index)
+    order = plan[-m:].long()
+    assert torch.equal(order, torch.argsort(slot, stable=True))
+    tiles, at = plan[4:4 + 4 * int(plan[0])].view(-1, 4), 0
+    assert plan[1] == m and plan[2] == slots
+    for s, start, count, _ in tiles.tolist():
+        assert start == at and 0 < count <= 64
+        want = slots if s < 0 else s
+        assert (slot[order[start:start + count]] == want).all()
+        at += count
+        assert count == 64 or at == m or slot[order[at]] != want
+    assert at == m
+
+
+def test_many_adapters(ops):
+    """Past the slots that a plan takes, and past 64 rows, the rows are grouped window by window."""
+    c = _case(150, 64, [40, 24], 900, 16, torch.bfloat16, seed=61)
+    assert ops.lora_batch(c["index"], 900).plan is None
+    _check(_run(ops, c), c)
+    c["index"] = (torch.arange(150) % 2 * 800).to(torch.int32).cuda()
+    _check(_run(ops, c), c)
+
+
+def test_a_plan_of_another_batch_writes_nothing(ops):
+    c = _case(100, 64, [40], 5, 16, torch.bfloat16, seed=62)
+    batch = ops.lora_batch(c["index"], 5)
+    batch.plan = ops.lora_batch(c["index"][:90].contiguous(), 5).plan
+    out = torch.full((100, 40), 3.0, dtype=torch.bfloat16, device="cuda")
+    ops.lora_add(c["base"], c["x"], batch, c["a"], c["b"], c["scaling"], c["ranks"], c["parts"], out=out)
+    assert (out == 3.0).all()
+
+
 def test_repeats_give_the_same_bits(ops):
     for m in (30, 500):
         c = _case(m, 1024, [512], 8, 16, torch.bfloat16, seed=51)

@@ -118,6 +118,22 @@ def test_lora_entry():
         assert call() == -2 and call(out=140000) == -2 and call(ranks=None) == -2 and call(ends=(0, 32, 32, 96), rank=4) == -2
 
 
+def test_lora_plan_entry():
+    L = _lib.load()
+    b = _buf()
+    at = (_at(b) + 15) & ~15
+    need = L.qtts_lora_plan_bytes(100, 4)
+    assert need >= 4 * 100 and L.qtts_lora_plan_bytes(0, 0) > 0
+    assert L.qtts_lora_plan_bytes(100, 769) == 0  # more than a plan takes
+    for m, slots in ((-1, 4), (100, -1), (1 << 31, 4), (100, 1 << 30)):
+        assert L.qtts_lora_plan_bytes(m, slots) == -1 and L.qtts_lora_plan(at, m, slots, at, 1 << 40, None) == -1
+    _refused(L.qtts_lora_plan(at, 100, 769, at, 1 << 20, None), "slots")
+    _refused(L.qtts_lora_plan(None, 100, 4, at, need, None), "null")
+    _refused(L.qtts_lora_plan(at, 100, 4, None, need, None), "null")
+    _refused(L.qtts_lora_plan(at, 100, 4, at + 4, need, None), "unaligned")
+    _refused(L.qtts_lora_plan(at, 100, 4, at, need - 1, None), "needed")
+
+
 def test_wrappers_check_shapes_and_types():
     bf, f32, i32 = torch.bfloat16, torch.float32, torch.int32
     x, w = torch.zeros(2, 64, dtype=bf), torch.ones(64, dtype=bf)

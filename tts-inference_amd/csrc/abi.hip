@@ -75,7 +75,8 @@ int qtts_launch_rms_norm_quant(const void* x, int x_dtype, int64_t m, int64_t k,
                                void* normed, int64_t ldn, hipStream_t st);
 int qtts_launch_silu_mul_quant(const void* gu, int x_dtype, int64_t m, int64_t k, int64_t ld, int codes, void* q, float* sx,
                                void* act, int64_t lda, hipStream_t st);
-int64_t qtts_lora_ws_bytes(int64_t m, int64_t rows_a);
+int64_t qtts_lora_ws_bytes(int64_t m, int64_t rows_a, int64_t k);
+int qtts_launch_lora_plan(const int32_t* index, int64_t m, int64_t slots, int32_t* plan, hipStream_t st);
 int qtts_launch_lora_add(const qtts::LoraArgs& args, int x_dtype, void* ws, hipStream_t st);
 
 static thread_local char g_last_error[512] = "";
@@ -260,8 +261,8 @@ int64_t qtts_workspace_bytes(int op, int64_t m, int64_t n, int64_t k, int algo) 
     case QTTS_OP_W8A16_SILU: return qtts_w8a16_silu_ws_bytes(m, n, k, algo, QTTS_BF16);
     case QTTS_OP_W8A16_FUSED: return qtts_w8a16_fused_ws_bytes(m, n, k, algo, QTTS_BF16);
     case QTTS_OP_LORA:
-      if (m > (1ll << 58) / n) return qtts_set_error(QTTS_ERR_INVALID_ARGUMENT, "bad workspace query");
-      return qtts_lora_ws_bytes(m, n);
+      if (m > (1ll << 54) / n) return qtts_set_error(QTTS_ERR_INVALID_ARGUMENT, "bad workspace query");
+      return qtts_lora_ws_bytes(m, n, k);
     default: return qtts_set_error(QTTS_ERR_INVALID_ARGUMENT, "unknown op %d", op);
   }
 }
@@ -711,11 +712,26 @@ int qtts_silu_mul_quant(const void* gate_up, int x_dtype, int64_t m, int64_t k, 
   return qtts_launch_silu_mul_quant(gate_up, x_dtype, m, k, ld_gate_up, codes, qx, sx, act, ldact, (hipStream_t)stream);
 }
 
+int64_t qtts_lora_plan_bytes(int64_t m, int64_t slots) {
+  if (m < 0 || slots < 0 || m >= (1ll << 31) || slots >= (1ll << 30))
+    return qtts_set_error(QTTS_ERR_INVALID_ARGUMENT, "lora_plan: bad sizes");
+  return slots > qtts::kPlanMaxSlots ? 0 : qtts::plan_words(m, slots) * 4;
+}
+
+int qtts_lora_plan(const int32_t* index, int64_t m, int64_t slots, int32_t* plan, int64_t plan_bytes, void* stream) {
+  const int64_t need = qtts_lora_plan_bytes(m, slots);
+  if (need < 0) return (int)need;
+  QTTS_REQUIRE(slots <= qtts::kPlanMaxSlots, "lora_plan: %lld slots, more than %d", (long long)slots, qtts::kPlanMaxSlots);
+  QTTS_REQUIRE(plan && (uintptr_t)plan % 16 == 0 && (m == 0 || index), "lora_plan: null or unaligned pointer");
+  QTTS_REQUIRE(plan_bytes >= need, "lora_plan: plan of %lld bytes < %lld needed", (long long)plan_bytes, (long long)need);
+  QTTS_TRY(current_device_check());
+  return qtts_launch_lora_plan(index, m, slots, plan, (hipStream_t)stream);
+}
+
 int qtts_lora_add(const void* x, int x_dtype, int64_t m, int64_t k, int64_t ldx, const int32_t* index, const int32_t* plan,
                   int64_t slots, const void* a, const void* b, int64_t rank, const int32_t* ranks, const float* scaling,
                   const int64_t* part_ends, int64_t parts, const void* base, int64_t ldb, void* out, int64_t n, int64_t ldo,
                   void* ws, int64_t ws_bytes, void* stream) {
-  (void)plan;
   QTTS_REQUIRE(m >= 0 && n >= 0 && k >= 0 && slots >= 0, "lora_add: negative size");
   QTTS_REQUIRE(m < (1ll << 31) && n < (1ll << 30) && k < (1ll << 30) && slots < (1ll << 30), "lora_add: size too large");
   QTTS_REQUIRE(x_dtype == QTTS_BF16 || x_dtype == QTTS_F16, "lora_add: activations must be bf16 or fp16");
@@ -730,11 +746,12 @@ int qtts_lora_add(const void* x, int x_dtype, int64_t m, int64_t k, int64_t ldx,
   QTTS_REQUIRE(ldx >= k && ldb >= n && ldo >= n, "lora_add: leading dimension smaller than the row");
   QTTS_REQUIRE(ws_bytes >= 0, "lora_add: negative workspace size");
   if (m == 0 || n == 0) return QTTS_OK;
+  QTTS_REQUIRE((uintptr_t)plan % 16 == 0, "lora_add: unaligned plan");
   QTTS_REQUIRE(base && out && index && (slots == 0 || (scaling && b && (k == 0 || (x && a)))), "lora_add: null pointer");
   QTTS_REQUIRE((out == base && ldo == ldb) || !spans_overlap(base, m, ldb, n, 2, out, m, ldo, n, 2),
                "lora_add: out overlaps base");
   QTTS_REQUIRE(!spans_overlap(x, m, ldx, k, 2, out, m, ldo, n, 2), "lora_add: out overlaps x");
-  const int64_t need = qtts_lora_ws_bytes(m, parts * rank);
+  const int64_t need = qtts_lora_ws_bytes(m, parts * rank, k);
   if (!ws || ws_bytes < need)
     return qtts_set_error(QTTS_ERR_WORKSPACE, "lora_add: workspace of %lld bytes < %lld needed", (long long)ws_bytes,
                           (long long)need);
@@ -743,6 +760,7 @@ int qtts_lora_add(const void* x, int x_dtype, int64_t m, int64_t k, int64_t ldx,
   g.x = x;
   g.ldx = ldx;
   g.index = index;
+  g.plan = plan;
   g.a = a;
   g.b = b;
   g.ranks = ranks;

@@ -1,4 +1,4 @@
-// Low-rank adapters of many requests beside one linear (lora.hip): the call's arguments.
+// Low-rank adapters of many requests beside one linear (lora.hip): the call's arguments and the plan's layout.
 #pragma once
 
 #include <stdint.h>
@@ -13,12 +13,14 @@ constexpr int kLoraMaxRank = 128;
 struct LoraParts {
   int count;
   int32_t end[kLoraMaxParts];
+  int32_t chunk_end[kLoraMaxParts];  // workgroups along the columns, each within one partition
 };
 
 struct LoraArgs {
+  const int32_t* index;  // [m], the row's slot; outside [0, slots): no adapter
+  const int32_t* plan;   // or null
   const void* x;
   int64_t ldx;
-  const int32_t* index;  // [m], the row's slot; outside [0, slots): no adapter
   const void* a;         // [slots, parts.count * rank, k]
   const void* b;         // [slots, n, rank]
   const int32_t* ranks;  // [slots] or null
@@ -27,10 +29,22 @@ struct LoraArgs {
   int64_t ldb;
   void* out;
   int64_t ldo;
-  float* t;  // [m, parts.count * rank]
+  float* t;  // [splits, m, t_stride]: partial sums over K of x A^T
   int64_t m;
-  int k, n, slots, rank;
+  int k, n, slots, rank, rows_a, t_stride, splits;
   LoraParts parts;
 };
+
+// ---- the plan: rows sorted by slot, cut into tiles of one slot each ----------------------------
+// int32 words: the number of tiles, m, slots, 0; then, from word 4, four words a tile (slot, or -1 for rows without an
+// adapter; its first entry of the order; its rows, at most kPlanTile; 0); then the order of the rows.
+constexpr int kPlanTile = 64;
+constexpr int kPlanMaxSlots = 768;  // the sort's counters are in LDS
+
+__host__ __device__ inline int64_t plan_max_tiles(int64_t m, int64_t slots) {
+  return (m + kPlanTile - 1) / kPlanTile + (m < slots + 1 ? m : slots + 1);
+}
+__host__ __device__ inline int64_t plan_order_at(int64_t m, int64_t slots) { return 4 + 4 * plan_max_tiles(m, slots); }
+__host__ __device__ inline int64_t plan_words(int64_t m, int64_t slots) { return plan_order_at(m, slots) + m; }
 
 }  // namespace qtts

@@ -102,6 +102,8 @@ EXPORTS = (
     "qtts_w8a16_gate_up_silu_strips",
     "qtts_rms_norm_quant",
     "qtts_silu_mul_quant",
+    "qtts_lora_plan_bytes",
+    "qtts_lora_plan",
     "qtts_lora_add",
     "qtts_kernel_timer_begin",
     "qtts_kernel_timer_end",
@@ -201,6 +203,10 @@ def load() -> ctypes.CDLL:
         L.qtts_rms_norm_quant.argtypes = [p, i32, i64, i64, i64, p, i64, p, ctypes.c_float, i32, p, p, p, i64, p, i64, p]
         L.qtts_silu_mul_quant.restype = i32
         L.qtts_silu_mul_quant.argtypes = [p, i32, i64, i64, i64, i32, p, p, p, i64, p]
+        L.qtts_lora_plan_bytes.restype = i64
+        L.qtts_lora_plan_bytes.argtypes = [i64, i64]
+        L.qtts_lora_plan.restype = i32
+        L.qtts_lora_plan.argtypes = [p, i64, i64, p, i64, p]
         L.qtts_lora_add.restype = i32
         L.qtts_lora_add.argtypes = [p, i32, i64, i64, i64, p, p, i64, p, p, i64, p, p, p, i64, p, i64, p, i64, i64, p, i64,
                                     p]

@@ -898,25 +898,40 @@ def silu_mul_quant(gate_up: torch.Tensor, codes: int = CODE_E4M3, want_act: bool
 
 # ---- low-rank adapters of many requests ----------------------------------------------------
 
+#: Rows up to which a batch needs no plan (qtts_lora_add groups the rows of each 64 by itself).
+LORA_WINDOW = 64
+
+
 class LoraBatch:
     """Which adapter slot each row of a batch takes: ``index`` ``[M]`` int32 on the GPU (-1, or any value outside
-    ``[0, slots)``: none).  Made once a step by :func:`lora_batch` and shared by every linear of the step.  A captured
-    graph reads the index it was given on every replay."""
+    ``[0, slots)``: none), and past :data:`LORA_WINDOW` rows the ``plan`` that sorts them.  Made by
+    :func:`lora_batch` whenever the index changes (inside the graph where a step is captured: replays then follow the
+    index) and shared by every linear of the step."""
 
-    __slots__ = ("index", "slots", "rows")
+    __slots__ = ("index", "slots", "rows", "plan")
 
-    def __init__(self, index: torch.Tensor, slots: int) -> None:
-        self.index, self.slots, self.rows = index, slots, index.shape[0]
+    def __init__(self, index: torch.Tensor, slots: int, plan: torch.Tensor | None = None) -> None:
+        self.index, self.slots, self.rows, self.plan = index, slots, index.shape[0], plan
 
 
 def lora_batch(index: torch.Tensor, slots: int) -> LoraBatch:
-    """The rows' adapter slots, ready for :func:`lora_add`."""
+    """The rows' adapter slots, ready for :func:`lora_add`: one kernel past :data:`LORA_WINDOW` rows, else none."""
     if index.dim() != 1 or index.dtype != torch.int32 or not index.is_contiguous():
         raise ValueError(f"index must be a contiguous 1-D int32 tensor, got {index.dtype} {tuple(index.shape)}")
     if slots < 0:
         raise ValueError(f"slots is negative: {slots}")
-    _require_cuda(index)
-    return LoraBatch(index, int(slots))
+    dev = _require_cuda(index)
+    m, lib = index.shape[0], _lib.load()
+    need = lib.qtts_lora_plan_bytes(m, slots) if m > LORA_WINDOW else 0
+    if need < 0:
+        _lib.check(int(need), "lora_plan")
+    if not need:
+        return LoraBatch(index, int(slots))
+    plan = torch.empty(need // 4, dtype=torch.int32, device=dev)
+    with _on(dev):
+        st = lib.qtts_lora_plan(index.data_ptr(), m, slots, plan.data_ptr(), need, _stream(dev))
+    _lib.check(st, "lora_plan")
+    return LoraBatch(index, int(slots), plan)
 
 
 @functools.lru_cache(maxsize=256)
@@ -968,7 +983,7 @@ def lora_add(base: torch.Tensor, x: torch.Tensor, batch: LoraBatch, a: torch.Ten
     ws, ws_n = _ws_for(dev)
     with _on(dev):
         st = _lib.load().qtts_lora_add(
-            xr.data_ptr(), dtype_code(dtype), m, k, xr.stride(0) if m > 1 else k, batch.index.data_ptr(), None,
+            xr.data_ptr(), dtype_code(dtype), m, k, xr.stride(0) if m > 1 else k, batch.index.data_ptr(), _ptr(batch.plan),
             batch.slots, a.data_ptr(), b.data_ptr(), rank, _ptr(ranks), scaling.data_ptr(), ends, len(ends),
             br.data_ptr(), br.stride(0) if m > 1 else n, y.data_ptr(), n, y.stride(0) if m > 1 else n, ws, ws_n,
             _stream(dev))
