@@ -5,19 +5,25 @@
 // with fp32 sums and one rounding, to the output's type.  Entries past a slot's rank are never used.
 //
 // Both products run on 16x16x32 MFMAs over groups of up to 16 rows that share a slot: A's rows and x's rows
-// lie along K, B's rows along the rank, so every operand is a 16-byte load from where it stands (a lane
-// holds row lane % 16, elements 8 (lane / 16) ... + 7).  t leaves the first product in fp32; the second
-// multiplies it as two 16-bit halves, hi = T(t) and lo = T(t - hi), which keeps 16 bits of it (bf16; 22 in
-// fp16, where the row is first scaled by the power of two that brings its largest entry to [1/2, 1)).
+// lie along K, B's rows along the rank, so an MFMA operand is 16 bytes of a row (a lane holds row lane % 16,
+// elements 8 (lane / 16) ... + 7).  Loaded that way each lane is on a line of its own, and a line is touched
+// at half or a quarter of its width; so x and A go to LDS in whole 128-byte lines (each wave its own part of K,
+// a ring of stages without a barrier), and the result meets base in LDS, whose rows are read and written in
+// 128-byte pieces.  t leaves the first product in fp32; the second multiplies it as two 16-bit halves,
+// hi = T(t) and lo = T(t - hi), which keeps 16 bits of it (bf16; 22 in fp16, where the row is first scaled by
+// the power of two that brings its largest entry to [1/2, 1)).
 //
 // Where the groups come from: up to 64 rows, each workgroup finds the rows of its slot by one load of the
 // window's indices and a ballot; past them from a plan (rows sorted by slot, made once a step).
 //
 //  * lora_one_kernel: both products in one launch, for few adapters of small rank (lora_rule.h);
 //  * lora_down_kernel, lora_up_kernel: one launch each, t through the workspace.
+#include <algorithm>
+
 #include "common.h"
 #include "lora.h"
 #include "lora_rule.h"
+#include "pipe.h"
 
 using namespace qtts;
 
@@ -69,16 +75,12 @@ __device__ __forceinline__ Group group_by_ballot(const LoraArgs& g, int64_t at) 
   return {slot, count, first + __builtin_amdgcn_ds_bpermute(4 * (before + (j < count ? j : 0)), order)};
 }
 
-// The plan's tiles; none where it was made for another batch or slot count.
-__device__ __forceinline__ int64_t plan_tiles(const LoraArgs& g) {
-  return g.plan[1] == g.m && g.plan[2] == g.slots ? g.plan[0] : 0;
-}
-
-// Sub-group `sub` (16 rows) of tile `tile` of the plan; count 0 past its end.
+// Sub-group `sub` (16 rows) of tile `tile` < plan_max_tiles; count 0 past its end, past the plan's tiles and where the
+// plan was made for another batch or slot count.
 __device__ __forceinline__ Group group_by_plan(const LoraArgs& g, int64_t tile, int sub) {
-  const i32x4_t e = *(const i32x4_t*)(g.plan + 4 + 4 * tile);
-  const int count = min(16, min(e[2], kPlanTile) - 16 * sub), j = threadIdx.x & 15;
-  if (count <= 0) return {e[0], 0, 0};
+  const i32x4_t head = *(const i32x4_t*)g.plan, e = *(const i32x4_t*)(g.plan + 4 + 4 * tile);
+  const int count = min(16, e[2] - 16 * sub), j = threadIdx.x & 15;
+  if (tile >= head[0] || head[1] != g.m || head[2] != g.slots || count <= 0) return {-1, 0, 0};
   const int64_t at = plan_order_at(g.m, g.slots) + e[1] + 16 * sub + (j < count ? j : 0);
   return {e[0], count, g.plan[at]};
 }
@@ -89,56 +91,81 @@ __device__ __forceinline__ int live_rank(const LoraArgs& g, int slot) {
 
 // ---- first product ---------------------------------------------------------------------------
 
-// Rows [16 tile, 16 (tile + N)) of the slot's A by the group's rows, over this wave's steps of 32 of K:
-// acc[i] holds, in lane l, rows 16 i + 4 (l / 16) ... + 3 of A for the group's row l % 16.
+// Stages of a wave's ring: 64 of K of the group's rows and of N 16-row tiles of A, each tile two direct loads of 1 KiB
+// (eight rows of 128 bytes, pieces swizzled as pipe.h's stages).
+template <int N> constexpr int kDownStages = N == 1 ? 4 : N == 2 ? 3 : 2;
+template <int N> constexpr int kDownBytes = kDownStages<N> * (N + 1) * 2048;  // of a wave
+
+// Rows [row0, row0 + 16 N) of a slot's A by the group's rows, over K from 32 s0 to 32 s1 (s0 even):
+// acc[i] holds, in lane l, rows 16 i + 4 (l / 16) ... + 3 of A for the group's row l % 16.  Rows past the slot's rank, or past
+// `rows`, give values that nothing reads.  lds: kDownBytes<N> of this wave alone.
 template <typename XT, int N, bool VEC>
-__device__ __forceinline__ void down_steps(const LoraArgs& g, const XT* x, const XT* a, int row0, int rows, int live, int s0,
-                                           int s1, f32x4_t* acc) {
-  const int lane = threadIdx.x & 63, j = lane & 15, off = 8 * (lane >> 4);
-  const XT* ap[N];
+__device__ __forceinline__ void down_steps(const LoraArgs& g, const Group& gr, const XT* a, int row0, int rows, int live, int s0,
+                                           int s1, uint8_t* lds, f32x4_t* acc) {
+  const int lane = threadIdx.x & 63, j = lane & 15, q = lane >> 4;
+  if constexpr (VEC) {
+    constexpr int S = kDownStages<N>, L = 2 * (N + 1);  // direct loads a stage
+    const XT* from[L];  // each direct load's row and piece, at K = 0
 #pragma unroll
-  for (int i = 0; i < N; ++i) {  // rows past the slot's rank (or past A) read its first row; nothing reads what they give
-    const int r = row0 + 16 * i + j;
-    ap[i] = a + (int64_t)(r < rows && r % g.rank < live ? r : 0) * g.k;
-  }
-  int s = s0;
-  // U steps at a time: all their loads in flight, then the MFMAs.  `part`: some of it is past the wave's steps or past K.
-  auto batch = [&](auto u, auto part) {
-    constexpr int U = u.value;
-    i32x4_t xv[U], av[U][N];
-    const int end = min(32 * s1, g.k);
-#pragma unroll
-    for (int t = 0; t < U; ++t) {
-      const int at = 32 * (s + t) + off, from = part.value ? min(at, g.k - 8) : at;  // clamped: in the row
-      xv[t] = *(const i32x4_t*)(x + from);
-#pragma unroll
-      for (int i = 0; i < N; ++i) av[t][i] = *(const i32x4_t*)(ap[i] + from);
-      if (part.value && at >= end) {
-        xv[t] = i32x4_t{0, 0, 0, 0};
-#pragma unroll
-        for (int i = 0; i < N; ++i) av[t][i] = i32x4_t{0, 0, 0, 0};
+    for (int i = 0; i < L; ++i) {
+      const int r = (i & 1) * 8 + (lane >> 3), piece = 8 * swizzle8(r, lane & 7);
+      if (i < 2) {
+        const int row = __builtin_amdgcn_ds_bpermute(4 * r, (int)gr.row);
+        from[i] = (const XT*)g.x + (int64_t)row * g.ldx + piece;
+      } else {  // hidden rows read the first one: in cache
+        const int ar = row0 + 16 * ((i - 2) >> 1) + r;
+        from[i] = a + (int64_t)(ar < rows && ar % g.rank < live ? ar : 0) * g.k + piece;
       }
     }
+    const int c1 = (s1 + 1) >> 1, tail = g.k - 8;
+    auto issue = [&](int c) {
+      uint8_t* stage = lds + c % S * (L * 1024);
 #pragma unroll
-    for (int t = 0; t < U; ++t)
+      for (int i = 0; i < L; ++i) {
+        const int r = (i & 1) * 8 + (lane >> 3), p = 8 * swizzle8(r, lane & 7);
+        const int past = max(64 * c + p - tail, 0);  // a piece past K: the row's last one, zeroed when it is read
+        load_to_lds16(from[i] + 64 * c - past, stage + i * 1024);
+      }
+    };
+    int c = s0 >> 1, ahead = c;
+    for (; ahead < min(c + S, c1); ++ahead) issue(ahead);
+    for (; c < c1; ++c) {
+      wait_stages<L, S - 1>(ahead - c - 1);
+      const uint8_t* stage = lds + c % S * (L * 1024);
+      i32x4_t xv[2], av[2][N];
 #pragma unroll
-      for (int i = 0; i < N; ++i)
-        acc[i] = mfma16<XT>::mma(__builtin_bit_cast(vec8<XT>, av[t][i]), __builtin_bit_cast(vec8<XT>, xv[t]), acc[i]);
-    s += U;
-  };
-  if constexpr (VEC) {
-    using std::integral_constant;
-    const int full = min(s1, g.k >> 5);
-    if constexpr (N <= 2)
-      while (s + 8 <= full) batch(integral_constant<int, 8>{}, std::false_type{});
-    while (s + 4 <= full) batch(integral_constant<int, 4>{}, std::false_type{});
-    if (s < s1) batch(integral_constant<int, 4>{}, std::true_type{});
+      for (int h = 0; h < 2; ++h) {
+        const int at = j * 128 + swizzle8(j, 4 * h + q) * 16;
+        xv[h] = *(const i32x4_t*)(stage + at);
+#pragma unroll
+        for (int i = 0; i < N; ++i) av[h][i] = *(const i32x4_t*)(stage + 2048 * (i + 1) + at);
+        if (64 * c + 32 * h + 8 * q > tail) {
+          xv[h] = i32x4_t{0, 0, 0, 0};
+#pragma unroll
+          for (int i = 0; i < N; ++i) av[h][i] = i32x4_t{0, 0, 0, 0};
+        }
+      }
+      wait_lgkmcnt0();  // the stage is read before it is loaded again
+      if (ahead < c1) issue(ahead++);
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+          acc[i] = mfma16<XT>::mma(__builtin_bit_cast(vec8<XT>, av[h][i]), __builtin_bit_cast(vec8<XT>, xv[h]), acc[i]);
+    }
   } else {
-    for (; s < s1; ++s) {
-      const vec8<XT> xv = __builtin_bit_cast(vec8<XT>, load8<false>(x, 32 * s + off, g.k));
+    const XT* x = (const XT*)g.x + gr.row * g.ldx;
+    const XT* ap[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int r = row0 + 16 * i + j;
+      ap[i] = a + (int64_t)(r < rows && r % g.rank < live ? r : 0) * g.k;
+    }
+    for (int s = s0; s < s1; ++s) {
+      const vec8<XT> xv = __builtin_bit_cast(vec8<XT>, load8<false>(x, 32 * s + 8 * q, g.k));
 #pragma unroll
       for (int i = 0; i < N; ++i)
-        acc[i] = mfma16<XT>::mma(__builtin_bit_cast(vec8<XT>, load8<false>(ap[i], 32 * s + off, g.k)), xv, acc[i]);
+        acc[i] = mfma16<XT>::mma(__builtin_bit_cast(vec8<XT>, load8<false>(ap[i], 32 * s + 8 * q, g.k)), xv, acc[i]);
     }
   }
 }
@@ -148,12 +175,12 @@ constexpr int kDownWaves = 4;
 // Grid: (blocks of A's tiles x splits of K, groups or tiles x 4).
 template <typename XT, int N, bool VEC, bool PLAN>
 __global__ __launch_bounds__(64 * kDownWaves) void lora_down_kernel(LoraArgs g) {
-  __shared__ f32x4_t red[kDownWaves][N][64];
+  __shared__ __align__(1024) uint8_t stages[kDownWaves][VEC ? kDownBytes<N> : 1024 * N];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int split = blockIdx.x % g.splits, row0 = blockIdx.x / g.splits * 16 * N;
-  const int64_t groups = PLAN ? 4 * plan_tiles(g) : g.m;
-  const int steps = (g.k + 31) >> 5, per = (steps + g.splits * kDownWaves - 1) / (g.splits * kDownWaves);
-  const int s0 = min((split * kDownWaves + wave) * per, steps), s1 = min(s0 + per, steps);
+  const int64_t groups = PLAN ? 4 * plan_max_tiles(g.m, g.slots) : g.m;
+  const int steps = (g.k + 31) >> 5, parts = g.splits * kDownWaves, per = ((steps + parts - 1) / parts + 1) & ~1;
+  const int s0 = min((split * kDownWaves + wave) * per, steps + 1 & ~1), s1 = min(s0 + per, steps);
   for (int64_t at = blockIdx.y; at < groups; at += gridDim.y) {
     const Group gr = PLAN ? group_by_plan(g, at >> 2, (int)(at & 3)) : group_by_ballot(g, at);
     if (gr.slot < 0 || !gr.count) continue;
@@ -162,18 +189,18 @@ __global__ __launch_bounds__(64 * kDownWaves) void lora_down_kernel(LoraArgs g) 
     f32x4_t acc[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) acc[i] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-    down_steps<XT, N, VEC>(g, (const XT*)g.x + gr.row * g.ldx, (const XT*)g.a + (int64_t)gr.slot * g.rows_a * g.k, row0,
-                           g.rows_a, live, s0, s1, acc);
-    __syncthreads();  // the previous group's readers are done
+    down_steps<XT, N, VEC>(g, gr, (const XT*)g.a + (int64_t)gr.slot * g.rows_a * g.k, row0, g.rows_a, live, s0, s1,
+                           stages[wave], acc);
 #pragma unroll
-    for (int i = 0; i < N; ++i) red[wave][i][lane] = acc[i];
+    for (int i = 0; i < N; ++i) ((f32x4_t*)stages[wave])[64 * i + lane] = acc[i];
     __syncthreads();
     if (wave < N && (lane & 15) < gr.count && row0 + 16 * wave < g.t_stride) {
-      f32x4_t v = red[0][wave][lane];
+      f32x4_t v = ((f32x4_t*)stages[0])[64 * wave + lane];
 #pragma unroll
-      for (int w = 1; w < kDownWaves; ++w) v += red[w][wave][lane];
+      for (int w = 1; w < kDownWaves; ++w) v += ((f32x4_t*)stages[w])[64 * wave + lane];
       *(f32x4_t*)(g.t + ((int64_t)split * g.m + gr.row) * g.t_stride + row0 + 16 * wave + 4 * (lane >> 4)) = v;
     }
+    __syncthreads();  // read before the next group's stages
   }
 }
 
@@ -243,8 +270,7 @@ template <typename XT, int NB, bool PACK> struct TOperand {
   }
 };
 
-// NT tiles of 16 columns a wave: MFMA row i of tile n is column c0 + 4 NT (i / 4) + 4 n + i % 4, so that lane l ends with
-// the 4 NT neighbouring columns from c0 + 4 NT (l / 16) of the group's row l % 16.
+// NT tiles of 16 columns a wave: lane l ends with columns c0 + 16 n + 4 (l / 16) ... + 3 of the group's row l % 16.
 template <typename XT, int NB, int NT, bool PACK, bool VEC> struct UpTile {
   vec8<XT> b[NT][NB];
 
@@ -252,7 +278,7 @@ template <typename XT, int NB, int NT, bool PACK, bool VEC> struct UpTile {
     const int i = threadIdx.x & 15;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      const int c = min(c0 + 4 * NT * (i >> 2) + 4 * n + (i & 3), end - 1);
+      const int c = min(c0 + 16 * n + i, end - 1);
       const XT* row = (const XT*)g.b + ((int64_t)slot * g.n + c) * g.rank;
 #pragma unroll
       for (int k = 0; k < NB; ++k) b[n][k] = __builtin_bit_cast(vec8<XT>, load8<VEC>(row, rl.first[k], g.rank));
@@ -279,53 +305,73 @@ template <typename XT, int NB, int NT, bool PACK, bool VEC> struct UpTile {
   }
 };
 
-// A lane's 4 NT neighbouring columns of one row: loaded as raw bits, so that the load is in flight early.
-template <typename XT, int NT, bool VEC> struct RowPiece {
-  i32x4_t raw[NT / 2];
+// A group's rows of base and out, 16 NT columns of a wave: 2 NT lanes a row, eight neighbouring columns a lane, NT / 2 pieces
+// a lane.  base is loaded as raw bits, in flight early.
+template <typename XT, int NT, bool VEC> struct Rows {
+  static constexpr int kLanes = 2 * NT, kPieces = NT / 2, kPitch = 16 * NT + 4;  // floats a row in LDS
+  static constexpr int kFloats = 16 * kPitch;
+  int64_t row[kPieces];
+  bool live[kPieces];
+  int c, end;
+  i32x4_t raw[kPieces];
 
-  __device__ __forceinline__ void load(const XT* row, int c, int end) {
+  // Every lane of the wave: the group's rows are read from its lanes.
+  __device__ __forceinline__ void load(const LoraArgs& g, const Group& gr, int c0, int part_end) {
+    const int lane = threadIdx.x & 63;
+    c = c0 + 8 * (lane % kLanes), end = part_end;
 #pragma unroll
-    for (int h = 0; h < NT / 2; ++h) raw[h] = load8<VEC>(row, c + 8 * h, end);
-  }
-
-  __device__ __forceinline__ float value(int e) const {
-    const uint32_t w = (uint32_t)raw[e >> 3][(e & 7) >> 1];
-    return to_f32(XT{(uint16_t)(e & 1 ? w >> 16 : w)});
-  }
-
-  __device__ __forceinline__ static void put(XT* row, int c, int end, i32x4_t v) {
-    if constexpr (VEC) {
-      if (c < end) *(i32x4_t*)(row + c) = v;
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (c + i < end) row[c + i] = XT{(uint16_t)((uint32_t)v[i >> 1] >> (16 * (i & 1)))};
+    for (int h = 0; h < kPieces; ++h) {
+      const int r = lane / kLanes + h * (64 / kLanes);
+      row[h] = __builtin_amdgcn_ds_bpermute(4 * r, (int)gr.row);
+      live[h] = r < gr.count && c < end;
+      if (live[h]) raw[h] = load8<VEC>((const XT*)g.base + row[h] * g.ldb, c, end);
     }
   }
 
-  __device__ __forceinline__ void copy_to(XT* row, int c, int end) const {
+  __device__ __forceinline__ void store(const LoraArgs& g, int h, i32x4_t v) const {
+    XT* out = (XT*)g.out + row[h] * g.ldo + c;
+    if constexpr (VEC) {
+      *(i32x4_t*)out = v;
+    } else {
 #pragma unroll
-    for (int h = 0; h < NT / 2; ++h) put(row, c + 8 * h, end, raw[h]);
+      for (int i = 0; i < 8; ++i)
+        if (c + i < end) out[i] = XT{(uint16_t)((uint32_t)v[i >> 1] >> (16 * (i & 1)))};
+    }
   }
 
-  // row = this + acc 2^exp, rounded once.
-  __device__ __forceinline__ void add_to(XT* row, int c, int end, const f32x4_t (&acc)[NT], int exp) const {
+  __device__ __forceinline__ void copy(const LoraArgs& g) const {
 #pragma unroll
-    for (int h = 0; h < NT / 2; ++h) {
+    for (int h = 0; h < kPieces; ++h)
+      if (live[h]) store(g, h, raw[h]);
+  }
+
+  // out = base + acc 2^exp, rounded once.  lds: kFloats of this wave alone.
+  __device__ __forceinline__ void add(const LoraArgs& g, const f32x4_t (&acc)[NT], int exp, float* lds) const {
+    const int lane = threadIdx.x & 63;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      f32x4_t v = acc[n];
+      if constexpr (std::is_same<XT, f16_t>::value)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = __builtin_amdgcn_ldexpf(v[i], exp);
+      *(f32x4_t*)(lds + (lane & 15) * kPitch + 16 * n + 4 * (lane >> 4)) = v;
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int h = 0; h < kPieces; ++h) {
+      const float* from = lds + (lane / kLanes + h * (64 / kLanes)) * kPitch + 8 * (lane % kLanes);
+      const f32x4_t d0 = *(const f32x4_t*)from, d1 = *(const f32x4_t*)(from + 4);
+      if (!live[h]) continue;
       i32x4_t v;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        float d[2];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int at = 8 * h + 2 * i + e;
-          float x = acc[at >> 2][at & 3];
-          if constexpr (std::is_same<XT, f16_t>::value) x = __builtin_amdgcn_ldexpf(x, exp);
-          d[e] = value(at) + x;
-        }
-        v[i] = (int)pack2_f32<XT>(d[0], d[1]);
+        const uint32_t w = (uint32_t)raw[h][i];
+        const float lo = i < 2 ? d0[2 * i] : d1[2 * i - 4], hi = i < 2 ? d0[2 * i + 1] : d1[2 * i - 3];
+        v[i] = (int)pack2_f32<XT>(to_f32(XT{(uint16_t)w}) + lo, to_f32(XT{(uint16_t)(w >> 16)}) + hi);
       }
-      put(row, c + 8 * h, end, v);
+      store(g, h, v);
     }
   }
 };
@@ -339,33 +385,34 @@ __device__ __forceinline__ Block block_of(const LoraArgs& g, int chunk, int cols
   return {p, first + (chunk - before) * cols, g.parts.end[p]};
 }
 
-constexpr int kUpWaves = 4, kUpTiles = kLoraUpCols / (16 * kUpWaves);
+constexpr int kUpWaves = 4, kUpTiles = kLoraUpCols / (16 * kUpWaves), kUpGroups = 2;
 
-// Grid: (column blocks, groups or tiles).  A tile of the plan is up to four groups of one slot, which share the B operands.
+// Grid: (column blocks, groups, or halves of the plan's tiles: two groups of one slot, which share the B operands).
 template <typename XT, int NB, bool PACK, bool VEC, bool PLAN>
 __global__ __launch_bounds__(64 * kUpWaves) void lora_up_kernel(LoraArgs g) {
-  constexpr int G = PLAN ? kPlanTile / 16 : 1, NT = kUpTiles;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  constexpr int G = PLAN ? kUpGroups : 1, NT = kUpTiles, PER = kPlanTile / 16 / G;
+  typedef Rows<XT, NT, VEC> R;
+  __shared__ __align__(16) float lds[kUpWaves][R::kFloats];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const Block blk = block_of(g, blockIdx.x, kLoraUpCols);
-  const int c0 = blk.c0 + 16 * NT * wave, c = c0 + 4 * NT * (lane >> 4), tok = lane & 15;
+  const int c0 = blk.c0 + 16 * NT * wave, tok = lane & 15;
   if (c0 >= blk.end) return;
   const RankLane<NB, PACK> rl(lane);
-  const int64_t groups = PLAN ? plan_tiles(g) : g.m;
+  const int64_t groups = PLAN ? PER * plan_max_tiles(g.m, g.slots) : g.m;
   for (int64_t at = blockIdx.y; at < groups; at += gridDim.y) {
     Group gr[G];
 #pragma unroll
-    for (int i = 0; i < G; ++i) gr[i] = PLAN ? group_by_plan(g, at, i) : group_by_ballot(g, at);
-    const int slot = gr[0].slot;
-    const int live = slot < 0 ? 0 : live_rank(g, slot);
-    if (!live && g.base == g.out) continue;
-    RowPiece<XT, NT, VEC> base[G];
-#pragma unroll
     for (int i = 0; i < G; ++i)
-      if (tok < gr[i].count) base[i].load((const XT*)g.base + gr[i].row * g.ldb, c, blk.end);
+      gr[i] = PLAN ? group_by_plan(g, at / PER, (int)(at % PER) * G + i) : group_by_ballot(g, at);
+    if (!gr[0].count) continue;
+    const int slot = gr[0].slot, live = slot < 0 ? 0 : live_rank(g, slot);
+    if (!live && g.base == g.out) continue;
+    R rows[G];
+#pragma unroll
+    for (int i = 0; i < G; ++i) rows[i].load(g, gr[i], c0, blk.end);
     if (!live) {
 #pragma unroll
-      for (int i = 0; i < G; ++i)
-        if (tok < gr[i].count) base[i].copy_to((XT*)g.out + gr[i].row * g.ldo, c, blk.end);
+      for (int i = 0; i < G; ++i) rows[i].copy(g);
       continue;
     }
     UpTile<XT, NB, NT, PACK, VEC> up;
@@ -384,7 +431,7 @@ __global__ __launch_bounds__(64 * kUpWaves) void lora_up_kernel(LoraArgs g) {
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
           if constexpr (VEC) {
-            if (rl.first[b] < live) {
+            if (rl.first[b] < live && tok < gr[i].count) {
               const f32x4_t v0 = *(const f32x4_t*)(t + rl.first[b]), v1 = *(const f32x4_t*)(t + rl.first[b] + 4);
 #pragma unroll
               for (int e = 0; e < 4; ++e) v[b][e] += v0[e], v[b][4 + e] += v1[e];
@@ -404,7 +451,7 @@ __global__ __launch_bounds__(64 * kUpWaves) void lora_up_kernel(LoraArgs g) {
       to.set(v, rl.low);
       f32x4_t acc[NT];
       up.mul(to, acc);
-      if (tok < gr[i].count) base[i].add_to((XT*)g.out + gr[i].row * g.ldo, c, blk.end, acc, to.exp);
+      rows[i].add(g, acc, to.exp, lds[wave]);
     }
   }
 }
@@ -414,50 +461,50 @@ __global__ __launch_bounds__(64 * kUpWaves) void lora_up_kernel(LoraArgs g) {
 constexpr int kOneWaves = 8, kOneTiles = kLoraFusedCols / (16 * kOneWaves);
 
 // Grid: (column blocks, rows).  The workgroup's waves share K of the first product, for its partition's rows of A alone, and
-// meet in LDS; then each multiplies its own columns.  B's and base's loads are in flight before the first product.
+// meet in LDS; then each multiplies its own columns.
 template <typename XT, int NB, bool PACK, bool VEC>
 __global__ __launch_bounds__(64 * kOneWaves) void lora_one_kernel(LoraArgs g) {
   constexpr int NT = kOneTiles, N = 2 * NB - (PACK ? 1 : 0);  // 16-row tiles of A
-  __shared__ f32x4_t red[kOneWaves][N][64];
+  typedef Rows<XT, NT, VEC> R;
+  constexpr int kBytes = std::max({VEC ? kDownBytes<N> : 0, 1024 * N, 4 * R::kFloats});
+  __shared__ __align__(1024) uint8_t stages[kOneWaves][(kBytes + 1023) & ~1023];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const Block blk = block_of(g, blockIdx.x, kLoraFusedCols);
-  const int c0 = blk.c0 + 16 * NT * wave, c = c0 + 4 * NT * (lane >> 4), tok = lane & 15;
+  const int c0 = blk.c0 + 16 * NT * wave, tok = lane & 15;
   const RankLane<NB, PACK> rl(lane);
-  const int steps = (g.k + 31) >> 5, per = (steps + kOneWaves - 1) / kOneWaves;
-  const int s0 = min(wave * per, steps), s1 = min(s0 + per, steps);
+  const int steps = (g.k + 31) >> 5, per = ((steps + kOneWaves - 1) / kOneWaves + 1) & ~1;
+  const int s0 = min(wave * per, steps + 1 & ~1), s1 = min(s0 + per, steps);
   for (int64_t at = blockIdx.y; at < g.m; at += gridDim.y) {
     const Group gr = group_by_ballot(g, at);
     if (!gr.count) continue;
     const int live = gr.slot < 0 ? 0 : live_rank(g, gr.slot);
     if (!live && g.base == g.out) continue;
-    const bool mine = tok < gr.count;
-    RowPiece<XT, NT, VEC> base;
-    if (mine) base.load((const XT*)g.base + gr.row * g.ldb, c, blk.end);
+    R rows;
+    rows.load(g, gr, c0, blk.end);
     if (!live) {
-      if (mine) base.copy_to((XT*)g.out + gr.row * g.ldo, c, blk.end);
+      rows.copy(g);
       continue;
     }
     UpTile<XT, NB, NT, PACK, VEC> up;
     up.load(g, gr.slot, c0, blk.end, live, rl);
     const float scaling = g.scaling[gr.slot];
+    __builtin_amdgcn_sched_barrier(0);  // in flight before the ring
     f32x4_t acc1[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) acc1[i] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-    down_steps<XT, N, VEC>(g, (const XT*)g.x + gr.row * g.ldx,
-                           (const XT*)g.a + ((int64_t)gr.slot * g.rows_a + blk.part * g.rank) * g.k, 0, g.rank, live, s0, s1,
-                           acc1);
-    __syncthreads();  // the previous group's readers are done
+    down_steps<XT, N, VEC>(g, gr, (const XT*)g.a + ((int64_t)gr.slot * g.rows_a + blk.part * g.rank) * g.k, 0, g.rank, live,
+                           s0, s1, stages[wave], acc1);
 #pragma unroll
-    for (int i = 0; i < N; ++i) red[wave][i][lane] = acc1[i];
+    for (int i = 0; i < N; ++i) ((f32x4_t*)stages[wave])[64 * i + lane] = acc1[i];
     __syncthreads();
     // entries first[b] ... + 7 are rows 16 tile + 4 q' ... of two neighbouring lane groups q' of one tile
     float v[NB][8];
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
-      const int tile = rl.first[b] >> 4, from = ((rl.first[b] & 15) >> 2) * 16 + tok;
-      f32x4_t lo = red[0][tile][from], hi = red[0][tile][from + 16];
+      const int from = 64 * (rl.first[b] >> 4) + ((rl.first[b] & 15) >> 2) * 16 + tok;
+      f32x4_t lo = ((f32x4_t*)stages[0])[from], hi = ((f32x4_t*)stages[0])[from + 16];
 #pragma unroll
-      for (int w = 1; w < kOneWaves; ++w) lo += red[w][tile][from], hi += red[w][tile][from + 16];
+      for (int w = 1; w < kOneWaves; ++w) lo += ((f32x4_t*)stages[w])[from], hi += ((f32x4_t*)stages[w])[from + 16];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         v[b][e] = rl.first[b] + e < live ? lo[e] * scaling : 0.0f;
@@ -468,7 +515,8 @@ __global__ __launch_bounds__(64 * kOneWaves) void lora_one_kernel(LoraArgs g) {
     to.set(v, rl.low);
     f32x4_t acc[NT];
     up.mul(to, acc);
-    if (mine) base.add_to((XT*)g.out + gr.row * g.ldo, c, blk.end, acc, to.exp);
+    __syncthreads();  // t is read before its place takes the result, and before the next group's stages
+    rows.add(g, acc, to.exp, (float*)stages[wave]);
   }
 }
 
@@ -601,9 +649,11 @@ template <typename XT> void launch_lora(LoraArgs& g, hipStream_t st) {
   const int chunks = cut_columns(g.parts, kLoraFusedCols);
   if (lora_one_launch(g.plan, g.m, g.k, g.rank, g.slots, chunks)) {
     by_rank(g.rank, [&](auto nb, auto pack) {
-      by_bool(vec_k && vec_n, [&](auto v) {
-        qtts::launch(&lora_one_kernel<XT, nb.value, pack.value, v.value>, dim3(chunks, grid_y(g.m)), dim3(64 * kOneWaves), 0, st, g);
-      });
+      if constexpr (32 * nb.value <= kLoraOneRank)
+        by_bool(vec_k && vec_n, [&](auto v) {
+          qtts::launch(&lora_one_kernel<XT, nb.value, pack.value, v.value>, dim3(chunks, grid_y(g.m)), dim3(64 * kOneWaves), 0,
+                       st, g);
+        });
     });
     return;
   }
@@ -620,7 +670,7 @@ template <typename XT> void launch_lora(LoraArgs& g, hipStream_t st) {
     const int up_chunks = cut_columns(g.parts, kLoraUpCols);
     by_rank(g.rank, [&](auto nb, auto pack) {
       by_bool(vec_n, [&](auto v) {
-        qtts::launch(&lora_up_kernel<XT, nb.value, pack.value, v.value, plan.value>, dim3(up_chunks, grid_y(tiles)),
+        qtts::launch(&lora_up_kernel<XT, nb.value, pack.value, v.value, plan.value>, dim3(up_chunks, grid_y(plan.value ? kPlanTile / 16 / kUpGroups * tiles : tiles)),
                      dim3(64 * kUpWaves), 0, st, g);
       });
     });
