@@ -79,7 +79,7 @@ typedef enum {
     QTTS_OP_FP8W = 5,
     QTTS_OP_W8A16_SILU = 6,
     QTTS_OP_W8A16_FUSED = 7,
-    QTTS_OP_LORA = 8 /* n: rows of one adapter's A (partitions * rank) */
+    QTTS_OP_LORA = 8 /* n: the linear's partitions, k: the rank */
 } qtts_op;
 
 /* What qtts_w8a16_fused_gemm_strips applies to its activations before the GEMM. */
@@ -462,7 +462,7 @@ int qtts_silu_mul_quant(const void* gate_up, int x_dtype, int64_t m, int64_t k, 
  * needs one to read the rows of an adapter together): one kernel, made anew whenever the
  * index changes (in the same graph where calls are captured), used by every linear of a
  * step.  index: [m] int32 on the device.  plan: qtts_lora_plan_bytes(m, slots) bytes, 16-byte
- * aligned; 0 bytes: more slots than a plan takes (768), calls then go without. */
+ * aligned; 0 bytes: more than a plan takes (768 slots, 2^30 rows), calls then go without. */
 int64_t qtts_lora_plan_bytes(int64_t m, int64_t slots);
 int qtts_lora_plan(const int32_t* index, int64_t m, int64_t slots, int32_t* plan, int64_t plan_bytes, void* stream);
 
@@ -472,7 +472,7 @@ int qtts_lora_plan(const int32_t* index, int64_t m, int64_t slots, int32_t* plan
  * for the output partition p of column j (part_ends: [parts] ascending column ends on the
  * host, the last n; a merged qkv or gate_up has an A block per partition).  Rows whose index
  * is outside [0, slots) have out = base.  Sums in fp32 (t is carried to the second product as
- * two 16-bit halves, 16 bits or more of it).  No counterpart in the reference.
+ * two 16-bit halves, 16 bits of it).  No counterpart in the reference.
  * x: [m, k] of x_dtype (bf16 or fp16), row stride ldx.  index: [m] int32, on the device.
  * a: [slots, parts * rank, k], b: [slots, n, rank], contiguous, of x_dtype.  ranks: [slots]
  * int32 or NULL (all `rank`); entries of a and b past a slot's rank are not used.  scaling:
@@ -480,7 +480,7 @@ int qtts_lora_plan(const int32_t* index, int64_t m, int64_t slots, int32_t* plan
  * and shares no byte with x.  rank <= QTTS_LORA_MAX_RANK, parts <= QTTS_LORA_MAX_PARTS.
  * plan: what qtts_lora_plan made of the same index, m and slots, or NULL (rows of one adapter
  * are then read together within each 64 rows); a plan of another m or slots writes nothing.  Workspace: qtts_workspace_bytes(QTTS_OP_LORA,
- * m, parts * rank, k, 0). */
+ * m, parts, rank, 0). */
 int qtts_lora_add(const void* x, int x_dtype, int64_t m, int64_t k, int64_t ldx, const int32_t* index,
                   const int32_t* plan, int64_t slots, const void* a, const void* b, int64_t rank, const int32_t* ranks,
                   const float* scaling, const int64_t* part_ends, int64_t parts, const void* base, int64_t ldb,

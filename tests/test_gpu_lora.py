@@ -92,6 +92,15 @@ def test_lora(ops, m, k, parts, slots, rank, dtype):
         _check(_run(ops, c), c, f"{m}x{k} parts {parts} slots {slots} rank {rank} {dtype}")
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("rank", [8, 16, 24, 40, 64, 72, 100])
+@pytest.mark.parametrize("m,parts,slots", [(2061, [4096, 4104], 3), (1100, [8000], 30), (66, [520, 24], 40)])
+def test_wide_outputs(ops, m, parts, slots, rank, dtype):
+    """The second product's 256, 128 and 64 columns a workgroup, with whole and broken tiles of rows."""
+    c = _case(m, 64, parts, slots, rank, dtype, seed=m + rank)
+    _check(_run(ops, c), c, f"{m} rows parts {parts} rank {rank} {dtype}")
+
+
 @pytest.mark.parametrize("m", [1, 5, 40, 100])
 @pytest.mark.parametrize("k,parts,rank", [(33, [17], 3), (65, [40, 1, 23], 4), (100, [13, 64], 12), (8, [8], 1),
                                           (2047, [31], 16), (64, [100], 17), (24, [7], 127), (16, [0, 24, 0], 8)])
@@ -221,16 +230,19 @@ def test_plan(ops, m, slots):
     index = torch.randint(-2, slots + 1, (m,), generator=g, dtype=torch.int32)
     plan = ops.lora_batch(index.cuda(), slots).plan.cpu()
     slot = torch.where((index < 0) | (index >= slots), slots, index)
-    order = plan[-m:].long()
-    assert torch.equal(order, torch.argsort(slot, stable=True))
-    tiles, at = plan[4:4 + 4 * int(plan[0])].view(-1, 4), 0
+    want = torch.argsort(slot, stable=True)
+    count = int(plan[0])
+    most = (m + 63) // 64 + min(m, slots + 1)
+    tiles = plan[4:4 + 2 * count].view(-1, 2)
+    order = plan[4 + (2 * most + 3) // 4 * 4:][:64 * count].view(-1, 64)
     assert plan[1] == m and plan[2] == slots
-    for s, start, count, _ in tiles.tolist():
-        assert start == at and 0 < count <= 64
-        want = slots if s < 0 else s
-        assert (slot[order[start:start + count]] == want).all()
-        at += count
-        assert count == 64 or at == m or slot[order[at]] != want
+    at = 0
+    for (s, n), rows in zip(tiles.tolist(), order):
+        assert 0 < n <= 64 and torch.equal(rows[:n].long(), want[at:at + n])
+        here = slots if s < 0 else s
+        assert (slot[want[at:at + n]] == here).all()
+        at += n
+        assert n == 64 or at == m or slot[want[at]] != here
     assert at == m
 
 

@@ -81,8 +81,9 @@ def test_silu_quant_entry():
 def test_lora_entry():
     L = _lib.load()
     b = _buf(1 << 20)
-    need = L.qtts_workspace_bytes(_lib.OP_LORA, 4, 16, 64, 0)
+    need = L.qtts_workspace_bytes(_lib.OP_LORA, 4, 1, 16, 0)
     assert need >= 4 * 16 * 4
+    assert L.qtts_workspace_bytes(_lib.OP_LORA, 4, 9, 16, 0) == -1 and L.qtts_workspace_bytes(_lib.OP_LORA, 4, 1, 129, 0) == -1
 
     def call(x=0, dt=1, m=4, k=64, ldx=64, index=4096, slots=3, a=8192, bb=65536, rank=16, ranks=131072, scaling=131200,
              ends=(96,), base=140000, ldb=96, out=160000, n=96, ldo=96, ws=262144, ws_n=None, parts=None):
@@ -115,7 +116,7 @@ def test_lora_entry():
         assert call(**ws) == -5 and "workspace" in _lib.last_error()
     assert call(m=0) == 0 and call(n=0, ends=(0,)) == 0
     if not torch.cuda.is_available():
-        assert call() == -2 and call(out=140000) == -2 and call(ranks=None) == -2 and call(ends=(0, 32, 32, 96), rank=4) == -2
+        assert call() == -2 and call(out=140000) == -2 and call(ranks=None) == -2 and call(ends=(0, 32, 32, 96), rank=4, ws_n=1 << 17) == -2
 
 
 def test_lora_plan_entry():
@@ -166,10 +167,11 @@ def test_wrappers_check_shapes_and_types():
 
     for match, kw in (("rows", {"base": base[:1]}), ("rows", {"batch": ops.LoraBatch(index[:1], 3)}),
                       ("one dtype", {"x": x.half()}), ("one dtype", {"a": a.float()}),
-                      ("contiguous", {"a": a.transpose(1, 2)}), ("contiguous", {"b": b[0]}), ("do not fit", {"parts": (96,)}),
+                      ("contiguous", {"a": a.transpose(1, 2)}), ("do not fit", {"b": b[0]}), ("do not fit", {"parts": (96,)}),
                       ("do not fit", {"parts": (64, 31)}), ("do not fit", {"a": a[:, :16].contiguous()}),
                       ("do not fit", {"b": b[:2]}),
-                      ("partition of", {"parts": (100, -4)}), ("scaling", {"s": s.to(bf)}), ("scaling", {"s": s[:2]}),
+                      ("partition of", {"parts": (100, -4)}),
+                      ("at most", {"a": torch.zeros(3, 258, 64, dtype=bf), "b": torch.zeros(3, 96, 129, dtype=bf)}), ("scaling", {"s": s.to(bf)}), ("scaling", {"s": s[:2]}),
                       ("ranks", {"ranks": torch.zeros(3)}), ("ranks", {"ranks": torch.zeros(2, dtype=i32)}),
                       ("GPU tensor", {})):
         with pytest.raises(ValueError, match=match):

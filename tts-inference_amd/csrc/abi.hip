@@ -75,7 +75,7 @@ int qtts_launch_rms_norm_quant(const void* x, int x_dtype, int64_t m, int64_t k,
                                void* normed, int64_t ldn, hipStream_t st);
 int qtts_launch_silu_mul_quant(const void* gu, int x_dtype, int64_t m, int64_t k, int64_t ld, int codes, void* q, float* sx,
                                void* act, int64_t lda, hipStream_t st);
-int64_t qtts_lora_ws_bytes(int64_t m, int64_t rows_a, int64_t k);
+int64_t qtts_lora_ws_bytes(int64_t m, int64_t parts, int64_t rank);
 int qtts_launch_lora_plan(const int32_t* index, int64_t m, int64_t slots, int32_t* plan, hipStream_t st);
 int qtts_launch_lora_add(const qtts::LoraArgs& args, int x_dtype, void* ws, hipStream_t st);
 
@@ -260,8 +260,9 @@ int64_t qtts_workspace_bytes(int op, int64_t m, int64_t n, int64_t k, int algo) 
     case QTTS_OP_FP8W: return qtts_fp8w_ws_bytes(m, n, k, algo);
     case QTTS_OP_W8A16_SILU: return qtts_w8a16_silu_ws_bytes(m, n, k, algo, QTTS_BF16);
     case QTTS_OP_W8A16_FUSED: return qtts_w8a16_fused_ws_bytes(m, n, k, algo, QTTS_BF16);
-    case QTTS_OP_LORA:
-      if (m > (1ll << 54) / n) return qtts_set_error(QTTS_ERR_INVALID_ARGUMENT, "bad workspace query");
+    case QTTS_OP_LORA:  // n partitions of rank k
+      if (n > QTTS_LORA_MAX_PARTS || k > QTTS_LORA_MAX_RANK)
+        return qtts_set_error(QTTS_ERR_INVALID_ARGUMENT, "bad workspace query");
       return qtts_lora_ws_bytes(m, n, k);
     default: return qtts_set_error(QTTS_ERR_INVALID_ARGUMENT, "unknown op %d", op);
   }
@@ -715,13 +716,14 @@ int qtts_silu_mul_quant(const void* gate_up, int x_dtype, int64_t m, int64_t k, 
 int64_t qtts_lora_plan_bytes(int64_t m, int64_t slots) {
   if (m < 0 || slots < 0 || m >= (1ll << 31) || slots >= (1ll << 30))
     return qtts_set_error(QTTS_ERR_INVALID_ARGUMENT, "lora_plan: bad sizes");
-  return slots > qtts::kPlanMaxSlots ? 0 : qtts::plan_words(m, slots) * 4;
+  return slots > qtts::kPlanMaxSlots || m > qtts::kPlanMaxRows ? 0 : qtts::plan_words(m, slots) * 4;
 }
 
 int qtts_lora_plan(const int32_t* index, int64_t m, int64_t slots, int32_t* plan, int64_t plan_bytes, void* stream) {
   const int64_t need = qtts_lora_plan_bytes(m, slots);
   if (need < 0) return (int)need;
-  QTTS_REQUIRE(slots <= qtts::kPlanMaxSlots, "lora_plan: %lld slots, more than %d", (long long)slots, qtts::kPlanMaxSlots);
+  QTTS_REQUIRE(slots <= qtts::kPlanMaxSlots && m <= qtts::kPlanMaxRows, "lora_plan: more than %d slots or %lld rows",
+               qtts::kPlanMaxSlots, (long long)qtts::kPlanMaxRows);
   QTTS_REQUIRE(plan && (uintptr_t)plan % 16 == 0 && (m == 0 || index), "lora_plan: null or unaligned pointer");
   QTTS_REQUIRE(plan_bytes >= need, "lora_plan: plan of %lld bytes < %lld needed", (long long)plan_bytes, (long long)need);
   QTTS_TRY(current_device_check());
@@ -751,7 +753,7 @@ int qtts_lora_add(const void* x, int x_dtype, int64_t m, int64_t k, int64_t ldx,
   QTTS_REQUIRE((out == base && ldo == ldb) || !spans_overlap(base, m, ldb, n, 2, out, m, ldo, n, 2),
                "lora_add: out overlaps base");
   QTTS_REQUIRE(!spans_overlap(x, m, ldx, k, 2, out, m, ldo, n, 2), "lora_add: out overlaps x");
-  const int64_t need = qtts_lora_ws_bytes(m, parts * rank, k);
+  const int64_t need = qtts_lora_ws_bytes(m, parts, rank);
   if (!ws || ws_bytes < need)
     return qtts_set_error(QTTS_ERR_WORKSPACE, "lora_add: workspace of %lld bytes < %lld needed", (long long)ws_bytes,
                           (long long)need);

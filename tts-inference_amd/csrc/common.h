@@ -369,7 +369,10 @@ inline void launch(void (*kernel)(Params...), dim3 grid, dim3 block, uint32_t sh
                    Args... args) {
   static_assert(sizeof...(Params) == sizeof...(Args), "kernel argument count");
   hipEvent_t a = nullptr, b = nullptr;
-  qtts_timer_slot(st, &a, &b);
+  if (!qtts_timer_slot(st, &a, &b)) {  // the plain launch: 0.6 us of host time less
+    hipLaunchKernelGGL(kernel, grid, block, shmem, st, static_cast<Params>(args)...);
+    return;
+  }
   hipExtLaunchKernelGGL(kernel, grid, block, shmem, st, a, b, 0u, static_cast<Params>(args)...);
 }
 

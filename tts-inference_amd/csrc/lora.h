@@ -29,22 +29,28 @@ struct LoraArgs {
   int64_t ldb;
   void* out;
   int64_t ldo;
-  float* t;  // [splits, m, t_stride]: partial sums over K of x A^T
+  uint8_t* t;     // [m, parts.count, blocks]: the first product's halves (lora.hip)
+  int32_t* exps;  // [m, parts.count, blocks], fp16
   int64_t m;
-  int k, n, slots, rank, rows_a, t_stride, splits;
+  int k, n, slots, rank, blocks, up_cols;
   LoraParts parts;
 };
 
 // ---- the plan: rows sorted by slot, cut into tiles of one slot each ----------------------------
-// int32 words: the number of tiles, m, slots, 0; then, from word 4, four words a tile (slot, or -1 for rows without an
-// adapter; its first entry of the order; its rows, at most kPlanTile; 0); then the order of the rows.
+// int32 words: the number of tiles, m, slots, 0; then, from word 4, two words a tile (slot, or -1 for rows without an
+// adapter; its rows, at most kPlanTile); then kPlanTile words a tile, its rows.
 constexpr int kPlanTile = 64;
 constexpr int kPlanMaxSlots = 768;  // the sort's counters are in LDS
+constexpr int64_t kPlanMaxRows = 1 << 30;  // places in int32
 
 __host__ __device__ inline int64_t plan_max_tiles(int64_t m, int64_t slots) {
   return (m + kPlanTile - 1) / kPlanTile + (m < slots + 1 ? m : slots + 1);
 }
-__host__ __device__ inline int64_t plan_order_at(int64_t m, int64_t slots) { return 4 + 4 * plan_max_tiles(m, slots); }
-__host__ __device__ inline int64_t plan_words(int64_t m, int64_t slots) { return plan_order_at(m, slots) + m; }
+__host__ __device__ inline int64_t plan_order_at(int64_t m, int64_t slots) {
+  return 4 + (2 * plan_max_tiles(m, slots) + 3) / 4 * 4;
+}
+__host__ __device__ inline int64_t plan_words(int64_t m, int64_t slots) {
+  return plan_order_at(m, slots) + kPlanTile * plan_max_tiles(m, slots);
+}
 
 }  // namespace qtts

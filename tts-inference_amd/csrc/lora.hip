@@ -9,9 +9,11 @@
 // elements 8 (lane / 16) ... + 7).  Loaded that way each lane is on a line of its own, and a line is touched
 // at half or a quarter of its width; so x and A go to LDS in whole 128-byte lines (each wave its own part of K,
 // a ring of stages without a barrier), and the result meets base in LDS, whose rows are read and written in
-// 128-byte pieces.  t leaves the first product in fp32; the second multiplies it as two 16-bit halves,
-// hi = T(t) and lo = T(t - hi), which keeps 16 bits of it (bf16; 22 in fp16, where the row is first scaled by
-// the power of two that brings its largest entry to [1/2, 1)).
+// 128-byte pieces.
+//
+// The second product multiplies t, scaled, as two 16-bit halves, hi = T(t) and lo = T(t - hi), which keeps 16 bits
+// of it (bf16; in fp16 22 of the largest entry of each 32, which are first scaled by a power of two into [1/2, 1)).
+// The first product's kernel writes them so: the second, whose time is the output's rows, only loads them.
 //
 // Where the groups come from: up to 64 rows, each workgroup finds the rows of its slot by one load of the
 // window's indices and a ballot; past them from a plan (rows sorted by slot, made once a step).
@@ -29,21 +31,20 @@ using namespace qtts;
 
 namespace qtts {
 
+typedef __attribute__((ext_vector_type(2))) int i32x2_t;
+
 static_assert(kLoraMaxParts == QTTS_LORA_MAX_PARTS && kLoraMaxRank == QTTS_LORA_MAX_RANK, "limits of the header");
 
 template <typename XT> using vec8 = typename mfma16<XT>::vec;
 
-// Eight elements of a row from `at`, zeros from `end` on.  VEC: the row starts on 16 bytes, at and end are multiples of 8.
-template <bool VEC, typename XT> __device__ __forceinline__ i32x4_t load8(const XT* row, int at, int end) {
-  i32x4_t v = {0, 0, 0, 0};
-  if constexpr (VEC) {
-    if (at < end) v = *(const i32x4_t*)(row + at);
-  } else {
+// Eight elements of a row from `at`, one by one; zeros from `end` on (the last one is read again there).
+template <typename XT> __device__ __forceinline__ i32x4_t load8(const XT* row, int at, int end) {
+  i32x4_t v;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t lo = at + 2 * i < end ? row[at + 2 * i].bits : 0, hi = at + 2 * i + 1 < end ? row[at + 2 * i + 1].bits : 0;
-      v[i] = (int)(lo | (hi << 16));
-    }
+  for (int i = 0; i < 4; ++i) {
+    const int e0 = at + 2 * i, e1 = e0 + 1;
+    const uint32_t lo = row[min(e0, end - 1)].bits, hi = row[min(e1, end - 1)].bits;
+    v[i] = (int)((e0 < end ? lo : 0) | (e1 < end ? hi << 16 : 0));
   }
   return v;
 }
@@ -75,303 +76,409 @@ __device__ __forceinline__ Group group_by_ballot(const LoraArgs& g, int64_t at) 
   return {slot, count, first + __builtin_amdgcn_ds_bpermute(4 * (before + (j < count ? j : 0)), order)};
 }
 
+// The rows of a tile, wherever the plan was made.
+__device__ __forceinline__ int plan_tile_rows(const LoraArgs& g, int64_t tile) { return g.plan[5 + 2 * tile]; }
+
 // Sub-group `sub` (16 rows) of tile `tile` < plan_max_tiles; count 0 past its end, past the plan's tiles and where the
-// plan was made for another batch or slot count.
+// plan was made for another batch or slot count.  The three loads do not wait for one another.
 __device__ __forceinline__ Group group_by_plan(const LoraArgs& g, int64_t tile, int sub) {
-  const i32x4_t head = *(const i32x4_t*)g.plan, e = *(const i32x4_t*)(g.plan + 4 + 4 * tile);
-  const int count = min(16, e[2] - 16 * sub), j = threadIdx.x & 15;
+  const int j = threadIdx.x & 15;
+  const i32x4_t head = *(const i32x4_t*)g.plan;
+  const i32x2_t e = *(const i32x2_t*)(g.plan + 4 + 2 * tile);
+  const int32_t* order = g.plan + plan_order_at(g.m, g.slots) + kPlanTile * tile + 16 * sub;
+  const int row = order[j], lead = order[0], count = min(16, e[1] - 16 * sub);
   if (tile >= head[0] || head[1] != g.m || head[2] != g.slots || count <= 0) return {-1, 0, 0};
-  const int64_t at = plan_order_at(g.m, g.slots) + e[1] + 16 * sub + (j < count ? j : 0);
-  return {e[0], count, g.plan[at]};
+  return {e[0], count, j < count ? row : lead};
 }
 
-__device__ __forceinline__ int live_rank(const LoraArgs& g, int slot) {
-  return g.ranks ? min(max(g.ranks[slot], 0), g.rank) : g.rank;
-}
+// The slots' ranks: the first 64 by lane, loaded beside what names the slot.
+struct Ranks {
+  int mine;
+  __device__ __forceinline__ explicit Ranks(const LoraArgs& g) {
+    const int lane = threadIdx.x & 63;
+    mine = g.ranks && lane < g.slots ? g.ranks[lane] : g.rank;
+  }
+  __device__ __forceinline__ int of(const LoraArgs& g, int slot) const {
+    if (slot < 0) return 0;
+    const int r = slot < 64 ? __builtin_amdgcn_readlane(mine, slot) : g.ranks ? g.ranks[slot] : g.rank;
+    return min(max(r, 0), g.rank);
+  }
+};
 
 // ---- first product ---------------------------------------------------------------------------
 
 // Stages of a wave's ring: 64 of K of the group's rows and of N 16-row tiles of A, each tile two direct loads of 1 KiB
 // (eight rows of 128 bytes, pieces swizzled as pipe.h's stages).
 template <int N> constexpr int kDownStages = N == 1 ? 4 : N == 2 ? 3 : 2;
-template <int N> constexpr int kDownBytes = kDownStages<N> * (N + 1) * 2048;  // of a wave
+template <int N, int S> constexpr int kDownBytes = S * (N + 1) * 2048;  // of a wave
 
-// Rows [row0, row0 + 16 N) of a slot's A by the group's rows, over K from 32 s0 to 32 s1 (s0 even):
-// acc[i] holds, in lane l, rows 16 i + 4 (l / 16) ... + 3 of A for the group's row l % 16.  Rows past the slot's rank, or past
-// `rows`, give values that nothing reads.  lds: kDownBytes<N> of this wave alone.
-template <typename XT, int N, bool VEC>
-__device__ __forceinline__ void down_steps(const LoraArgs& g, const Group& gr, const XT* a, int row0, int rows, int live, int s0,
-                                           int s1, uint8_t* lds, f32x4_t* acc) {
+// N 16-row tiles of a slot's A, row(i, j) the j-th row of tile i (rows past the slot's rank give values that nothing
+// reads, and are taken from its first row, which is in cache), by the group's rows, over K from 32 s0 to 32 s1
+// (s0 even): acc[i] holds, in lane l, rows 4 (l / 16) ... + 3 of tile i for the group's row l % 16.  lds: kDownBytes<N, S> of
+// this wave alone.
+template <typename XT, int N, int S, bool VEC, typename F>
+__device__ __forceinline__ void down_steps(const LoraArgs& g, const Group& gr, const XT* a, F&& row, int s0, int s1,
+                                           uint8_t* lds, f32x4_t* acc) {
   const int lane = threadIdx.x & 63, j = lane & 15, q = lane >> 4;
   if constexpr (VEC) {
-    constexpr int S = kDownStages<N>, L = 2 * (N + 1);  // direct loads a stage
-    const XT* from[L];  // each direct load's row and piece, at K = 0
+    constexpr int L = 2 * (N + 1);  // direct loads a stage
+    const XT* from[L];              // each direct load's row and piece, at the next stage's K
+    const int c0 = s0 >> 1, c1 = (s1 + 1) >> 1, whole = min(c1, g.k >> 6);
 #pragma unroll
     for (int i = 0; i < L; ++i) {
-      const int r = (i & 1) * 8 + (lane >> 3), piece = 8 * swizzle8(r, lane & 7);
-      if (i < 2) {
-        const int row = __builtin_amdgcn_ds_bpermute(4 * r, (int)gr.row);
-        from[i] = (const XT*)g.x + (int64_t)row * g.ldx + piece;
-      } else {  // hidden rows read the first one: in cache
-        const int ar = row0 + 16 * ((i - 2) >> 1) + r;
-        from[i] = a + (int64_t)(ar < rows && ar % g.rank < live ? ar : 0) * g.k + piece;
-      }
+      const int r = (i & 1) * 8 + (lane >> 3), at = 64 * c0 + 8 * swizzle8(r, lane & 7);
+      if (i < 2) from[i] = (const XT*)g.x + (int64_t)__builtin_amdgcn_ds_bpermute(4 * r, (int)gr.row) * g.ldx + at;
+      else from[i] = a + (int64_t)row((i - 2) >> 1, r) * g.k + at;
     }
-    const int c1 = (s1 + 1) >> 1, tail = g.k - 8;
-    auto issue = [&](int c) {
-      uint8_t* stage = lds + c % S * (L * 1024);
+    int into = 0, out = 0, ahead = c0;  // stages of the ring
+    auto issue = [&]() {
 #pragma unroll
       for (int i = 0; i < L; ++i) {
-        const int r = (i & 1) * 8 + (lane >> 3), p = 8 * swizzle8(r, lane & 7);
-        const int past = max(64 * c + p - tail, 0);  // a piece past K: the row's last one, zeroed when it is read
-        load_to_lds16(from[i] + 64 * c - past, stage + i * 1024);
+        load_to_lds16(from[i], lds + (into * L + i) * 1024);
+        from[i] += 64;
       }
+      into = into + 1 == S ? 0 : into + 1;
+      ++ahead;
     };
-    int c = s0 >> 1, ahead = c;
-    for (; ahead < min(c + S, c1); ++ahead) issue(ahead);
-    for (; c < c1; ++c) {
-      wait_stages<L, S - 1>(ahead - c - 1);
-      const uint8_t* stage = lds + c % S * (L * 1024);
-      i32x4_t xv[2], av[2][N];
+    i32x4_t xv[2], av[2][N];
+    auto read = [&](const uint8_t* stage) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int at = j * 128 + swizzle8(j, 4 * h + q) * 16;
         xv[h] = *(const i32x4_t*)(stage + at);
 #pragma unroll
         for (int i = 0; i < N; ++i) av[h][i] = *(const i32x4_t*)(stage + 2048 * (i + 1) + at);
-        if (64 * c + 32 * h + 8 * q > tail) {
-          xv[h] = i32x4_t{0, 0, 0, 0};
-#pragma unroll
-          for (int i = 0; i < N; ++i) av[h][i] = i32x4_t{0, 0, 0, 0};
-        }
       }
-      wait_lgkmcnt0();  // the stage is read before it is loaded again
-      if (ahead < c1) issue(ahead++);
+    };
+    auto multiply = [&]() {
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int i = 0; i < N; ++i)
           acc[i] = mfma16<XT>::mma(__builtin_bit_cast(vec8<XT>, av[h][i]), __builtin_bit_cast(vec8<XT>, xv[h]), acc[i]);
+    };
+    while (ahead < min(c0 + S, whole)) issue();
+    for (int c = c0; c < whole; ++c) {
+      wait_stages<L, S - 1>(ahead - c - 1);
+      read(lds + out * (L * 1024));
+      out = out + 1 == S ? 0 : out + 1;
+      wait_lgkmcnt0();  // the stage is read before it is loaded again
+      if (ahead < whole) issue();
+      multiply();
+    }
+    if (max(c0, whole) < c1) {  // the last stage of a K that is no multiple of 64: its missing pieces are zeros
+      const int left = g.k - 64 * whole;  // of K, a multiple of 8
+#pragma unroll
+      for (int i = 0; i < L; ++i) {
+        const int piece = 8 * swizzle8((i & 1) * 8 + (lane >> 3), lane & 7);
+        load_to_lds16(from[i] - (piece < left ? 0 : piece), lds + i * 1024);
+      }
+      wait_vmcnt<0>();
+      read(lds);
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        if (32 * h + 8 * q >= left) {
+          xv[h] = i32x4_t{0, 0, 0, 0};
+#pragma unroll
+          for (int i = 0; i < N; ++i) av[h][i] = i32x4_t{0, 0, 0, 0};
+        }
+      wait_lgkmcnt0();
+      multiply();
     }
   } else {
     const XT* x = (const XT*)g.x + gr.row * g.ldx;
     const XT* ap[N];
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int r = row0 + 16 * i + j;
-      ap[i] = a + (int64_t)(r < rows && r % g.rank < live ? r : 0) * g.k;
-    }
+    for (int i = 0; i < N; ++i) ap[i] = a + (int64_t)row(i, j) * g.k;
     for (int s = s0; s < s1; ++s) {
-      const vec8<XT> xv = __builtin_bit_cast(vec8<XT>, load8<false>(x, 32 * s + 8 * q, g.k));
+      const vec8<XT> xv = __builtin_bit_cast(vec8<XT>, load8(x, 32 * s + 8 * q, g.k));
 #pragma unroll
       for (int i = 0; i < N; ++i)
-        acc[i] = mfma16<XT>::mma(__builtin_bit_cast(vec8<XT>, load8<false>(ap[i], 32 * s + 8 * q, g.k)), xv, acc[i]);
+        acc[i] = mfma16<XT>::mma(__builtin_bit_cast(vec8<XT>, load8(ap[i], 32 * s + 8 * q, g.k)), xv, acc[i]);
     }
   }
 }
 
-constexpr int kDownWaves = 4;
+// ---- t's halves ------------------------------------------------------------------------------
+// The rank in blocks: up to 16 entries one block of 16 (PACK), past them NB blocks of 32.  A block of a row in the workspace:
+// its hi halves, then its lo halves.  A lane's operand: whole blocks, entries 8 (lane / 16) ... + 7 of hi and then of lo
+// (two MFMAs); PACK, hi for lanes 0-31 and lo for lanes 32-63 (one).
 
-// Grid: (blocks of A's tiles x splits of K, groups or tiles x 4).
-template <typename XT, int N, bool VEC, bool PLAN>
+template <bool PACK> constexpr int kBlockTiles = PACK ? 1 : 2;
+template <bool PACK> constexpr int kBlockBytes = PACK ? 64 : 128;
+
+// Four neighbouring entries of t (already zero past the slot's rank) as halves.
+template <typename XT> struct Halves {
+  uint2 hi, lo;
+  __device__ __forceinline__ explicit Halves(f32x4_t v) {
+    uint32_t h[2], l[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      h[i] = pack2_f32<XT>(v[2 * i], v[2 * i + 1]);
+      const float h0 = to_f32(XT{(uint16_t)h[i]}), h1 = to_f32(XT{(uint16_t)(h[i] >> 16)});
+      // an infinite half has no remainder
+      l[i] = pack2_f32<XT>(fabsf(h0) <= 3.4e38f ? v[2 * i] - h0 : 0.0f, fabsf(h1) <= 3.4e38f ? v[2 * i + 1] - h1 : 0.0f);
+    }
+    hi = make_uint2(h[0], h[1]), lo = make_uint2(l[0], l[1]);
+  }
+};
+
+// fp16: the exponent that brings the largest of a block's entries to [1/2, 1) (four lanes a row), and the entries scaled by it.
+template <typename XT, int T> __device__ __forceinline__ int scale_block(f32x4_t (&v)[T]) {
+  if constexpr (!std::is_same<XT, f16_t>::value) return 0;
+  float top = 0.0f;
+#pragma unroll
+  for (int t = 0; t < T; ++t)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) top = fmaxf(top, fabsf(v[t][i]));
+  top = fmaxf(top, __shfl_xor(top, 16, 64));
+  top = fmaxf(top, __shfl_xor(top, 32, 64));
+  const int exp = __builtin_amdgcn_frexp_expf(top);  // 0 for zero, infinity and NaN
+#pragma unroll
+  for (int t = 0; t < T; ++t)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[t][i] = __builtin_amdgcn_ldexpf(v[t][i], -exp);
+  return exp;
+}
+
+// Tiles [tile, tile + T) of the waves' sums in LDS (wave w's at sums + w * pitch bytes), added, scaled, zero past the rank;
+// r0: the first tile's first entry of its partition.
+template <int W, int T>
+__device__ __forceinline__ void meet_waves(const uint8_t* sums, int pitch, int tile, int r0, int live, float scaling,
+                                           f32x4_t (&v)[T]) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int t = 0; t < T; ++t) {
+    v[t] = *(const f32x4_t*)(sums + (64 * (tile + t) + lane) * 16);
+#pragma unroll
+    for (int w = 1; w < W; ++w) v[t] += *(const f32x4_t*)(sums + w * pitch + (64 * (tile + t) + lane) * 16);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[t][i] = r0 + 16 * t + 4 * (lane >> 4) + i < live ? v[t][i] * scaling : 0.0f;
+  }
+}
+
+constexpr int kDownWaves = 8;
+
+// Grid: (N tiles of the partitions' A each, groups or tiles x 4).  Eight waves share K.
+template <typename XT, int N, bool PACK, bool VEC, bool PLAN>
 __global__ __launch_bounds__(64 * kDownWaves) void lora_down_kernel(LoraArgs g) {
-  __shared__ __align__(1024) uint8_t stages[kDownWaves][VEC ? kDownBytes<N> : 1024 * N];
+  constexpr int T = kBlockTiles<PACK>, kPitch = VEC ? kDownBytes<N, kDownStages<N>> : 1024 * N;
+  __shared__ __align__(1024) uint8_t stages[kDownWaves][kPitch];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int split = blockIdx.x % g.splits, row0 = blockIdx.x / g.splits * 16 * N;
+  const int per_part = T * g.blocks, tile0 = blockIdx.x * N;  // tiles of a partition; the workgroup's first
   const int64_t groups = PLAN ? 4 * plan_max_tiles(g.m, g.slots) : g.m;
-  const int steps = (g.k + 31) >> 5, parts = g.splits * kDownWaves, per = ((steps + parts - 1) / parts + 1) & ~1;
-  const int s0 = min((split * kDownWaves + wave) * per, steps + 1 & ~1), s1 = min(s0 + per, steps);
+  const Ranks ranks(g);
+  const int steps = (g.k + 31) >> 5, per = ((steps + kDownWaves - 1) / kDownWaves + 1) & ~1;
+  const int s0 = min(wave * per, (steps + 1) & ~1), s1 = min(s0 + per, steps);
   for (int64_t at = blockIdx.y; at < groups; at += gridDim.y) {
     const Group gr = PLAN ? group_by_plan(g, at >> 2, (int)(at & 3)) : group_by_ballot(g, at);
-    if (gr.slot < 0 || !gr.count) continue;
-    const int live = live_rank(g, gr.slot);
+    if (!gr.count) continue;
+    const int live = ranks.of(g, gr.slot);
     if (!live) continue;
     f32x4_t acc[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) acc[i] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-    down_steps<XT, N, VEC>(g, gr, (const XT*)g.a + (int64_t)gr.slot * g.rows_a * g.k, row0, g.rows_a, live, s0, s1,
-                           stages[wave], acc);
+    const float scaling = g.scaling[gr.slot];
+    auto row = [&](int i, int j) {
+      const int part = (tile0 + i) / per_part, r = 16 * ((tile0 + i) % per_part) + j;
+      return part < g.parts.count && r < live ? part * g.rank + r : 0;
+    };
+    down_steps<XT, N, kDownStages<N>, VEC>(g, gr, (const XT*)g.a + (int64_t)gr.slot * g.parts.count * g.rank * g.k, row, s0,
+                                           s1, stages[wave], acc);
 #pragma unroll
     for (int i = 0; i < N; ++i) ((f32x4_t*)stages[wave])[64 * i + lane] = acc[i];
     __syncthreads();
-    if (wave < N && (lane & 15) < gr.count && row0 + 16 * wave < g.t_stride) {
-      f32x4_t v = ((f32x4_t*)stages[0])[64 * wave + lane];
+    const int tile = tile0 + T * wave;  // the wave's block
+    if (wave < N / T && tile < per_part * g.parts.count) {
+      f32x4_t v[T];
+      meet_waves<kDownWaves, T>(stages[0], kPitch, T * wave, tile % per_part * 16, live, scaling, v);
+      const int exp = scale_block<XT, T>(v);
+      const int64_t block = gr.row * (g.parts.count * g.blocks) + tile / T;
+      if ((lane & 15) < gr.count) {
+        uint8_t* to = g.t + block * kBlockBytes<PACK> + 8 * (lane >> 4);
 #pragma unroll
-      for (int w = 1; w < kDownWaves; ++w) v += ((f32x4_t*)stages[w])[64 * wave + lane];
-      *(f32x4_t*)(g.t + ((int64_t)split * g.m + gr.row) * g.t_stride + row0 + 16 * wave + 4 * (lane >> 4)) = v;
+        for (int t = 0; t < T; ++t) {
+          const Halves<XT> h(v[t]);
+          *(uint2*)(to + 32 * t) = h.hi;
+          *(uint2*)(to + 32 * t + kBlockBytes<PACK> / 2) = h.lo;
+        }
+        if (std::is_same<XT, f16_t>::value && lane < 16) g.exps[block] = exp;
+      }
     }
     __syncthreads();  // read before the next group's stages
   }
 }
 
 // ---- second product --------------------------------------------------------------------------
-// The rank in blocks of 32 (NB of them).  A whole block: lane group q = lane / 16 holds entries 8 q ... + 7, and two
-// MFMAs multiply them by t's high and low halves.  PACK: the last block has 16 entries or fewer, so one MFMA does
-// both, groups 0-1 with the high halves and 2-3 with the low ones.
+// The t operands of one group's rows: (hi, lo) of each block, and fp16's exponents.
+template <typename XT, int NB, bool PACK> struct TOperand {
+  static constexpr int kHalves = PACK ? 1 : 2;
+  i32x4_t v[NB][kHalves];
+  int exp[NB];
 
-template <int NB, bool PACK> struct RankLane {
-  int first[NB];  // the lane's first entry of each block
-  bool low;       // PACK: the lane's half in the last block
-  __device__ __forceinline__ explicit RankLane(int lane) {
-    const int q = lane >> 4;
+  // `row`: the lane's row of the workspace (of a group's first for lanes past its rows), `part` of the partition.
+  __device__ __forceinline__ void load(const LoraArgs& g, int64_t row, int part) {
+    const int64_t block = (row * g.parts.count + part) * NB;
+    const uint8_t* from = g.t + block * kBlockBytes<PACK> + 16 * ((threadIdx.x & 63) >> 4);
 #pragma unroll
-    for (int b = 0; b < NB; ++b) first[b] = 32 * b + 8 * (PACK && b == NB - 1 ? q & 1 : q);
-    low = q >= 2;
+    for (int b = 0; b < NB; ++b) {
+#pragma unroll
+      for (int h = 0; h < kHalves; ++h) v[b][h] = *(const i32x4_t*)(from + kBlockBytes<PACK> * b + 64 * h);
+      if constexpr (std::is_same<XT, f16_t>::value) exp[b] = g.exps[block + b];
+    }
   }
 };
 
-// Zeroes the entries of an operand from `at` on that are past the slot's rank: they may hold anything.
-__device__ __forceinline__ i32x4_t hide(i32x4_t v, int at, int live) {
+// A slot's B by columns: an operand of 16 columns from c is the lane's eight entries of each block of rows c + lane % 16.  VEC: a
+// lane's place as bytes in the slot's B (32 bits: the host checks), clamped to the partition's last column.  Entries past the
+// slot's rank may hold anything, and those past the rank are no part of the row: a lane of such entries reads others of its row,
+// and masks them.  (No load is in a branch: the compiler may give each side of one its own copy of the MFMAs after it.)
+template <typename XT, int NB, bool PACK, bool VEC> struct Columns {
+  const char* slot_b;
+  uint32_t at, last, step;  // of column c0 + lane % 16, of the last column, from one operand to the next
+  int rank, c, end;
+  bool masks;
+  int first[NB];
+  i32x4_t shown[NB];
+
+  __device__ __forceinline__ Columns(const LoraArgs& g, int slot, int c0, int part_end, int live) {
+    const int q = (threadIdx.x & 63) >> 4;
+    slot_b = (const char*)((const XT*)g.b + (int64_t)slot * g.n * g.rank);
+    rank = g.rank, c = c0 + (int)(threadIdx.x & 15), end = part_end;
+    at = (uint32_t)c * (uint32_t)rank * 2, last = (uint32_t)(end - 1) * (uint32_t)rank * 2, step = 32 * (uint32_t)rank;
+    masks = live != (PACK ? 16 : 32 * NB);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int n = live - at - 2 * i;
-    v[i] = n >= 2 ? v[i] : n == 1 ? v[i] & 0xffff : 0;
+    for (int b = 0; b < NB; ++b) {
+      const int e = 32 * b + 8 * (PACK ? q & 1 : q);
+      first[b] = VEC && e >= rank ? 0 : e;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) shown[b][i] = live - e - 2 * i >= 2 ? -1 : live - e - 2 * i == 1 ? 0xffff : 0;
+    }
   }
-  return v;
-}
 
-// The t operands of one group's row: (hi, lo) halves of each block, and the exponent that fp16 rows are scaled by.
-template <typename XT, int NB, bool PACK> struct TOperand {
-  vec8<XT> hi[NB], lo[NB];
-  int exp;
-
-  // v[b][i]: entry first[b] + i of t, scaled and zero past the slot's rank.
-  __device__ __forceinline__ void set(float (&v)[NB][8], bool low) {
-    exp = 0;
-    if constexpr (std::is_same<XT, f16_t>::value) {
-      float top = 0.0f;
+  // The operand of the next 16 columns.
+  __device__ __forceinline__ void next(vec8<XT> (&v)[NB]) {
+    i32x4_t r[NB];
+    if constexpr (VEC) {
+      const uint32_t from = at < last ? at : last;
 #pragma unroll
-      for (int b = 0; b < NB; ++b)
+      for (int b = 0; b < NB; ++b) r[b] = *(const i32x4_t*)(slot_b + (from + 2 * first[b]));
+      at += step;
+    } else {
+      const XT* row = (const XT*)slot_b + (int64_t)min(c, end - 1) * rank;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[b][i]));
-      top = fmaxf(top, __shfl_xor(top, 16, 64));
-      top = fmaxf(top, __shfl_xor(top, 32, 64));
-      exp = __builtin_amdgcn_frexp_expf(top);  // 0 for zero, infinity and NaN
-#pragma unroll
-      for (int b = 0; b < NB; ++b)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[b][i] = __builtin_amdgcn_ldexpf(v[b][i], -exp);
+      for (int b = 0; b < NB; ++b) r[b] = load8(row, first[b], rank);
+      c += 16;
     }
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
-      i32x4_t h, l;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        h[i] = (int)pack2_f32<XT>(v[b][2 * i], v[b][2 * i + 1]);
-        const float h0 = to_f32(XT{(uint16_t)h[i]}), h1 = to_f32(XT{(uint16_t)((uint32_t)h[i] >> 16)});
-        // an infinite or NaN half has no remainder
-        const float l0 = fabsf(h0) <= 3.4e38f ? v[b][2 * i] - h0 : 0.0f, l1 = fabsf(h1) <= 3.4e38f ? v[b][2 * i + 1] - h1 : 0.0f;
-        l[i] = (int)pack2_f32<XT>(l0, l1);
-      }
-      if (PACK && b == NB - 1) h = low ? l : h;  // one MFMA: the lane's half
-      hi[b] = __builtin_bit_cast(vec8<XT>, h);
-      lo[b] = __builtin_bit_cast(vec8<XT>, l);
+      if (masks) r[b] &= shown[b];
+      v[b] = __builtin_bit_cast(vec8<XT>, r[b]);
     }
   }
 };
 
-// NT tiles of 16 columns a wave: lane l ends with columns c0 + 16 n + 4 (l / 16) ... + 3 of the group's row l % 16.
-template <typename XT, int NB, int NT, bool PACK, bool VEC> struct UpTile {
-  vec8<XT> b[NT][NB];
-
-  __device__ __forceinline__ void load(const LoraArgs& g, int slot, int c0, int end, int live, const RankLane<NB, PACK>& rl) {
-    const int i = threadIdx.x & 15;
+template <typename XT, int NB, bool PACK>
+__device__ __forceinline__ f32x4_t up_mma(const vec8<XT> (&b)[NB], const TOperand<XT, NB, PACK>& t) {
+  f32x4_t sum = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const int c = min(c0 + 16 * n + i, end - 1);
-      const XT* row = (const XT*)g.b + ((int64_t)slot * g.n + c) * g.rank;
+  for (int k = 0; k < NB; ++k) {
+    constexpr bool kExp = std::is_same<XT, f16_t>::value;  // a block at a time: each has an exponent of its own
+    f32x4_t acc = kExp ? f32x4_t{0.0f, 0.0f, 0.0f, 0.0f} : sum;
 #pragma unroll
-      for (int k = 0; k < NB; ++k) b[n][k] = __builtin_bit_cast(vec8<XT>, load8<VEC>(row, rl.first[k], g.rank));
-    }
-    if (live != g.rank) {
+    for (int h = 0; h < TOperand<XT, NB, PACK>::kHalves; ++h)
+      acc = mfma16<XT>::mma(b[k], __builtin_bit_cast(vec8<XT>, t.v[k][h]), acc);
+    if constexpr (kExp) {
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int k = 0; k < NB; ++k)
-          b[n][k] = __builtin_bit_cast(vec8<XT>, hide(__builtin_bit_cast(i32x4_t, b[n][k]), rl.first[k], live));
+      for (int i = 0; i < 4; ++i) sum[i] += __builtin_amdgcn_ldexpf(acc[i], t.exp[k]);
+    } else {
+      sum = acc;
     }
   }
+  return sum;
+}
 
-  __device__ __forceinline__ void mul(const TOperand<XT, NB, PACK>& t, f32x4_t (&acc)[NT]) const {
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      acc[n] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-      for (int k = 0; k < NB; ++k) {
-        acc[n] = mfma16<XT>::mma(b[n][k], t.hi[k], acc[n]);
-        if (!(PACK && k == NB - 1)) acc[n] = mfma16<XT>::mma(b[n][k], t.lo[k], acc[n]);
-      }
-    }
-  }
-};
-
-// A group's rows of base and out, 16 NT columns of a wave: 2 NT lanes a row, eight neighbouring columns a lane, NT / 2 pieces
-// a lane.  base is loaded as raw bits, in flight early.
+// A group's rows of base and out, 16 NT columns at a time: 2 NT lanes a row, eight neighbouring columns a lane, NT / 2 pieces
+// a lane.  base is loaded as raw bits, in flight early.  Every lane of the wave takes part.
 template <typename XT, int NT, bool VEC> struct Rows {
   static constexpr int kLanes = 2 * NT, kPieces = NT / 2, kPitch = 16 * NT + 4;  // floats a row in LDS
   static constexpr int kFloats = 16 * kPitch;
-  int64_t row[kPieces];
-  bool live[kPieces];
+  const XT* base[kPieces];
+  XT* out[kPieces];
+  bool mine[kPieces];
   int c, end;
   i32x4_t raw[kPieces];
 
-  // Every lane of the wave: the group's rows are read from its lanes.
-  __device__ __forceinline__ void load(const LoraArgs& g, const Group& gr, int c0, int part_end) {
+  __device__ __forceinline__ Rows(const LoraArgs& g, const Group& gr, int c0, int part_end) {
     const int lane = threadIdx.x & 63;
     c = c0 + 8 * (lane % kLanes), end = part_end;
 #pragma unroll
     for (int h = 0; h < kPieces; ++h) {
       const int r = lane / kLanes + h * (64 / kLanes);
-      row[h] = __builtin_amdgcn_ds_bpermute(4 * r, (int)gr.row);
-      live[h] = r < gr.count && c < end;
-      if (live[h]) raw[h] = load8<VEC>((const XT*)g.base + row[h] * g.ldb, c, end);
+      const int64_t row = __builtin_amdgcn_ds_bpermute(4 * r, (int)gr.row);
+      base[h] = (const XT*)g.base + row * g.ldb + c;
+      out[h] = (XT*)g.out + row * g.ldo + c;
+      mine[h] = r < gr.count;
     }
   }
 
-  __device__ __forceinline__ void store(const LoraArgs& g, int h, i32x4_t v) const {
-    XT* out = (XT*)g.out + row[h] * g.ldo + c;
+  __device__ __forceinline__ void load() {
+    // clamped, not in a branch: rows past the group's are its first, columns past the partition the last ones before it
+#pragma unroll
+    for (int h = 0; h < kPieces; ++h) {
+      const int back = max(c - (end - (VEC ? 8 : 1)), 0);
+      if constexpr (VEC) raw[h] = *(const i32x4_t*)(base[h] - back);
+      else raw[h] = load8(base[h] - back, 0, end - c + back);
+    }
+  }
+
+  __device__ __forceinline__ void store(int h, i32x4_t v) const {
     if constexpr (VEC) {
-      *(i32x4_t*)out = v;
+      *(i32x4_t*)out[h] = v;
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        if (c + i < end) out[i] = XT{(uint16_t)((uint32_t)v[i >> 1] >> (16 * (i & 1)))};
+        if (c + i < end) out[h][i] = XT{(uint16_t)((uint32_t)v[i >> 1] >> (16 * (i & 1)))};
     }
   }
 
-  __device__ __forceinline__ void copy(const LoraArgs& g) const {
+  __device__ __forceinline__ void copy() const {
 #pragma unroll
     for (int h = 0; h < kPieces; ++h)
-      if (live[h]) store(g, h, raw[h]);
+      if (mine[h] && c < end) store(h, raw[h]);
   }
 
-  // out = base + acc 2^exp, rounded once.  lds: kFloats of this wave alone.
-  __device__ __forceinline__ void add(const LoraArgs& g, const f32x4_t (&acc)[NT], int exp, float* lds) const {
+  __device__ __forceinline__ void advance() {  // to the next 16 NT columns
+    c += 16 * NT;
+#pragma unroll
+    for (int h = 0; h < kPieces; ++h) base[h] += 16 * NT, out[h] += 16 * NT;
+  }
+
+  // out = base + acc(tile), rounded once.  lds: kFloats of this wave alone.
+  template <typename F> __device__ __forceinline__ void add(F&& acc, float* lds) const {
     const int lane = threadIdx.x & 63;
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // the last result has been read
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      f32x4_t v = acc[n];
-      if constexpr (std::is_same<XT, f16_t>::value)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = __builtin_amdgcn_ldexpf(v[i], exp);
-      *(f32x4_t*)(lds + (lane & 15) * kPitch + 16 * n + 4 * (lane >> 4)) = v;
-    }
+    for (int n = 0; n < NT; ++n)
+      *(f32x4_t*)(lds + (lane & 15) * kPitch + 16 * n + 4 * (lane >> 4)) = acc(n);
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
+    f32x4_t d[kPieces][2];
 #pragma unroll
     for (int h = 0; h < kPieces; ++h) {
       const float* from = lds + (lane / kLanes + h * (64 / kLanes)) * kPitch + 8 * (lane % kLanes);
-      const f32x4_t d0 = *(const f32x4_t*)from, d1 = *(const f32x4_t*)(from + 4);
-      if (!live[h]) continue;
+      d[h][0] = *(const f32x4_t*)from, d[h][1] = *(const f32x4_t*)(from + 4);
+    }
+#pragma unroll
+    for (int h = 0; h < kPieces; ++h) {
       i32x4_t v;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const uint32_t w = (uint32_t)raw[h][i];
-        const float lo = i < 2 ? d0[2 * i] : d1[2 * i - 4], hi = i < 2 ? d0[2 * i + 1] : d1[2 * i - 3];
-        v[i] = (int)pack2_f32<XT>(to_f32(XT{(uint16_t)w}) + lo, to_f32(XT{(uint16_t)(w >> 16)}) + hi);
+        v[i] = (int)pack2_f32<XT>(to_f32(XT{(uint16_t)w}) + d[h][i >> 1][2 * (i & 1)],
+                                  to_f32(XT{(uint16_t)(w >> 16)}) + d[h][i >> 1][2 * (i & 1) + 1]);
       }
-      store(g, h, v);
+      if (mine[h] && c < end) store(h, v);
     }
   }
 };
@@ -385,138 +492,137 @@ __device__ __forceinline__ Block block_of(const LoraArgs& g, int chunk, int cols
   return {p, first + (chunk - before) * cols, g.parts.end[p]};
 }
 
-constexpr int kUpWaves = 4, kUpTiles = kLoraUpCols / (16 * kUpWaves), kUpGroups = 2;
+constexpr int kUpWaves = 4, kUpTiles = 4, kUpBlock = 16 * kUpTiles;
 
-// Grid: (column blocks, groups, or halves of the plan's tiles: two groups of one slot, which share the B operands).
+// Grid: (blocks of g.up_cols columns, groups or the plan's tiles).  A tile of the plan is up to four groups of one slot: a wave
+// takes a whole group, or with fewer than four of them a part of a group's columns, 64 at a time.
+#ifndef LBA
+#define LBA 1
+#define LBB 1
+#endif
 template <typename XT, int NB, bool PACK, bool VEC, bool PLAN>
-__global__ __launch_bounds__(64 * kUpWaves) void lora_up_kernel(LoraArgs g) {
-  constexpr int G = PLAN ? kUpGroups : 1, NT = kUpTiles, PER = kPlanTile / 16 / G;
-  typedef Rows<XT, NT, VEC> R;
+__global__ __launch_bounds__(64 * kUpWaves, !VEC || NB > 2 ? 1 : NB == 1 ? LBA : LBB) void lora_up_kernel(LoraArgs g) {
+  typedef Rows<XT, kUpTiles, VEC> R;
   __shared__ __align__(16) float lds[kUpWaves][R::kFloats];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const Block blk = block_of(g, blockIdx.x, kLoraUpCols);
-  const int c0 = blk.c0 + 16 * NT * wave, tok = lane & 15;
-  if (c0 >= blk.end) return;
-  const RankLane<NB, PACK> rl(lane);
-  const int64_t groups = PLAN ? PER * plan_max_tiles(g.m, g.slots) : g.m;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const Block blk = block_of(g, blockIdx.x, g.up_cols);
+  const Ranks ranks(g);
+  const int64_t groups = PLAN ? plan_max_tiles(g.m, g.slots) : g.m;
+  const int blocks = g.up_cols / kUpBlock;
   for (int64_t at = blockIdx.y; at < groups; at += gridDim.y) {
-    Group gr[G];
-#pragma unroll
-    for (int i = 0; i < G; ++i)
-      gr[i] = PLAN ? group_by_plan(g, at / PER, (int)(at % PER) * G + i) : group_by_ballot(g, at);
-    if (!gr[0].count) continue;
-    const int slot = gr[0].slot, live = slot < 0 ? 0 : live_rank(g, slot);
+    int parts = kUpWaves;  // waves a group
+    if constexpr (PLAN) {
+      const int rows = plan_tile_rows(g, at);
+      parts = rows > 32 ? 1 : rows > 16 ? 2 : 4;
+    }
+    const Group gr = PLAN ? group_by_plan(g, at, wave / parts) : group_by_ballot(g, at);
+    if (!gr.count) continue;
+    const int per = (blocks + parts - 1) / parts, first = wave % parts * per;  // the wave's blocks of 64 columns
+    const int c0 = blk.c0 + kUpBlock * first, c1 = min(blk.c0 + kUpBlock * min(first + per, blocks), blk.end);
+    if (c0 >= c1) continue;
+    const int live = ranks.of(g, gr.slot);
     if (!live && g.base == g.out) continue;
-    R rows[G];
-#pragma unroll
-    for (int i = 0; i < G; ++i) rows[i].load(g, gr[i], c0, blk.end);
+    R rows(g, gr, c0, blk.end);
+    rows.load();
     if (!live) {
-#pragma unroll
-      for (int i = 0; i < G; ++i) rows[i].copy(g);
+      for (int c = c0;;) {
+        rows.copy();
+        if ((c += kUpBlock) >= c1) break;
+        rows.advance();
+        rows.load();
+      }
       continue;
     }
-    UpTile<XT, NB, NT, PACK, VEC> up;
-    up.load(g, slot, c0, blk.end, live, rl);
-    const float scaling = g.scaling[slot];
+    TOperand<XT, NB, PACK> t;
+    t.load(g, gr.row, blk.part);
+    Columns<XT, NB, PACK, VEC> columns(g, gr.slot, c0, blk.end, live);
+    vec8<XT> b[kUpTiles][NB];
 #pragma unroll
-    for (int i = 0; i < G; ++i) {
-      if (!gr[i].count) break;
-      float v[NB][8];
+    for (int n = 0; n < kUpTiles; ++n) columns.next(b[n]);
+    for (int c = c0;;) {
+      rows.add([&](int n) { return up_mma<XT, NB, PACK>(b[n], t); }, lds[wave]);
+      if ((c += kUpBlock) >= c1) break;
+      rows.advance();
+      rows.load();
 #pragma unroll
-      for (int b = 0; b < NB; ++b)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[b][e] = 0.0f;
-      const float* t = g.t + gr[i].row * g.t_stride + blk.part * g.rank;
-      for (int s = 0; s < g.splits; ++s, t += g.m * g.t_stride) {
-#pragma unroll
-        for (int b = 0; b < NB; ++b) {
-          if constexpr (VEC) {
-            if (rl.first[b] < live && tok < gr[i].count) {
-              const f32x4_t v0 = *(const f32x4_t*)(t + rl.first[b]), v1 = *(const f32x4_t*)(t + rl.first[b] + 4);
-#pragma unroll
-              for (int e = 0; e < 4; ++e) v[b][e] += v0[e], v[b][4 + e] += v1[e];
-            }
-          } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-              if (rl.first[b] + e < live) v[b][e] += t[rl.first[b] + e];
-          }
-        }
-      }
-#pragma unroll
-      for (int b = 0; b < NB; ++b)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[b][e] = rl.first[b] + e < live ? v[b][e] * scaling : 0.0f;
-      TOperand<XT, NB, PACK> to;
-      to.set(v, rl.low);
-      f32x4_t acc[NT];
-      up.mul(to, acc);
-      rows[i].add(g, acc, to.exp, lds[wave]);
+      for (int n = 0; n < kUpTiles; ++n) columns.next(b[n]);
     }
   }
 }
 
 // ---- both in one launch ----------------------------------------------------------------------
 
-constexpr int kOneWaves = 8, kOneTiles = kLoraFusedCols / (16 * kOneWaves);
+constexpr int kOneStages = 2, kOneWaves = 8, kOneTiles = kLoraFusedCols / (16 * kOneWaves);
 
 // Grid: (column blocks, rows).  The workgroup's waves share K of the first product, for its partition's rows of A alone, and
 // meet in LDS; then each multiplies its own columns.
 template <typename XT, int NB, bool PACK, bool VEC>
 __global__ __launch_bounds__(64 * kOneWaves) void lora_one_kernel(LoraArgs g) {
-  constexpr int NT = kOneTiles, N = 2 * NB - (PACK ? 1 : 0);  // 16-row tiles of A
+  constexpr int NT = kOneTiles, T = kBlockTiles<PACK>, N = T * NB;  // 16-row tiles of A
   typedef Rows<XT, NT, VEC> R;
-  constexpr int kBytes = std::max({VEC ? kDownBytes<N> : 0, 1024 * N, 4 * R::kFloats});
-  __shared__ __align__(1024) uint8_t stages[kOneWaves][(kBytes + 1023) & ~1023];
+  // A wave's stages; then its sums, later its result, in the first 4 KiB, and in the first wave's part the halves past them.
+  constexpr int kHalves = NB * 16 * kBlockBytes<PACK>, kUsed = 4096 + kHalves + NB * 64;
+  constexpr int kPitch = (std::max(VEC ? kDownBytes<N, kOneStages> : 0, kUsed) + 1023) & ~1023;
+  static_assert(1024 * N <= 4096 && 4 * R::kFloats <= 4096, "the sums and the result");
+  __shared__ __align__(1024) uint8_t stages[kOneWaves][kPitch];
+  uint8_t(*halves)[16][kBlockBytes<PACK>] = (uint8_t(*)[16][kBlockBytes<PACK>])(stages[0] + 4096);
+  int(*exps)[16] = (int(*)[16])(stages[0] + 4096 + kHalves);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const Block blk = block_of(g, blockIdx.x, kLoraFusedCols);
   const int c0 = blk.c0 + 16 * NT * wave, tok = lane & 15;
-  const RankLane<NB, PACK> rl(lane);
+  const Ranks ranks(g);
   const int steps = (g.k + 31) >> 5, per = ((steps + kOneWaves - 1) / kOneWaves + 1) & ~1;
-  const int s0 = min(wave * per, steps + 1 & ~1), s1 = min(s0 + per, steps);
+  const int s0 = min(wave * per, (steps + 1) & ~1), s1 = min(s0 + per, steps);
   for (int64_t at = blockIdx.y; at < g.m; at += gridDim.y) {
     const Group gr = group_by_ballot(g, at);
     if (!gr.count) continue;
-    const int live = gr.slot < 0 ? 0 : live_rank(g, gr.slot);
+    const int live = ranks.of(g, gr.slot);
     if (!live && g.base == g.out) continue;
-    R rows;
-    rows.load(g, gr, c0, blk.end);
+    R rows(g, gr, c0, blk.end);
+    rows.load();
     if (!live) {
-      rows.copy(g);
+      rows.copy();
       continue;
     }
-    UpTile<XT, NB, NT, PACK, VEC> up;
-    up.load(g, gr.slot, c0, blk.end, live, rl);
+    Columns<XT, NB, PACK, VEC> columns(g, gr.slot, c0, blk.end, live);
+    vec8<XT> b[NT][NB];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) columns.next(b[n]);
     const float scaling = g.scaling[gr.slot];
     __builtin_amdgcn_sched_barrier(0);  // in flight before the ring
-    f32x4_t acc1[N];
+    f32x4_t acc[N];
 #pragma unroll
-    for (int i = 0; i < N; ++i) acc1[i] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-    down_steps<XT, N, VEC>(g, gr, (const XT*)g.a + ((int64_t)gr.slot * g.rows_a + blk.part * g.rank) * g.k, 0, g.rank, live,
-                           s0, s1, stages[wave], acc1);
+    for (int i = 0; i < N; ++i) acc[i] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    auto row = [&](int i, int j) { return 16 * i + j < live ? 16 * i + j : 0; };
+    down_steps<XT, N, kOneStages, VEC>(g, gr, (const XT*)g.a + ((int64_t)gr.slot * g.parts.count + blk.part) * g.rank * g.k,
+                                       row, s0, s1, stages[wave], acc);
 #pragma unroll
-    for (int i = 0; i < N; ++i) ((f32x4_t*)stages[wave])[64 * i + lane] = acc1[i];
+    for (int i = 0; i < N; ++i) ((f32x4_t*)stages[wave])[64 * i + lane] = acc[i];
     __syncthreads();
-    // entries first[b] ... + 7 are rows 16 tile + 4 q' ... of two neighbouring lane groups q' of one tile
-    float v[NB][8];
+    if (wave < NB) {
+      f32x4_t v[T];
+      meet_waves<kOneWaves, T>(stages[0], kPitch, T * wave, 16 * T * wave, live, scaling, v);
+      const int exp = scale_block<XT, T>(v);
+      uint8_t* to = &halves[wave][tok][8 * (lane >> 4)];
 #pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      const int from = 64 * (rl.first[b] >> 4) + ((rl.first[b] & 15) >> 2) * 16 + tok;
-      f32x4_t lo = ((f32x4_t*)stages[0])[from], hi = ((f32x4_t*)stages[0])[from + 16];
-#pragma unroll
-      for (int w = 1; w < kOneWaves; ++w) lo += ((f32x4_t*)stages[w])[from], hi += ((f32x4_t*)stages[w])[from + 16];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        v[b][e] = rl.first[b] + e < live ? lo[e] * scaling : 0.0f;
-        v[b][4 + e] = rl.first[b] + 4 + e < live ? hi[e] * scaling : 0.0f;
+      for (int t = 0; t < T; ++t) {
+        const Halves<XT> h(v[t]);
+        *(uint2*)(to + 32 * t) = h.hi;
+        *(uint2*)(to + 32 * t + kBlockBytes<PACK> / 2) = h.lo;
       }
+      if (std::is_same<XT, f16_t>::value && lane < 16) exps[wave][tok] = exp;
     }
-    TOperand<XT, NB, PACK> to;
-    to.set(v, rl.low);
-    f32x4_t acc[NT];
-    up.mul(to, acc);
-    __syncthreads();  // t is read before its place takes the result, and before the next group's stages
-    rows.add(g, acc, to.exp, (float*)stages[wave]);
+    __syncthreads();  // (the sums are read: the result may take their place)
+    TOperand<XT, NB, PACK> t;
+#pragma unroll
+    for (int k = 0; k < NB; ++k) {
+#pragma unroll
+      for (int h = 0; h < TOperand<XT, NB, PACK>::kHalves; ++h)
+        t.v[k][h] = *(const i32x4_t*)&halves[k][tok][64 * h + 16 * (lane >> 4)];
+      if constexpr (std::is_same<XT, f16_t>::value) t.exp[k] = exps[k][tok];
+    }
+    rows.add([&](int n) { return up_mma<XT, NB, PACK>(b[n], t); }, (float*)stages[wave]);
+    __syncthreads();  // before the next group's stages and halves
   }
 }
 
@@ -546,9 +652,9 @@ template <typename F> __device__ __forceinline__ void by_slot(const int32_t* ind
 // slot and wave by wave, and the waves place their rows.
 __global__ __launch_bounds__(kPlanThreads) void lora_plan_kernel(const int32_t* __restrict__ index, int64_t m, int slots,
                                                                  int32_t* __restrict__ plan) {
-  extern __shared__ int32_t lds[];  // [kPlanWaves][slots + 1] counts, then places; [slots + 1] rows, first rows, first tiles
+  extern __shared__ int32_t lds[];  // [kPlanWaves][slots + 1] counts, then places; [slots + 1] rows, first tiles
   const int n = slots + 1, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  int32_t *rows = lds + kPlanWaves * n, *first_row = rows + n, *first_tile = first_row + n;
+  int32_t *rows = lds + kPlanWaves * n, *first_tile = rows + n;
   for (int i = tid; i < kPlanWaves * n; i += kPlanThreads) lds[i] = 0;
   __syncthreads();
   const int64_t run = (m + 64 * kPlanWaves - 1) / (64 * kPlanWaves) * 64;
@@ -566,28 +672,26 @@ __global__ __launch_bounds__(kPlanThreads) void lora_plan_kernel(const int32_t* 
   }
   __syncthreads();
   if (wave == 0) {  // exclusive sums over the slots
-    int row = 0, tile = 0;
+    int tile = 0;
     for (int s0 = 0; s0 < n; s0 += 64) {
-      const int c = s0 + lane < n ? rows[s0 + lane] : 0, t = (c + kPlanTile - 1) / kPlanTile;
-      int cs = c, ts = t;
+      const int t = s0 + lane < n ? (rows[s0 + lane] + kPlanTile - 1) / kPlanTile : 0;
+      int ts = t;
 #pragma unroll
       for (int o = 1; o < 64; o <<= 1) {
-        const int cu = __shfl_up(cs, o, 64), tu = __shfl_up(ts, o, 64);
-        if (lane >= o) cs += cu, ts += tu;
+        const int tu = __shfl_up(ts, o, 64);
+        if (lane >= o) ts += tu;
       }
-      if (s0 + lane < n) first_row[s0 + lane] = row + cs - c, first_tile[s0 + lane] = tile + ts - t;
-      row += __shfl(cs, 63, 64);
+      if (s0 + lane < n) first_tile[s0 + lane] = tile + ts - t;
       tile += __shfl(ts, 63, 64);
     }
     if (lane == 0) plan[0] = tile, plan[1] = (int32_t)m, plan[2] = slots;
   }
   __syncthreads();
   for (int s = tid; s < n; s += kPlanThreads) {
-    const int total = rows[s], start = first_row[s], tile = first_tile[s];
+    const int total = rows[s], tile = first_tile[s];
     for (int i = 0; i * kPlanTile < total; ++i)
-      *(i32x4_t*)(plan + 4 + 4 * (int64_t)(tile + i)) =
-          i32x4_t{s < slots ? s : -1, start + i * kPlanTile, min(kPlanTile, total - i * kPlanTile), 0};
-    int place = start;
+      *(i32x2_t*)(plan + 4 + 2 * (int64_t)(tile + i)) = i32x2_t{s < slots ? s : -1, min(kPlanTile, total - i * kPlanTile)};
+    int place = tile * kPlanTile;
     for (int w = 0; w < kPlanWaves; ++w) {
       const int c = lds[w * n + s];
       lds[w * n + s] = place;
@@ -618,7 +722,6 @@ template <typename F> void by_rank(int rank, F&& f) {
   using std::integral_constant;
   if (rank <= 16) f(integral_constant<int, 1>{}, std::true_type{});
   else if (rank <= 32) f(integral_constant<int, 1>{}, std::false_type{});
-  else if (rank <= 48) f(integral_constant<int, 2>{}, std::true_type{});
   else if (rank <= 64) f(integral_constant<int, 2>{}, std::false_type{});
   else if (rank <= 96) f(integral_constant<int, 3>{}, std::false_type{});
   else f(integral_constant<int, 4>{}, std::false_type{});
@@ -646,6 +749,7 @@ template <typename XT> void launch_lora(LoraArgs& g, hipStream_t st) {
   const bool vec_k = g.k % 8 == 0 && aligned(g.x, g.ldx) && aligned(g.a, 0);
   bool vec_n = g.rank % 8 == 0 && aligned(g.b, 0) && aligned(g.base, g.ldb) && aligned(g.out, g.ldo);
   for (int p = 0; p < g.parts.count; ++p) vec_n = vec_n && g.parts.end[p] % 8 == 0;
+  vec_n = vec_n && (int64_t)g.n * g.rank < (1 << 30);  // a slot's B by 32-bit offsets
   const int chunks = cut_columns(g.parts, kLoraFusedCols);
   if (lora_one_launch(g.plan, g.m, g.k, g.rank, g.slots, chunks)) {
     by_rank(g.rank, [&](auto nb, auto pack) {
@@ -658,19 +762,29 @@ template <typename XT> void launch_lora(LoraArgs& g, hipStream_t st) {
     return;
   }
   const int64_t tiles = g.plan ? plan_max_tiles(g.m, g.slots) : g.m;
-  const int n = std::min((g.rows_a + 15) / 16, kLoraAtiles), blocks = (g.rows_a + 16 * n - 1) / (16 * n);
   by_bool(g.plan, [&](auto plan) {
-    by_bool(vec_k, [&](auto v) {
-      const dim3 grid(blocks * g.splits, grid_y(plan.value ? 4 * tiles : tiles)), block(64 * kDownWaves);
-      if (n == 1) qtts::launch(&lora_down_kernel<XT, 1, v.value, plan.value>, grid, block, 0, st, g);
-      else if (n == 2) qtts::launch(&lora_down_kernel<XT, 2, v.value, plan.value>, grid, block, 0, st, g);
-      else if (n == 3) qtts::launch(&lora_down_kernel<XT, 3, v.value, plan.value>, grid, block, 0, st, g);
-      else qtts::launch(&lora_down_kernel<XT, 4, v.value, plan.value>, grid, block, 0, st, g);
+    by_bool(g.rank <= 16, [&](auto pack) {
+      by_bool(vec_k, [&](auto v) {
+        const int a_tiles = g.parts.count * g.blocks * kBlockTiles<pack.value>;
+        auto down = [&](auto n) {
+          qtts::launch(&lora_down_kernel<XT, n.value, pack.value, v.value, plan.value>,
+                       dim3((a_tiles + n.value - 1) / n.value, grid_y(plan.value ? 4 * tiles : tiles)), dim3(64 * kDownWaves), 0,
+                       st, g);
+        };
+        using std::integral_constant;
+        if constexpr (pack.value) {
+          if (a_tiles == 1) return down(integral_constant<int, 1>{});
+          if (a_tiles == 3) return down(integral_constant<int, 3>{});
+        }
+        if (a_tiles == 2) down(integral_constant<int, 2>{});
+        else down(integral_constant<int, 4>{});
+      });
     });
-    const int up_chunks = cut_columns(g.parts, kLoraUpCols);
+    g.up_cols = lora_up_cols(g.m, g.n);
+    const int up_chunks = cut_columns(g.parts, g.up_cols);
     by_rank(g.rank, [&](auto nb, auto pack) {
       by_bool(vec_n, [&](auto v) {
-        qtts::launch(&lora_up_kernel<XT, nb.value, pack.value, v.value, plan.value>, dim3(up_chunks, grid_y(plan.value ? kPlanTile / 16 / kUpGroups * tiles : tiles)),
+        qtts::launch(&lora_up_kernel<XT, nb.value, pack.value, v.value, plan.value>, dim3(up_chunks, grid_y(tiles)),
                      dim3(64 * kUpWaves), 0, st, g);
       });
     });
@@ -679,24 +793,24 @@ template <typename XT> void launch_lora(LoraArgs& g, hipStream_t st) {
 
 }  // namespace
 
-int64_t qtts_lora_ws_bytes(int64_t m, int64_t rows_a, int64_t k) {
-  return kCounterBytes + align256(lora_splits(m, rows_a, k) * m * lora_t_stride(rows_a) * 4);
+// The workspace: t's blocks, row by row, then fp16's exponents.
+static int64_t lora_t_bytes(int64_t m, int64_t parts, int64_t rank) { return align256(m * parts * lora_blocks(rank) * (rank <= 16 ? 64 : 128)); }
+
+int64_t qtts_lora_ws_bytes(int64_t m, int64_t parts, int64_t rank) {
+  return kCounterBytes + lora_t_bytes(m, parts, rank) + align256(m * parts * lora_blocks(rank) * 4);
 }
 
-int64_t qtts_lora_plan_words(int64_t m, int64_t slots) { return slots <= kPlanMaxSlots ? plan_words(m, slots) : 0; }
-
 int qtts_launch_lora_plan(const int32_t* index, int64_t m, int64_t slots, int32_t* plan, hipStream_t st) {
-  const uint32_t shmem = (uint32_t)((kPlanWaves + 3) * (slots + 1) * 4);
+  const uint32_t shmem = (uint32_t)((kPlanWaves + 2) * (slots + 1) * 4);
   qtts::launch(&lora_plan_kernel, dim3(1), dim3(kPlanThreads), shmem, st, index, m, slots, plan);
   return qtts_check_launch("lora_plan");
 }
 
 int qtts_launch_lora_add(const LoraArgs& args, int x_dtype, void* ws, hipStream_t st) {
   LoraArgs g = args;
-  g.t = (float*)((char*)ws + kCounterBytes);
-  g.rows_a = g.parts.count * g.rank;
-  g.t_stride = (int)lora_t_stride(g.rows_a);
-  g.splits = lora_splits(g.m, g.rows_a, g.k);
+  g.t = (uint8_t*)ws + kCounterBytes;
+  g.exps = (int32_t*)(g.t + lora_t_bytes(g.m, g.parts.count, g.rank));
+  g.blocks = lora_blocks(g.rank);
   if (x_dtype == QTTS_BF16) launch_lora<bf16_t>(g, st);
   else launch_lora<f16_t>(g, st);
   return qtts_check_launch("lora_add");

@@ -8,7 +8,6 @@ CPU or eager-PyTorch fallback: a missing library or an unsupported device raises
 
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import functools
 import threading
@@ -827,19 +826,34 @@ def w8a16_gate_up_silu_strips(x: torch.Tensor, qs: torch.Tensor, n: int, scale: 
 # ---- 8-bit activations from their producers ------------------------------------------------
 
 _CODE_DTYPES = {CODE_INT8: torch.int8, CODE_E4M3: torch.float8_e4m3fn}
-_NO_GUARD = contextlib.nullcontext()
 
 
-def _on(dev: torch.device):
-    """``dev`` made the current device for a launch on it (nothing to do where it is)."""
-    return _NO_GUARD if dev.index == torch._C._cuda_getDevice() else torch.cuda.device(dev)
+def _gpu_index(first: torch.Tensor, *others: torch.Tensor | None) -> int:
+    """The index of the GPU that all of these are on (what _require_cuda checks, at a third of its time)."""
+    idx = first.get_device()
+    if idx < 0:
+        _require_cuda(first)
+    for t in others:
+        if t is not None and t.get_device() != idx:
+            _require_cuda(first, t)
+    return idx
 
 
-def _codes_out(rows: int, k: int, codes: int, dev: torch.device) -> tuple[torch.Tensor, torch.Tensor]:
+def _call(idx: int, fn, *args) -> int:
+    """``fn(*args)`` with GPU ``idx`` current."""
+    if idx == torch._C._cuda_getDevice():
+        return fn(*args)
+    with torch.cuda.device(idx):
+        return fn(*args)
+
+
+def _codes_out(a: torch.Tensor, k: int, codes: int) -> tuple[torch.Tensor, torch.Tensor]:
+    """Room for the codes of ``a``'s rows, ``k`` a row, and their scales."""
     dtype = _CODE_DTYPES.get(codes)
     if dtype is None:
         raise ValueError(f"codes must be CODE_INT8 or CODE_E4M3, got {codes}")
-    return torch.empty((rows, k), dtype=dtype, device=dev), torch.empty(rows, dtype=torch.float32, device=dev)
+    m, dev = a.shape[0], a.device
+    return torch.empty(m, k, dtype=dtype, device=dev), torch.empty(m, dtype=torch.float32, device=dev)
 
 
 def rms_norm_quant(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual: torch.Tensor | None = None,
@@ -853,25 +867,26 @@ def rms_norm_quant(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, res
     :func:`w8a8_fp8_gemm_strips` / :func:`w8a8_int8_gemm_strips`."""
     a = _flatten(x)
     rows, k = a.shape
+    dtype = a.dtype
     if weight.numel() != k:
         raise ValueError(f"norm weight has {weight.numel()} entries for rows of {k}")
     res = None
     if residual is not None:
-        if residual.shape != x.shape or residual.dtype != x.dtype:
+        if residual.shape != x.shape or residual.dtype != dtype:
             raise ValueError(f"residual must be {tuple(x.shape)} {x.dtype}, got {tuple(residual.shape)} {residual.dtype}")
         res = _flatten(residual)
-    dev = _require_cuda(a, weight, res)
-    dtype = a.dtype
+    idx = _gpu_index(a, weight, res)
     w = weight if weight.dtype == dtype and weight.is_contiguous() else weight.to(dtype).contiguous()
-    qx, sx = _codes_out(rows, k, codes, dev)
-    hidden = None if res is None else torch.empty((rows, k), dtype=dtype, device=dev)
-    normed = torch.empty((rows, k), dtype=dtype, device=dev) if want_normed else None
-    with _on(dev):
-        st = _lib.load().qtts_rms_norm_quant(
-            a.data_ptr(), dtype_code(dtype), rows, k, a.stride(0) if rows > 1 else k, _ptr(res),
-            res.stride(0) if res is not None and rows > 1 else k, w.data_ptr(), eps, codes, qx.data_ptr(), sx.data_ptr(),
-            _ptr(hidden), k, _ptr(normed), k, _stream(dev))
-    _lib.check(st, "rms_norm_quant")
+    code = dtype_code(dtype)
+    qx, sx = _codes_out(a, k, codes)
+    hidden = None if res is None else torch.empty(rows, k, dtype=dtype, device=a.device)
+    normed = torch.empty(rows, k, dtype=dtype, device=a.device) if want_normed else None
+    st = _call(idx, _lib.load().qtts_rms_norm_quant, a.data_ptr(), code, rows, k, a.stride(0) if rows > 1 else k,
+               None if res is None else res.data_ptr(), res.stride(0) if res is not None and rows > 1 else k, w.data_ptr(),
+               eps, codes, qx.data_ptr(), sx.data_ptr(), None if hidden is None else hidden.data_ptr(), k,
+               None if normed is None else normed.data_ptr(), k, torch._C._cuda_getCurrentRawStream(idx))
+    if st:
+        _lib.check(st, "rms_norm_quant")
     if x.dim() != 2:
         hidden = None if hidden is None else hidden.view(x.shape)
         normed = None if normed is None else normed.view(x.shape)
@@ -885,14 +900,14 @@ def silu_mul_quant(gate_up: torch.Tensor, codes: int = CODE_E4M3, want_act: bool
     shape = gate_up.shape
     a = _gate_up_rows(gate_up)
     rows, k = a.shape[0], a.shape[1] // 2
-    dev = _require_cuda(a)
-    qx, sx = _codes_out(rows, k, codes, dev)
-    act = torch.empty((rows, k), dtype=a.dtype, device=dev) if want_act else None
-    with _on(dev):
-        st = _lib.load().qtts_silu_mul_quant(a.data_ptr(), dtype_code(a.dtype), rows, k,
-                                             a.stride(0) if rows > 1 else 2 * k, codes, qx.data_ptr(), sx.data_ptr(),
-                                             _ptr(act), k, _stream(dev))
-    _lib.check(st, "silu_mul_quant")
+    idx, code = _gpu_index(a), dtype_code(a.dtype)
+    qx, sx = _codes_out(a, k, codes)
+    act = torch.empty(rows, k, dtype=a.dtype, device=a.device) if want_act else None
+    st = _call(idx, _lib.load().qtts_silu_mul_quant, a.data_ptr(), code, rows, k, a.stride(0) if rows > 1 else 2 * k, codes,
+               qx.data_ptr(), sx.data_ptr(), None if act is None else act.data_ptr(), k,
+               torch._C._cuda_getCurrentRawStream(idx))
+    if st:
+        _lib.check(st, "silu_mul_quant")
     return qx, sx, act if act is None else _shaped(act, shape)
 
 
@@ -920,29 +935,36 @@ def lora_batch(index: torch.Tensor, slots: int) -> LoraBatch:
         raise ValueError(f"index must be a contiguous 1-D int32 tensor, got {index.dtype} {tuple(index.shape)}")
     if slots < 0:
         raise ValueError(f"slots is negative: {slots}")
-    dev = _require_cuda(index)
+    idx = _gpu_index(index)
     m, lib = index.shape[0], _lib.load()
     need = lib.qtts_lora_plan_bytes(m, slots) if m > LORA_WINDOW else 0
     if need < 0:
         _lib.check(int(need), "lora_plan")
     if not need:
         return LoraBatch(index, int(slots))
-    plan = torch.empty(need // 4, dtype=torch.int32, device=dev)
-    with _on(dev):
-        st = lib.qtts_lora_plan(index.data_ptr(), m, slots, plan.data_ptr(), need, _stream(dev))
-    _lib.check(st, "lora_plan")
+    plan = torch.empty(need // 4, dtype=torch.int32, device=index.device)
+    st = _call(idx, lib.qtts_lora_plan, index.data_ptr(), m, slots, plan.data_ptr(), need,
+               torch._C._cuda_getCurrentRawStream(idx))
+    if st:
+        _lib.check(st, "lora_plan")
     return LoraBatch(index, int(slots), plan)
 
 
-@functools.lru_cache(maxsize=256)
-def _part_ends(partitions: tuple[int, ...]):
+@functools.lru_cache(maxsize=1024)
+def _lora_sizes(m: int, k: int, n: int, slots: int, a: torch.Size, b: torch.Size, partitions: tuple[int, ...]):
+    """The partitions' ends, their count, the rank and the workspace bytes of a call, a function of its sizes alone."""
     ends, at = [], 0
     for size in partitions:
         if size < 0:
             raise ValueError(f"partition of {size} columns")
         at += size
         ends.append(at)
-    return (ctypes.c_int64 * len(ends))(*ends), at
+    if len(a) != 3 or len(b) != 3 or at != n or a != (slots, len(ends) * b[2], k) or b != (slots, n, b[2]):
+        raise ValueError(f"a {tuple(a)} and b {tuple(b)} do not fit {slots} adapters of a [{n}, {k}] linear with "
+                         f"{len(ends)} partitions of {at} columns in all")
+    if len(ends) > LORA_MAX_PARTS or not 1 <= b[2] <= LORA_MAX_RANK:
+        raise ValueError(f"{len(ends)} partitions of rank {b[2]}: at most {LORA_MAX_PARTS}, of rank 1 to {LORA_MAX_RANK}")
+    return (ctypes.c_int64 * len(ends))(*ends), len(ends), b[2], workspace_bytes(OP_LORA, m, len(ends), b[2])
 
 
 def lora_add(base: torch.Tensor, x: torch.Tensor, batch: LoraBatch, a: torch.Tensor, b: torch.Tensor,
@@ -956,38 +978,37 @@ def lora_add(base: torch.Tensor, x: torch.Tensor, batch: LoraBatch, a: torch.Ten
     Rows without an adapter are base.  Returns a fresh tensor in base's shape, or ``out`` (which may be base)."""
     xr, br = _flatten(x), _flatten(base)
     m, k = xr.shape
-    n, dtype = br.shape[1], xr.dtype
+    n, dtype, slots = br.shape[1], xr.dtype, batch.slots
     if br.shape[0] != m or batch.rows != m:
         raise ValueError(f"x has {m} rows, base {br.shape[0]} and the index {batch.rows}")
     if br.dtype != dtype or a.dtype != dtype or b.dtype != dtype:
         raise ValueError(f"x, base, a and b must have one dtype, got {dtype}, {br.dtype}, {a.dtype} and {b.dtype}")
-    if a.dim() != 3 or b.dim() != 3 or not a.is_contiguous() or not b.is_contiguous():
+    if not a.is_contiguous() or not b.is_contiguous():
         raise ValueError("a and b must be contiguous [S, P * R, K] and [S, N, R] tensors")
-    ends, width = _part_ends((n,) if partitions is None else tuple(partitions))
-    rank = b.shape[2]
-    if width != n or a.shape != (batch.slots, len(ends) * rank, k) or b.shape != (batch.slots, n, rank):
-        raise ValueError(f"a {tuple(a.shape)} and b {tuple(b.shape)} do not fit {batch.slots} adapters of a [{n}, {k}] "
-                         f"linear with {len(ends)} partitions of {width} columns in all")
-    if scaling.numel() != batch.slots or scaling.dtype != torch.float32 or not scaling.is_contiguous():
-        raise ValueError(f"scaling must be {batch.slots} contiguous fp32 entries")
-    if ranks is not None and (ranks.numel() != batch.slots or ranks.dtype != torch.int32 or not ranks.is_contiguous()):
-        raise ValueError(f"ranks must be {batch.slots} contiguous int32 entries")
-    dev = _require_cuda(xr, br, a, b, scaling, ranks, batch.index)
+    ends, parts, rank, need = _lora_sizes(m, k, n, slots, a.shape, b.shape, (n,) if partitions is None else tuple(partitions))
+    if scaling.numel() != slots or scaling.dtype != torch.float32 or not scaling.is_contiguous():
+        raise ValueError(f"scaling must be {slots} contiguous fp32 entries")
+    if ranks is not None and (ranks.numel() != slots or ranks.dtype != torch.int32 or not ranks.is_contiguous()):
+        raise ValueError(f"ranks must be {slots} contiguous int32 entries")
+    idx, code = _gpu_index(xr, br, a, b, scaling, ranks, batch.index), dtype_code(dtype)
     if out is None:
-        y = torch.empty((m, n), dtype=dtype, device=dev)
+        y, ldy = torch.empty(m, n, dtype=dtype, device=xr.device), n
     else:
         y = _flatten(out)
-        if y.shape != (m, n) or y.dtype != dtype or y.device != dev or y.data_ptr() != out.data_ptr():
-            raise ValueError(f"out must be a [{m}, {n}] {dtype} tensor on {dev}")
-    _ensure_workspace(dev, workspace_bytes(OP_LORA, m, a.shape[1], k), "lora_add")
-    ws, ws_n = _ws_for(dev)
-    with _on(dev):
-        st = _lib.load().qtts_lora_add(
-            xr.data_ptr(), dtype_code(dtype), m, k, xr.stride(0) if m > 1 else k, batch.index.data_ptr(), _ptr(batch.plan),
-            batch.slots, a.data_ptr(), b.data_ptr(), rank, _ptr(ranks), scaling.data_ptr(), ends, len(ends),
-            br.data_ptr(), br.stride(0) if m > 1 else n, y.data_ptr(), n, y.stride(0) if m > 1 else n, ws, ws_n,
-            _stream(dev))
-    _lib.check(st, "lora_add")
+        if y.shape != (m, n) or y.dtype != dtype or y.get_device() != idx or y.data_ptr() != out.data_ptr():
+            raise ValueError(f"out must be a [{m}, {n}] {dtype} tensor on {xr.device}")
+        ldy = y.stride(0) if m > 1 else n
+    ws = _workspaces.get(idx)
+    if ws is None or ws.numel() < need:
+        _ensure_workspace(xr.device, need, "lora_add")
+        ws = _workspaces[idx]
+    st = _call(idx, _lib.load().qtts_lora_add, xr.data_ptr(), code, m, k, xr.stride(0) if m > 1 else k,
+               batch.index.data_ptr(), None if batch.plan is None else batch.plan.data_ptr(), slots, a.data_ptr(),
+               b.data_ptr(), rank, None if ranks is None else ranks.data_ptr(), scaling.data_ptr(), ends, parts,
+               br.data_ptr(), br.stride(0) if m > 1 else n, y.data_ptr(), n, ldy, ws.data_ptr(), ws.numel(),
+               torch._C._cuda_getCurrentRawStream(idx))
+    if st:
+        _lib.check(st, "lora_add")
     if out is not None:
         return out
     return y if base.dim() == 2 else y.view(base.shape)
