@@ -33,6 +33,8 @@ struct LoraArgs {
   int32_t* exps;  // [m, parts.count, blocks], fp16
   int64_t m;
   int k, n, slots, rank, blocks, up_cols;
+  int ordinal;     // without a plan: workgroups by group, not by row
+  int64_t groups;  // and how many
   LoraParts parts;
 };
 

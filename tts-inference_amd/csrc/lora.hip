@@ -57,23 +57,44 @@ struct Group {
   int64_t row;  // the row of lane % 16 (of the first one past count)
 };
 
-// The group that row `at` leads among its window of 64 rows: rows of its slot, in steps of 16; count 0 for a row that
-// another one leads.  A row without an adapter is a group by itself.
+// The group of workgroup row `at`, without a plan; count 0 for none.  Up to 64 rows with fewer adapters (g.ordinal) it is the
+// at-th of the groups in the order of their first rows; otherwise the group that row `at` leads among its window of 64 rows,
+// every 16th of its slot.
 __device__ __forceinline__ Group group_by_ballot(const LoraArgs& g, int64_t at) {
-  const int lane = threadIdx.x & 63, here = (int)(at & 63);
-  const int64_t first = at - here;
-  int s = first + lane < g.m ? g.index[first + lane] : -1;
+  const int lane = threadIdx.x & 63;
+  const int64_t window = g.ordinal ? 0 : at & ~(int64_t)63;
+  const bool in = window + lane < g.m;
+  int s = in ? g.index[window + lane] : -1;
   if (s < 0 || s >= g.slots) s = -1;
-  const int slot = __builtin_amdgcn_readlane(s, here);
-  if (slot < 0) return {-1, 1, at};
-  const uint64_t same = __ballot(s == slot), below = (1ull << lane) - 1;
-  const int before = __popcll(same & ((1ull << here) - 1)), total = __popcll(same);
-  if (before % 16) return {slot, 0, at};
+  uint64_t same;
+  int slot, before = 0, total;
+  if (g.ordinal) {
+    uint64_t left = __ballot(in);
+    for (int ahead = (int)at;;) {
+      if (!left) return {-1, 0, 0};
+      slot = __builtin_amdgcn_readlane(s, __builtin_ctzll(left));
+      same = __ballot(in && s == slot), total = __popcll(same);
+      const int groups = (total + 15) >> 4;
+      if (ahead < groups) {
+        before = 16 * ahead;
+        break;
+      }
+      ahead -= groups;
+      left &= ~same;
+    }
+  } else {
+    const int here = (int)(at & 63);
+    slot = __builtin_amdgcn_readlane(s, here);
+    same = __ballot(in && s == slot), total = __popcll(same);
+    before = __popcll(same & ((1ull << here) - 1));
+    if (before % 16) return {slot, 0, 0};
+  }
   // lane i of the window to lane `rank of i among the slot's rows` (the others past them): one permutation
-  const int to = s == slot ? __popcll(same & below) : total + __popcll(~same & below);
+  const uint64_t below = (1ull << lane) - 1;
+  const int to = same >> lane & 1 ? __popcll(same & below) : total + __popcll(~same & below);
   const int order = __builtin_amdgcn_ds_permute(4 * to, lane);
   const int count = min(16, total - before), j = lane & 15;
-  return {slot, count, first + __builtin_amdgcn_ds_bpermute(4 * (before + (j < count ? j : 0)), order)};
+  return {slot, count, window + __builtin_amdgcn_ds_bpermute(4 * (before + (j < count ? j : 0)), order)};
 }
 
 // The rows of a tile, wherever the plan was made.
@@ -266,7 +287,7 @@ __global__ __launch_bounds__(64 * kDownWaves) void lora_down_kernel(LoraArgs g) 
   __shared__ __align__(1024) uint8_t stages[kDownWaves][kPitch];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int per_part = T * g.blocks, tile0 = blockIdx.x * N;  // tiles of a partition; the workgroup's first
-  const int64_t groups = PLAN ? 4 * plan_max_tiles(g.m, g.slots) : g.m;
+  const int64_t groups = PLAN ? 4 * plan_max_tiles(g.m, g.slots) : g.groups;
   const Ranks ranks(g);
   const int steps = (g.k + 31) >> 5, per = ((steps + kDownWaves - 1) / kDownWaves + 1) & ~1;
   const int s0 = min(wave * per, (steps + 1) & ~1), s1 = min(s0 + per, steps);
@@ -496,18 +517,14 @@ constexpr int kUpWaves = 4, kUpTiles = 4, kUpBlock = 16 * kUpTiles;
 
 // Grid: (blocks of g.up_cols columns, groups or the plan's tiles).  A tile of the plan is up to four groups of one slot: a wave
 // takes a whole group, or with fewer than four of them a part of a group's columns, 64 at a time.
-#ifndef LBA
-#define LBA 1
-#define LBB 1
-#endif
 template <typename XT, int NB, bool PACK, bool VEC, bool PLAN>
-__global__ __launch_bounds__(64 * kUpWaves, !VEC || NB > 2 ? 1 : NB == 1 ? LBA : LBB) void lora_up_kernel(LoraArgs g) {
+__global__ __launch_bounds__(64 * kUpWaves) void lora_up_kernel(LoraArgs g) {
   typedef Rows<XT, kUpTiles, VEC> R;
   __shared__ __align__(16) float lds[kUpWaves][R::kFloats];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const Block blk = block_of(g, blockIdx.x, g.up_cols);
   const Ranks ranks(g);
-  const int64_t groups = PLAN ? plan_max_tiles(g.m, g.slots) : g.m;
+  const int64_t groups = PLAN ? plan_max_tiles(g.m, g.slots) : g.groups;
   const int blocks = g.up_cols / kUpBlock;
   for (int64_t at = blockIdx.y; at < groups; at += gridDim.y) {
     int parts = kUpWaves;  // waves a group
@@ -573,7 +590,7 @@ __global__ __launch_bounds__(64 * kOneWaves) void lora_one_kernel(LoraArgs g) {
   const Ranks ranks(g);
   const int steps = (g.k + 31) >> 5, per = ((steps + kOneWaves - 1) / kOneWaves + 1) & ~1;
   const int s0 = min(wave * per, (steps + 1) & ~1), s1 = min(s0 + per, steps);
-  for (int64_t at = blockIdx.y; at < g.m; at += gridDim.y) {
+  for (int64_t at = blockIdx.y; at < g.groups; at += gridDim.y) {
     const Group gr = group_by_ballot(g, at);
     if (!gr.count) continue;
     const int live = ranks.of(g, gr.slot);
@@ -751,17 +768,19 @@ template <typename XT> void launch_lora(LoraArgs& g, hipStream_t st) {
   for (int p = 0; p < g.parts.count; ++p) vec_n = vec_n && g.parts.end[p] % 8 == 0;
   vec_n = vec_n && (int64_t)g.n * g.rank < (1 << 30);  // a slot's B by 32-bit offsets
   const int chunks = cut_columns(g.parts, kLoraFusedCols);
+  const int64_t ballots = lora_groups(g.m, g.slots);
+  g.groups = ballots, g.ordinal = ballots < g.m;
   if (lora_one_launch(g.plan, g.m, g.k, g.rank, g.slots, chunks)) {
     by_rank(g.rank, [&](auto nb, auto pack) {
       if constexpr (32 * nb.value <= kLoraOneRank)
         by_bool(vec_k && vec_n, [&](auto v) {
-          qtts::launch(&lora_one_kernel<XT, nb.value, pack.value, v.value>, dim3(chunks, grid_y(g.m)), dim3(64 * kOneWaves), 0,
+          qtts::launch(&lora_one_kernel<XT, nb.value, pack.value, v.value>, dim3(chunks, grid_y(ballots)), dim3(64 * kOneWaves), 0,
                        st, g);
         });
     });
     return;
   }
-  const int64_t tiles = g.plan ? plan_max_tiles(g.m, g.slots) : g.m;
+  const int64_t tiles = g.plan ? plan_max_tiles(g.m, g.slots) : ballots;
   by_bool(g.plan, [&](auto plan) {
     by_bool(g.rank <= 16, [&](auto pack) {
       by_bool(vec_k, [&](auto v) {
