@@ -1,0 +1,208 @@
+"""Low-rank adapters on the linears' hook (qtts_amd.layers.adapters), the decoder helpers for W8A8 layers, their custom
+ops' fakes and the dispatch rules of the kernels behind them, all without a GPU."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+import torch.nn.functional as F
+from torch import nn
+from torch._subclasses.fake_tensor import FakeTensorMode
+
+from qtts_amd import AdapterRouting, attach_adapters, ops, torch_ops
+from qtts_amd.layers import GatedMLP, LinearBase, MergedLinear
+from qtts_amd.layers.adapters import AdapterMethod, LinearAdapters
+from qtts_amd.layers.decoder import add_norm_linear, add_norm_mlp
+from test_decoder_helpers import Norm
+from test_dispatch_rules import _run
+
+
+def _fill(m: nn.Module) -> nn.Module:
+    with torch.no_grad():
+        for p in m.parameters():
+            p.normal_(0, 0.05)
+    return m
+
+
+@pytest.mark.parametrize("with_residual", [False, True])
+def test_add_norm_fallbacks_are_the_composition(with_residual):
+    torch.manual_seed(1)
+    norm, lin = Norm(64), _fill(LinearBase(64, 96, bias=True))
+    x = torch.randn(3, 2, 64)
+    r = torch.randn(3, 2, 64) if with_residual else None
+    h = x if r is None else r + x
+    y, hidden = add_norm_linear(norm, lin, x, r)
+    assert torch.equal(hidden, h) and torch.equal(y, lin(norm(h)))
+    for fuse in (True, False):
+        mlp = _fill(GatedMLP(64, 128, fuse=fuse))
+        y, hidden = add_norm_mlp(norm, mlp, x, r)
+        assert torch.equal(hidden, h) and torch.equal(y, mlp(norm(h)))
+
+
+class Block(nn.Module):
+    def __init__(self) -> None:
+        super().__init__()
+        self.qkv_proj = MergedLinear(64, [32, 16, 16])
+        self.o_proj = LinearBase(32, 64)
+        self.mlp = GatedMLP(64, 128)
+
+
+def test_attach_finds_the_named_linears_and_their_partitions():
+    block = _fill(Block())
+    routing = AdapterRouting(4, 32, device="cpu")
+    banks = attach_adapters(block, slots=4, rank=12, routing=routing, targets=("qkv", "down"))
+    assert sorted(banks) == ["mlp.down_proj", "qkv_proj"]
+    q = banks["qkv_proj"]
+    assert q.lora_a.shape == (4, 3 * 16, 64) and q.lora_b.shape == (4, 64, 16) and q.rank == 16
+    assert banks["mlp.down_proj"].lora_a.shape == (4, 16, 128)
+    assert isinstance(block.qkv_proj.quant_method, AdapterMethod) and block.o_proj.quant_method is None
+    assert block.qkv_proj.quant_method.applies_to(block.qkv_proj)
+    assert not list(q.state_dict())  # adapters are loaded by slot, not from the checkpoint
+    with pytest.raises(ValueError, match="has adapters already"):
+        attach_adapters(block, slots=4, rank=12, routing=routing)
+    assert block.o_proj.quant_method is None  # refused before any layer changed
+    with pytest.raises(ValueError, match="routing has 4 slots"):
+        attach_adapters(_fill(Block()), slots=5, rank=12, routing=routing)
+    for bad in ({"slots": 0}, {"rank": 0}, {"rank": 129}):
+        kw = {"slots": 4, "rank": 8, **bad}
+        with pytest.raises(ValueError):
+            attach_adapters(_fill(Block()), routing=AdapterRouting(max(kw["slots"], 1), 8, device="cpu") if kw["slots"] else routing,
+                            **kw)
+
+
+def test_load_lays_adapters_out_by_partition():
+    bank = LinearAdapters(8, [6, 4], 3, 5, torch.float32, "cpu")
+    assert bank.rank == 8
+    a0, a1, b0, b1 = torch.randn(5, 8), torch.randn(2, 8), torch.randn(6, 5), torch.randn(4, 2)
+    bank.load(1, [a0, a1], [b0, b1], scaling=0.5)
+    assert torch.equal(bank.lora_a[1, :5], a0) and torch.equal(bank.lora_a[1, 8:10], a1)
+    assert torch.equal(bank.lora_b[1, :6, :5], b0) and torch.equal(bank.lora_b[1, 6:, :2], b1)
+    assert not bank.lora_a[1, 5:8].any() and not bank.lora_a[1, 10:].any() and not bank.lora_b[1, 6:, 2:].any()
+    assert bank.lora_ranks.tolist() == [0, 5, 0] and bank.lora_scaling.tolist() == [0.0, 0.5, 0.0]
+    bank.load(1, a1, torch.cat([b0[:, :2], b1]))  # one A and one B for the whole linear
+    assert torch.equal(bank.lora_a[1, :2], a1) and torch.equal(bank.lora_a[1, 8:10], a1) and not bank.lora_a[1, 2:8].any()
+    assert bank.lora_ranks[1] == 2 and bank.lora_scaling[1] == 1
+    bank.load(2, [None, a1], [None, b1])
+    assert not bank.lora_a[2, :8].any() and bank.lora_ranks[2] == 2
+    bank.clear(1)
+    assert not bank.lora_a[1].any() and not bank.lora_b[1].any() and bank.lora_ranks.tolist() == [0, 0, 2]
+
+
+def test_load_refusals_leave_the_slot():
+    bank = LinearAdapters(8, [6, 4], 3, 5, torch.float32, "cpu")
+    a, b0, b1 = torch.randn(5, 8), torch.randn(6, 5), torch.randn(4, 5)
+    bank.load(0, [a, a], [b0, b1])
+    kept = bank.lora_a.clone(), bank.lora_b.clone()
+    for slot, la, lb in ((3, [a, a], [b0, b1]), (-1, [a, a], [b0, b1]), (0, [a], [b0]), (0, [a, a], [b1, b0]),
+                         (0, [a, None], [b0, b1]), (0, [torch.randn(6, 8)] * 2, [torch.randn(6, 6), torch.randn(4, 6)]),
+                         (0, [a[:, :7]] * 2, [b0, b1]), (0, [a, a], [b0, b1[0]]), (0, a, b0), (0, a[0], torch.cat([b0, b1]))):
+        with pytest.raises(ValueError):
+            bank.load(slot, la, lb)
+    assert torch.equal(bank.lora_a, kept[0]) and torch.equal(bank.lora_b, kept[1])
+
+
+def test_routing_refusals():
+    for bad in ((0, 8), (4, 0)):
+        with pytest.raises(ValueError):
+            AdapterRouting(*bad, device="cpu")
+    routing = AdapterRouting(4, 8, device="cpu")
+    for index, rows in (([0] * 9, None), ([0, 1], 1), ([0, 1], 9), ([[0, 1]], None)):
+        with pytest.raises(ValueError):
+            routing.set(index, rows)
+    if not torch.cuda.is_available():
+        with pytest.raises(ValueError):  # the kernels need a GPU, and no batch stands after a failed set
+            routing.set([0, 1])
+    assert routing.batch is None
+    layer = _fill(LinearBase(64, 32))
+    attach_adapters(layer, slots=4, rank=8, routing=routing)
+    with pytest.raises(ValueError, match="set for no rows, the call has 3"):
+        layer(torch.randn(3, 64))
+
+
+def test_fakes():
+    bf = torch.bfloat16
+    assert {"rms_norm_quant", "silu_mul_quant", "lora_add"} <= set(torch_ops.OPS)
+    with FakeTensorMode():
+        x = torch.empty(3, 5, 1024, dtype=bf, device="cuda")
+        w = torch.empty(1024, dtype=bf, device="cuda")
+        q = torch.ops.qtts
+        for codes, dtype in ((ops.CODE_E4M3, torch.float8_e4m3fn), (ops.CODE_INT8, torch.int8)):
+            for res, want in ((x, True), (None, False)):
+                qx, sx, hidden, normed = q.rms_norm_quant(x, w, 1e-6, res, codes, want)
+                assert qx.shape == (15, 1024) and qx.dtype == dtype and sx.shape == (15,) and sx.dtype == torch.float32
+                assert hidden.shape == (x.shape if want else (0,)) == normed.shape and normed.dtype == bf
+                qx, sx, act = q.silu_mul_quant(x, codes, want)
+                assert qx.shape == (15, 512) and qx.dtype == dtype and sx.shape == (15,)
+                assert act.shape == ((3, 5, 512) if want else (0,)) and act.dtype == bf
+        sw = torch.empty(96, device="cuda")
+        bias = torch.empty(96, dtype=bf, device="cuda")
+        ws = torch.empty(96 * 512, dtype=torch.int8, device="cuda")
+        for gemm in (q.w8a8_fp8_gemm_strips, q.w8a8_int8_gemm_strips):
+            y = gemm(qx, sx, ws, 96, sw, bias, torch.float16, 0)
+            assert y.shape == (15, 96) and y.dtype == torch.float16
+        base = torch.empty(3, 5, 96, dtype=bf, device="cuda")
+        index = torch.empty(15, dtype=torch.int32, device="cuda")
+        y = q.lora_add(base, x, index, None, 4, torch.empty(4, 16, 1024, dtype=bf, device="cuda"),
+                       torch.empty(4, 96, 16, dtype=bf, device="cuda"), torch.empty(4, device="cuda"), None, [96])
+        assert y.shape == base.shape and y.dtype == bf
+
+
+def test_row_forms_hold_the_row(tmp_path):
+    """Rows of 8-bit codes: in registers up to 8192 columns, and a grid whose threads fit 32 bits; read twice past that."""
+    rows = _run(tmp_path, """
+#include <stdio.h>
+#include "quant_rows_rule.h"
+int main() {
+  const long long ms[] = {1, 1003, 1 << 22, (1 << 22) + 1, 1 << 25};
+  for (long long m : ms) {
+    for (long long k = 0; k <= 8300; ++k) { auto f = qtts::row_form(m, k); printf("%lld %lld %d %d\\n", m, k, f.threads, f.vectors); }
+    auto f = qtts::row_form(m, 1 << 20); printf("%lld %d %d %d\\n", m, 1 << 20, f.threads, f.vectors);
+  }
+}
+""")
+    assert len(rows) == 5 * 8302
+    forms = set()
+    for m, k, threads, vectors in rows:
+        if 0 < k <= 8192 and m <= 1 << 22:
+            assert threads * vectors * 8 >= k and threads * m < 1 << 32, (m, k)
+            forms.add((threads, vectors))
+        else:
+            assert threads == 0, (m, k)
+    assert forms == {(64, 1), (128, 1), (256, 1), (256, 2), (256, 3), (256, 4)}  # the kernels that are built
+
+
+def test_adapter_launches_cover_their_work(tmp_path):
+    """Every rank has its blocks, every group of rows a workgroup, and one launch is taken only where it is allowed."""
+    rows = _run(tmp_path, """
+#include <stdio.h>
+#include "lora_rule.h"
+using namespace qtts;
+int main() {
+  for (int rank = 1; rank <= 128; ++rank) printf("0 %d %d\\n", rank, lora_blocks(rank));
+  for (int m = 1; m <= 64; ++m)
+    for (int slots = 0; slots <= 80; ++slots) printf("1 %d %d %lld\\n", m, slots, (long long)lora_groups(m, slots));
+  const int ms[] = {1, 5, 64, 65, 1003, 2048, 8192, 1 << 20}, ns[] = {1, 64, 256, 2048, 4096, 12288};
+  for (int m : ms) for (int n : ns) printf("2 %d %d %d\\n", m, n, lora_up_cols(m, n));
+  for (int rank = 1; rank <= 128; ++rank)
+    for (int chunks = 1; chunks <= 48; ++chunks)
+      for (int m = 1; m <= 64; m += 7)
+        printf("3 %d %d %d %d %d\\n", rank, chunks, m, (int)lora_one_launch(false, m, 2048, rank, 8, chunks),
+               (int)lora_one_launch(true, m, 2048, rank, 8, chunks));
+}
+""")
+    one = two = 0
+    for kind, *v in rows:
+        if kind == 0:
+            rank, blocks = v
+            assert blocks * (16 if rank <= 16 else 32) >= rank and blocks <= 4
+        elif kind == 1:
+            m, slots, groups = v
+            # the rows of at most slots adapters and of none, in groups of up to 16, fit the workgroups
+            assert groups >= min(m, min(m, slots + 1) + m // 16) or groups == m, (m, slots)
+        elif kind == 2:
+            assert v[2] in (64, 128, 256)
+        else:
+            rank, chunks, m, free, plan = v
+            assert not plan and (not free or rank <= 64)
+            one, two = one + free, two + (not free)
+    assert one and two

@@ -9,6 +9,7 @@ from . import ops, torch_ops  # torch_ops registers torch.ops.qtts.*
 from .config import QuantConfig
 from .layers.linear import LinearBase, MergedLinear, iter_linears
 from .quant import apply_quantization, build_method, fp8_supported, quantize_module
+from .layers.adapters import AdapterRouting, attach_adapters  # after quant, which the layers' modules import
 
 __all__ = ["ops", "torch_ops", "QuantConfig", "LinearBase", "MergedLinear", "iter_linears", "apply_quantization",
-           "build_method", "fp8_supported", "quantize_module"]
+           "build_method", "fp8_supported", "quantize_module", "AdapterRouting", "attach_adapters"]

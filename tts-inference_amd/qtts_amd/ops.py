@@ -929,21 +929,37 @@ class LoraBatch:
         self.index, self.slots, self.rows, self.plan = index, slots, index.shape[0], plan
 
 
-def lora_batch(index: torch.Tensor, slots: int) -> LoraBatch:
-    """The rows' adapter slots, ready for :func:`lora_add`: one kernel past :data:`LORA_WINDOW` rows, else none."""
+def _plan_bytes(m: int, slots: int) -> int:
+    """Bytes of the plan of m rows, grows with m; 0 where a call takes none."""
+    need = _lib.load().qtts_lora_plan_bytes(m, slots) if m > LORA_WINDOW else 0
+    if need < 0:
+        _lib.check(int(need), "lora_plan")
+    return need
+
+
+def lora_plan_buffer(max_rows: int, slots: int, device: torch.device) -> torch.Tensor:
+    """A buffer that holds the plan of any batch of up to ``max_rows`` rows (:func:`lora_batch`)."""
+    return torch.empty(_plan_bytes(max_rows, slots) // 4, dtype=torch.int32, device=device)
+
+
+def lora_batch(index: torch.Tensor, slots: int, plan: torch.Tensor | None = None) -> LoraBatch:
+    """The rows' adapter slots, ready for :func:`lora_add`: one kernel past :data:`LORA_WINDOW` rows, else none.
+    ``plan``: a :func:`lora_plan_buffer` to write the plan into (a captured graph that reads it then follows the
+    index of the last batch); a fresh tensor otherwise."""
     if index.dim() != 1 or index.dtype != torch.int32 or not index.is_contiguous():
         raise ValueError(f"index must be a contiguous 1-D int32 tensor, got {index.dtype} {tuple(index.shape)}")
     if slots < 0:
         raise ValueError(f"slots is negative: {slots}")
     idx = _gpu_index(index)
-    m, lib = index.shape[0], _lib.load()
-    need = lib.qtts_lora_plan_bytes(m, slots) if m > LORA_WINDOW else 0
-    if need < 0:
-        _lib.check(int(need), "lora_plan")
+    m = index.shape[0]
+    need = _plan_bytes(m, slots)
     if not need:
         return LoraBatch(index, int(slots))
-    plan = torch.empty(need // 4, dtype=torch.int32, device=index.device)
-    st = _call(idx, lib.qtts_lora_plan, index.data_ptr(), m, slots, plan.data_ptr(), need,
+    if plan is None:
+        plan = torch.empty(need // 4, dtype=torch.int32, device=index.device)
+    elif plan.dtype != torch.int32 or not plan.is_contiguous() or plan.numel() * 4 < need or plan.get_device() != idx:
+        raise ValueError(f"plan must hold {need // 4} contiguous int32 entries on {index.device}")
+    st = _call(idx, _lib.load().qtts_lora_plan, index.data_ptr(), m, slots, plan.data_ptr(), need,
                torch._C._cuda_getCurrentRawStream(idx))
     if st:
         _lib.check(st, "lora_plan")

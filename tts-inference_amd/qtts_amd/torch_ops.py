@@ -187,7 +187,92 @@ def _(x, qs, n, scale, bias, prologue, norm_weight, eps, algo):
     return x.new_empty(_rows_shape(x, n // 2))
 
 
+# ---- the W8A8 GEMMs on given codes, and the codes' producers --------------------------------
+
+def _reserve(op: int, qx: torch.Tensor, n: int, algo: int) -> None:
+    """Workspace for rows past what the quant method reserved at load time."""
+    rows, k = qx.shape
+    ops._ensure_workspace(qx.device, ops.workspace_bytes(op, rows, n, k, algo), "w8a8_gemm_strips")
+
+
+@torch.library.custom_op(f"{_LIB}::w8a8_fp8_gemm_strips", mutates_args=())
+def w8a8_fp8_gemm_strips(qx: torch.Tensor, sx: torch.Tensor, qws: torch.Tensor, n: int, sw: torch.Tensor,
+                         bias: Optional[torch.Tensor], out_dtype: torch.dtype, algo: int) -> torch.Tensor:
+    _reserve(ops.OP_W8A8_FP8, qx, n, algo)
+    return ops.w8a8_fp8_gemm_strips(qx, sx, qws, n, sw, bias, out_dtype, algo)
+
+
+@torch.library.custom_op(f"{_LIB}::w8a8_int8_gemm_strips", mutates_args=())
+def w8a8_int8_gemm_strips(qx: torch.Tensor, sx: torch.Tensor, qws: torch.Tensor, n: int, sw: torch.Tensor,
+                          bias: Optional[torch.Tensor], out_dtype: torch.dtype, algo: int) -> torch.Tensor:
+    _reserve(ops.OP_W8A8_INT8, qx, n, algo)
+    return ops.w8a8_int8_gemm_strips(qx, sx, qws, n, sw, bias, out_dtype, algo)
+
+
+@w8a8_fp8_gemm_strips.register_fake
+@w8a8_int8_gemm_strips.register_fake
+def _(qx, sx, qws, n, sw, bias, out_dtype, algo):
+    return qx.new_empty((qx.shape[0], n), dtype=out_dtype)
+
+
+_CODES = {ops.CODE_INT8: torch.int8, ops.CODE_E4M3: torch.float8_e4m3fn}
+
+
+def _fake_codes(x, k, codes):
+    rows = 1
+    for d in x.shape[:-1]:
+        rows = rows * d
+    return x.new_empty((rows, k), dtype=_CODES[codes]), x.new_empty((rows,), dtype=torch.float32)
+
+
+def _or_empty(t: Optional[torch.Tensor], x: torch.Tensor) -> torch.Tensor:
+    return x.new_empty(0) if t is None else t
+
+
+@torch.library.custom_op(f"{_LIB}::rms_norm_quant", mutates_args=())
+def rms_norm_quant(x: torch.Tensor, weight: torch.Tensor, eps: float, residual: Optional[torch.Tensor], codes: int,
+                   want_normed: bool) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """``ops.rms_norm_quant``; an output that was not asked for is an empty tensor."""
+    qx, sx, hidden, normed = ops.rms_norm_quant(x, weight, eps, residual, codes, want_normed)
+    return qx, sx, _or_empty(hidden, x), _or_empty(normed, x)
+
+
+@rms_norm_quant.register_fake
+def _(x, weight, eps, residual, codes, want_normed):
+    qx, sx = _fake_codes(x, x.shape[-1], codes)
+    return qx, sx, x.new_empty(x.shape if residual is not None else 0), x.new_empty(x.shape if want_normed else 0)
+
+
+@torch.library.custom_op(f"{_LIB}::silu_mul_quant", mutates_args=())
+def silu_mul_quant(gate_up: torch.Tensor, codes: int, want_act: bool) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """``ops.silu_mul_quant``; the 16-bit value is an empty tensor unless asked for."""
+    qx, sx, act = ops.silu_mul_quant(gate_up, codes, want_act)
+    return qx, sx, _or_empty(act, gate_up)
+
+
+@silu_mul_quant.register_fake
+def _(gate_up, codes, want_act):
+    k = gate_up.shape[-1] // 2
+    qx, sx = _fake_codes(gate_up, k, codes)
+    return qx, sx, gate_up.new_empty(_rows_shape(gate_up, k) if want_act else 0)
+
+
+# ---- low-rank adapters (layers/adapters.py) ---------------------------------------------------
+
+@torch.library.custom_op(f"{_LIB}::lora_add", mutates_args=())
+def lora_add(base: torch.Tensor, x: torch.Tensor, index: torch.Tensor, plan: Optional[torch.Tensor], slots: int,
+             a: torch.Tensor, b: torch.Tensor, scaling: torch.Tensor, ranks: Optional[torch.Tensor],
+             partitions: list[int]) -> torch.Tensor:
+    return ops.lora_add(base, x, ops.LoraBatch(index, slots, plan), a, b, scaling, ranks, partitions)
+
+
+@lora_add.register_fake
+def _(base, x, index, plan, slots, a, b, scaling, ranks, partitions):
+    return base.new_empty(base.shape)
+
+
 #: Every op this module registers, by name (``torch.ops.qtts.<name>``).
 OPS = ("w8a16_gemm", "w8a16_gemm_strips", "fp8_linear", "fp8_linear_strips", "int8_linear", "int8_linear_strips",
        "fp8w_gemm_strips", "dequant_linear", "rms_norm", "silu_mul", "w8a16_silu_mul_gemm_strips",
-       "w8a16_fused_gemm_strips", "w8a16_gate_up_silu_strips")
+       "w8a16_fused_gemm_strips", "w8a16_gate_up_silu_strips", "w8a8_fp8_gemm_strips", "w8a8_int8_gemm_strips",
+       "rms_norm_quant", "silu_mul_quant", "lora_add")
