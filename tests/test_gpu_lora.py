@@ -225,24 +225,24 @@ def test_graph_follows_the_index(ops, m):
 
 @pytest.mark.parametrize("m,slots", [(65, 1), (100, 3), (1000, 7), (4097, 768), (5000, 40), (70000, 500), (64 * 1024, 1)])
 def test_plan(ops, m, slots):
-    """The plan holds every row once, stably sorted by slot, in tiles of at most 64 rows of one slot."""
+    """The plan holds every row once, stably sorted by slot, in groups of at most 16 rows of one slot."""
     g = torch.Generator().manual_seed(m)
     index = torch.randint(-2, slots + 1, (m,), generator=g, dtype=torch.int32)
     plan = ops.lora_batch(index.cuda(), slots).plan.cpu()
     slot = torch.where((index < 0) | (index >= slots), slots, index)
     want = torch.argsort(slot, stable=True)
     count = int(plan[0])
-    most = (m + 63) // 64 + min(m, slots + 1)
-    tiles = plan[4:4 + 2 * count].view(-1, 2)
-    order = plan[4 + (2 * most + 3) // 4 * 4:][:64 * count].view(-1, 64)
+    most = (m + 15) // 16 + min(m, slots + 1)
+    groups = plan[4:4 + 2 * count].view(-1, 2)
+    order = plan[4 + (2 * most + 3) // 4 * 4:][:16 * count].view(-1, 16)
     assert plan[1] == m and plan[2] == slots
     at = 0
-    for (s, n), rows in zip(tiles.tolist(), order):
-        assert 0 < n <= 64 and torch.equal(rows[:n].long(), want[at:at + n])
+    for (s, n), rows in zip(groups.tolist(), order):
+        assert 0 < n <= 16 and torch.equal(rows[:n].long(), want[at:at + n])
         here = slots if s < 0 else s
         assert (slot[want[at:at + n]] == here).all()
         at += n
-        assert n == 64 or at == m or slot[want[at]] != here
+        assert n == 16 or at == m or slot[want[at]] != here
     assert at == m
 
 
@@ -257,11 +257,19 @@ def test_many_adapters(ops):
 
 def test_a_plan_of_another_batch_writes_nothing(ops):
     c = _case(100, 64, [40], 5, 16, torch.bfloat16, seed=62)
-    batch = ops.lora_batch(c["index"], 5)
-    batch.plan = ops.lora_batch(c["index"][:90].contiguous(), 5).plan
+    plan = ops.lora_plan_buffer(100, 5, c["x"].device)
+    batch = ops.lora_batch(c["index"], 5, plan)
+    ops.lora_batch(c["index"][:90].contiguous(), 5, plan)  # the buffer now holds another batch's
     out = torch.full((100, 40), 3.0, dtype=torch.bfloat16, device="cuda")
     ops.lora_add(c["base"], c["x"], batch, c["a"], c["b"], c["scaling"], c["ranks"], c["parts"], out=out)
     assert (out == 3.0).all()
+    ops.lora_batch(c["index"], 5, plan)
+    _check(ops.lora_add(c["base"], c["x"], batch, c["a"], c["b"], c["scaling"], c["ranks"], c["parts"]), c)
+    for bad in (plan[:100], plan.long(), plan.cpu(), plan[::2]):  # too short for the rows, or no plan buffer here
+        with pytest.raises(ValueError, match="plan must hold"):
+            ops.lora_batch(c["index"], 5, bad)
+        with pytest.raises(ValueError, match="plan must hold"):
+            torch.ops.qtts.lora_add(c["base"], c["x"], c["index"], bad, 5, c["a"], c["b"], c["scaling"], c["ranks"], c["parts"])
 
 
 def test_repeats_give_the_same_bits(ops):

@@ -38,21 +38,21 @@ struct LoraArgs {
   LoraParts parts;
 };
 
-// ---- the plan: rows sorted by slot, cut into tiles of one slot each ----------------------------
-// int32 words: the number of tiles, m, slots, 0; then, from word 4, two words a tile (slot, or -1 for rows without an
-// adapter; its rows, at most kPlanTile); then kPlanTile words a tile, its rows.
-constexpr int kPlanTile = 64;
+// ---- the plan: rows sorted by slot, cut into groups of one slot each ---------------------------
+// int32 words: the number of groups, m, slots, 0; then, from word 4, two words a group (slot, or -1 for rows without an
+// adapter; its rows, at most kPlanGroup); then kPlanGroup words a group, its rows.
+constexpr int kPlanGroup = 16;
 constexpr int kPlanMaxSlots = 768;  // the sort's counters are in LDS
 constexpr int64_t kPlanMaxRows = 1 << 30;  // places in int32
 
-__host__ __device__ inline int64_t plan_max_tiles(int64_t m, int64_t slots) {
-  return (m + kPlanTile - 1) / kPlanTile + (m < slots + 1 ? m : slots + 1);
+__host__ __device__ inline int64_t plan_max_groups(int64_t m, int64_t slots) {
+  return (m + kPlanGroup - 1) / kPlanGroup + (m < slots + 1 ? m : slots + 1);
 }
 __host__ __device__ inline int64_t plan_order_at(int64_t m, int64_t slots) {
-  return 4 + (2 * plan_max_tiles(m, slots) + 3) / 4 * 4;
+  return 4 + (2 * plan_max_groups(m, slots) + 3) / 4 * 4;
 }
 __host__ __device__ inline int64_t plan_words(int64_t m, int64_t slots) {
-  return plan_order_at(m, slots) + kPlanTile * plan_max_tiles(m, slots);
+  return plan_order_at(m, slots) + kPlanGroup * plan_max_groups(m, slots);
 }
 
 }  // namespace qtts

@@ -97,19 +97,16 @@ __device__ __forceinline__ Group group_by_ballot(const LoraArgs& g, int64_t at) 
   return {slot, count, window + __builtin_amdgcn_ds_bpermute(4 * (before + (j < count ? j : 0)), order)};
 }
 
-// The rows of a tile, wherever the plan was made.
-__device__ __forceinline__ int plan_tile_rows(const LoraArgs& g, int64_t tile) { return g.plan[5 + 2 * tile]; }
-
-// Sub-group `sub` (16 rows) of tile `tile` < plan_max_tiles; count 0 past its end, past the plan's tiles and where the
-// plan was made for another batch or slot count.  The three loads do not wait for one another.
-__device__ __forceinline__ Group group_by_plan(const LoraArgs& g, int64_t tile, int sub) {
+// Group `at` < plan_max_groups of the plan; count 0 past the plan's groups and where the plan was made for another batch or
+// slot count.  The three loads do not wait for one another.
+__device__ __forceinline__ Group group_by_plan(const LoraArgs& g, int64_t at) {
   const int j = threadIdx.x & 15;
   const i32x4_t head = *(const i32x4_t*)g.plan;
-  const i32x2_t e = *(const i32x2_t*)(g.plan + 4 + 2 * tile);
-  const int32_t* order = g.plan + plan_order_at(g.m, g.slots) + kPlanTile * tile + 16 * sub;
-  const int row = order[j], lead = order[0], count = min(16, e[1] - 16 * sub);
-  if (tile >= head[0] || head[1] != g.m || head[2] != g.slots || count <= 0) return {-1, 0, 0};
-  return {e[0], count, j < count ? row : lead};
+  const i32x2_t e = *(const i32x2_t*)(g.plan + 4 + 2 * at);
+  const int32_t* order = g.plan + plan_order_at(g.m, g.slots) + kPlanGroup * at;
+  const int row = order[j], lead = order[0];
+  if (at >= head[0] || head[1] != g.m || head[2] != g.slots) return {-1, 0, 0};
+  return {e[0], e[1], j < e[1] ? row : lead};
 }
 
 // The slots' ranks: the first 64 by lane, loaded beside what names the slot.
@@ -280,19 +277,18 @@ __device__ __forceinline__ void meet_waves(const uint8_t* sums, int pitch, int t
 
 constexpr int kDownWaves = 8;
 
-// Grid: (N tiles of the partitions' A each, groups or tiles x 4).  Eight waves share K.
+// Grid: (N tiles of the partitions' A each, groups).  Eight waves share K.
 template <typename XT, int N, bool PACK, bool VEC, bool PLAN>
 __global__ __launch_bounds__(64 * kDownWaves) void lora_down_kernel(LoraArgs g) {
   constexpr int T = kBlockTiles<PACK>, kPitch = VEC ? kDownBytes<N, kDownStages<N>> : 1024 * N;
   __shared__ __align__(1024) uint8_t stages[kDownWaves][kPitch];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int per_part = T * g.blocks, tile0 = blockIdx.x * N;  // tiles of a partition; the workgroup's first
-  const int64_t groups = PLAN ? 4 * plan_max_tiles(g.m, g.slots) : g.groups;
   const Ranks ranks(g);
   const int steps = (g.k + 31) >> 5, per = ((steps + kDownWaves - 1) / kDownWaves + 1) & ~1;
   const int s0 = min(wave * per, (steps + 1) & ~1), s1 = min(s0 + per, steps);
-  for (int64_t at = blockIdx.y; at < groups; at += gridDim.y) {
-    const Group gr = PLAN ? group_by_plan(g, at >> 2, (int)(at & 3)) : group_by_ballot(g, at);
+  for (int64_t at = blockIdx.y; at < g.groups; at += gridDim.y) {
+    const Group gr = PLAN ? group_by_plan(g, at) : group_by_ballot(g, at);
     if (!gr.count) continue;
     const int live = ranks.of(g, gr.slot);
     if (!live) continue;
@@ -515,8 +511,8 @@ __device__ __forceinline__ Block block_of(const LoraArgs& g, int chunk, int cols
 
 constexpr int kUpWaves = 4, kUpTiles = 4, kUpBlock = 16 * kUpTiles;
 
-// Grid: (blocks of g.up_cols columns, groups or the plan's tiles).  A tile of the plan is up to four groups of one slot: a wave
-// takes a whole group, or with fewer than four of them a part of a group's columns, 64 at a time.
+// Grid: (blocks of g.up_cols columns, groups).  A wave takes 64 columns at a time: with a plan, whose groups of one slot follow
+// one another, all columns of a group of its own; else a part of the workgroup's group.
 template <typename XT, int NB, bool PACK, bool VEC, bool PLAN>
 __global__ __launch_bounds__(64 * kUpWaves) void lora_up_kernel(LoraArgs g) {
   typedef Rows<XT, kUpTiles, VEC> R;
@@ -524,18 +520,13 @@ __global__ __launch_bounds__(64 * kUpWaves) void lora_up_kernel(LoraArgs g) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const Block blk = block_of(g, blockIdx.x, g.up_cols);
   const Ranks ranks(g);
-  const int64_t groups = PLAN ? plan_max_tiles(g.m, g.slots) : g.groups;
-  const int blocks = g.up_cols / kUpBlock;
-  for (int64_t at = blockIdx.y; at < groups; at += gridDim.y) {
-    int parts = kUpWaves;  // waves a group
-    if constexpr (PLAN) {
-      const int rows = plan_tile_rows(g, at);
-      parts = rows > 32 ? 1 : rows > 16 ? 2 : 4;
-    }
-    const Group gr = PLAN ? group_by_plan(g, at, wave / parts) : group_by_ballot(g, at);
+  constexpr int kShare = PLAN ? 1 : kUpWaves;  // waves a group
+  const int blocks = g.up_cols / kUpBlock, per = (blocks + kShare - 1) / kShare, first = wave % kShare * per;
+  const int c0 = blk.c0 + kUpBlock * first, c1 = min(blk.c0 + kUpBlock * min(first + per, blocks), blk.end);
+  for (int64_t at = PLAN ? (int64_t)blockIdx.y * kUpWaves + wave : blockIdx.y; at < g.groups;
+       at += (int64_t)gridDim.y * (PLAN ? kUpWaves : 1)) {
+    const Group gr = PLAN ? group_by_plan(g, at) : group_by_ballot(g, at);
     if (!gr.count) continue;
-    const int per = (blocks + parts - 1) / parts, first = wave % parts * per;  // the wave's blocks of 64 columns
-    const int c0 = blk.c0 + kUpBlock * first, c1 = min(blk.c0 + kUpBlock * min(first + per, blocks), blk.end);
     if (c0 >= c1) continue;
     const int live = ranks.of(g, gr.slot);
     if (!live && g.base == g.out) continue;
@@ -647,40 +638,43 @@ __global__ __launch_bounds__(64 * kOneWaves) void lora_one_kernel(LoraArgs g) {
 
 constexpr int kPlanThreads = 1024, kPlanWaves = kPlanThreads / 64;
 
-// f(slot, rows of this wave's window with it) for each slot among 64 rows (slots: the rows without an adapter).
-template <typename F> __device__ __forceinline__ void by_slot(const int32_t* index, int64_t m, int slots, int64_t first, F&& f) {
-  const int lane = threadIdx.x & 63;
-  int s = slots;
-  const bool in = first + lane < m;
-  if (in) {
-    s = index[first + lane];
-    if (s < 0 || s >= slots) s = slots;
+// 64 rows, one a lane: the lane's slot (slots: no adapter) and the lanes with the same one, found bit by bit of the slot (a
+// loop over the slots among 64 rows, of up to 64 steps that wait for LDS, took 10 us more for 300 rows of 64 adapters).
+struct Window {
+  bool in;
+  int slot;
+  uint64_t same;
+  __device__ __forceinline__ Window(const int32_t* index, int64_t m, int slots, int64_t first) {
+    const int lane = threadIdx.x & 63;
+    in = first + lane < m;
+    slot = in ? index[first + lane] : -1;
+    if (slot < 0 || slot >= slots) slot = slots;
+    same = __ballot(in);
+    for (int bit = 1; bit <= slots; bit <<= 1) {
+      const uint64_t set = __ballot((slot & bit) != 0);
+      same &= slot & bit ? set : ~set;
+    }
   }
-  uint64_t left = __ballot(in);
-  while (left) {
-    const int one = __builtin_amdgcn_readlane(s, __builtin_ctzll(left));
-    const uint64_t same = __ballot(in && s == one);
-    f(one, same);
-    left &= ~same;
-  }
-}
+  __device__ __forceinline__ int before() const { return __popcll(same & ((1ull << (threadIdx.x & 63)) - 1)); }
+  __device__ __forceinline__ bool leads() const { return in && before() == 0; }
+};
 
 // A stable counting sort by slot in one workgroup: each wave counts a run of rows, the counts become first places, slot by
 // slot and wave by wave, and the waves place their rows.
 __global__ __launch_bounds__(kPlanThreads) void lora_plan_kernel(const int32_t* __restrict__ index, int64_t m, int slots,
                                                                  int32_t* __restrict__ plan) {
-  extern __shared__ int32_t lds[];  // [kPlanWaves][slots + 1] counts, then places; [slots + 1] rows, first tiles
+  extern __shared__ int32_t lds[];  // [kPlanWaves][slots + 1] counts, then places; [slots + 1] rows, first groups
   const int n = slots + 1, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  int32_t *rows = lds + kPlanWaves * n, *first_tile = rows + n;
+  int32_t *rows = lds + kPlanWaves * n, *first_group = rows + n;
   for (int i = tid; i < kPlanWaves * n; i += kPlanThreads) lds[i] = 0;
   __syncthreads();
   const int64_t run = (m + 64 * kPlanWaves - 1) / (64 * kPlanWaves) * 64;
   const int64_t r0 = wave * run, r1 = r0 + run < m ? r0 + run : m;
   int32_t* mine = lds + wave * n;
-  for (int64_t r = r0; r < r1; r += 64)
-    by_slot(index, m, slots, r, [&](int s, uint64_t same) {
-      if (lane == 0) mine[s] += __popcll(same);
-    });
+  for (int64_t r = r0; r < r1; r += 64) {
+    const Window w(index, m, slots, r);
+    if (w.leads()) mine[w.slot] += __popcll(w.same);  // one lane a slot
+  }
   __syncthreads();
   for (int s = tid; s < n; s += kPlanThreads) {
     int total = 0;
@@ -689,26 +683,28 @@ __global__ __launch_bounds__(kPlanThreads) void lora_plan_kernel(const int32_t* 
   }
   __syncthreads();
   if (wave == 0) {  // exclusive sums over the slots
-    int tile = 0;
+    int groups = 0;
     for (int s0 = 0; s0 < n; s0 += 64) {
-      const int t = s0 + lane < n ? (rows[s0 + lane] + kPlanTile - 1) / kPlanTile : 0;
+      const int t = s0 + lane < n ? (rows[s0 + lane] + kPlanGroup - 1) / kPlanGroup : 0;
       int ts = t;
 #pragma unroll
       for (int o = 1; o < 64; o <<= 1) {
         const int tu = __shfl_up(ts, o, 64);
         if (lane >= o) ts += tu;
       }
-      if (s0 + lane < n) first_tile[s0 + lane] = tile + ts - t;
-      tile += __shfl(ts, 63, 64);
+      if (s0 + lane < n) first_group[s0 + lane] = groups + ts - t;
+      groups += __shfl(ts, 63, 64);
     }
-    if (lane == 0) plan[0] = tile, plan[1] = (int32_t)m, plan[2] = slots;
+    if (lane == 0) plan[0] = groups, plan[1] = (int32_t)m, plan[2] = slots;
   }
   __syncthreads();
+  for (int s = wave; s < n; s += kPlanWaves) {
+    const int total = rows[s], first = first_group[s];
+    for (int i = lane; i * kPlanGroup < total; i += 64)
+      *(i32x2_t*)(plan + 4 + 2 * (int64_t)(first + i)) = i32x2_t{s < slots ? s : -1, min(kPlanGroup, total - i * kPlanGroup)};
+  }
   for (int s = tid; s < n; s += kPlanThreads) {
-    const int total = rows[s], tile = first_tile[s];
-    for (int i = 0; i * kPlanTile < total; ++i)
-      *(i32x2_t*)(plan + 4 + 2 * (int64_t)(tile + i)) = i32x2_t{s < slots ? s : -1, min(kPlanTile, total - i * kPlanTile)};
-    int place = tile * kPlanTile;
+    int place = first_group[s] * kPlanGroup;
     for (int w = 0; w < kPlanWaves; ++w) {
       const int c = lds[w * n + s];
       lds[w * n + s] = place;
@@ -717,13 +713,14 @@ __global__ __launch_bounds__(kPlanThreads) void lora_plan_kernel(const int32_t* 
   }
   __syncthreads();
   int32_t* order = plan + plan_order_at(m, slots);
-  for (int64_t r = r0; r < r1; r += 64)
-    by_slot(index, m, slots, r, [&](int s, uint64_t same) {
-      int place = 0;
-      if (lane == 0) place = mine[s], mine[s] = place + __popcll(same);  // lane 0 alone reads and writes the wave's places
-      place = __builtin_amdgcn_readfirstlane(place);
-      if (same >> lane & 1) order[place + __popcll(same & ((1ull << lane) - 1))] = (int32_t)(r + lane);
-    });
+  for (int64_t r = r0; r < r1; r += 64) {
+    const Window w(index, m, slots, r);
+    const int place = mine[w.slot];
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // every lane has read its slot's place
+    if (w.leads()) mine[w.slot] = place + __popcll(w.same);
+    if (w.in) order[place + w.before()] = (int32_t)(r + lane);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  }
 }
 
 }  // namespace qtts
@@ -780,14 +777,14 @@ template <typename XT> void launch_lora(LoraArgs& g, hipStream_t st) {
     });
     return;
   }
-  const int64_t tiles = g.plan ? plan_max_tiles(g.m, g.slots) : ballots;
+  if (g.plan) g.groups = plan_max_groups(g.m, g.slots);
   by_bool(g.plan, [&](auto plan) {
     by_bool(g.rank <= 16, [&](auto pack) {
       by_bool(vec_k, [&](auto v) {
         const int a_tiles = g.parts.count * g.blocks * kBlockTiles<pack.value>;
         auto down = [&](auto n) {
           qtts::launch(&lora_down_kernel<XT, n.value, pack.value, v.value, plan.value>,
-                       dim3((a_tiles + n.value - 1) / n.value, grid_y(plan.value ? 4 * tiles : tiles)), dim3(64 * kDownWaves), 0,
+                       dim3((a_tiles + n.value - 1) / n.value, grid_y(g.groups)), dim3(64 * kDownWaves), 0,
                        st, g);
         };
         using std::integral_constant;
@@ -803,7 +800,7 @@ template <typename XT> void launch_lora(LoraArgs& g, hipStream_t st) {
     const int up_chunks = cut_columns(g.parts, g.up_cols);
     by_rank(g.rank, [&](auto nb, auto pack) {
       by_bool(vec_n, [&](auto v) {
-        qtts::launch(&lora_up_kernel<XT, nb.value, pack.value, v.value, plan.value>, dim3(up_chunks, grid_y(tiles)),
+        qtts::launch(&lora_up_kernel<XT, nb.value, pack.value, v.value, plan.value>, dim3(up_chunks, grid_y(plan.value ? (g.groups + kUpWaves - 1) / kUpWaves : g.groups)),
                      dim3(64 * kUpWaves), 0, st, g);
       });
     });

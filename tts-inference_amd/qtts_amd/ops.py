@@ -917,6 +917,15 @@ def silu_mul_quant(gate_up: torch.Tensor, codes: int = CODE_E4M3, want_act: bool
 LORA_WINDOW = 64
 
 
+@functools.lru_cache(maxsize=1024)
+def _plan_bytes(m: int, slots: int) -> int:
+    """Bytes of the plan of m rows, grows with m; 0 where a call takes none."""
+    need = _lib.load().qtts_lora_plan_bytes(m, slots) if m > LORA_WINDOW else 0
+    if need < 0:
+        _lib.check(int(need), "lora_plan")
+    return int(need)
+
+
 class LoraBatch:
     """Which adapter slot each row of a batch takes: ``index`` ``[M]`` int32 on the GPU (-1, or any value outside
     ``[0, slots)``: none), and past :data:`LORA_WINDOW` rows the ``plan`` that sorts them.  Made by
@@ -926,15 +935,18 @@ class LoraBatch:
     __slots__ = ("index", "slots", "rows", "plan")
 
     def __init__(self, index: torch.Tensor, slots: int, plan: torch.Tensor | None = None) -> None:
-        self.index, self.slots, self.rows, self.plan = index, slots, index.shape[0], plan
-
-
-def _plan_bytes(m: int, slots: int) -> int:
-    """Bytes of the plan of m rows, grows with m; 0 where a call takes none."""
-    need = _lib.load().qtts_lora_plan_bytes(m, slots) if m > LORA_WINDOW else 0
-    if need < 0:
-        _lib.check(int(need), "lora_plan")
-    return need
+        if index.dim() != 1 or index.dtype != torch.int32 or not index.is_contiguous():
+            raise ValueError(f"index must be a contiguous 1-D int32 tensor, got {index.dtype} {tuple(index.shape)}")
+        if slots < 0:
+            raise ValueError(f"slots is negative: {slots}")
+        self.index, self.slots, self.rows, self.plan = index, int(slots), index.shape[0], plan
+        if plan is not None:
+            need = _plan_bytes(self.rows, self.slots)
+            if (plan.dtype != torch.int32 or not plan.is_contiguous() or plan.numel() * 4 < need
+                    or plan.device != index.device):
+                raise ValueError(f"plan must hold {need // 4} contiguous int32 entries on {index.device}")
+            if not need:
+                self.plan = None  # so few rows, or so many slots, that none is taken
 
 
 def lora_plan_buffer(max_rows: int, slots: int, device: torch.device) -> torch.Tensor:
@@ -946,24 +958,17 @@ def lora_batch(index: torch.Tensor, slots: int, plan: torch.Tensor | None = None
     """The rows' adapter slots, ready for :func:`lora_add`: one kernel past :data:`LORA_WINDOW` rows, else none.
     ``plan``: a :func:`lora_plan_buffer` to write the plan into (a captured graph that reads it then follows the
     index of the last batch); a fresh tensor otherwise."""
-    if index.dim() != 1 or index.dtype != torch.int32 or not index.is_contiguous():
-        raise ValueError(f"index must be a contiguous 1-D int32 tensor, got {index.dtype} {tuple(index.shape)}")
-    if slots < 0:
-        raise ValueError(f"slots is negative: {slots}")
+    batch = LoraBatch(index, slots, plan)
     idx = _gpu_index(index)
-    m = index.shape[0]
-    need = _plan_bytes(m, slots)
-    if not need:
-        return LoraBatch(index, int(slots))
-    if plan is None:
-        plan = torch.empty(need // 4, dtype=torch.int32, device=index.device)
-    elif plan.dtype != torch.int32 or not plan.is_contiguous() or plan.numel() * 4 < need or plan.get_device() != idx:
-        raise ValueError(f"plan must hold {need // 4} contiguous int32 entries on {index.device}")
-    st = _call(idx, _lib.load().qtts_lora_plan, index.data_ptr(), m, slots, plan.data_ptr(), need,
-               torch._C._cuda_getCurrentRawStream(idx))
-    if st:
-        _lib.check(st, "lora_plan")
-    return LoraBatch(index, int(slots), plan)
+    need = _plan_bytes(batch.rows, batch.slots)
+    if need:
+        if plan is None:
+            batch.plan = plan = torch.empty(need // 4, dtype=torch.int32, device=index.device)
+        st = _call(idx, _lib.load().qtts_lora_plan, index.data_ptr(), batch.rows, batch.slots, plan.data_ptr(),
+                   plan.numel() * 4, torch._C._cuda_getCurrentRawStream(idx))
+        if st:
+            _lib.check(st, "lora_plan")
+    return batch
 
 
 @functools.lru_cache(maxsize=1024)
