@@ -183,6 +183,17 @@ int main() {
     for (int slots = 0; slots <= 80; ++slots) printf("1 %d %d %lld\\n", m, slots, (long long)lora_groups(m, slots));
   const int ms[] = {1, 5, 64, 65, 1003, 2048, 8192, 1 << 20}, ns[] = {1, 64, 256, 2048, 4096, 12288};
   for (int m : ms) for (int n : ns) printf("2 %d %d %d\\n", m, n, lora_up_cols(m, n));
+  for (int groups = 1; groups <= 700; groups += 9)
+    for (int tiles = 1; tiles <= 64; ++tiles)
+      for (int pack = 0; pack < 2; ++pack)
+        if (pack || tiles % 2 == 0) {
+          const int t = lora_down_tiles(groups, tiles, pack);
+          printf("4 %d %d %d %d %d %d\n", groups, tiles, pack, t, lora_splits(64, 6144, 16, groups * ((tiles + t - 1) / t)),
+                 lora_splits(64, 1024, 16, 1));
+        }
+  for (int m = 1; m < 5000; m += 7)
+    for (int rank = 8; rank <= 128; rank += 8)
+      printf("5 %d %d %d %d\n", m, rank, (int)lora_max_splits(m, rank), lora_splits(m, 6144, rank, (m + 15) / 16));
   for (int rank = 1; rank <= 128; ++rank)
     for (int chunks = 1; chunks <= 48; ++chunks)
       for (int m = 1; m <= 64; m += 7)
@@ -191,6 +202,7 @@ int main() {
 }
 """)
     one = two = 0
+    seen = set()
     for kind, *v in rows:
         if kind == 0:
             rank, blocks = v
@@ -201,8 +213,17 @@ int main() {
             assert groups >= min(m, min(m, slots + 1) + m // 16) or groups == m, (m, slots)
         elif kind == 2:
             assert v[2] in (64, 128, 256)
+        elif kind == 4:
+            groups, tiles, pack, t, splits, short = v
+            assert t in ((1, 2, 3, 4) if pack else (2, 4)), v  # the kernels that are built
+            assert splits == (2 if groups * -(-tiles // t) <= 128 else 1) and short == 1, v
+            seen.add((pack, t))
+        elif kind == 5:
+            m, rank, most, splits = v
+            assert 1 <= splits <= most <= 2 and (rank <= 64 or most == 1), v  # within the workspace
         else:
             rank, chunks, m, free, plan = v
             assert not plan and (not free or rank <= 64)
             one, two = one + free, two + (not free)
     assert one and two
+    assert seen == {(1, 1), (1, 2), (1, 3), (1, 4), (0, 2), (0, 4)}

@@ -29,10 +29,10 @@ struct LoraArgs {
   int64_t ldb;
   void* out;
   int64_t ldo;
-  uint8_t* t;     // [m, parts.count, blocks]: the first product's halves (lora.hip)
-  int32_t* exps;  // [m, parts.count, blocks], fp16
+  uint8_t* t;     // [splits, m, parts.count, blocks]: the first product's halves (lora.hip)
+  int32_t* exps;  // as many, fp16
   int64_t m;
-  int k, n, slots, rank, blocks, up_cols;
+  int k, n, slots, rank, blocks, up_cols, splits;
   int ordinal;     // without a plan: workgroups by group, not by row
   int64_t groups;  // and how many
   LoraParts parts;

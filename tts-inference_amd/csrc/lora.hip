@@ -277,7 +277,7 @@ __device__ __forceinline__ void meet_waves(const uint8_t* sums, int pitch, int t
 
 constexpr int kDownWaves = 8;
 
-// Grid: (N tiles of the partitions' A each, groups).  Eight waves share K.
+// Grid: (N tiles of the partitions' A each, groups, splits of K).  Eight waves share the split's K.
 template <typename XT, int N, bool PACK, bool VEC, bool PLAN>
 __global__ __launch_bounds__(64 * kDownWaves) void lora_down_kernel(LoraArgs g) {
   constexpr int T = kBlockTiles<PACK>, kPitch = VEC ? kDownBytes<N, kDownStages<N>> : 1024 * N;
@@ -285,8 +285,8 @@ __global__ __launch_bounds__(64 * kDownWaves) void lora_down_kernel(LoraArgs g) 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int per_part = T * g.blocks, tile0 = blockIdx.x * N;  // tiles of a partition; the workgroup's first
   const Ranks ranks(g);
-  const int steps = (g.k + 31) >> 5, per = ((steps + kDownWaves - 1) / kDownWaves + 1) & ~1;
-  const int s0 = min(wave * per, (steps + 1) & ~1), s1 = min(s0 + per, steps);
+  const int cuts = kDownWaves * g.splits, steps = (g.k + 31) >> 5, per = ((steps + cuts - 1) / cuts + 1) & ~1;
+  const int s0 = min((int)(kDownWaves * blockIdx.z + wave) * per, (steps + 1) & ~1), s1 = min(s0 + per, steps);
   for (int64_t at = blockIdx.y; at < g.groups; at += gridDim.y) {
     const Group gr = PLAN ? group_by_plan(g, at) : group_by_ballot(g, at);
     if (!gr.count) continue;
@@ -310,7 +310,7 @@ __global__ __launch_bounds__(64 * kDownWaves) void lora_down_kernel(LoraArgs g) 
       f32x4_t v[T];
       meet_waves<kDownWaves, T>(stages[0], kPitch, T * wave, tile % per_part * 16, live, scaling, v);
       const int exp = scale_block<XT, T>(v);
-      const int64_t block = gr.row * (g.parts.count * g.blocks) + tile / T;
+      const int64_t block = (blockIdx.z * g.m + gr.row) * (g.parts.count * g.blocks) + tile / T;
       if ((lane & 15) < gr.count) {
         uint8_t* to = g.t + block * kBlockBytes<PACK> + 8 * (lane >> 4);
 #pragma unroll
@@ -327,21 +327,22 @@ __global__ __launch_bounds__(64 * kDownWaves) void lora_down_kernel(LoraArgs g) 
 }
 
 // ---- second product --------------------------------------------------------------------------
-// The t operands of one group's rows: (hi, lo) of each block, and fp16's exponents.
-template <typename XT, int NB, bool PACK> struct TOperand {
-  static constexpr int kHalves = PACK ? 1 : 2;
-  i32x4_t v[NB][kHalves];
-  int exp[NB];
+// The t operands of one group's rows: (hi, lo) of each block of each split's sum, and fp16's exponents.  The splits of K meet
+// here, as more MFMAs by the same operand of B.
+template <typename XT, int NB, bool PACK, int S = 1> struct TOperand {
+  static constexpr int kHalves = PACK ? 1 : 2, kBlocks = NB * S;
+  i32x4_t v[kBlocks][kHalves];
+  int exp[kBlocks];
 
   // `row`: the lane's row of the workspace (of a group's first for lanes past its rows), `part` of the partition.
   __device__ __forceinline__ void load(const LoraArgs& g, int64_t row, int part) {
-    const int64_t block = (row * g.parts.count + part) * NB;
-    const uint8_t* from = g.t + block * kBlockBytes<PACK> + 16 * ((threadIdx.x & 63) >> 4);
 #pragma unroll
-    for (int b = 0; b < NB; ++b) {
+    for (int b = 0; b < kBlocks; ++b) {
+      const int64_t block = ((b / NB * g.m + row) * g.parts.count + part) * NB + b % NB;
+      const uint8_t* from = g.t + block * kBlockBytes<PACK> + 16 * ((threadIdx.x & 63) >> 4);
 #pragma unroll
-      for (int h = 0; h < kHalves; ++h) v[b][h] = *(const i32x4_t*)(from + kBlockBytes<PACK> * b + 64 * h);
-      if constexpr (std::is_same<XT, f16_t>::value) exp[b] = g.exps[block + b];
+      for (int h = 0; h < kHalves; ++h) v[b][h] = *(const i32x4_t*)(from + 64 * h);
+      if constexpr (std::is_same<XT, f16_t>::value) exp[b] = g.exps[block];
     }
   }
 };
@@ -395,16 +396,16 @@ template <typename XT, int NB, bool PACK, bool VEC> struct Columns {
   }
 };
 
-template <typename XT, int NB, bool PACK>
-__device__ __forceinline__ f32x4_t up_mma(const vec8<XT> (&b)[NB], const TOperand<XT, NB, PACK>& t) {
+template <typename XT, int NB, bool PACK, int S>
+__device__ __forceinline__ f32x4_t up_mma(const vec8<XT> (&b)[NB], const TOperand<XT, NB, PACK, S>& t) {
   f32x4_t sum = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-  for (int k = 0; k < NB; ++k) {
+  for (int k = 0; k < NB * S; ++k) {
     constexpr bool kExp = std::is_same<XT, f16_t>::value;  // a block at a time: each has an exponent of its own
     f32x4_t acc = kExp ? f32x4_t{0.0f, 0.0f, 0.0f, 0.0f} : sum;
 #pragma unroll
     for (int h = 0; h < TOperand<XT, NB, PACK>::kHalves; ++h)
-      acc = mfma16<XT>::mma(b[k], __builtin_bit_cast(vec8<XT>, t.v[k][h]), acc);
+      acc = mfma16<XT>::mma(b[k % NB], __builtin_bit_cast(vec8<XT>, t.v[k][h]), acc);
     if constexpr (kExp) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) sum[i] += __builtin_amdgcn_ldexpf(acc[i], t.exp[k]);
@@ -513,7 +514,7 @@ constexpr int kUpWaves = 4, kUpTiles = 4, kUpBlock = 16 * kUpTiles;
 
 // Grid: (blocks of g.up_cols columns, groups).  A wave takes 64 columns at a time: with a plan, whose groups of one slot follow
 // one another, all columns of a group of its own; else a part of the workgroup's group.
-template <typename XT, int NB, bool PACK, bool VEC, bool PLAN>
+template <typename XT, int NB, bool PACK, bool VEC, bool PLAN, int S>
 __global__ __launch_bounds__(64 * kUpWaves) void lora_up_kernel(LoraArgs g) {
   typedef Rows<XT, kUpTiles, VEC> R;
   __shared__ __align__(16) float lds[kUpWaves][R::kFloats];
@@ -541,14 +542,14 @@ __global__ __launch_bounds__(64 * kUpWaves) void lora_up_kernel(LoraArgs g) {
       }
       continue;
     }
-    TOperand<XT, NB, PACK> t;
+    TOperand<XT, NB, PACK, S> t;
     t.load(g, gr.row, blk.part);
     Columns<XT, NB, PACK, VEC> columns(g, gr.slot, c0, blk.end, live);
     vec8<XT> b[kUpTiles][NB];
 #pragma unroll
     for (int n = 0; n < kUpTiles; ++n) columns.next(b[n]);
     for (int c = c0;;) {
-      rows.add([&](int n) { return up_mma<XT, NB, PACK>(b[n], t); }, lds[wave]);
+      rows.add([&](int n) { return up_mma(b[n], t); }, lds[wave]);
       if ((c += kUpBlock) >= c1) break;
       rows.advance();
       rows.load();
@@ -629,7 +630,7 @@ __global__ __launch_bounds__(64 * kOneWaves) void lora_one_kernel(LoraArgs g) {
         t.v[k][h] = *(const i32x4_t*)&halves[k][tok][64 * h + 16 * (lane >> 4)];
       if constexpr (std::is_same<XT, f16_t>::value) t.exp[k] = exps[k][tok];
     }
-    rows.add([&](int n) { return up_mma<XT, NB, PACK>(b[n], t); }, (float*)stages[wave]);
+    rows.add([&](int n) { return up_mma(b[n], t); }, (float*)stages[wave]);
     __syncthreads();  // before the next group's stages and halves
   }
 }
@@ -778,21 +779,22 @@ template <typename XT> void launch_lora(LoraArgs& g, hipStream_t st) {
     return;
   }
   if (g.plan) g.groups = plan_max_groups(g.m, g.slots);
+  const int a_tiles = g.parts.count * g.blocks * (g.rank <= 16 ? 1 : 2);
+  const int down_tiles = lora_down_tiles(g.groups, a_tiles, g.rank <= 16), down_wide = (a_tiles + down_tiles - 1) / down_tiles;
+  g.splits = vec_k && vec_n ? lora_splits(g.m, g.k, g.rank, g.groups * down_wide) : 1;
   by_bool(g.plan, [&](auto plan) {
     by_bool(g.rank <= 16, [&](auto pack) {
       by_bool(vec_k, [&](auto v) {
-        const int a_tiles = g.parts.count * g.blocks * kBlockTiles<pack.value>;
         auto down = [&](auto n) {
           qtts::launch(&lora_down_kernel<XT, n.value, pack.value, v.value, plan.value>,
-                       dim3((a_tiles + n.value - 1) / n.value, grid_y(g.groups)), dim3(64 * kDownWaves), 0,
-                       st, g);
+                       dim3(down_wide, grid_y(g.groups), g.splits), dim3(64 * kDownWaves), 0, st, g);
         };
         using std::integral_constant;
         if constexpr (pack.value) {
-          if (a_tiles == 1) return down(integral_constant<int, 1>{});
-          if (a_tiles == 3) return down(integral_constant<int, 3>{});
+          if (down_tiles == 1) return down(integral_constant<int, 1>{});
+          if (down_tiles == 3) return down(integral_constant<int, 3>{});
         }
-        if (a_tiles == 2) down(integral_constant<int, 2>{});
+        if (down_tiles == 2) down(integral_constant<int, 2>{});
         else down(integral_constant<int, 4>{});
       });
     });
@@ -800,8 +802,15 @@ template <typename XT> void launch_lora(LoraArgs& g, hipStream_t st) {
     const int up_chunks = cut_columns(g.parts, g.up_cols);
     by_rank(g.rank, [&](auto nb, auto pack) {
       by_bool(vec_n, [&](auto v) {
-        qtts::launch(&lora_up_kernel<XT, nb.value, pack.value, v.value, plan.value>, dim3(up_chunks, grid_y(plan.value ? (g.groups + kUpWaves - 1) / kUpWaves : g.groups)),
-                     dim3(64 * kUpWaves), 0, st, g);
+        auto up = [&](auto s) {
+          qtts::launch(&lora_up_kernel<XT, nb.value, pack.value, v.value, plan.value, s.value>,
+                       dim3(up_chunks, grid_y(plan.value ? (g.groups + kUpWaves - 1) / kUpWaves : g.groups)),
+                       dim3(64 * kUpWaves), 0, st, g);
+        };
+        if constexpr (v.value && 32 * nb.value <= kLoraSplitRank) {
+          if (g.splits == 2) return up(std::integral_constant<int, 2>{});
+        }
+        up(std::integral_constant<int, 1>{});
       });
     });
   });
@@ -809,11 +818,14 @@ template <typename XT> void launch_lora(LoraArgs& g, hipStream_t st) {
 
 }  // namespace
 
-// The workspace: t's blocks, row by row, then fp16's exponents.
-static int64_t lora_t_bytes(int64_t m, int64_t parts, int64_t rank) { return align256(m * parts * lora_blocks(rank) * (rank <= 16 ? 64 : 128)); }
+// The workspace: t's blocks, split by split and row by row, then fp16's exponents.
+static int64_t lora_t_blocks(int64_t m, int64_t parts, int64_t rank) { return lora_max_splits(m, rank) * m * parts * lora_blocks(rank); }
+static int64_t lora_t_bytes(int64_t m, int64_t parts, int64_t rank) {
+  return align256(lora_t_blocks(m, parts, rank) * (rank <= 16 ? 64 : 128));
+}
 
 int64_t qtts_lora_ws_bytes(int64_t m, int64_t parts, int64_t rank) {
-  return kCounterBytes + lora_t_bytes(m, parts, rank) + align256(m * parts * lora_blocks(rank) * 4);
+  return kCounterBytes + lora_t_bytes(m, parts, rank) + align256(lora_t_blocks(m, parts, rank) * 4);
 }
 
 int qtts_launch_lora_plan(const int32_t* index, int64_t m, int64_t slots, int32_t* plan, hipStream_t st) {

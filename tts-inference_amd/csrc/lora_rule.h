@@ -21,6 +21,28 @@ inline int64_t lora_groups(int64_t m, int64_t slots) {
   return m <= 64 && 8 * slots <= m ? most : m;
 }
 
+// 16-row tiles of A (all partitions' `tiles`; past rank 16, PACK false, two a block) that a workgroup of the first product takes:
+// few, and x read more often, while each of the workgroups has a compute unit; else as many as its LDS holds.  Captured with the
+// second product, few / many: rank 16 of qkv, 300 rows of 4 adapters (70 workgroups of 1) 12.8 / 14.2 us, 2048 of 8 (411)
+// 24.8 / 21.0; rank 32 of gate_up, 300 of 4 (46 of 2) 16.7 / 18.5, 2048 of 64 (386) 51.5 / 51.4; rank 32 of qkv, 300 of 64 (252)
+// 19.9 / 21.0, 2048 of 8 (411) 28.7 / 25.1.
+inline int lora_down_tiles(int64_t groups, int tiles, bool pack) {
+  const int few = pack ? 1 : 2;
+  if (groups * ((tiles + few - 1) / few) <= 256) return few;
+  return pack ? std::min(tiles, 4) : tiles == 2 ? 2 : 4;
+}
+
+// Parts of K with workgroups of their own in the first product, which the second adds: two for a long K while the workgroups are
+// few.  K = 6144, one / two: rank 16, 64 rows of 32 adapters 10.7 / 9.2 us, 300 of 4 14.9 / 13.2, 1003 of 32 (95 workgroups)
+// 17.4 / 16.5; rank 64, 300 of 4 19.2 / 16.8.  K = 2048: rank 16, 300 of 4 through o_proj 11.5 / 11.0, 64 of 64 through qkv (192
+// workgroups) 10.7 / 12.7.  (Four: K = 6144, rank 16, 300 of 4 12.6.)
+constexpr int64_t kLoraSplitRows = 2048;  // 128 workgroups at the least
+constexpr int kLoraSplitRank = 64;
+inline int lora_max_splits(int64_t m, int64_t rank) { return m <= kLoraSplitRows && rank <= kLoraSplitRank ? 2 : 1; }
+inline int lora_splits(int64_t m, int64_t k, int64_t rank, int64_t workgroups) {
+  return workgroups <= 128 && k >= 2048 ? lora_max_splits(m, rank) : 1;
+}
+
 // Columns of a workgroup of the second product: a wave that takes 256 of a group's columns makes its t operand once for all of
 // them, but the GPU wants some 4096 waves.
 inline int lora_up_cols(int64_t m, int64_t n) {
