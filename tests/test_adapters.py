@@ -188,12 +188,12 @@ int main() {
       for (int pack = 0; pack < 2; ++pack)
         if (pack || tiles % 2 == 0) {
           const int t = lora_down_tiles(groups, tiles, pack);
-          printf("4 %d %d %d %d %d %d\n", groups, tiles, pack, t, lora_splits(64, 6144, 16, groups * ((tiles + t - 1) / t)),
+          printf("4 %d %d %d %d %d %d\\n", groups, tiles, pack, t, lora_splits(64, 6144, 16, groups * ((tiles + t - 1) / t)),
                  lora_splits(64, 1024, 16, 1));
         }
   for (int m = 1; m < 5000; m += 7)
     for (int rank = 8; rank <= 128; rank += 8)
-      printf("5 %d %d %d %d\n", m, rank, (int)lora_max_splits(m, rank), lora_splits(m, 6144, rank, (m + 15) / 16));
+      printf("5 %d %d %d %d\\n", m, rank, (int)lora_max_splits(m, rank), lora_splits(m, 6144, rank, (m + 15) / 16));
   for (int rank = 1; rank <= 128; ++rank)
     for (int chunks = 1; chunks <= 48; ++chunks)
       for (int m = 1; m <= 64; m += 7)
