@@ -101,6 +101,17 @@ def test_wide_outputs(ops, m, parts, slots, rank, dtype):
     _check(_run(ops, c), c, f"{m} rows parts {parts} rank {rank} {dtype}")
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("k", [2048, 2056, 2104, 6144])
+@pytest.mark.parametrize("m,parts,slots,rank", [(60, [4096], 30, 16), (60, [1024], 40, 64), (63, [520, 264], 63, 24), (70, [1024], 3, 8),
+                                                (300, [520, 264], 4, 40), (1003, [1024], 30, 16), (130, [64] * 5, 2, 16)])
+def test_long_k_in_parts(ops, m, parts, slots, rank, k, dtype):
+    """Few groups and a long K: the first product in two parts of K, which the second adds.  Each part's sum is carried in 2^-17 of
+    its own magnitude, which is at most that of all of K's products: within the bound's fp32 term, 2 K u >= 2^-12 of those."""
+    c = _case(m, k, parts, slots, rank, dtype, seed=m + k + rank)
+    _check(_run(ops, c), c)
+
+
 @pytest.mark.parametrize("m", [1, 5, 40, 100])
 @pytest.mark.parametrize("k,parts,rank", [(33, [17], 3), (65, [40, 1, 23], 4), (100, [13, 64], 12), (8, [8], 1),
                                           (2047, [31], 16), (64, [100], 17), (24, [7], 127), (16, [0, 24, 0], 8)])
