@@ -479,8 +479,9 @@ int qtts_lora_plan(const int32_t* index, int64_t m, int64_t slots, int32_t* plan
  * [slots] fp32.  base, out: [m, n] of x_dtype, row strides ldb, ldo; out may be base itself
  * and shares no byte with x.  rank <= QTTS_LORA_MAX_RANK, parts <= QTTS_LORA_MAX_PARTS.
  * plan: what qtts_lora_plan made of the same index, m and slots, or NULL (rows of one adapter
- * are then read together within each 64 rows); a plan of another m or slots writes nothing.  Workspace: qtts_workspace_bytes(QTTS_OP_LORA,
- * m, parts, rank, 0). */
+ * are then read together within each 64 rows); with a plan of another m or slots, in a buffer
+ * of qtts_lora_plan_bytes(m, slots), nothing is written.
+ * Workspace: qtts_workspace_bytes(QTTS_OP_LORA, m, parts, rank, 0). */
 int qtts_lora_add(const void* x, int x_dtype, int64_t m, int64_t k, int64_t ldx, const int32_t* index,
                   const int32_t* plan, int64_t slots, const void* a, const void* b, int64_t rank, const int32_t* ranks,
                   const float* scaling, const int64_t* part_ends, int64_t parts, const void* base, int64_t ldb,

@@ -148,27 +148,27 @@ def test_fakes():
 
 
 def test_row_forms_hold_the_row(tmp_path):
-    """Rows of 8-bit codes: in registers up to 8192 columns, and a grid whose threads fit 32 bits; read twice past that."""
+    """Rows of 8-bit codes: in registers up to 16384 columns, and a grid whose threads fit 32 bits; read twice past that."""
     rows = _run(tmp_path, """
 #include <stdio.h>
 #include "quant_rows_rule.h"
 int main() {
   const long long ms[] = {1, 1003, 1 << 22, (1 << 22) + 1, 1 << 25};
   for (long long m : ms) {
-    for (long long k = 0; k <= 8300; ++k) { auto f = qtts::row_form(m, k); printf("%lld %lld %d %d\\n", m, k, f.threads, f.vectors); }
+    for (long long k = 0; k <= 16500; ++k) { auto f = qtts::row_form(m, k); printf("%lld %lld %d %d\\n", m, k, f.threads, f.vectors); }
     auto f = qtts::row_form(m, 1 << 20); printf("%lld %d %d %d\\n", m, 1 << 20, f.threads, f.vectors);
   }
 }
 """)
-    assert len(rows) == 5 * 8302
+    assert len(rows) == 5 * 16502
     forms = set()
     for m, k, threads, vectors in rows:
-        if 0 < k <= 8192 and m <= 1 << 22:
+        if 0 < k <= 16384 and m <= 1 << 22:
             assert threads * vectors * 8 >= k and threads * m < 1 << 32, (m, k)
             forms.add((threads, vectors))
         else:
             assert threads == 0, (m, k)
-    assert forms == {(64, 1), (128, 1), (256, 1), (256, 2), (256, 3), (256, 4)}  # the kernels that are built
+    assert forms == {(64, 1), (128, 1), (256, 1), (256, 2), (256, 3), (256, 4), (512, 3), (512, 4)}  # the kernels that are built
 
 
 def test_adapter_launches_cover_their_work(tmp_path):

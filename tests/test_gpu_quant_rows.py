@@ -74,7 +74,7 @@ def _silu64(gu):
 
 
 SHAPES = [(1, 8), (1, 2048), (3, 100), (5, 1003), (17, 1024), (9, 520), (2, 6144), (3, 7), (70, 1), (4, 8192), (2, 9001),
-          (2, 12296), (1, 33000), (2000, 72)]
+          (2, 12296), (2, 16384), (3, 16385), (1, 33000), (2000, 72)]
 
 
 @pytest.mark.parametrize("codes", [1, 0], ids=["e4m3", "int8"])

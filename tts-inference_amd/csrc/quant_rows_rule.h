@@ -8,14 +8,16 @@ namespace qtts {
 // The row in registers of `threads` threads, `vectors` times eight elements each; threads == 0: the row read twice.
 struct RowForm { int threads, vectors; };
 
-// Rows of up to 8192 columns stay in registers: the fewest threads, 64 to 256, that hold the row in eight elements
-// each, then two to four times eight.  One workgroup a row, so up to 2^22 rows (the grid's threads stay within 2^30).
+// Rows of up to 16384 columns stay in registers: the fewest threads, 64 to 256, that hold the row in eight elements each, then two
+// to four times eight, then 512 of three or four times eight.  One workgroup a row, so up to 2^22 rows (the grid's threads stay
+// within 2^31).  Beyond either the row is read twice, element by element (16384 columns: one norm row 46 us so, 4.7 in registers; 4096 rows 231, 66).
 inline RowForm row_form(int64_t m, int64_t k) {
   const int64_t nv = (k + 7) / 8;
-  if (k <= 0 || nv > 1024 || m > (1 << 22)) return {0, 0};
+  if (k <= 0 || nv > 2048 || m > (1 << 22)) return {0, 0};
   if (nv <= 64) return {64, 1};
   if (nv <= 128) return {128, 1};
-  return {256, (int)((nv + 255) / 256)};
+  const int threads = nv <= 1024 ? 256 : 512;
+  return {threads, (int)((nv + threads - 1) / threads)};
 }
 
 }  // namespace qtts
