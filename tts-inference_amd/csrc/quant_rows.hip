@@ -208,8 +208,8 @@ __global__ __launch_bounds__(T) void rms_norm_quant_kernel(
   if (threadIdx.x == 0) sx[row] = s;
 }
 
-// As above, without the sum: the gate and up values of a row meet in registers.  4096 x 6144 fp16, 5 bytes an element, in 28.7 us
-// (4.4 TB/s, the exponential and the reciprocal beside the loads); 1501 rows in 9.6, 5 rows in 3.2.
+// As above, without the sum: the gate and up values of a row meet in registers.  4096 x 6144 fp16 with act, 7 bytes an element, in
+// 28.7 us (6.1 TB/s); 1501 bf16 rows without it, 5 bytes, in 9.6 (4.8); 5 rows in 3.2.
 template <typename XT, bool FP8, bool VEC, int T, int V>
 __global__ __launch_bounds__(T) void silu_mul_quant_kernel(const XT* __restrict__ gu, int64_t ld, int k,
                                                            uint8_t* __restrict__ q, float* __restrict__ sx,
