@@ -60,7 +60,9 @@ def test_attach_finds_the_named_linears_and_their_partitions():
     assert not list(q.state_dict())  # adapters are loaded by slot, not from the checkpoint
     with pytest.raises(ValueError, match="has adapters already"):
         attach_adapters(block, slots=4, rank=12, routing=routing)
-    assert block.o_proj.quant_method is None  # refused before any layer changed
+    with pytest.raises(ValueError, match="mlp.down_proj has adapters already"):  # after layers without any
+        attach_adapters(block, slots=4, rank=12, routing=routing, targets=("o_proj", "mlp"))
+    assert block.o_proj.quant_method is None and not hasattr(block.mlp.gate_up_proj, "adapters")
     with pytest.raises(ValueError, match="routing has 4 slots"):
         attach_adapters(_fill(Block()), slots=5, rank=12, routing=routing)
     for bad in ({"slots": 0}, {"rank": 0}, {"rank": 129}):
@@ -145,6 +147,18 @@ def test_fakes():
         y = q.lora_add(base, x, index, None, 4, torch.empty(4, 16, 1024, dtype=bf, device="cuda"),
                        torch.empty(4, 96, 16, dtype=bf, device="cuda"), torch.empty(4, device="cuda"), None, [96])
         assert y.shape == base.shape and y.dtype == bf
+
+
+def test_dynamo_traces_a_layer_with_adapters():
+    """A linear with adapters is its own method's op and lora_add, without a graph break."""
+    import torch._dynamo
+    layer = MergedLinear(64, [32, 32], dtype=torch.bfloat16, device="meta")
+    routing = AdapterRouting(4, 8, device="meta")
+    attach_adapters(layer, slots=4, rank=8, routing=routing)
+    routing.batch = ops.LoraBatch(routing.index[:3], 4)
+    torch._dynamo.reset()
+    report = torch._dynamo.explain(lambda x: layer(x) + 1)(torch.empty(3, 64, dtype=torch.bfloat16, device="meta"))
+    assert report.graph_break_count == 0, report.break_reasons
 
 
 def test_row_forms_hold_the_row(tmp_path):

@@ -157,17 +157,16 @@ def attach_adapters(module: nn.Module, slots: int, rank: int, routing: AdapterRo
     adapters of rank up to ``rank``; returns them by name.  ``dtype``: the activations' (default: the weight's)."""
     if routing.slots != slots:
         raise ValueError(f"the routing has {routing.slots} slots, the adapters {slots}")
+    layers = {name: layer for name, layer in iter_linears(module) if not targets or any(t in name for t in targets)}
     banks = {}
-    for name, layer in iter_linears(module):
-        if targets and not any(t in name for t in targets):
-            continue
+    for name, layer in layers.items():  # all of them before any layer changes: a refusal leaves the module as it was
         if isinstance(layer.quant_method, AdapterMethod):
             raise ValueError(f"{name} has adapters already")
-        parts = getattr(layer, "partitions", None) or [layer.out_features]
-        device = layer.weight.device
-        layer.adapters = LinearAdapters(layer.in_features, parts, slots, rank, dtype or layer.weight.dtype, device)
+        parts, device = getattr(layer, "partitions", None) or [layer.out_features], layer.weight.device
+        bank = banks[name] = LinearAdapters(layer.in_features, parts, slots, rank, dtype or layer.weight.dtype, device)
         if device.type == "cuda":  # a captured call allocates no workspace
-            ops.reserve_for_rows(device, ops.OP_LORA, len(parts), layer.adapters.rank)
+            ops.reserve_for_rows(device, ops.OP_LORA, len(parts), bank.rank, max(ops.WORKSPACE_ROWS, routing.max_rows))
+    for name, layer in layers.items():
+        layer.adapters = banks[name]
         layer.quant_method = AdapterMethod(layer.quant_method, routing)
-        banks[name] = layer.adapters
     return banks
