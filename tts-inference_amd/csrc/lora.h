@@ -33,8 +33,7 @@ struct LoraArgs {
   int32_t* exps;  // as many, fp16
   int64_t m;
   int k, n, slots, rank, blocks, up_cols, splits;
-  int ordinal;     // without a plan: workgroups by group, not by row
-  int64_t groups;  // and how many
+  int64_t groups;  // at most, of the batch: the workgroups along the rows
   LoraParts parts;
 };
 

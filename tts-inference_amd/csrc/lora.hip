@@ -67,44 +67,42 @@ struct Group {
   int64_t row;  // the row of lane % 16 (of the first one past count)
 };
 
-// The group of workgroup row `at`, without a plan; count 0 for none.  Up to 64 rows with fewer adapters (g.ordinal) it is the
-// at-th of the groups in the order of their first rows; otherwise the group that row `at` leads among its window of 64 rows,
-// every 16th of its slot.
+// The lanes of `in` whose slot (0 to slots) is this lane's, bit by bit of the slot (a loop over the slots among 64 rows waits 90 ns
+// or more for each).
+__device__ __forceinline__ uint64_t same_slot(int slot, int slots, bool in) {
+  uint64_t same = __ballot(in);
+  for (int bit = 1; bit <= slots; bit <<= 1) {
+    const uint64_t set = __ballot((slot & bit) != 0);
+    same &= slot & bit ? set : ~set;
+  }
+  return same;
+}
+
+// Group `at` without a plan, count 0 for none; every 16th row of a slot among 64 rows leads one.  With a place for each row
+// (g.groups == g.m) it is the one that row `at` leads; with fewer, of up to 64 rows, the at-th in the order of their first rows.
 __device__ __forceinline__ Group group_by_ballot(const LoraArgs& g, int64_t at) {
   const int lane = threadIdx.x & 63;
-  const int64_t window = g.ordinal ? 0 : at & ~(int64_t)63;
+  const int64_t window = at & ~(int64_t)63;
+  const uint64_t below = (1ull << lane) - 1;
   const bool in = window + lane < g.m;
   int s = in ? g.index[window + lane] : -1;
-  if (s < 0 || s >= g.slots) s = -1;
-  uint64_t same;
-  int slot, before = 0, total;
-  if (g.ordinal) {
-    uint64_t left = __ballot(in);
-    for (int ahead = (int)at;;) {
-      if (!left) return {-1, 0, 0};
-      slot = __builtin_amdgcn_readlane(s, __builtin_ctzll(left));
-      same = __ballot(in && s == slot), total = __popcll(same);
-      const int groups = (total + 15) >> 4;
-      if (ahead < groups) {
-        before = 16 * ahead;
-        break;
-      }
-      ahead -= groups;
-      left &= ~same;
-    }
-  } else {
-    const int here = (int)(at & 63);
-    slot = __builtin_amdgcn_readlane(s, here);
-    same = __ballot(in && s == slot), total = __popcll(same);
-    before = __popcll(same & ((1ull << here) - 1));
-    if (before % 16) return {slot, 0, 0};
+  if (s < 0 || s >= g.slots) s = g.slots;
+  int leader = (int)(at & 63);
+  if (g.groups < g.m) {
+    const uint64_t leaders = __ballot(in && __popcll(same_slot(s, g.slots, in) & below) % 16 == 0);
+    const uint64_t found = __ballot((leaders >> lane & 1) && __popcll(leaders & below) == leader);
+    if (!found) return {-1, 0, 0};
+    leader = __builtin_ctzll(found);
   }
+  const int slot = __builtin_amdgcn_readlane(s, leader);
+  const uint64_t same = __ballot(in && s == slot);
+  const int total = __popcll(same), before = __popcll(same & ((1ull << leader) - 1));
+  if (before % 16) return {-1, 0, 0};
   // lane i of the window to lane `rank of i among the slot's rows` (the others past them): one permutation
-  const uint64_t below = (1ull << lane) - 1;
   const int to = same >> lane & 1 ? __popcll(same & below) : total + __popcll(~same & below);
   const int order = __builtin_amdgcn_ds_permute(4 * to, lane);
   const int count = min(16, total - before), j = lane & 15;
-  return {slot, count, window + __builtin_amdgcn_ds_bpermute(4 * (before + (j < count ? j : 0)), order)};
+  return {slot < g.slots ? slot : -1, count, window + __builtin_amdgcn_ds_bpermute(4 * (before + (j < count ? j : 0)), order)};
 }
 
 // Group `at` < plan_max_groups of the plan; count 0 past the plan's groups and where the plan was made for another batch or
@@ -649,8 +647,7 @@ __global__ __launch_bounds__(64 * kOneWaves) void lora_one_kernel(LoraArgs g) {
 
 constexpr int kPlanThreads = 1024, kPlanWaves = kPlanThreads / 64;
 
-// 64 rows, one a lane: the lane's slot (slots: no adapter) and the lanes with the same one, found bit by bit of the slot (a
-// loop over the slots among 64 rows, of up to 64 steps that wait for LDS, took 10 us more for 300 rows of 64 adapters).
+// 64 rows, one a lane: the lane's slot (slots: no adapter), and the lanes with the same one.
 struct Window {
   bool in;
   int slot;
@@ -660,11 +657,7 @@ struct Window {
     in = first + lane < m;
     slot = in ? index[first + lane] : -1;
     if (slot < 0 || slot >= slots) slot = slots;
-    same = __ballot(in);
-    for (int bit = 1; bit <= slots; bit <<= 1) {
-      const uint64_t set = __ballot((slot & bit) != 0);
-      same &= slot & bit ? set : ~set;
-    }
+    same = same_slot(slot, slots, in);
   }
   __device__ __forceinline__ int before() const { return __popcll(same & ((1ull << (threadIdx.x & 63)) - 1)); }
   __device__ __forceinline__ bool leads() const { return in && before() == 0; }
@@ -777,13 +770,12 @@ template <typename XT> void launch_lora(LoraArgs& g, hipStream_t st) {
   for (int p = 0; p < g.parts.count; ++p) vec_n = vec_n && g.parts.end[p] % 8 == 0;
   vec_n = vec_n && (int64_t)g.n * g.rank < (1 << 30);  // a slot's B by 32-bit offsets
   const int chunks = cut_columns(g.parts, kLoraFusedCols);
-  const int64_t ballots = lora_groups(g.m, g.slots);
-  g.groups = ballots, g.ordinal = ballots < g.m;
+  g.groups = lora_groups(g.m, g.slots);
   if (lora_one_launch(g.plan, g.m, g.k, g.rank, g.slots, chunks)) {
     by_rank(g.rank, [&](auto nb, auto pack) {
       if constexpr (32 * nb.value <= kLoraOneRank)
         by_bool(vec_k && vec_n, [&](auto v) {
-          qtts::launch(&lora_one_kernel<XT, nb.value, pack.value, v.value>, dim3(chunks, grid_y(ballots)), dim3(64 * kOneWaves), 0,
+          qtts::launch(&lora_one_kernel<XT, nb.value, pack.value, v.value>, dim3(chunks, grid_y(g.groups)), dim3(64 * kOneWaves), 0,
                        st, g);
         });
     });

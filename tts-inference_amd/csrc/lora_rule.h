@@ -13,12 +13,11 @@ constexpr int kLoraOneRank = 64;     // the largest rank of the one-launch kerne
 // Blocks of the rank: one of 16 entries, or of 32 each.
 inline int lora_blocks(int64_t rank) { return rank <= 16 ? 1 : (int)((rank + 31) / 32); }
 
-// Workgroups along the rows without a plan: m, one a row, most of which lead no group and end at once, but hold a
-// compute unit's LDS until they have read the index (64 rows of one adapter through gate_up, rank 16: 11.0 us); or
-// fewer than m, one a group, each of which walks the slots before its own, 90 ns each (that case: 5.5 us).
+// Workgroups along the rows without a plan: of up to 64 rows the groups of 16 rows of one slot, at most, if they are fewer (each
+// workgroup then looks for its own, 0.3 us; 64 rows of 8 adapters through gate_up, rank 64: 13.5 us with one a row, 12.7), else
+// one a row (64 of 64: 39.2, and 41.0 with the search).
 inline int64_t lora_groups(int64_t m, int64_t slots) {
-  const int64_t most = std::min<int64_t>(m, slots + 1) + m / 16;
-  return m <= 64 && 8 * slots <= m ? most : m;
+  return m <= 64 ? std::min<int64_t>(m, std::min<int64_t>(m, slots + 1) + m / 16) : m;
 }
 
 // 16-row tiles of A (all partitions' `tiles`; past rank 16, PACK false, two a block) that a workgroup of the first product takes:
