@@ -839,12 +839,7 @@ def _gpu_index(first: torch.Tensor, *others: torch.Tensor | None) -> int:
     return idx
 
 
-def _call(idx: int, fn, *args) -> int:
-    """``fn(*args)`` with GPU ``idx`` current."""
-    if idx == torch._C._cuda_getDevice():
-        return fn(*args)
-    with torch.cuda.device(idx):
-        return fn(*args)
+_current_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 
 
 def _codes_out(a: torch.Tensor, k: int, codes: int) -> tuple[torch.Tensor, torch.Tensor]:
@@ -865,31 +860,33 @@ def rms_norm_quant(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, res
     normed the norm's 16-bit value (None unless ``want_normed``), both in x's shape.  The norm's value goes to its
     code from fp32, ``sx = max(amax, 1e-6) / 448`` (e4m3) or ``/ 127`` (int8); feed ``qx, sx`` to
     :func:`w8a8_fp8_gemm_strips` / :func:`w8a8_int8_gemm_strips`."""
-    a = _flatten(x)
+    a, shape, dtype = _flatten(x), x.shape, x.dtype
     rows, k = a.shape
-    dtype = a.dtype
     if weight.numel() != k:
         raise ValueError(f"norm weight has {weight.numel()} entries for rows of {k}")
     res = None
     if residual is not None:
-        if residual.shape != x.shape or residual.dtype != dtype:
-            raise ValueError(f"residual must be {tuple(x.shape)} {x.dtype}, got {tuple(residual.shape)} {residual.dtype}")
+        if residual.shape != shape or residual.dtype != dtype:
+            raise ValueError(f"residual must be {tuple(shape)} {dtype}, got {tuple(residual.shape)} {residual.dtype}")
         res = _flatten(residual)
     idx = _gpu_index(a, weight, res)
+    if idx != _current_device():
+        with torch.cuda.device(idx):
+            return rms_norm_quant(x, weight, eps, residual, codes, want_normed)
     w = weight if weight.dtype == dtype and weight.is_contiguous() else weight.to(dtype).contiguous()
     code = dtype_code(dtype)
     qx, sx = _codes_out(a, k, codes)
     hidden = None if res is None else torch.empty(rows, k, dtype=dtype, device=a.device)
     normed = torch.empty(rows, k, dtype=dtype, device=a.device) if want_normed else None
-    st = _call(idx, _lib.load().qtts_rms_norm_quant, a.data_ptr(), code, rows, k, a.stride(0) if rows > 1 else k,
-               None if res is None else res.data_ptr(), res.stride(0) if res is not None and rows > 1 else k, w.data_ptr(),
-               eps, codes, qx.data_ptr(), sx.data_ptr(), None if hidden is None else hidden.data_ptr(), k,
-               None if normed is None else normed.data_ptr(), k, torch._C._cuda_getCurrentRawStream(idx))
+    st = _lib.load().qtts_rms_norm_quant(
+        a.data_ptr(), code, rows, k, a.stride(0) if rows > 1 else k, None if res is None else res.data_ptr(),
+        res.stride(0) if res is not None and rows > 1 else k, w.data_ptr(), eps, codes, qx.data_ptr(), sx.data_ptr(),
+        None if hidden is None else hidden.data_ptr(), k, None if normed is None else normed.data_ptr(), k, _raw_stream(idx))
     if st:
         _lib.check(st, "rms_norm_quant")
-    if x.dim() != 2:
-        hidden = None if hidden is None else hidden.view(x.shape)
-        normed = None if normed is None else normed.view(x.shape)
+    if len(shape) != 2:
+        hidden = None if hidden is None else hidden.view(shape)
+        normed = None if normed is None else normed.view(shape)
     return qx, sx, hidden, normed
 
 
@@ -901,11 +898,14 @@ def silu_mul_quant(gate_up: torch.Tensor, codes: int = CODE_E4M3, want_act: bool
     a = _gate_up_rows(gate_up)
     rows, k = a.shape[0], a.shape[1] // 2
     idx, code = _gpu_index(a), dtype_code(a.dtype)
+    if idx != _current_device():
+        with torch.cuda.device(idx):
+            return silu_mul_quant(gate_up, codes, want_act)
     qx, sx = _codes_out(a, k, codes)
     act = torch.empty(rows, k, dtype=a.dtype, device=a.device) if want_act else None
-    st = _call(idx, _lib.load().qtts_silu_mul_quant, a.data_ptr(), code, rows, k, a.stride(0) if rows > 1 else 2 * k, codes,
-               qx.data_ptr(), sx.data_ptr(), None if act is None else act.data_ptr(), k,
-               torch._C._cuda_getCurrentRawStream(idx))
+    st = _lib.load().qtts_silu_mul_quant(
+        a.data_ptr(), code, rows, k, a.stride(0) if rows > 1 else 2 * k, codes, qx.data_ptr(), sx.data_ptr(),
+        None if act is None else act.data_ptr(), k, _raw_stream(idx))
     if st:
         _lib.check(st, "silu_mul_quant")
     return qx, sx, act if act is None else _shaped(act, shape)
@@ -962,10 +962,13 @@ def lora_batch(index: torch.Tensor, slots: int, plan: torch.Tensor | None = None
     idx = _gpu_index(index)
     need = _plan_bytes(batch.rows, batch.slots)
     if need:
+        if idx != _current_device():
+            with torch.cuda.device(idx):
+                return lora_batch(index, slots, plan)
         if plan is None:
             batch.plan = plan = torch.empty(need // 4, dtype=torch.int32, device=index.device)
-        st = _call(idx, _lib.load().qtts_lora_plan, index.data_ptr(), batch.rows, batch.slots, plan.data_ptr(),
-                   plan.numel() * 4, torch._C._cuda_getCurrentRawStream(idx))
+        st = _lib.load().qtts_lora_plan(index.data_ptr(), batch.rows, batch.slots, plan.data_ptr(), plan.numel() * 4,
+                                        _raw_stream(idx))
         if st:
             _lib.check(st, "lora_plan")
     return batch
@@ -1012,6 +1015,9 @@ def lora_add(base: torch.Tensor, x: torch.Tensor, batch: LoraBatch, a: torch.Ten
     if ranks is not None and (ranks.numel() != slots or ranks.dtype != torch.int32 or not ranks.is_contiguous()):
         raise ValueError(f"ranks must be {slots} contiguous int32 entries")
     idx, code = _gpu_index(xr, br, a, b, scaling, ranks, batch.index), dtype_code(dtype)
+    if idx != _current_device():
+        with torch.cuda.device(idx):
+            return lora_add(base, x, batch, a, b, scaling, ranks, partitions, out)
     if out is None:
         y, ldy = torch.empty(m, n, dtype=dtype, device=xr.device), n
     else:
@@ -1023,11 +1029,11 @@ def lora_add(base: torch.Tensor, x: torch.Tensor, batch: LoraBatch, a: torch.Ten
     if ws is None or ws.numel() < need:
         _ensure_workspace(xr.device, need, "lora_add")
         ws = _workspaces[idx]
-    st = _call(idx, _lib.load().qtts_lora_add, xr.data_ptr(), code, m, k, xr.stride(0) if m > 1 else k,
-               batch.index.data_ptr(), None if batch.plan is None else batch.plan.data_ptr(), slots, a.data_ptr(),
-               b.data_ptr(), rank, None if ranks is None else ranks.data_ptr(), scaling.data_ptr(), ends, parts,
-               br.data_ptr(), br.stride(0) if m > 1 else n, y.data_ptr(), n, ldy, ws.data_ptr(), ws.numel(),
-               torch._C._cuda_getCurrentRawStream(idx))
+    st = _lib.load().qtts_lora_add(
+        xr.data_ptr(), code, m, k, xr.stride(0) if m > 1 else k, batch.index.data_ptr(),
+        None if batch.plan is None else batch.plan.data_ptr(), slots, a.data_ptr(), b.data_ptr(), rank,
+        None if ranks is None else ranks.data_ptr(), scaling.data_ptr(), ends, parts, br.data_ptr(),
+        br.stride(0) if m > 1 else n, y.data_ptr(), n, ldy, ws.data_ptr(), ws.numel(), _raw_stream(idx))
     if st:
         _lib.check(st, "lora_add")
     if out is not None:
