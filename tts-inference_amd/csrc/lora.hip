@@ -23,13 +23,13 @@
 //
 // What bounds them, bf16 (a large copy runs at 5.1 TB/s here):
 //  * one launch: latency, three round trips to memory (the index; x, A, B and base; the result).  Rank 16, one row through 2048 x
-//    2048 in 5.6 us, 27 rows of 9 adapters through 2048 -> 12288 in 9.3 (14 MB of A and B);
+//    2048 in 5.6 us, 27 rows of 9 adapters through 2048 -> 12288 in 8.5 (14 MB of A and B);
 //  * the first product: how much one compute unit can load, which is why K's parts and A's tiles get workgroups of their own while
-//    groups are few.  64 rows of 32 rank-64 adapters, two partitions of 2048 (17 MB of A), in 6.4 us; 2048 rows of 8 rank-16
+//    groups are few.  64 rows of 32 rank-64 adapters, two partitions of 2048 (17 MB of A), in 7.3 us; 2048 rows of 8 rank-16
 //    adapters, K = 2048, in 5.6 (8 MB of x), K = 6144 in 10.4; past rank 32 and a thousand rows A's re-reads, once a group through
 //    L2 (4096 rows, rank 64, three partitions of K = 2048: 280 MB of them in 42);
 //  * the second product: base and the result, or B where rows are few.  2048 rows through 2048 -> 12288, rank 16, in 23.4 us
-//    (101 MB, 4.3 TB/s); 64 rows of 32 rank-64 adapters (51 MB of B) in 14.7.
+//    (101 MB, 4.3 TB/s); 64 rows of 32 rank-64 adapters (51 MB of B) in 12.0.
 #include <algorithm>
 
 #include "common.h"
