@@ -298,3 +298,20 @@ def test_a_row_does_not_depend_on_its_batch(ops):
     perm = torch.randperm(40, generator=torch.Generator().manual_seed(1)).cuda()
     d = dict(c, x=c["x"][perm], base=c["base"][perm], index=c["index"][perm])
     assert torch.equal(_run(ops, d), want[perm])
+
+
+def test_first_calls_of_a_process(ops, monkeypatch):
+    """Without a workspace yet: a call of no rows or no columns needs none, any other reserves its own."""
+    monkeypatch.setattr(ops, "_workspaces", {})
+    for shape in ((0, 40), (2, 0, 40), (3, 0)):
+        base = torch.empty(shape, dtype=torch.bfloat16, device="cuda")
+        m, n = base.numel() // shape[-1] if shape[-1] else 3, shape[-1]
+        batch = ops.lora_batch(torch.zeros(m, dtype=torch.int32, device="cuda"), 2)
+        a, b = (torch.zeros(2, *s, dtype=torch.bfloat16, device="cuda") for s in ((8, 64), (n, 8)))
+        x = torch.zeros((*shape[:-1], 64), dtype=torch.bfloat16, device="cuda")
+        y = ops.lora_add(base, x, batch, a, b, torch.ones(2, device="cuda"))
+        assert y.shape == base.shape and not ops._workspaces
+        assert ops.lora_add(base, x, batch, a, b, torch.ones(2, device="cuda"), out=base) is base
+    c = _case(5, 64, [40], 2, 8, torch.bfloat16, seed=71)
+    _check(_run(ops, c), c)
+    assert len(ops._workspaces) == 1

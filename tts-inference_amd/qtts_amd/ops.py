@@ -1025,6 +1025,8 @@ def lora_add(base: torch.Tensor, x: torch.Tensor, batch: LoraBatch, a: torch.Ten
         if y.shape != (m, n) or y.dtype != dtype or y.get_device() != idx or y.data_ptr() != out.data_ptr():
             raise ValueError(f"out must be a [{m}, {n}] {dtype} tensor on {xr.device}")
         ldy = y.stride(0) if m > 1 else n
+    if not m or not n:
+        return y.view(base.shape) if out is None else out
     ws = _workspaces.get(idx)
     if ws is None or ws.numel() < need:
         _ensure_workspace(xr.device, need, "lora_add")
