@@ -68,8 +68,7 @@ def test_attach_finds_the_named_linears_and_their_partitions():
     for bad in ({"slots": 0}, {"rank": 0}, {"rank": 129}):
         kw = {"slots": 4, "rank": 8, **bad}
         with pytest.raises(ValueError):
-            attach_adapters(_fill(Block()), routing=AdapterRouting(max(kw["slots"], 1), 8, device="cpu") if kw["slots"] else routing,
-                            **kw)
+            attach_adapters(_fill(Block()), routing=AdapterRouting(4, 8, device="cpu"), **kw)
 
 
 def test_load_lays_adapters_out_by_partition():
@@ -169,7 +168,10 @@ def test_row_forms_hold_the_row(tmp_path):
 int main() {
   const long long ms[] = {1, 1003, 1 << 22, (1 << 22) + 1, 1 << 25};
   for (long long m : ms) {
-    for (long long k = 0; k <= 16500; ++k) { auto f = qtts::row_form(m, k); printf("%lld %lld %d %d\\n", m, k, f.threads, f.vectors); }
+    for (long long k = 0; k <= 16500; ++k) {
+      auto f = qtts::row_form(m, k);
+      printf("%lld %lld %d %d\\n", m, k, f.threads, f.vectors);
+    }
     auto f = qtts::row_form(m, 1 << 20); printf("%lld %d %d %d\\n", m, 1 << 20, f.threads, f.vectors);
   }
 }

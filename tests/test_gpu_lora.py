@@ -103,8 +103,9 @@ def test_wide_outputs(ops, m, parts, slots, rank, dtype):
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
 @pytest.mark.parametrize("k", [2048, 2056, 2104, 6144])
-@pytest.mark.parametrize("m,parts,slots,rank", [(60, [4096], 30, 16), (60, [1024], 40, 64), (63, [520, 264], 63, 24), (70, [1024], 3, 8),
-                                                (300, [520, 264], 4, 40), (1003, [1024], 30, 16), (130, [64] * 5, 2, 16)])
+@pytest.mark.parametrize("m,parts,slots,rank", [
+    (60, [4096], 30, 16), (60, [1024], 40, 64), (63, [520, 264], 63, 24), (70, [1024], 3, 8), (300, [520, 264], 4, 40),
+    (1003, [1024], 30, 16), (130, [64] * 5, 2, 16)])
 def test_long_k_in_parts(ops, m, parts, slots, rank, k, dtype):
     """Few groups and a long K: the first product in two parts of K, which the second adds.  Each part's sum is carried in 2^-17 of
     its own magnitude, which is at most that of all of K's products: within the bound's fp32 term, 2 K u >= 2^-12 of those."""
@@ -315,3 +316,36 @@ def test_first_calls_of_a_process(ops, monkeypatch):
     c = _case(5, 64, [40], 2, 8, torch.bfloat16, seed=71)
     _check(_run(ops, c), c)
     assert len(ops._workspaces) == 1
+
+
+@pytest.mark.parametrize("m", [6, 70])
+@pytest.mark.parametrize("k,parts,slots,rank", [(4096, [64] * 8, 540, 128), (64, [65536], 300, 128)], ids=["a", "b"])
+def test_adapters_past_32_bits(ops, k, parts, slots, rank, m):
+    """Adapters whose bytes pass 2^32: rows of the first slots, the last and those on either side of that offset."""
+    n = sum(parts)
+    shapes = (slots, len(parts) * rank, k), (slots, n, rank)
+    used = sorted({0, 1, slots - 1} | {min(slots - 1, (1 << sh) // (2 * s[1] * s[2]) + d) for s in shapes for sh in (31, 32)
+                                       for d in (0, 1)})
+    a, b = (torch.empty(s, dtype=torch.bfloat16, device="cuda") for s in shapes)
+    assert max(a.numel(), b.numel()) * 2 > 1 << 32
+    for i, slot in enumerate(used):
+        a[slot], b[slot] = _rand(shapes[0][1:], torch.bfloat16, i, k ** -0.5), _rand(shapes[1][1:], torch.bfloat16, 50 + i, 0.2)
+    index = torch.tensor([used[i % len(used)] for i in range(m)], dtype=torch.int32)
+    c = {"base": _rand((m, n), torch.bfloat16, 1), "x": _rand((m, k), torch.bfloat16, 2), "index": index.cuda(), "a": a, "b": b,
+         "scaling": torch.full((slots,), 0.5, device="cuda"), "ranks": None, "parts": parts, "slots": slots, "rank": rank}
+    _check(_run(ops, c), c)
+
+
+@pytest.mark.parametrize("m", [50, 70])
+def test_rows_past_32_bits(ops, m):
+    """x, base and out with rows so far apart that their offsets pass 2^32 elements' bytes; what lies between stays as it was."""
+    pitch = (1 << 26) + 8
+    wide = [torch.empty((m - 1) * pitch + 64, dtype=torch.bfloat16, device="cuda") for _ in range(3)]
+    x, base, out = (w.as_strided((m, 64), (pitch, 1)) for w in wide)
+    c = _case(m, 64, [40, 24], 5, 16, torch.bfloat16, seed=81)
+    x.copy_(c["x"]), base.copy_(c["base"])
+    edges = wide[2].as_strided((m - 1, 64), (pitch, 1), 64)
+    edges.fill_(3.0)
+    ops.lora_add(base, x, ops.lora_batch(c["index"], 5), c["a"], c["b"], c["scaling"], c["ranks"], c["parts"], out=out)
+    _check(out.contiguous(), c)
+    assert (edges == 3.0).all()

@@ -263,3 +263,18 @@ def test_more_rows_than_workgroups(ops):
     _check_codes(q[pick], s[pick], _norm64(x[pick], w, 1e-6), 0, rel(k), "many rows")
     q, s, _ = ops.silu_mul_quant(x, 1)
     _check_codes(q[pick], s[pick], _silu64(x[pick]), 1, rel(0), "many rows")
+
+
+@pytest.mark.parametrize("k", [64, 63])
+def test_rows_past_32_bits(ops, k):
+    """Rows so far apart that their offsets pass 2^32 elements' bytes give what the same rows do side by side."""
+    m, pitch = 40, (1 << 26) + 8
+    wide = [torch.empty((m - 1) * pitch + 2 * k, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    x, res, gu = (w.as_strided((m, c), (pitch, 1)) for w, c in zip(wide + wide[:1], (k, k, 2 * k)))
+    g = torch.Generator(device="cuda").manual_seed(k)
+    gu.copy_(torch.randn(m, 2 * k, generator=g, device="cuda")), res.copy_(torch.randn(m, k, generator=g, device="cuda"))
+    w = torch.ones(k, dtype=torch.bfloat16, device="cuda")
+    near = ops.rms_norm_quant(x.contiguous(), w, 1e-6, res.contiguous(), 1, True)
+    for got, want in ((ops.rms_norm_quant(x, w, 1e-6, res, 1, True), near),
+                      (ops.silu_mul_quant(gu, 0, True), ops.silu_mul_quant(gu.contiguous(), 0, True))):
+        assert all(torch.equal(p.view(torch.uint8), q.view(torch.uint8)) for p, q in zip(got, want))
