@@ -102,6 +102,22 @@ def test_wide_outputs(ops, m, parts, slots, rank, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("rank", [1, 2, 3, 4, 5, 7, 9, 12, 15, 17, 20, 31, 33, 50, 63, 65, 90, 100, 127])
+def test_ranks_off_eight(ops, rank, dtype):
+    """B's rows start anywhere: every slot's last columns, the last slot's among them, with values behind B that are no part of it."""
+    for m, k, parts, slots in ((1, 64, [8], 1), (7, 256, [24, 8], 3), (60, 512, [2048, 72], 33), (150, 128, [264, 520], 4)):
+        index = torch.arange(m, dtype=torch.int32) % (slots + 1)
+        index[index == slots] = slots - 1
+        c = _case(m, k, parts, slots, rank, dtype, seed=m + rank, index=index, mixed=False)
+        room = torch.full((c["b"].numel() + 64,), float("nan"), dtype=dtype, device="cuda")
+        room[:c["b"].numel()] = c["b"].flatten()
+        c["b"] = room[:c["b"].numel()].view(c["b"].shape)
+        _check(_run(ops, c), c, f"m={m}")
+        c["ranks"] = torch.full((slots,), max(1, rank - 1), dtype=torch.int32, device="cuda")
+        _check(_run(ops, c), c, f"m={m}, ranks short by one")
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
 @pytest.mark.parametrize("k", [2048, 2056, 2104, 6144])
 @pytest.mark.parametrize("m,parts,slots,rank", [
     (60, [4096], 30, 16), (60, [1024], 40, 64), (63, [520, 264], 63, 24), (70, [1024], 3, 8), (300, [520, 264], 4, 40),

@@ -355,13 +355,31 @@ template <typename XT, int NB, bool PACK, int S = 1> struct TOperand {
   }
 };
 
-// A slot's B by columns: an operand of 16 columns from c is the lane's eight entries of each block of rows c + lane % 16.  VEC: a
-// lane's place as bytes in the slot's B (32 bits: the host checks), clamped to the partition's last column.  Entries past the
-// slot's rank may hold anything, and those past the rank are no part of the row: a lane of such entries reads others of its row,
-// and masks them.  (No load is in a branch: the compiler may give each side of one its own copy of the MFMAs after it.)
-template <typename XT, int NB, bool PACK, bool VEC> struct Columns {
+// A slot's B by columns: an operand of 16 columns from c is the lane's eight entries of each block of rows c + lane % 16.  Read as
+// 16 bytes (a lane's place as bytes in the slot's B, 32 bits: the host checks; clamped to the partition's last column), aligned where
+// the rank is a multiple of 8, at any address elsewhere (gate_up of 2048 rows, rank 4: entry by entry 80.6 us, so 30.2, as rank 8
+// aligned; one form for both cost rank 64 up to 6%), or entry by entry where base or out forbid vectors.  Entries past the slot's
+// rank may hold anything, and those past the rank are no part of the row: a lane of such entries reads others of its row, a rank
+// that is no multiple of 8 has its last lane read into the next row, and all of them are masked; the last slot's last rows have none
+// behind them, and are read from further ahead and shifted.  (No load is in a branch: the compiler may give each side of one its
+// own copy of the MFMAs after it.)
+enum { kByEntry, kAligned, kAnywhere };
+
+struct __attribute__((packed, aligned(2))) Unaligned16 { i32x4_t v; };
+
+// v's bytes from `back` (even, below 16) on, zeros behind.
+__device__ __forceinline__ i32x4_t from_byte(i32x4_t v, uint32_t back) {
+  const uint64_t lo = (uint64_t)(uint32_t)v[1] << 32 | (uint32_t)v[0], hi = (uint64_t)(uint32_t)v[3] << 32 | (uint32_t)v[2];
+  const uint32_t s = 8 * (back & 7);
+  const uint64_t low = lo >> s | (s ? hi << (64 - s) : 0), high = hi >> s;
+  const uint64_t l = back >= 8 ? high : low, h = back >= 8 ? 0 : high;
+  return i32x4_t{(int)l, (int)(l >> 32), (int)h, (int)(h >> 32)};
+}
+
+template <typename XT, int NB, bool PACK, int B> struct Columns {
   const char* slot_b;
   uint32_t at, last, step;  // of column c0 + lane % 16, of the last column, from one operand to the next
+  uint32_t most;            // the last place with 16 bytes of all B from it
   int rank, c, end;
   bool masks;
   int first[NB];
@@ -373,10 +391,11 @@ template <typename XT, int NB, bool PACK, bool VEC> struct Columns {
     rank = g.rank, c = c0 + (int)(threadIdx.x & 15), end = part_end;
     at = (uint32_t)c * (uint32_t)rank * 2, last = (uint32_t)(end - 1) * (uint32_t)rank * 2, step = 32 * (uint32_t)rank;
     masks = live != (PACK ? 16 : 32 * NB);
+    most = slot == g.slots - 1 ? (uint32_t)g.n * (uint32_t)rank * 2 - 16 : 0xffffffffu;
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
       const int e = 32 * b + 8 * (PACK ? q & 1 : q);
-      first[b] = VEC && e >= rank ? 0 : e;
+      first[b] = B != kByEntry && e >= rank ? 0 : e;
 #pragma unroll
       for (int i = 0; i < 4; ++i) shown[b][i] = live - e - 2 * i >= 2 ? -1 : live - e - 2 * i == 1 ? 0xffff : 0;
     }
@@ -385,10 +404,14 @@ template <typename XT, int NB, bool PACK, bool VEC> struct Columns {
   // The operand of the next 16 columns.
   __device__ __forceinline__ void next(vec8<XT> (&v)[NB]) {
     i32x4_t r[NB];
-    if constexpr (VEC) {
+    if constexpr (B != kByEntry) {
       const uint32_t from = at < last ? at : last;
 #pragma unroll
-      for (int b = 0; b < NB; ++b) r[b] = *(const i32x4_t*)(slot_b + (from + 2 * first[b]));
+      for (int b = 0; b < NB; ++b) {
+        const uint32_t place = from + 2 * first[b];
+        if constexpr (B == kAligned) r[b] = *(const i32x4_t*)(slot_b + place);
+        else r[b] = from_byte(((const Unaligned16*)(slot_b + min(place, most)))->v, place - min(place, most));
+      }
       at += step;
     } else {
       const XT* row = (const XT*)slot_b + (int64_t)min(c, end - 1) * rank;
@@ -522,9 +545,9 @@ constexpr int kUpWaves = 4, kUpTiles = 4, kUpBlock = 16 * kUpTiles;
 
 // Grid: (blocks of g.up_cols columns, groups).  A wave takes 64 columns at a time: with a plan, whose groups of one slot follow
 // one another, all columns of a group of its own; else a part of the workgroup's group.
-template <typename XT, int NB, bool PACK, bool VEC, bool PLAN, int S>
+template <typename XT, int NB, bool PACK, int B, bool PLAN, int S>
 __global__ __launch_bounds__(64 * kUpWaves) void lora_up_kernel(LoraArgs g) {
-  typedef Rows<XT, kUpTiles, VEC> R;
+  typedef Rows<XT, kUpTiles, B != kByEntry> R;
   __shared__ __align__(16) float lds[kUpWaves][R::kFloats];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const Block blk = block_of(g, blockIdx.x, g.up_cols);
@@ -552,7 +575,7 @@ __global__ __launch_bounds__(64 * kUpWaves) void lora_up_kernel(LoraArgs g) {
     }
     TOperand<XT, NB, PACK, S> t;
     t.load(g, gr.row, blk.part);
-    Columns<XT, NB, PACK, VEC> columns(g, gr.slot, c0, blk.end, live);
+    Columns<XT, NB, PACK, B> columns(g, gr.slot, c0, blk.end, live);
     vec8<XT> b[kUpTiles][NB];
 #pragma unroll
     for (int n = 0; n < kUpTiles; ++n) columns.next(b[n]);
@@ -573,9 +596,10 @@ constexpr int kOneStages = 2, kOneWaves = 8, kOneTiles = kLoraFusedCols / (16 * 
 
 // Grid: (column blocks, rows).  The workgroup's waves share K of the first product, for its partition's rows of A alone, and
 // meet in LDS; then each multiplies its own columns.
-template <typename XT, int NB, bool PACK, bool VEC>
+template <typename XT, int NB, bool PACK, int B>
 __global__ __launch_bounds__(64 * kOneWaves) void lora_one_kernel(LoraArgs g) {
   constexpr int NT = kOneTiles, T = kBlockTiles<PACK>, N = T * NB;  // 16-row tiles of A
+  constexpr bool VEC = B != kByEntry;
   typedef Rows<XT, NT, VEC> R;
   // A wave's stages; then its sums, later its result, in the first 4 KiB, and in the first wave's part the halves past them.
   constexpr int kHalves = NB * 16 * kBlockBytes<PACK>, kUsed = 4096 + kHalves + NB * 64;
@@ -601,7 +625,7 @@ __global__ __launch_bounds__(64 * kOneWaves) void lora_one_kernel(LoraArgs g) {
       rows.copy();
       continue;
     }
-    Columns<XT, NB, PACK, VEC> columns(g, gr.slot, c0, blk.end, live);
+    Columns<XT, NB, PACK, B> columns(g, gr.slot, c0, blk.end, live);
     vec8<XT> b[NT][NB];
 #pragma unroll
     for (int n = 0; n < NT; ++n) columns.next(b[n]);
@@ -751,6 +775,12 @@ template <typename F> void by_bool(bool v, F&& f) {
   else f(std::false_type{});
 }
 
+template <typename F> void by_kind(int b, F&& f) {
+  if (b == kAligned) f(std::integral_constant<int, kAligned>{});
+  else if (b == kAnywhere) f(std::integral_constant<int, kAnywhere>{});
+  else f(std::integral_constant<int, kByEntry>{});
+}
+
 // Column blocks of `cols` columns, none across a partition's end.
 int cut_columns(LoraParts& parts, int cols) {
   int chunks = 0;
@@ -764,17 +794,19 @@ int cut_columns(LoraParts& parts, int cols) {
 bool aligned(const void* p, int64_t ld) { return (uintptr_t)p % 16 == 0 && ld % 8 == 0; }
 
 template <typename XT> void launch_lora(LoraArgs& g, hipStream_t st) {
-  // The operands of each product as 16-byte vectors: its rows start on 16 bytes and its widths are multiples of 8.
+  // The operands of each product as 16-byte vectors: x's, A's, base's and out's rows start on 16 bytes and K and the partitions are
+  // multiples of 8; B's rows start anywhere, but a slot's B has 32-bit offsets, and 16 bytes at the least.
   const bool vec_k = g.k % 8 == 0 && aligned(g.x, g.ldx) && aligned(g.a, 0);
-  bool vec_n = g.rank % 8 == 0 && aligned(g.b, 0) && aligned(g.base, g.ldb) && aligned(g.out, g.ldo);
+  const int64_t slot_b = (int64_t)g.n * g.rank;
+  bool vec_n = aligned(g.base, g.ldb) && aligned(g.out, g.ldo) && slot_b >= 8 && slot_b < (1 << 30);
   for (int p = 0; p < g.parts.count; ++p) vec_n = vec_n && g.parts.end[p] % 8 == 0;
-  vec_n = vec_n && (int64_t)g.n * g.rank < (1 << 30);  // a slot's B by 32-bit offsets
+  const int b_kind = !vec_n ? kByEntry : g.rank % 8 == 0 && aligned(g.b, 0) ? kAligned : kAnywhere;
   const int chunks = cut_columns(g.parts, kLoraFusedCols);
   g.groups = lora_groups(g.m, g.slots);
   if (lora_one_launch(g.plan, g.m, g.k, g.rank, g.slots, chunks)) {
     by_rank(g.rank, [&](auto nb, auto pack) {
       if constexpr (32 * nb.value <= kLoraOneRank)
-        by_bool(vec_k && vec_n, [&](auto v) {
+        by_kind(vec_k ? b_kind : kByEntry, [&](auto v) {
           qtts::launch(&lora_one_kernel<XT, nb.value, pack.value, v.value>, dim3(chunks, grid_y(g.groups)), dim3(64 * kOneWaves), 0,
                        st, g);
         });
@@ -784,7 +816,7 @@ template <typename XT> void launch_lora(LoraArgs& g, hipStream_t st) {
   if (g.plan) g.groups = plan_max_groups(g.m, g.slots);
   const int a_tiles = g.parts.count * g.blocks * (g.rank <= 16 ? 1 : 2);
   const int down_tiles = lora_down_tiles(g.groups, a_tiles, g.rank <= 16), down_wide = (a_tiles + down_tiles - 1) / down_tiles;
-  g.splits = vec_k && vec_n ? lora_splits(g.m, g.k, g.rank, g.groups * down_wide) : 1;
+  g.splits = vec_k && b_kind == kAligned ? lora_splits(g.m, g.k, g.rank, g.groups * down_wide) : 1;
   by_bool(g.plan, [&](auto plan) {
     by_bool(g.rank <= 16, [&](auto pack) {
       by_bool(vec_k, [&](auto v) {
@@ -804,13 +836,13 @@ template <typename XT> void launch_lora(LoraArgs& g, hipStream_t st) {
     g.up_cols = lora_up_cols(g.m, g.n);
     const int up_chunks = cut_columns(g.parts, g.up_cols);
     by_rank(g.rank, [&](auto nb, auto pack) {
-      by_bool(vec_n, [&](auto v) {
+      by_kind(b_kind, [&](auto v) {
         auto up = [&](auto s) {
           qtts::launch(&lora_up_kernel<XT, nb.value, pack.value, v.value, plan.value, s.value>,
                        dim3(up_chunks, grid_y(plan.value ? (g.groups + kUpWaves - 1) / kUpWaves : g.groups)),
                        dim3(64 * kUpWaves), 0, st, g);
         };
-        if constexpr (v.value && 32 * nb.value <= kLoraSplitRank) {
+        if constexpr (v.value == kAligned && 32 * nb.value <= kLoraSplitRank) {
           if (g.splits == 2) return up(std::integral_constant<int, 2>{});
         }
         up(std::integral_constant<int, 1>{});
