@@ -137,7 +137,7 @@ def _hold(layer, y, qx, sx, x, index, adapters):
 @pytest.mark.parametrize("adapters", [False, True])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
 @pytest.mark.parametrize("method", ["fp8", "int8"])
-@pytest.mark.parametrize("m", [1, 7, 64, 131])
+@pytest.mark.parametrize("m", [0, 1, 7, 64, 131])
 def test_layer_stages(ops, method, dtype, adapters, m):
     from qtts_amd.layers.decoder import add_norm_linear, add_norm_mlp
     block, routing = _block(method, dtype, adapters=adapters)
