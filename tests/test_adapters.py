@@ -213,8 +213,8 @@ int main() {
   for (int rank = 1; rank <= 128; ++rank)
     for (int chunks = 1; chunks <= 48; ++chunks)
       for (int m = 1; m <= 64; m += 7)
-        printf("3 %d %d %d %d %d\\n", rank, chunks, m, (int)lora_one_launch(false, m, 2048, rank, 8, chunks),
-               (int)lora_one_launch(true, m, 2048, rank, 8, chunks));
+        printf("3 %d %d %d %d %d\\n", rank, chunks, m, (int)lora_one_launch(false, m, 2048, rank, 8, chunks, chunks < 8 ? chunks : 8),
+               (int)lora_one_launch(true, m, 2048, rank, 8, chunks, 1));
 }
 """)
     one = two = 0

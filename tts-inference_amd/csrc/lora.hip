@@ -803,7 +803,9 @@ template <typename XT> void launch_lora(LoraArgs& g, hipStream_t st) {
   const int b_kind = !vec_n ? kByEntry : g.rank % 8 == 0 && aligned(g.b, 0) ? kAligned : kAnywhere;
   const int chunks = cut_columns(g.parts, kLoraFusedCols);
   g.groups = lora_groups(g.m, g.slots);
-  if (lora_one_launch(g.plan, g.m, g.k, g.rank, g.slots, chunks)) {
+  int reads = 0;
+  for (int p = 0; p < g.parts.count; ++p) reads += std::min(8, g.parts.chunk_end[p] - (p ? g.parts.chunk_end[p - 1] : 0));
+  if (lora_one_launch(g.plan, g.m, g.k, g.rank, g.slots, chunks, reads)) {
     by_rank(g.rank, [&](auto nb, auto pack) {
       if constexpr (32 * nb.value <= kLoraOneRank)
         by_kind(vec_k ? b_kind : kByEntry, [&](auto v) {

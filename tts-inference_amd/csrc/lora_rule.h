@@ -49,15 +49,18 @@ inline int lora_up_cols(int64_t m, int64_t n) {
   return waves >= 16384 || m <= 64 ? 256 : waves >= 8192 ? 128 : 64;
 }
 
-// One launch, the first product recomputed by each workgroup along the columns, while its workgroups (two a compute unit to
-// rank 16, else one) and the A blocks that they all read stay few.  Captured calls over three adapters' worth of memory, us,
-// one launch / two: rank 16, o_proj of 1 row 4.9 / 7.3, gate_up of 8 rows of 8 adapters (384 workgroups, 24 MB) 7.7 / 8.4, of
-// 16 of 16 (768, 48 MB) 11.1 / 9.1; rank 32, qkv of 16 of 16 (256, 32 MB) 9.9 / 11.3, of 32 of 32 (64 MB) 17.5 / 12.5; rank 64,
-// gate_up of 4 of 4 (192, 48 MB) 9.7 / 10.9, of 8 of 8 (96 MB) 17.0 / 14.2; rank 8, gate_up of 16 of 16 (768, 24 MB)
-// 10.7 / 8.9.  Called one by one, the second launch costs 3 us of host time more.
-inline bool lora_one_launch(bool plan, int64_t m, int64_t k, int64_t rank, int64_t slots, int64_t chunks) {
-  const int64_t workgroups = chunks * std::min(m, std::min(m, slots) + m / 16);
-  return !plan && rank <= kLoraOneRank && workgroups <= 640 && workgroups * rank * k * 2 <= (40ll << 20);
+// One launch, the first product recomputed by each workgroup along the columns, while the workgroups (two a compute unit to rank 16,
+// else one) are little more than a round of them, and both a workgroup's A (what one compute unit then loads by itself) and all
+// reads of A past the L2s are small: every group's, once a die for each partition (`reads`: the partitions' workgroups along the
+// columns, at most 8 of each).  Captured calls over three adapters' worth of memory, us, one launch / two: rank 16, o_proj of 1 row
+// 5.0 / 6.9, qkv of 16 rows of 16 adapters (17 MB) 7.2 / 7.3, of 32 of 32 (34 MB) 10.2 / 8.5; rank 32, gate_up of 32 of 4 (13 MB)
+// 7.3 / 8.7, o_proj of 32 of 32 (34 MB) 9.9 / 8.4; rank 64, qkv of 4 of 4 (17 MB) 9.3 / 8.9, of 8 of 8 (34 MB) 10.6 / 9.7,
+// down_proj of 1 row (768 KiB a workgroup) 12.4 / 10.1, rank 32 (384 KiB) 8.6 / 9.1; gate_up, rank 16, of 16 of 16 (768 workgroups)
+// 10.8 / 8.1, rank 32, of 8 of 8 (384) 11.9 / 8.5.  Called one by one, the second launch costs 3 us of host time more.
+inline bool lora_one_launch(bool plan, int64_t m, int64_t k, int64_t rank, int64_t slots, int64_t chunks, int64_t reads) {
+  const int64_t groups = std::min(m, std::min(m, slots) + m / 16), a = rank * k * 2;
+  return !plan && rank <= kLoraOneRank && groups * chunks <= (rank <= 16 ? 640 : 320) && a <= 400 << 10 &&
+         groups * reads * a <= 20 << 20;
 }
 
 }  // namespace qtts
