@@ -430,7 +430,8 @@ int qtts_fp8w_gemm_strips(const void* x, int x_dtype, int64_t m, int64_t k, int6
  *   v[r, c] = h[r, c] * inv * f32(weight[c]),  inv = 1 / sqrt(sum_c h[r, c]^2 / k + eps)
  *   sx[r] = max(max_c |v[r, c]|, 1e-6) / L,    L = 448 (QTTS_CODE_E4M3) or 127 (QTTS_CODE_INT8)
  *   qx[r, c] = code(v[r, c] / sx[r])           (nearest, ties to even)
- * in one pass, with v in fp32 up to its code.  No counterpart in the reference, which adds
+ * in one pass, with v in fp32 up to its code and the quotient rounded once (above the scale's
+ * floor it is h weight L / max |h weight|, before v's and sx's own roundings).  No counterpart in the reference, which adds
  * (qtts/models/talker.py:270-271), normalizes (qtts/layers/norm.py:50-76) and quantizes
  * (qtts/quant/fp8.py:77-78, qtts/quant/int8.py:146-149) in separate kernels and rounds to
  * x_dtype between them; there the 1e-6 and, for int8, the scale are in x_dtype too.

@@ -278,3 +278,43 @@ def test_rows_past_32_bits(ops, k):
     for got, want in ((ops.rms_norm_quant(x, w, 1e-6, res, 1, True), near),
                       (ops.silu_mul_quant(gu, 0, True), ops.silu_mul_quant(gu.contiguous(), 0, True))):
         assert all(torch.equal(p.view(torch.uint8), q.view(torch.uint8)) for p, q in zip(got, want))
+
+
+@pytest.mark.parametrize("codes", [1, 0], ids=["e4m3", "int8"])
+@pytest.mark.parametrize("dtype", DTYPES[:2], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("m,k", [(1, 8), (64, 2048), (33, 4095), (5, 16386), (700, 1024)])
+def test_norm_codes_are_the_nearest(ops, m, k, dtype, codes):
+    """v / sx = h w L / max |h w| has ties, as h w and its maximum have few bits: each code is the nearest of that quotient, a tie's
+    the even one.  64 bits hold h w L exactly (16 or 22 bits by 9) and the division hits every tie; no other quotient of bf16 rows
+    is within 2^-24 of one, so their codes are equal.  fp16 (h w of 22 bits): quotients that are no tie but round to one in fp32, of
+    a relative distance under 2^-24 and of the other parity, are one code off; a hit needs a / b within 2^-24 of one of 127 ties,
+    for which no more than 1 in 2^10 of all quotients can be counted (each tie's interval is 2^-23 of its own size, 2^-8 or more
+    apart: 2^-14, and room for a row of few values)."""
+    w = (1 + _rand((k,), torch.float32, 41, 0.1)).to(dtype)
+    x, res = _rand((m, k), dtype, 42), _rand((m, k), dtype, 43, 2.0)
+    x[0], res[0], w[:8] = torch.arange(k, device="cuda") % 17 - 8, 0, 1  # whole numbers: ties in plenty
+    for r in (None, res):
+        q, s, _, _ = ops.rms_norm_quant(x, w, 1e-6, r, codes)
+        h = x if r is None else x + r
+        hw = h.double() * w.double()
+        want = hw * LIMIT[codes] / hw.abs().amax(1, keepdim=True)
+        want = want.round() if codes == 0 else want.to(torch.float32).to(torch.float8_e4m3fn).double()
+        off = int((q.double() != want).sum())
+        assert off == 0 if dtype == torch.bfloat16 else off <= want.numel() >> 10, f"{off} of {want.numel()} codes"
+
+
+@pytest.mark.parametrize("codes", [1, 0], ids=["e4m3", "int8"])
+def test_norm_codes_at_the_ends_of_the_range(ops, codes):
+    """Values whose product with the code range passes fp32, rows at and under the scale's floor, and eps of zero."""
+    k = 64
+    x = _rand((6, k), torch.float32, 44)
+    w = torch.ones(k, device="cuda")
+    w[5], w[9] = 1e20, -7e19
+    x[0] *= 1e18  # h w of 1e38 (and |x| < 3.4 of these few), h w L past fp32
+    x[1] *= 1e-30  # under eps: v of 1e-27
+    x[2] *= 1e-18
+    x[3] = 0
+    for eps in (1e-6, 0.0):
+        rows = [0, 1, 2, 3, 4, 5] if eps else [0, 2, 4, 5]  # (squares of 1e-30 vanish in fp32: without eps there is no norm)
+        q, s, _, _ = ops.rms_norm_quant(x[rows], w, eps, None, codes)
+        _check_codes(q, s, _norm64(x[rows], w, eps), codes, rel(k), f"eps {eps}")
