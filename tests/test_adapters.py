@@ -89,6 +89,21 @@ def test_load_lays_adapters_out_by_partition():
     assert not bank.lora_a[1].any() and not bank.lora_b[1].any() and bank.lora_ranks.tolist() == [0, 0, 2]
 
 
+def test_load_takes_a_training_modules_parameters():
+    """The bank holds values: loading tensors that require grad leaves no graph behind, however often a slot is reloaded."""
+    import copy
+
+    bank = LinearAdapters(8, [6, 4], 3, 5, torch.float32, "cpu")
+    a, b = nn.Parameter(torch.randn(5, 8)), nn.Parameter(torch.randn(10, 5))
+    for _ in range(3):
+        bank.load(1, a, b)
+        assert not any(t.requires_grad or t.grad_fn is not None for t in bank.buffers())
+    assert torch.equal(bank.lora_a[1, :5], a.detach()) and torch.equal(bank.lora_b[1, 6:, :5], b.detach()[6:])
+    assert torch.equal(copy.deepcopy(bank).lora_a, bank.lora_a)
+    bank.clear(1)
+    assert not any(t.requires_grad for t in bank.buffers()) and a.grad is None
+
+
 def test_load_refusals_leave_the_slot():
     bank = LinearAdapters(8, [6, 4], 3, 5, torch.float32, "cpu")
     a, b0, b1 = torch.randn(5, 8), torch.randn(6, 5), torch.randn(4, 5)

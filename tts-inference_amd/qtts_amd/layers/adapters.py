@@ -82,6 +82,7 @@ class LinearAdapters(nn.Module):
         self.register_buffer("lora_scaling", torch.zeros(slots, dtype=torch.float32, device=device), persistent=False)
         self.register_buffer("lora_ranks", torch.zeros(slots, dtype=torch.int32, device=device), persistent=False)
 
+    @torch.no_grad()  # the values alone: a's and b's graph does not become the bank's
     def load(self, slot: int, a, b, scaling: float = 1.0) -> None:
         """Adapter ``slot``: A ``[r, K]`` and B ``[N, r]``, or lists of one of each a partition (None: that partition
         has none).  One A serves every partition, and one B of all output channels is cut by partition."""
@@ -113,6 +114,7 @@ class LinearAdapters(nn.Module):
         self.lora_scaling[slot] = float(scaling)
         self.lora_ranks[slot] = max((ap.shape[0] for ap in a if ap is not None), default=0)
 
+    @torch.no_grad()
     def clear(self, slot: int) -> None:
         """Slot ``slot`` without an adapter: its rows get the shared projection alone."""
         self.lora_a[slot].zero_()
