@@ -176,3 +176,31 @@ def test_wrappers_check_shapes_and_types():
                       ("GPU tensor", {})):
         with pytest.raises(ValueError, match=match):
             call(**kw)
+
+
+def test_a_torch_without_gpu_bindings_imports_and_refuses():
+    """A CPU build of torch has no device and stream calls in its bindings: the package imports there (its checkers, packers' formats
+    and configuration need no GPU) and an operator refuses the CPU tensor."""
+    import os
+    import subprocess
+    import sys
+
+    code = """
+import torch
+for name in ("_cuda_getDevice", "_cuda_getCurrentRawStream"):
+    if hasattr(torch._C, name):
+        delattr(torch._C, name)
+from qtts_amd import ops
+for call in (lambda: ops.rms_norm_quant(torch.zeros(2, 64), torch.ones(64)), lambda: ops.silu_mul_quant(torch.zeros(2, 64)),
+             lambda: ops.lora_batch(torch.zeros(2, dtype=torch.int32), 3)):
+    try:
+        call()
+    except ValueError as e:
+        assert "GPU tensor" in str(e), e
+    else:
+        raise AssertionError("ran on the CPU")
+print("refused")
+"""
+    env = dict(os.environ, PYTHONPATH=os.pathsep.join(sys.path))
+    done = subprocess.run([sys.executable, "-c", code], env=env, capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0 and "refused" in done.stdout, done.stderr
