@@ -258,3 +258,35 @@ int main() {
             one, two = one + free, two + (not free)
     assert one and two
     assert seen == {(1, 1), (1, 2), (1, 3), (1, 4), (0, 2), (0, 4)}
+
+
+def test_quantizing_after_attaching_keeps_the_adapters():
+    """quantize_module puts its method under a linear's adapters, as attaching afterwards would; excluded and declined linears keep
+    what they had."""
+    from qtts_amd import QuantConfig, quantize_module
+    from qtts_amd.quant.base import QuantMethodBase
+
+    class Method(QuantMethodBase):
+        name = "marked"
+
+        def process_weights(self, layer):
+            layer.marked = layer.out_features != 32  # declines o_proj's width below
+
+        def applies_to(self, layer):
+            return layer.marked
+
+    block = _fill(Block())
+    block.o_proj = LinearBase(32, 32)
+    routing = AdapterRouting(4, 32, device="cpu")
+    attach_adapters(block, slots=4, rank=8, routing=routing, targets=("qkv", "o_proj", "down"))
+    method = Method()
+    report = quantize_module(block, method, QuantConfig(method="int8", exclude_substrings=("down_proj",)), "talker")
+    assert report["converted"] == 2 and report["declined"] == 1 and report["excluded"] == 1
+    qkv = block.qkv_proj.quant_method
+    assert isinstance(qkv, AdapterMethod) and qkv.inner is method and qkv.routing is routing
+    assert block.mlp.gate_up_proj.quant_method is method
+    for linear in (block.o_proj, block.mlp.down_proj):
+        assert isinstance(linear.quant_method, AdapterMethod) and linear.quant_method.inner is None
+    again = Method()
+    quantize_module(block, again, QuantConfig(method="int8"), "talker")  # another method: under the same adapters
+    assert block.qkv_proj.quant_method.inner is again and block.qkv_proj.quant_method.routing is routing

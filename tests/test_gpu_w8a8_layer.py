@@ -258,3 +258,19 @@ def test_what_the_helpers_leave_to_the_linear(ops):
     weight_only, _ = _block("int8_weight_only", torch.bfloat16, adapters=False)
     y, hidden = add_norm_linear(weight_only.norm1, weight_only.qkv, x, res)
     assert torch.equal(y, weight_only.qkv(weight_only.norm1(res + x))) and torch.equal(hidden, res + x)
+
+
+@pytest.mark.parametrize("method", ["fp8", "int8_weight_only"])
+def test_quantizing_before_or_after_attaching(ops, method):
+    """The order of attach_adapters and quantization is the caller's: the same bits either way."""
+    from qtts_amd import QuantConfig
+    from qtts_amd.quant.base import build_method, quantize_module
+    before, first = _block(method, torch.bfloat16)
+    after, second = _block("none", torch.bfloat16)
+    config = QuantConfig(method=method, calibrate=False)
+    assert quantize_module(after, build_method(config), config, "talker")["converted"] == 4
+    x, index = _rows(9, torch.bfloat16, 3), _index(9, 4)
+    first.set(index), second.set(index)
+    want = before.qkv(x)
+    first.set([-1] * 9)
+    assert not torch.equal(want, before.qkv(x)) and torch.equal(after.qkv(x), want)

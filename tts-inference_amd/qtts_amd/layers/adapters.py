@@ -9,7 +9,7 @@ hangs them on the same hook its quant methods use, so the model code does not ch
   each of its partitions;
 * :class:`AdapterRouting` says which slot each row of the step takes, for every linear of the model;
 * :class:`AdapterMethod` is the quant method that adds the one to the other;
-* :func:`attach_adapters` puts them on a model after ``apply_quantization``.
+* :func:`attach_adapters` puts them on a model, before or after ``apply_quantization``.
 
 Per step, a serving loop sets the routing, then runs the model::
 
@@ -135,6 +135,10 @@ class AdapterMethod(QuantMethodBase):
 
     def __init__(self, inner, routing: AdapterRouting) -> None:
         self.inner, self.routing = inner, routing
+
+    def over(self, method) -> AdapterMethod:
+        """These adapters on top of ``method`` (a linear that is quantized after its adapters were attached)."""
+        return AdapterMethod(method, self.routing)
 
     def applies_to(self, layer) -> bool:
         return getattr(layer, "adapters", None) is not None

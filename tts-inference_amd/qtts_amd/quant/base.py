@@ -90,7 +90,8 @@ def quantize_module(module: nn.Module, method: QuantMethodBase, config: QuantCon
         if not method.applies_to(layer):
             declined += 1
             continue
-        layer.quant_method = method
+        outer = getattr(layer, "quant_method", None)  # adapters attached before stay on top
+        layer.quant_method = outer.over(method) if hasattr(outer, "over") else method
         layer.quant_stream = stream
         converted += 1
         # a converted layer whose calibration routed some row bucket to F.linear keeps its weight
