@@ -488,6 +488,15 @@ int qtts_lora_add(const void* x, int x_dtype, int64_t m, int64_t k, int64_t ldx,
                   const float* scaling, const int64_t* part_ends, int64_t parts, const void* base, int64_t ldb,
                   void* out, int64_t n, int64_t ldo, void* ws, int64_t ws_bytes, void* stream);
 
+/* qtts_lora_add into an out that holds nothing yet: every row is written, whatever the plan holds.  A plan
+ * of another m or slots (a captured step replayed after the routing of another batch) is left aside, and the
+ * rows take the slots that index names, as without a plan. */
+int qtts_lora_add_fresh(const void* x, int x_dtype, int64_t m, int64_t k, int64_t ldx, const int32_t* index,
+                        const int32_t* plan, int64_t slots, const void* a, const void* b, int64_t rank,
+                        const int32_t* ranks, const float* scaling, const int64_t* part_ends, int64_t parts,
+                        const void* base, int64_t ldb, void* out, int64_t n, int64_t ldo, void* ws, int64_t ws_bytes,
+                        void* stream);
+
 /* Kernel timer.  No counterpart in the reference: benchmark instrumentation.
  * Between qtts_kernel_timer_begin and qtts_kernel_timer_end, each kernel the
  * library launches on a stream that is not capturing a graph records a start and

@@ -365,3 +365,30 @@ def test_rows_past_32_bits(ops, m):
     ops.lora_add(base, x, ops.lora_batch(c["index"], 5), c["a"], c["b"], c["scaling"], c["ranks"], c["parts"], out=out)
     _check(out.contiguous(), c)
     assert (edges == 3.0).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("m,k,parts,slots,rank", [(100, 64, [40], 5, 16), (1003, 128, [64, 72], 1, 24), (70, 2048, [264], 30, 16),
+                                                  (3000, 64, [520, 16], 2, 64), (130, 96, [136], 150, 100), (300, 33, [17, 4], 6, 3)])
+def test_a_fresh_output_is_whole_whatever_the_plan(ops, m, k, parts, slots, rank, dtype):
+    """With a plan of another batch a fresh output has every row, by the index, also through the custom op and a captured call."""
+    c = _case(m, k, parts, slots, rank, dtype, seed=m + rank)
+    index, n = c["index"], sum(parts)
+    plan = ops.lora_plan_buffer(m + 64, max(slots, 2), index.device)
+    batch = ops.lora_batch(index, slots, plan)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = ops.lora_add(c["base"], c["x"], batch, c["a"], c["b"], c["scaling"], c["ranks"], c["parts"])
+    for rows, of in ((m - 5, slots), (m + 33, slots), (m, 1 if slots > 1 else 2)):
+        other = torch.zeros(rows, dtype=torch.int32, device="cuda")
+        ops.lora_batch(other, of, plan)  # the buffer now holds another batch's
+        torch.full((m, n), float("nan"), dtype=dtype, device="cuda")  # what torch.empty finds
+        _check(ops.lora_add(c["base"], c["x"], batch, c["a"], c["b"], c["scaling"], c["ranks"], c["parts"]), c, f"plan of {rows}, {of}")
+        torch.full((m, n), float("nan"), dtype=dtype, device="cuda")
+        _check(torch.ops.qtts.lora_add(c["base"], c["x"], index, plan, slots, c["a"], c["b"], c["scaling"], c["ranks"], c["parts"]), c)
+        held.fill_(float("nan"))
+        graph.replay()
+        _check(held, c, f"replay with a plan of {rows}, {of}")
+    ops.lora_batch(index, slots, plan)
+    graph.replay()
+    assert torch.equal(held, ops.lora_add(c["base"], c["x"], batch, c["a"], c["b"], c["scaling"], c["ranks"], c["parts"]))

@@ -204,3 +204,15 @@ print("refused")
     env = dict(os.environ, PYTHONPATH=os.pathsep.join(sys.path))
     done = subprocess.run([sys.executable, "-c", code], env=env, capture_output=True, text=True, timeout=300)
     assert done.returncode == 0 and "refused" in done.stdout, done.stderr
+
+
+def test_lora_add_fresh_entry_checks_as_lora_add_does():
+    L = _lib.load()
+    b = _buf(1 << 20)
+    ends = (ctypes.c_int64 * 1)(96)
+    for m, rank, out, ws_n, text in ((-1, 16, 160000, 1 << 18, "negative"), (4, 129, 160000, 1 << 18, "rank"),
+                                     (4, 16, 140002, 1 << 18, "out overlaps base"), (4, 16, 160000, 8, "workspace")):
+        status = [add(_at(b), 1, m, 64, 64, _at(b, 4096), None, 3, _at(b, 8192), _at(b, 65536), rank, None, _at(b, 131200), ends, 1,
+                      _at(b, 140000), 96, _at(b, out), 96, 96, _at(b, 262144), ws_n, None)
+                  for add in (L.qtts_lora_add, L.qtts_lora_add_fresh)]
+        assert status[0] == status[1] < 0 and text in _lib.last_error()

@@ -730,10 +730,10 @@ int qtts_lora_plan(const int32_t* index, int64_t m, int64_t slots, int32_t* plan
   return qtts_launch_lora_plan(index, m, slots, plan, (hipStream_t)stream);
 }
 
-int qtts_lora_add(const void* x, int x_dtype, int64_t m, int64_t k, int64_t ldx, const int32_t* index, const int32_t* plan,
-                  int64_t slots, const void* a, const void* b, int64_t rank, const int32_t* ranks, const float* scaling,
-                  const int64_t* part_ends, int64_t parts, const void* base, int64_t ldb, void* out, int64_t n, int64_t ldo,
-                  void* ws, int64_t ws_bytes, void* stream) {
+static int lora_add(const void* x, int x_dtype, int64_t m, int64_t k, int64_t ldx, const int32_t* index, const int32_t* plan,
+                    int64_t slots, const void* a, const void* b, int64_t rank, const int32_t* ranks, const float* scaling,
+                    const int64_t* part_ends, int64_t parts, const void* base, int64_t ldb, void* out, int64_t n, int64_t ldo,
+                    bool whole, void* ws, int64_t ws_bytes, void* stream) {
   QTTS_REQUIRE(m >= 0 && n >= 0 && k >= 0 && slots >= 0, "lora_add: negative size");
   QTTS_REQUIRE(m < (1ll << 31) && n < (1ll << 30) && k < (1ll << 30) && slots < (1ll << 30), "lora_add: size too large");
   QTTS_REQUIRE(x_dtype == QTTS_BF16 || x_dtype == QTTS_F16, "lora_add: activations must be bf16 or fp16");
@@ -778,7 +778,24 @@ int qtts_lora_add(const void* x, int x_dtype, int64_t m, int64_t k, int64_t ldx,
   g.rank = (int)rank;
   g.parts.count = (int)parts;
   for (int64_t p = 0; p < parts; ++p) g.parts.end[p] = (int32_t)part_ends[p];
+  g.whole = whole;
   return qtts_launch_lora_add(g, x_dtype, ws, (hipStream_t)stream);
+}
+
+int qtts_lora_add(const void* x, int x_dtype, int64_t m, int64_t k, int64_t ldx, const int32_t* index, const int32_t* plan,
+                  int64_t slots, const void* a, const void* b, int64_t rank, const int32_t* ranks, const float* scaling,
+                  const int64_t* part_ends, int64_t parts, const void* base, int64_t ldb, void* out, int64_t n, int64_t ldo,
+                  void* ws, int64_t ws_bytes, void* stream) {
+  return lora_add(x, x_dtype, m, k, ldx, index, plan, slots, a, b, rank, ranks, scaling, part_ends, parts, base, ldb, out, n,
+                  ldo, false, ws, ws_bytes, stream);
+}
+
+int qtts_lora_add_fresh(const void* x, int x_dtype, int64_t m, int64_t k, int64_t ldx, const int32_t* index,
+                        const int32_t* plan, int64_t slots, const void* a, const void* b, int64_t rank, const int32_t* ranks,
+                        const float* scaling, const int64_t* part_ends, int64_t parts, const void* base, int64_t ldb, void* out,
+                        int64_t n, int64_t ldo, void* ws, int64_t ws_bytes, void* stream) {
+  return lora_add(x, x_dtype, m, k, ldx, index, plan, slots, a, b, rank, ranks, scaling, part_ends, parts, base, ldb, out, n,
+                  ldo, true, ws, ws_bytes, stream);
 }
 
 int qtts_w8a16_fused_gemm_strips(const void* x, int x_dtype, int64_t m, int64_t k, int64_t ldx, int prologue,

@@ -34,6 +34,7 @@ struct LoraArgs {
   int64_t m;
   int k, n, slots, rank, blocks, up_cols, splits;
   int64_t groups;  // at most, of the batch: the workgroups along the rows
+  bool whole;      // every row is written, by the index alone where the plan is another batch's
   LoraParts parts;
 };
 

@@ -105,7 +105,7 @@ __device__ __forceinline__ Group group_by_ballot(const LoraArgs& g, int64_t at) 
   return {slot < g.slots ? slot : -1, count, window + __builtin_amdgcn_ds_bpermute(4 * (before + (j < count ? j : 0)), order)};
 }
 
-// Group `at` < plan_max_groups of the plan; count 0 past the plan's groups and where the plan was made for another batch or
+// Group `at` < plan_max_groups of the plan; count 0 past the plan's groups, -1 where the plan was made for another batch or
 // slot count.  The three loads do not wait for one another.
 __device__ __forceinline__ Group group_by_plan(const LoraArgs& g, int64_t at) {
   const int j = threadIdx.x & 15;
@@ -113,7 +113,8 @@ __device__ __forceinline__ Group group_by_plan(const LoraArgs& g, int64_t at) {
   const i32x2_t e = *(const i32x2_t*)(g.plan + 4 + 2 * at);
   const int32_t* order = g.plan + plan_order_at(g.m, g.slots) + kPlanGroup * at;
   const int row = order[j], lead = order[0];
-  if (at >= head[0] || head[1] != g.m || head[2] != g.slots) return {-1, 0, 0};
+  if (head[1] != g.m || head[2] != g.slots) return {-1, -1, 0};
+  if (at >= head[0]) return {-1, 0, 0};
   return {e[0], e[1], j < e[1] ? row : lead};
 }
 
@@ -283,12 +284,55 @@ __device__ __forceinline__ void meet_waves(const uint8_t* sums, int pitch, int t
   }
 }
 
+// Both products of rows `row`, row + step, ..., from the index: what a call that writes every row falls back on where its plan is
+// another batch's (a captured step replayed after the routing of other rows).  Row by row and in fp32.  It is in the first product's
+// kernel, whose waves a compute unit are counted by LDS: its registers, and those of groups of 16 rows in its place, cost the second's
+// a wave of five, 6% of a layer of 2048 rows.  It reads the kernel's arguments anew, where the compiler does not see that they are
+// those: it held them all from the kernel's start (33 scalar registers spilled, 0.4 us a launch; 0.1 so).  t: kLoraMaxRank of this wave alone.
+template <typename XT> __device__ __forceinline__ void rows_by_index(int64_t row, int64_t step, float* t) {
+  uint64_t args = (uint64_t)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(args));
+  const LoraArgs& g = *(const LoraArgs*)args;
+  const int lane = threadIdx.x & 63;
+#pragma unroll 1
+  for (; row < g.m; row += step) {
+    const int slot = g.index[row];
+    const bool has = slot >= 0 && slot < g.slots;
+    const int live = has ? min(max(g.ranks ? g.ranks[slot] : g.rank, 0), g.rank) : 0;
+    const XT *x = (const XT*)g.x + row * g.ldx, *base = (const XT*)g.base + row * g.ldb;
+    XT* out = (XT*)g.out + row * g.ldo;
+#pragma unroll 1
+    for (int part = 0, c0 = 0; part < g.parts.count; c0 = g.parts.end[part++]) {
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // the last t has been read
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+      for (int i = 0; i < live; ++i) {
+        const XT* a = (const XT*)g.a + (((int64_t)slot * g.parts.count + part) * g.rank + i) * g.k;
+        float sum = 0.0f;
+        for (int c = lane; c < g.k; c += 64) sum = __builtin_fmaf(to_f32(x[c]), to_f32(a[c]), sum);
+        sum = wave_sum(sum);
+        if (lane == 0) t[i] = sum * g.scaling[slot];
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+      for (int c = c0 + lane; c < g.parts.end[part]; c += 64) {
+        const XT* b = (const XT*)g.b + ((int64_t)slot * g.n + c) * g.rank;  // (not read without a slot)
+        float sum = 0.0f;
+        for (int i = 0; i < live; ++i) sum = __builtin_fmaf(t[i], to_f32(b[i]), sum);
+        out[c] = live ? from_f32<XT>(to_f32(base[c]) + sum) : base[c];
+      }
+    }
+  }
+}
+
 constexpr int kDownWaves = 8;
 
 // Grid: (N tiles of the partitions' A each, groups, splits of K).  Eight waves share the split's K.
 template <typename XT, int N, bool PACK, bool VEC, bool PLAN>
 __global__ __launch_bounds__(64 * kDownWaves) void lora_down_kernel(LoraArgs g) {
   constexpr int T = kBlockTiles<PACK>, kPitch = VEC ? kDownBytes<N, kDownStages<N>> : 1024 * N;
+  static_assert(kLoraMaxRank * 4 <= kPitch, "rows_by_index");
   __shared__ __align__(1024) uint8_t stages[kDownWaves][kPitch];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int per_part = T * g.blocks, tile0 = blockIdx.x * N;  // tiles of a partition; the workgroup's first
@@ -297,6 +341,11 @@ __global__ __launch_bounds__(64 * kDownWaves) void lora_down_kernel(LoraArgs g) 
   const int s0 = min((int)(kDownWaves * blockIdx.z + wave) * per, (steps + 1) & ~1), s1 = min(s0 + per, steps);
   for (int64_t at = blockIdx.y; at < g.groups; at += gridDim.y) {
     const Group gr = PLAN ? group_by_plan(g, at) : group_by_ballot(g, at);
+    if (PLAN && gr.count < 0) {  // for every group: each workgroup is here once, the second product's not at all
+      if (g.whole && blockIdx.x == 0 && blockIdx.z == 0)
+        rows_by_index<XT>((int64_t)blockIdx.y * kDownWaves + wave, (int64_t)gridDim.y * kDownWaves, (float*)stages[wave]);
+      return;
+    }
     if (!gr.count) continue;
     const int live = ranks.of(g, gr.slot);
     if (!live) continue;
@@ -558,7 +607,7 @@ __global__ __launch_bounds__(64 * kUpWaves) void lora_up_kernel(LoraArgs g) {
   for (int64_t at = PLAN ? (int64_t)blockIdx.y * kUpWaves + wave : blockIdx.y; at < g.groups;
        at += (int64_t)gridDim.y * (PLAN ? kUpWaves : 1)) {
     const Group gr = PLAN ? group_by_plan(g, at) : group_by_ballot(g, at);
-    if (!gr.count) continue;
+    if (gr.count <= 0) continue;
     if (c0 >= c1) continue;
     const int live = ranks.of(g, gr.slot);
     if (!live && g.base == g.out) continue;

@@ -105,6 +105,7 @@ EXPORTS = (
     "qtts_lora_plan_bytes",
     "qtts_lora_plan",
     "qtts_lora_add",
+    "qtts_lora_add_fresh",
     "qtts_kernel_timer_begin",
     "qtts_kernel_timer_end",
 )
@@ -207,9 +208,9 @@ def load() -> ctypes.CDLL:
         L.qtts_lora_plan_bytes.argtypes = [i64, i64]
         L.qtts_lora_plan.restype = i32
         L.qtts_lora_plan.argtypes = [p, i64, i64, p, i64, p]
-        L.qtts_lora_add.restype = i32
-        L.qtts_lora_add.argtypes = [p, i32, i64, i64, i64, p, p, i64, p, p, i64, p, p, p, i64, p, i64, p, i64, i64, p, i64,
-                                    p]
+        for add in (L.qtts_lora_add, L.qtts_lora_add_fresh):
+            add.restype = i32
+            add.argtypes = [p, i32, i64, i64, i64, p, p, i64, p, p, i64, p, p, p, i64, p, i64, p, i64, i64, p, i64, p]
         L.qtts_kernel_timer_begin.restype = i32
         L.qtts_kernel_timer_begin.argtypes = [i32]
         L.qtts_kernel_timer_end.restype = i32

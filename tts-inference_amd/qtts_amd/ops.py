@@ -1001,7 +1001,9 @@ def lora_add(base: torch.Tensor, x: torch.Tensor, batch: LoraBatch, a: torch.Ten
     base ``[..., N]`` is the shared projection's output, x ``[..., K]`` its input (bf16 or fp16).  a ``[S, P * R, K]``
     and b ``[S, N, R]`` hold S adapters of rank up to R for a linear of P output ``partitions`` (their widths; None:
     one of N), scaling ``[S]`` fp32, ranks ``[S]`` int32 or None (all R): entries past a slot's rank are not used.
-    Rows without an adapter are base.  Returns a fresh tensor in base's shape, or ``out`` (which may be base)."""
+    Rows without an adapter are base.  Returns a fresh tensor in base's shape, or ``out`` (which may be base).  Where the
+    batch's plan buffer has been rewritten for another row or slot count, a fresh tensor takes the rows' slots from
+    ``batch.index`` and ``out`` stays as it was."""
     xr, br = _flatten(x), _flatten(base)
     m, k = xr.shape
     n, dtype, slots = br.shape[1], xr.dtype, batch.slots
@@ -1033,7 +1035,8 @@ def lora_add(base: torch.Tensor, x: torch.Tensor, batch: LoraBatch, a: torch.Ten
     if ws is None or ws.numel() < need:
         _ensure_workspace(xr.device, need, "lora_add")
         ws = _workspaces[idx]
-    st = _lib.load().qtts_lora_add(
+    lib = _lib.load()
+    st = (lib.qtts_lora_add_fresh if out is None else lib.qtts_lora_add)(
         xr.data_ptr(), code, m, k, xr.stride(0) if m > 1 else k, batch.index.data_ptr(),
         None if batch.plan is None else batch.plan.data_ptr(), slots, a.data_ptr(), b.data_ptr(), rank,
         None if ranks is None else ranks.data_ptr(), scaling.data_ptr(), ends, parts, br.data_ptr(),
