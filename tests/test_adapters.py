@@ -290,3 +290,29 @@ def test_quantizing_after_attaching_keeps_the_adapters():
     again = Method()
     quantize_module(block, again, QuantConfig(method="int8"), "talker")  # another method: under the same adapters
     assert block.qkv_proj.quant_method.inner is again and block.qkv_proj.quant_method.routing is routing
+
+
+@pytest.mark.parametrize("max_rows", [8, 200])
+def test_a_routing_holds_its_last_index_alone(max_rows):
+    """Behind the rows of the last set there is no adapter and no plan: a captured step of more rows, or of a plan's, finds nothing of
+    an earlier one.  (The kernels need a GPU: set writes its buffers, then refuses here.)"""
+    routing = AdapterRouting(4, max_rows, device="cpu")
+
+    def held(index, rows=None):
+        with pytest.raises(ValueError, match="GPU tensor"):
+            routing.set(index, rows)
+        n = len(index)
+        assert routing.index[:n].tolist() == [int(i) for i in index] and (routing.index[n:] == -1).all()
+        if max_rows > 64:
+            assert routing._plan.data_ptr() % 16 == 0 and routing._plan.numel() * 4 >= ops._plan_bytes(max_rows, 4)
+            assert (routing._plan[:4] == -1).all()  # of no row count
+
+    if not torch.cuda.is_available():
+        address = routing.index.data_ptr()
+        held([3, 2, 1, 0, 3, 2, 1, 0])
+        if max_rows > 64:
+            routing._plan[:4] = torch.tensor([9, 100, 4, 0], dtype=torch.int32)
+        held([1, 2], 7)
+        held(torch.tensor([3] * max_rows))
+        held([])
+        assert routing.index.data_ptr() == address

@@ -274,3 +274,32 @@ def test_quantizing_before_or_after_attaching(ops, method):
     want = before.qkv(x)
     first.set([-1] * 9)
     assert not torch.equal(want, before.qkv(x)) and torch.equal(after.qkv(x), want)
+
+
+@pytest.mark.parametrize("captured", [100, 48])
+def test_a_replay_after_a_routing_of_other_rows(ops, captured):
+    """A captured step's rows take the last routing's slots, and none where it has no row, whatever its row count."""
+    block, routing = _block("fp8", torch.bfloat16)
+    x = _rows(captured, torch.bfloat16, 1)
+    routing.set(_index(captured, 2))
+    block.qkv(x)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = block.qkv(x)
+    bank = block.qkv.adapters
+    routing.set([-1] * captured)
+    base = block.qkv(x)
+    for turn, rows in enumerate((20, captured, 131, 66, 5, captured - 1, 200)):
+        index = _index(rows, 30 + turn)
+        routing.set([SLOTS - 2] * 256), routing.set(index if turn % 2 else index.cuda())
+        graph.replay()
+        mine = torch.full((captured,), -1, dtype=torch.int32)
+        mine[:min(rows, captured)] = index[:captured]
+        want = ops.lora_add(base, x, ops.lora_batch(mine.cuda(), SLOTS), bank.lora_a, bank.lora_b, bank.lora_scaling, bank.lora_ranks,
+                            bank.partitions)
+        # a call without this batch's plan sums in another order: at most a step of the output apart, and fp32's K + R roundings
+        step = torch.finfo(out.dtype).eps * want.abs() + 2 * (HIDDEN + 16) * U * (want - base).abs().amax()
+        assert ((out.float() - want.float()).abs() <= step.float()).all(), rows
+        none = (mine < 0).nonzero().flatten().cuda()
+        assert torch.equal(out[none], base[none]), rows

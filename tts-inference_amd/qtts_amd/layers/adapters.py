@@ -36,15 +36,18 @@ from .linear import iter_linears
 
 class AdapterRouting:
     """Which adapter slot each row takes (-1: none), in buffers that keep their addresses: a graph captured while the
-    routing was set for a row count reads, on every replay, what the last :meth:`set` wrote.  That one has to be of the
-    graph's row count, as the buffers serve every row count."""
+    routing was set reads, on every replay, what the last :meth:`set` wrote.  A graph of another row count than that one's
+    takes its rows' slots from it all the same, and no adapter for rows that it does not have."""
 
     def __init__(self, slots: int, max_rows: int, device: torch.device | str = "cuda") -> None:
         if slots < 1 or max_rows < 1:
             raise ValueError(f"an adapter routing needs slots and rows, got {slots} and {max_rows}")
         self.slots, self.max_rows = int(slots), int(max_rows)
-        self.index = torch.full((self.max_rows,), -1, dtype=torch.int32, device=device)
-        self._plan = ops.lora_plan_buffer(self.max_rows, self.slots, self.index.device)
+        # One buffer, the index (as far as 16 bytes go), then the plan: one write clears the index's end and the plan's head.
+        words, at = ops.lora_plan_buffer(self.max_rows, self.slots, torch.device("meta")).numel(), (self.max_rows + 3) // 4 * 4
+        buffer = torch.full((at + words,), -1, dtype=torch.int32, device=device)
+        self.index, self._plan = buffer[:self.max_rows], buffer[at:]
+        self._live = buffer[:at + min(words, 4)]  # what a set writes
         self.batch: ops.LoraBatch | None = None
 
     def set(self, index: torch.Tensor | Sequence[int], rows: int | None = None) -> ops.LoraBatch:
@@ -57,8 +60,12 @@ class AdapterRouting:
         if not given <= rows <= self.max_rows:
             raise ValueError(f"{given} rows padded to {rows} do not fit a routing of {self.max_rows}")
         self.batch = None  # nothing stands if what follows fails
-        self.index[:given].copy_(index)
-        self.index[given:rows].fill_(-1)
+        # The rows behind the given ones have no adapter and the plan is of no batch, also for captured steps of other row counts.
+        if index.device == self._live.device:
+            self._live[:given].copy_(index)
+            self._live[given:].fill_(-1)
+        else:
+            self._live.copy_(F.pad(index, (0, self._live.shape[0] - given), value=-1))
         self.batch = ops.lora_batch(self.index[:rows], self.slots, self._plan)
         return self.batch
 
