@@ -316,3 +316,23 @@ def test_a_routing_holds_its_last_index_alone(max_rows):
         held(torch.tensor([3] * max_rows))
         held([])
         assert routing.index.data_ptr() == address
+
+
+def test_a_routing_takes_whole_numbers():
+    """Values that int32 cannot hold are no slot; what is no whole number is refused, not cut."""
+    routing = AdapterRouting(4, 8, device="cpu")
+    for bad in ([0.5, 1.0], torch.zeros(2), torch.tensor([True, False])):
+        with pytest.raises(ValueError, match="whole numbers"):
+            routing.set(bad)
+    if not torch.cuda.is_available():
+        for dtype in (torch.int64, torch.uint8, torch.int16):
+            given = torch.tensor([2, 3, 1], dtype=dtype)
+            with pytest.raises(ValueError, match="GPU tensor"):
+                routing.set(given)
+            assert routing.index[:3].tolist() == [2, 3, 1]
+        given = torch.tensor([1, 2 ** 32, 2 ** 32 + 3, -2 ** 40])
+        kept = given.clone()
+        with pytest.raises(ValueError, match="GPU tensor"):
+            routing.set(given)
+        index = routing.index[:4]
+        assert index[0] == 1 and not ((index[1:] >= 0) & (index[1:] < 4)).any() and torch.equal(given, kept)

@@ -52,13 +52,17 @@ class AdapterRouting:
 
     def set(self, index: torch.Tensor | Sequence[int], rows: int | None = None) -> ops.LoraBatch:
         """The slots of the step's rows, ``rows`` of them with padding rows (no adapter) behind ``index``."""
-        index = torch.as_tensor(index, dtype=torch.int32)
+        index = torch.as_tensor(index)
         if index.dim() != 1:
             raise ValueError(f"index must be 1-D, got shape {tuple(index.shape)}")
         given = index.shape[0]
+        if given and (index.dtype == torch.bool or index.is_floating_point() or index.is_complex()):
+            raise ValueError(f"index must hold whole numbers, got {index.dtype}")
         rows = given if rows is None else int(rows)
         if not given <= rows <= self.max_rows:
             raise ValueError(f"{given} rows padded to {rows} do not fit a routing of {self.max_rows}")
+        if index.dtype != torch.int32:  # what int32 cannot hold is no slot either
+            index = index.to(torch.int64).clamp(-1, self.slots).to(torch.int32)
         self.batch = None  # nothing stands if what follows fails
         # The rows behind the given ones have no adapter and the plan is of no batch, also for captured steps of other row counts.
         if index.device == self._live.device:
