@@ -303,3 +303,50 @@ def test_a_replay_after_a_routing_of_other_rows(ops, captured):
         assert ((out.float() - want.float()).abs() <= step.float()).all(), rows
         none = (mine < 0).nonzero().flatten().cuda()
         assert torch.equal(out[none], base[none]), rows
+
+
+@pytest.mark.parametrize("kind", ["ShiftedNorm", "BiasNorm", "CenteredNorm", "OuterEpsNorm"])
+def test_norms_that_only_look_like_rms_norm(ops, kind):
+    """A norm of another formula with RMSNorm's attributes keeps the composition's bits in every helper."""
+    import test_decoder_helpers as helpers
+    from qtts_amd.layers.decoder import add_norm_linear, add_norm_mlp, norm_linear, norm_mlp_residual
+    norm = getattr(helpers, kind)(HIDDEN).cuda().to(torch.bfloat16)
+    if kind == "BiasNorm":
+        norm.bias.data.fill_(0.5)
+    x, res = _rows(5, torch.bfloat16, 1) + 0.25, _rows(5, torch.bfloat16, 2)
+    block, _ = _block("fp8", torch.bfloat16, adapters=False)
+    y, hidden = add_norm_linear(norm, block.qkv, x, res)
+    assert torch.equal(hidden, res + x) and torch.equal(y, block.qkv(norm(res + x)))
+    y, hidden = add_norm_mlp(norm, block.mlp, x, res)
+    assert torch.equal(y, block.mlp(norm(res + x)))
+    block, _ = _block("int8_weight_only", torch.bfloat16, adapters=False)
+    assert torch.equal(norm_linear(norm, block.qkv, x), block.qkv(norm(x)))
+    gate, up = block.mlp.gate_up_proj.split(block.mlp.gate_up_proj(norm(x)))
+    assert torch.equal(norm_mlp_residual(norm, block.mlp, x), x + block.mlp.down_proj(torch.nn.functional.silu(gate) * up))
+
+
+def test_a_norm_of_a_gpu_kernel_alone(ops):
+    """It is asked on its own device, in its own type; a captured step that meets it first runs the norm itself."""
+    import test_decoder_helpers as helpers
+    from qtts_amd.layers.norm import is_rms_norm
+
+    class KernelNorm(Norm):
+        def forward(self, x):
+            return ops.rms_norm(x, self.weight, self.eps)
+
+    for dtype in (torch.bfloat16, torch.float16, torch.float32):
+        assert is_rms_norm(KernelNorm(HIDDEN, dtype)) and is_rms_norm(helpers.GpuNorm(HIDDEN).cuda().to(dtype))
+
+    class ShiftedKernelNorm(Norm):
+        def forward(self, x):
+            return ops.rms_norm(x, 1 + self.weight, self.eps)
+
+    assert not is_rms_norm(ShiftedKernelNorm(HIDDEN, torch.bfloat16))
+    norm, x = KernelNorm(HIDDEN, torch.bfloat16), _rows(3, torch.bfloat16, 1)
+    want = norm(x)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        assert not is_rms_norm(norm)
+        out = norm(x)
+    graph.replay()
+    assert torch.equal(out, want) and is_rms_norm(norm)

@@ -33,6 +33,7 @@ from torch import nn
 from .. import ops, torch_ops  # noqa: F401  (torch_ops registers torch.ops.qtts)
 from ..quant.base import weight_flags
 from .adapters import AdapterMethod
+from .norm import is_rms_norm, norm_eps
 
 
 def _int8_strips(linear: nn.Module, x: torch.Tensor) -> bool:
@@ -48,19 +49,18 @@ def _int8_strips(linear: nn.Module, x: torch.Tensor) -> bool:
     return routed is None or routed(linear, x)
 
 
-def _norm_eps(norm: nn.Module) -> float:
-    for attr in ("eps", "variance_epsilon"):
-        if hasattr(norm, attr):
-            return float(getattr(norm, attr))
-    raise AttributeError(f"{type(norm).__name__} has no eps")
+def _rms_norm_of(norm: nn.Module, x: torch.Tensor) -> bool:
+    """Whether the kernels compute what ``norm`` does to x's rows: an RMSNorm of their width."""
+    weight = getattr(norm, "weight", None)
+    return weight is not None and weight.dim() == 1 and weight.shape[0] == x.shape[-1] and is_rms_norm(norm)
 
 
 def norm_linear(norm: nn.Module, linear: nn.Module, x: torch.Tensor) -> torch.Tensor:
     """``linear(norm(x))``: input_layernorm + qkv_proj (talker.py:249), with the RMSNorm computed
     inside the int8 weight-only GEMM's prologue."""
-    if _int8_strips(linear, x):
+    if _int8_strips(linear, x) and _rms_norm_of(norm, x):
         return torch.ops.qtts.w8a16_fused_gemm_strips(x, linear.int8_weight, linear.out_features, linear.int8_scale,
-                                                      linear.bias, ops.PRO_RMS_NORM, norm.weight, _norm_eps(norm),
+                                                      linear.bias, ops.PRO_RMS_NORM, norm.weight, norm_eps(norm),
                                                       None, ops.ALGO_AUTO | weight_flags(linear))
     return linear(norm(x))
 
@@ -80,10 +80,11 @@ def norm_mlp_residual(norm: nn.Module, mlp: nn.Module, hidden: torch.Tensor) -> 
     in the gate_up GEMM's prologue, ``silu(gate) * up`` in its epilogue, the residual add in the
     down GEMM's epilogue: two launches."""
     fused = getattr(mlp, "fuse", False)
-    if fused and _int8_strips(mlp.gate_up_proj, hidden) and mlp.gate_up_proj.out_features % 2 == 0:
+    if (fused and _int8_strips(mlp.gate_up_proj, hidden) and mlp.gate_up_proj.out_features % 2 == 0
+            and _rms_norm_of(norm, hidden)):
         up = mlp.gate_up_proj
         act = torch.ops.qtts.w8a16_gate_up_silu_strips(hidden, up.int8_weight, up.out_features, up.int8_scale,
-                                                       up.bias, ops.PRO_RMS_NORM, norm.weight, _norm_eps(norm),
+                                                       up.bias, ops.PRO_RMS_NORM, norm.weight, norm_eps(norm),
                                                        ops.ALGO_AUTO | weight_flags(up))
         return linear_residual(mlp.down_proj, act, hidden)
     if fused:
@@ -126,16 +127,14 @@ def _w8a8_linear(linear: nn.Module, method, codes: int, qx: torch.Tensor, sx: to
 def _add_norm_w8a8(norm: nn.Module, linear: nn.Module, found, x: torch.Tensor, residual: torch.Tensor | None):
     method, codes = found
     adapted = isinstance(method, AdapterMethod)
-    qx, sx, hidden, normed = torch.ops.qtts.rms_norm_quant(x, norm.weight, _norm_eps(norm), residual, codes, adapted)
+    qx, sx, hidden, normed = torch.ops.qtts.rms_norm_quant(x, norm.weight, norm_eps(norm), residual, codes, adapted)
     y = _w8a8_linear(linear, method, codes, qx, sx, normed if adapted else None, x.shape, x.dtype)
     return y, x if residual is None else hidden
 
 
 def _norm_fits(norm: nn.Module, x: torch.Tensor, residual: torch.Tensor | None) -> bool:
     """Whether the kernel computes what ``norm`` does: an RMSNorm in x's type, of a residual like x."""
-    weight = getattr(norm, "weight", None)
-    return (weight is not None and weight.dtype == x.dtype and not isinstance(norm, nn.LayerNorm)
-            and getattr(norm, "eps", 0.0) is not None
+    return (_rms_norm_of(norm, x) and norm.weight.dtype == x.dtype
             and (residual is None or (residual.shape == x.shape and residual.dtype == x.dtype)))
 
 

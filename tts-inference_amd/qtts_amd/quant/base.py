@@ -16,6 +16,7 @@ from torch import nn
 
 from ..config import QuantConfig
 from ..layers.linear import iter_linears
+from ..layers.norm import mark_rms_norms
 
 logger = logging.getLogger("qtts_amd.quant")
 
@@ -97,6 +98,7 @@ def quantize_module(module: nn.Module, method: QuantMethodBase, config: QuantCon
         # a converted layer whose calibration routed some row bucket to F.linear keeps its weight
         weight = getattr(layer, "weight", None)
         kept_weight += int(weight is not None and weight.numel() > 0)
+    mark_rms_norms(module)  # what the decoder helpers may fuse, known before any step is traced or captured
     after = _param_bytes(module) + _buffer_bytes(module)
     logger.info("%s: %s converted %d linears (%d keeping their weight for F.linear at some row bucket), "
                 "skipped %d by exclusion, kept %d on F.linear; weights %s -> %s, %s",
