@@ -392,3 +392,63 @@ def test_a_fresh_output_is_whole_whatever_the_plan(ops, m, k, parts, slots, rank
     ops.lora_batch(index, slots, plan)
     graph.replay()
     assert torch.equal(held, ops.lora_add(c["base"], c["x"], batch, c["a"], c["b"], c["scaling"], c["ranks"], c["parts"]))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("cancels", ["entries", "halves"])
+@pytest.mark.parametrize("m,k,parts,slots,rank", [
+    (1, 2048, [512], 2, 16), (16, 64, [72], 1, 8), (27, 2048, [256, 128, 128], 9, 16), (16, 2048, [512], 4, 32), (8, 2048, [264], 3, 64),
+    (60, 2048, [512], 30, 16), (63, 6144, [264], 40, 24), (64, 6144, [520], 64, 64), (64, 1024, [136], 64, 100), (70, 2048, [264], 3, 8),
+    (300, 6144, [520, 264], 4, 40), (300, 2048, [520], 4, 64), (1003, 6144, [72], 30, 16), (2100, 2048, [520], 8, 32), (130, 512, [264], 7, 128),
+    (5000, 64, [4096], 5, 72), (40, 1003, [17, 40], 3, 12), (200, 333, [41], 5, 36), (100, 2040, [64], 2, 7)])
+def test_what_cancels_is_exact(ops, m, k, parts, slots, rank, cancels, dtype):
+    """The first product's sums keep fp32's 24 bits to the second: whole numbers of up to 2^21 whose terms cancel to fewer than 2^8,
+    between neighbouring entries of the rank or between the two halves of K.  Every product, every partial sum in any order (8 terms of
+    2^21, below 2^24) and the result are whole numbers that fp32, and the output's type, hold exactly, so the result is exact too."""
+    g = torch.Generator().manual_seed(m + k + rank)
+    most = max(1, min(200, (1 << 20) // (k * 100)))
+
+    def whole(lo, hi, *shape):
+        return torch.randint(lo, hi + 1, shape, generator=g).double()
+
+    n, pairs = sum(parts), rank // 2
+    x = whole(1, most, m, k)
+    if cancels == "entries":  # rows of A in pairs that differ by one in a few places, B + and - of them
+        a = whole(40, 200, slots, len(parts) * rank, k)
+        for p in range(len(parts)):
+            even = a[:, p * rank:p * rank + 2 * pairs:2]
+            a[:, p * rank + 1:p * rank + 2 * pairs:2] = even + (torch.arange(k) == 0).double() - (torch.arange(k) == k - 1).double()
+        b = torch.zeros(slots, n, rank, dtype=torch.float64)
+        used = torch.randperm(pairs, generator=g)[:4]
+        sign = whole(0, 1, slots, n, len(used)) * 2 - 1
+        b[:, :, 2 * used], b[:, :, 2 * used + 1] = sign, -sign
+        if most > 40:  # four of x's first and last, within 2^8
+            x[:, 0], x[:, -1] = x[:, 0] % 20, x[:, -1] % 20
+    else:  # the second half of K takes the first away, but for one place
+        half = k // 2
+        a = whole(40, 200, slots, len(parts) * rank, k)
+        a[:, :, half:2 * half], x[:, half:2 * half] = -a[:, :, :half], x[:, :half]
+        a[:, :, k - 1] = a[:, :, k - 1] + 1 if k % 2 == 0 else 1
+        if most > 40:
+            x[:, k - 1] = x[:, k - 1] % 30
+            x[:, half - 1] = x[:, k - 1] if k % 2 == 0 else x[:, half - 1]
+        b = torch.zeros(slots, n, rank, dtype=torch.float64)
+        used = torch.randperm(rank, generator=g)[:2]
+        b[:, :, used] = whole(0, 1, slots, n, len(used)) * 2 - 1
+    base = whole(-20, 20, m, n)
+    index = torch.randint(-1, slots, (m,), generator=g, dtype=torch.int32)
+    scaling = whole(0, 1, slots) * 2 - 1
+    want, lo = base.clone(), 0
+    for p, width in enumerate(parts):
+        for s in range(slots):
+            rows = (index == s).nonzero().flatten()
+            t = x[rows] @ a[s, p * rank:(p + 1) * rank].t()
+            assert t.numel() == 0 or (t.abs().max() < 1 << 21 and (x[rows].abs() @ a[s, p * rank].abs()).max() < 1 << 21)
+            want[rows, lo:lo + width] += scaling[s] * (t @ b[s, lo:lo + width].t())
+        lo += width
+    assert want.abs().max() <= 256 and torch.equal(want.to(dtype).double(), want)
+    c = [v.to(dtype).cuda() for v in (base, x, a, b)]
+    assert all(torch.equal(v.double().cpu(), w) for v, w in zip(c, (base, x, a, b)))
+    out = ops.lora_add(c[0], c[1], ops.lora_batch(index.cuda(), slots), c[2], c[3], scaling.float().cuda(), None, parts)
+    wrong = out.double().cpu() != want
+    assert not wrong.any(), f"{int(wrong.sum())} of {wrong.numel()}, the first {float(out.double().cpu()[wrong][0])} for {float(want[wrong][0])}"

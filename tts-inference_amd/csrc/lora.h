@@ -29,7 +29,7 @@ struct LoraArgs {
   int64_t ldb;
   void* out;
   int64_t ldo;
-  uint8_t* t;     // [splits, m, parts.count, blocks]: the first product's halves (lora.hip)
+  uint8_t* t;     // [splits, m, parts.count, blocks]: the first product's sums as 16-bit parts (lora.hip)
   int32_t* exps;  // as many, fp16
   int64_t m;
   int k, n, slots, rank, blocks, up_cols, splits;

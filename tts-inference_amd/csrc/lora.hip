@@ -11,8 +11,10 @@
 // a ring of stages without a barrier), and the result meets base in LDS, whose rows are read and written in
 // 128-byte pieces.
 //
-// The second product multiplies t, scaled, as two 16-bit halves, hi = T(t) and lo = T(t - hi), which keeps 16 bits
-// of it (bf16; in fp16 22 of the largest entry of each 32, which are first scaled by a power of two into [1/2, 1)).
+// The second product multiplies t, scaled, as 16-bit parts, each the rounding of what those before it leave: in bf16
+// three, which hold all 24 bits of fp32 (with two, 16 bits, an adapter whose terms cancel lost the rest; the third costs a
+// layer of 27 rows 0.7%, of 2048 2.8%, ranks past 16 and many rows 4-5%); in fp16 two, 22 bits of the largest entry of
+// each 32, which are first scaled by a power of two into [1/2, 1).
 // The first product's kernel writes them so: the second, whose time is the output's rows, only loads them.
 //
 // Where the groups come from: up to 64 rows, each workgroup finds the rows of its slot by one load of the
@@ -226,29 +228,40 @@ __device__ __forceinline__ void down_steps(const LoraArgs& g, const Group& gr, c
   }
 }
 
-// ---- t's halves ------------------------------------------------------------------------------
-// The rank in blocks: up to 16 entries one block of 16 (PACK), past them NB blocks of 32.  A block of a row in the workspace:
-// its hi halves, then its lo halves.  A lane's operand: whole blocks, entries 8 (lane / 16) ... + 7 of hi and then of lo
-// (two MFMAs); PACK, hi for lanes 0-31 and lo for lanes 32-63 (one).
+// ---- t's parts -------------------------------------------------------------------------------
+// The rank in blocks: up to 16 entries one block of 16 (PACK), past them NB blocks of 32.  A block of a row in the workspace: its
+// parts, one after another.  A lane's operands, one an MFMA: whole blocks, entries 8 (lane / 16) ... + 7 of each part; PACK, the
+// first part for lanes 0-31 and the second for lanes 32-63, then the third for lanes 0-31 alone.
 
+template <typename XT> constexpr int kParts = std::is_same<XT, f16_t>::value ? 2 : 3;
 template <bool PACK> constexpr int kBlockTiles = PACK ? 1 : 2;
-template <bool PACK> constexpr int kBlockBytes = PACK ? 64 : 128;
+template <bool PACK> constexpr int kPartBytes = PACK ? 32 : 64;
+template <typename XT, bool PACK> constexpr int kBlockBytes = kParts<XT> * kPartBytes<PACK>;
+template <typename XT, bool PACK> constexpr int kOperands = PACK ? (kParts<XT> + 1) / 2 : kParts<XT>;
 
-// Four neighbouring entries of t (already zero past the slot's rank) as halves.
-template <typename XT> struct Halves {
-  uint2 hi, lo;
-  __device__ __forceinline__ explicit Halves(f32x4_t v) {
-    uint32_t h[2], l[2];
+// Operand h of a block.
+template <bool PACK> __device__ __forceinline__ i32x4_t load_part(const uint8_t* block, int h) {
+  const int q = (threadIdx.x & 63) >> 4;
+  if (!PACK || h == 0) return *(const i32x4_t*)(block + 64 * h + 16 * q);
+  const i32x4_t v = *(const i32x4_t*)(block + 64 + 16 * (q & 1));
+  return q < 2 ? v : i32x4_t{0, 0, 0, 0};
+}
+
+// Four neighbouring entries of t (already zero past the slot's rank) as parts, to their place in a block.
+template <typename XT, bool PACK> __device__ __forceinline__ void store_parts(f32x4_t v, uint8_t* to) {
+#pragma unroll
+  for (int p = 0; p < kParts<XT>; ++p) {
+    uint32_t h[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       h[i] = pack2_f32<XT>(v[2 * i], v[2 * i + 1]);
       const float h0 = to_f32(XT{(uint16_t)h[i]}), h1 = to_f32(XT{(uint16_t)(h[i] >> 16)});
-      // an infinite half has no remainder
-      l[i] = pack2_f32<XT>(fabsf(h0) <= 3.4e38f ? v[2 * i] - h0 : 0.0f, fabsf(h1) <= 3.4e38f ? v[2 * i + 1] - h1 : 0.0f);
+      // an infinite part leaves nothing
+      v[2 * i] = fabsf(h0) <= 3.4e38f ? v[2 * i] - h0 : 0.0f, v[2 * i + 1] = fabsf(h1) <= 3.4e38f ? v[2 * i + 1] - h1 : 0.0f;
     }
-    hi = make_uint2(h[0], h[1]), lo = make_uint2(l[0], l[1]);
+    *(uint2*)(to + p * kPartBytes<PACK>) = make_uint2(h[0], h[1]);
   }
-};
+}
 
 // fp16: the exponent that brings the largest of a block's entries to [1/2, 1) (four lanes a row), and the entries scaled by it.
 template <typename XT, int T> __device__ __forceinline__ int scale_block(f32x4_t (&v)[T]) {
@@ -369,13 +382,9 @@ __global__ __launch_bounds__(64 * kDownWaves) void lora_down_kernel(LoraArgs g) 
       const int exp = scale_block<XT, T>(v);
       const int64_t block = (blockIdx.z * g.m + gr.row) * (g.parts.count * g.blocks) + tile / T;
       if ((lane & 15) < gr.count) {
-        uint8_t* to = g.t + block * kBlockBytes<PACK> + 8 * (lane >> 4);
+        uint8_t* to = g.t + block * kBlockBytes<XT, PACK> + 8 * (lane >> 4);
 #pragma unroll
-        for (int t = 0; t < T; ++t) {
-          const Halves<XT> h(v[t]);
-          *(uint2*)(to + 32 * t) = h.hi;
-          *(uint2*)(to + 32 * t + kBlockBytes<PACK> / 2) = h.lo;
-        }
+        for (int t = 0; t < T; ++t) store_parts<XT, PACK>(v[t], to + 32 * t);
         if (std::is_same<XT, f16_t>::value && lane < 16) g.exps[block] = exp;
       }
     }
@@ -384,11 +393,11 @@ __global__ __launch_bounds__(64 * kDownWaves) void lora_down_kernel(LoraArgs g) 
 }
 
 // ---- second product --------------------------------------------------------------------------
-// The t operands of one group's rows: (hi, lo) of each block of each split's sum, and fp16's exponents.  The splits of K meet
+// The t operands of one group's rows: the parts of each block of each split's sum, and fp16's exponents.  The splits of K meet
 // here, as more MFMAs by the same operand of B.
 template <typename XT, int NB, bool PACK, int S = 1> struct TOperand {
-  static constexpr int kHalves = PACK ? 1 : 2, kBlocks = NB * S;
-  i32x4_t v[kBlocks][kHalves];
+  static constexpr int kEach = kOperands<XT, PACK>, kBlocks = NB * S;
+  i32x4_t v[kBlocks][kEach];
   int exp[kBlocks];
 
   // `row`: the lane's row of the workspace (of a group's first for lanes past its rows), `part` of the partition.
@@ -396,9 +405,8 @@ template <typename XT, int NB, bool PACK, int S = 1> struct TOperand {
 #pragma unroll
     for (int b = 0; b < kBlocks; ++b) {
       const int64_t block = ((b / NB * g.m + row) * g.parts.count + part) * NB + b % NB;
-      const uint8_t* from = g.t + block * kBlockBytes<PACK> + 16 * ((threadIdx.x & 63) >> 4);
 #pragma unroll
-      for (int h = 0; h < kHalves; ++h) v[b][h] = *(const i32x4_t*)(from + 64 * h);
+      for (int h = 0; h < kEach; ++h) v[b][h] = load_part<PACK>(g.t + block * kBlockBytes<XT, PACK>, h);
       if constexpr (std::is_same<XT, f16_t>::value) exp[b] = g.exps[block];
     }
   }
@@ -484,7 +492,7 @@ __device__ __forceinline__ f32x4_t up_mma(const vec8<XT> (&b)[NB], const TOperan
     constexpr bool kExp = std::is_same<XT, f16_t>::value;  // a block at a time: each has an exponent of its own
     f32x4_t acc = kExp ? f32x4_t{0.0f, 0.0f, 0.0f, 0.0f} : sum;
 #pragma unroll
-    for (int h = 0; h < TOperand<XT, NB, PACK>::kHalves; ++h)
+    for (int h = 0; h < kOperands<XT, PACK>; ++h)
       acc = mfma16<XT>::mma(b[k % NB], __builtin_bit_cast(vec8<XT>, t.v[k][h]), acc);
     if constexpr (kExp) {
 #pragma unroll
@@ -593,8 +601,9 @@ __device__ __forceinline__ Block block_of(const LoraArgs& g, int chunk, int cols
 constexpr int kUpWaves = 4, kUpTiles = 4, kUpBlock = 16 * kUpTiles;
 
 // Grid: (blocks of g.up_cols columns, groups).  A wave takes 64 columns at a time: with a plan, whose groups of one slot follow
-// one another, all columns of a group of its own; else a part of the workgroup's group.
-template <typename XT, int NB, bool PACK, int B, bool PLAN, int S>
+// one another, all columns of a group of its own; else a part of the workgroup's group.  ONE (with a plan): those are 64 and no more,
+// which without the next ones' loads takes 12 registers less (2048 rows of a layer 76.8 -> 75.2 us).
+template <typename XT, int NB, bool PACK, int B, bool PLAN, int S, bool ONE>
 __global__ __launch_bounds__(64 * kUpWaves) void lora_up_kernel(LoraArgs g) {
   typedef Rows<XT, kUpTiles, B != kByEntry> R;
   __shared__ __align__(16) float lds[kUpWaves][R::kFloats];
@@ -616,7 +625,7 @@ __global__ __launch_bounds__(64 * kUpWaves) void lora_up_kernel(LoraArgs g) {
     if (!live) {
       for (int c = c0;;) {
         rows.copy();
-        if ((c += kUpBlock) >= c1) break;
+        if (ONE || (c += kUpBlock) >= c1) break;
         rows.advance();
         rows.load();
       }
@@ -630,7 +639,7 @@ __global__ __launch_bounds__(64 * kUpWaves) void lora_up_kernel(LoraArgs g) {
     for (int n = 0; n < kUpTiles; ++n) columns.next(b[n]);
     for (int c = c0;;) {
       rows.add([&](int n) { return up_mma(b[n], t); }, lds[wave]);
-      if ((c += kUpBlock) >= c1) break;
+      if (ONE || (c += kUpBlock) >= c1) break;
       rows.advance();
       rows.load();
 #pragma unroll
@@ -650,13 +659,14 @@ __global__ __launch_bounds__(64 * kOneWaves) void lora_one_kernel(LoraArgs g) {
   constexpr int NT = kOneTiles, T = kBlockTiles<PACK>, N = T * NB;  // 16-row tiles of A
   constexpr bool VEC = B != kByEntry;
   typedef Rows<XT, NT, VEC> R;
-  // A wave's stages; then its sums, later its result, in the first 4 KiB, and in the first wave's part the halves past them.
-  constexpr int kHalves = NB * 16 * kBlockBytes<PACK>, kUsed = 4096 + kHalves + NB * 64;
+  // A wave's stages; then its sums, later its result, in the first 4 KiB, and in the first wave's the parts of t past them.
+  constexpr int kPartsBytes = NB * 16 * kBlockBytes<XT, PACK>, kUsed = 4096 + kPartsBytes + NB * 64;
   constexpr int kPitch = (std::max(VEC ? kDownBytes<N, kOneStages> : 0, kUsed) + 1023) & ~1023;
   static_assert(1024 * N <= 4096 && 4 * R::kFloats <= 4096, "the sums and the result");
   __shared__ __align__(1024) uint8_t stages[kOneWaves][kPitch];
-  uint8_t(*halves)[16][kBlockBytes<PACK>] = (uint8_t(*)[16][kBlockBytes<PACK>])(stages[0] + 4096);
-  int(*exps)[16] = (int(*)[16])(stages[0] + 4096 + kHalves);
+  typedef uint8_t TBlock[kBlockBytes<XT, PACK>];
+  TBlock(*blocks)[16] = (TBlock(*)[16])(stages[0] + 4096);  // [NB][16]
+  int(*exps)[16] = (int(*)[16])(stages[0] + 4096 + kPartsBytes);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const Block blk = block_of(g, blockIdx.x, kLoraFusedCols);
   const int c0 = blk.c0 + 16 * NT * wave, tok = lane & 15;
@@ -693,13 +703,9 @@ __global__ __launch_bounds__(64 * kOneWaves) void lora_one_kernel(LoraArgs g) {
       f32x4_t v[T];
       meet_waves<kOneWaves, T>(stages[0], kPitch, T * wave, 16 * T * wave, live, scaling, v);
       const int exp = scale_block<XT, T>(v);
-      uint8_t* to = &halves[wave][tok][8 * (lane >> 4)];
+      uint8_t* to = &blocks[wave][tok][8 * (lane >> 4)];
 #pragma unroll
-      for (int t = 0; t < T; ++t) {
-        const Halves<XT> h(v[t]);
-        *(uint2*)(to + 32 * t) = h.hi;
-        *(uint2*)(to + 32 * t + kBlockBytes<PACK> / 2) = h.lo;
-      }
+      for (int t = 0; t < T; ++t) store_parts<XT, PACK>(v[t], to + 32 * t);
       if (std::is_same<XT, f16_t>::value && lane < 16) exps[wave][tok] = exp;
     }
     __syncthreads();  // (the sums are read: the result may take their place)
@@ -707,12 +713,11 @@ __global__ __launch_bounds__(64 * kOneWaves) void lora_one_kernel(LoraArgs g) {
 #pragma unroll
     for (int k = 0; k < NB; ++k) {
 #pragma unroll
-      for (int h = 0; h < TOperand<XT, NB, PACK>::kHalves; ++h)
-        t.v[k][h] = *(const i32x4_t*)&halves[k][tok][64 * h + 16 * (lane >> 4)];
+      for (int h = 0; h < kOperands<XT, PACK>; ++h) t.v[k][h] = load_part<PACK>(blocks[k][tok], h);
       if constexpr (std::is_same<XT, f16_t>::value) t.exp[k] = exps[k][tok];
     }
     rows.add([&](int n) { return up_mma(b[n], t); }, (float*)stages[wave]);
-    __syncthreads();  // before the next group's stages and halves
+    __syncthreads();  // before the next group's stages and parts
   }
 }
 
@@ -888,10 +893,16 @@ template <typename XT> void launch_lora(LoraArgs& g, hipStream_t st) {
     const int up_chunks = cut_columns(g.parts, g.up_cols);
     by_rank(g.rank, [&](auto nb, auto pack) {
       by_kind(b_kind, [&](auto v) {
-        auto up = [&](auto s) {
-          qtts::launch(&lora_up_kernel<XT, nb.value, pack.value, v.value, plan.value, s.value>,
+        auto launch_up = [&](auto s, auto one) {
+          qtts::launch(&lora_up_kernel<XT, nb.value, pack.value, v.value, plan.value, s.value, one.value>,
                        dim3(up_chunks, grid_y(plan.value ? (g.groups + kUpWaves - 1) / kUpWaves : g.groups)),
                        dim3(64 * kUpWaves), 0, st, g);
+        };
+        auto up = [&](auto s) {
+          if constexpr (plan.value && v.value == kAligned) {
+            if (g.up_cols == kUpBlock) return launch_up(s, std::true_type{});
+          }
+          launch_up(s, std::false_type{});
         };
         if constexpr (v.value == kAligned && 32 * nb.value <= kLoraSplitRank) {
           if (g.splits == 2) return up(std::integral_constant<int, 2>{});
@@ -907,7 +918,7 @@ template <typename XT> void launch_lora(LoraArgs& g, hipStream_t st) {
 // The workspace: t's blocks, split by split and row by row, then fp16's exponents.
 static int64_t lora_t_blocks(int64_t m, int64_t parts, int64_t rank) { return lora_max_splits(m, rank) * m * parts * lora_blocks(rank); }
 static int64_t lora_t_bytes(int64_t m, int64_t parts, int64_t rank) {
-  return align256(lora_t_blocks(m, parts, rank) * (rank <= 16 ? 64 : 128));
+  return align256(lora_t_blocks(m, parts, rank) * (rank <= 16 ? kBlockBytes<bf16_t, true> : kBlockBytes<bf16_t, false>));
 }
 
 int64_t qtts_lora_ws_bytes(int64_t m, int64_t parts, int64_t rank) {
