@@ -473,8 +473,8 @@ int qtts_lora_plan(const int32_t* index, int64_t m, int64_t slots, int32_t* plan
  * for the output partition p of column j (part_ends: [parts] ascending column ends on the
  * host, the last n; a merged qkv or gate_up has an A block per partition).  Rows whose index
  * is outside [0, slots) have out = base.  Sums in fp32, t's among them: the second product takes
- * it in 16-bit parts, fp32's 24 bits (bf16) or 22 of the largest of each 32 entries (fp16).  No
- * counterpart in the reference.
+ * it in 16-bit parts, fp32's 24 bits (bf16) or 22 (fp16; entries under 2^-17 of the largest
+ * of their 32 fewer).  No counterpart in the reference.
  * x: [m, k] of x_dtype (bf16 or fp16), row stride ldx.  index: [m] int32, on the device.
  * a: [slots, parts * rank, k], b: [slots, n, rank], contiguous, of x_dtype.  ranks: [slots]
  * int32 or NULL (all `rank`); entries of a and b past a slot's rank are not used.  scaling:

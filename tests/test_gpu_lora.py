@@ -452,3 +452,30 @@ def test_what_cancels_is_exact(ops, m, k, parts, slots, rank, cancels, dtype):
     out = ops.lora_add(c[0], c[1], ops.lora_batch(index.cuda(), slots), c[2], c[3], scaling.float().cuda(), None, parts)
     wrong = out.double().cpu() != want
     assert not wrong.any(), f"{int(wrong.sum())} of {wrong.numel()}, the first {float(out.double().cpu()[wrong][0])} for {float(want[wrong][0])}"
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("m,k,parts,slots,rank", [(1, 256, [72], 1, 16), (20, 2048, [264], 3, 16), (30, 512, [512], 8, 32),
+                                                  (64, 2048, [264, 8], 20, 64), (100, 2048, [72], 3, 40), (900, 320, [520], 4, 24)])
+def test_large_entries_leave_the_small_ones_their_bits(ops, m, k, parts, slots, rank, dtype):
+    """Entries of t 2^18 to 2^26 apart in one row, the large ones with a B of zero: the small ones' sums are exact, and so is the
+    result (one product of the type's full mantissa)."""
+    g = torch.Generator().manual_seed(m + rank)
+    n, one = sum(parts), 1 + torch.finfo(dtype).eps
+    x = torch.ones(m, k, dtype=torch.float64)
+    a = torch.zeros(slots, len(parts) * rank, k, dtype=torch.float64)
+    b = torch.zeros(slots, n, rank, dtype=torch.float64)
+    small = torch.randint(0, rank, (slots,), generator=g)
+    for s in range(slots):
+        for p in range(len(parts)):
+            rows = a[s, p * rank:(p + 1) * rank]
+            rows[:] = (1 << 15) // (1 << s % 6)  # t: k times as much
+            rows[small[s]] = 0
+            rows[small[s], s % k] = one  # t: that value alone
+        b[s, :, small[s]] = 1
+    index = torch.randint(0, slots, (m,), generator=g, dtype=torch.int32)
+    scaling = 2.0 ** torch.randint(-3, 4, (slots,), generator=g).double()
+    want = (scaling[index.long()] * one)[:, None].expand(m, n)
+    c = [v.to(dtype).cuda() for v in (torch.zeros(m, n), x, a, b)]
+    out = ops.lora_add(c[0], c[1], ops.lora_batch(index.cuda(), slots), c[2], c[3], scaling.float().cuda(), None, parts)
+    assert torch.equal(out.double().cpu(), want), f"{float(out.double().cpu()[0, 0])} for {float(want[0, 0])}"

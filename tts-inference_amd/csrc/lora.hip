@@ -13,8 +13,8 @@
 //
 // The second product multiplies t, scaled, as 16-bit parts, each the rounding of what those before it leave: in bf16
 // three, which hold all 24 bits of fp32 (with two, 16 bits, an adapter whose terms cancel lost the rest; the third costs a
-// layer of 27 rows 0.7%, of 2048 2.8%, ranks past 16 and many rows 4-5%); in fp16 two, 22 bits of the largest entry of
-// each 32, which are first scaled by a power of two into [1/2, 1).
+// layer of 27 rows 0.7%, of 2048 2.8%, ranks past 16 and many rows 4-5%); in fp16 two, 22 bits of entries down to
+// 2^-17 of the largest of each 32, which are first scaled by a power of two.
 // The first product's kernel writes them so: the second, whose time is the output's rows, only loads them.
 //
 // Where the groups come from: up to 64 rows, each workgroup finds the rows of its slot by one load of the
@@ -263,7 +263,8 @@ template <typename XT, bool PACK> __device__ __forceinline__ void store_parts(f3
   }
 }
 
-// fp16: the exponent that brings the largest of a block's entries to [1/2, 1) (four lanes a row), and the entries scaled by it.
+// fp16: the exponent that brings the largest of a block's entries to [2^14, 2^15) (four lanes a row), and the entries scaled by it: as
+// far up as halves go, so that entries down to 2^-17 of it keep 22 bits and to 2^-28 the first part's 11.
 template <typename XT, int T> __device__ __forceinline__ int scale_block(f32x4_t (&v)[T]) {
   if constexpr (!std::is_same<XT, f16_t>::value) return 0;
   float top = 0.0f;
@@ -273,7 +274,7 @@ template <typename XT, int T> __device__ __forceinline__ int scale_block(f32x4_t
     for (int i = 0; i < 4; ++i) top = fmaxf(top, fabsf(v[t][i]));
   top = fmaxf(top, __shfl_xor(top, 16, 64));
   top = fmaxf(top, __shfl_xor(top, 32, 64));
-  const int exp = __builtin_amdgcn_frexp_expf(top);  // 0 for zero, infinity and NaN
+  const int exp = top < __builtin_inff() ? __builtin_amdgcn_frexp_expf(top) - 15 : 0;  // (an infinity's finite neighbours as they are)
 #pragma unroll
   for (int t = 0; t < T; ++t)
 #pragma unroll
