@@ -318,3 +318,32 @@ def test_norm_codes_at_the_ends_of_the_range(ops, codes):
         rows = [0, 1, 2, 3, 4, 5] if eps else [0, 2, 4, 5]  # (squares of 1e-30 vanish in fp32: without eps there is no norm)
         q, s, _, _ = ops.rms_norm_quant(x[rows], w, eps, None, codes)
         _check_codes(q, s, _norm64(x[rows], w, eps), codes, rel(k), f"eps {eps}")
+
+
+@pytest.mark.parametrize("codes", [1, 0], ids=["e4m3", "int8"])
+@pytest.mark.parametrize("k", [16, 15])
+def test_rows_that_share_a_workgroup(ops, k, codes):
+    """Past 2^22 rows the long kernels take a call, 2^20 workgroups of every 2^20-th row each: rows on both sides of every multiple,
+    and all rows of a few workgroups, hold to 64 bits with and without a residual and the 16-bit outputs."""
+    m, step = (1 << 22) + 77, 1 << 20
+    x = torch.empty(m, 2 * k, dtype=torch.bfloat16, device="cuda").normal_(generator=torch.Generator(device="cuda").manual_seed(k))
+    x[3 * step + 5] = 0
+    x[2 * step + 6, 1] = float("nan")  # its workgroup's other rows are 6, step + 6, 3 step + 6 and 4 step + 6
+    w = (1 + _rand((k,), torch.float32, 51, 0.1)).to(torch.bfloat16)
+    near = {r + d for r in range(0, m, step) for d in range(-3, 12)}
+    pick = torch.tensor(sorted(r for r in near | {m - 1, m - 2} if 0 <= r < m and r != 2 * step + 6), device="cuda")
+    rows, res = x[:, :k], x[:, k:]
+    for residual in (None, res):
+        q, s, hidden, normed = ops.rms_norm_quant(rows, w, 1e-6, residual, codes, True)
+        h = rows[pick] if residual is None else rows[pick] + res[pick]
+        v = _norm64(h, w, 1e-6)
+        _check_codes(q[pick], s[pick], v, codes, rel(k), "norm")
+        _check_16bit(normed[pick], v, rel(k), "normed")
+        assert hidden is None or torch.equal(hidden[pick], h)
+        assert torch.isnan(s).nonzero().flatten().tolist() == [2 * step + 6]
+        del q, s, hidden, normed
+    q, s, act = ops.silu_mul_quant(x, codes, want_act=True)
+    v = _silu64(x[pick])
+    _check_codes(q[pick], s[pick], v, codes, rel(0), "silu")
+    _check_16bit(act[pick], v, rel(0), "act")
+    assert torch.isnan(s).nonzero().flatten().tolist() == [2 * step + 6]
