@@ -336,3 +336,46 @@ def test_a_routing_takes_whole_numbers():
             routing.set(given)
         index = routing.index[:4]
         assert index[0] == 1 and not ((index[1:] >= 0) & (index[1:] < 4)).any() and torch.equal(given, kept)
+
+
+def test_places_for_every_routing(tmp_path):
+    """lora_groups against the most groups of 16 rows of one slot that any routing of m rows over the slots and none makes, counted
+    apart: most[c][r], of r rows in up to c classes, by trying every size of the last class."""
+    rows = _run(tmp_path, """
+#include <stdio.h>
+#include "lora_rule.h"
+int main() {
+  for (int m = 1; m <= 64; ++m)
+    for (int slots = 0; slots <= 80; ++slots) printf("%d %d %lld\\n", m, slots, (long long)qtts::lora_groups(m, slots));
+}
+""")
+    most = [[0] + [-1] * 64]
+    for _ in range(81):
+        last = most[-1]
+        most.append([max(last[r], max((last[r - c] - (-c // 16) for c in range(1, r + 1) if last[r - c] >= 0), default=-1))
+                     for r in range(65)])
+    assert most[1][33] == 3 and most[2][34] == 4 and most[81][64] == 64
+    for m, slots, groups in rows:
+        assert groups >= most[slots + 1][m], (m, slots, groups, most[slots + 1][m])
+
+
+def test_parts_of_k_stay_in_their_workspace(tmp_path):
+    """The workspace holds each row's sums for every part of K that a call may take, whatever the workgroups are."""
+    from qtts_amd import _lib
+
+    rows = _run(tmp_path, """
+#include <stdio.h>
+#include "lora_rule.h"
+int main() {
+  const int ks[] = {1, 2040, 2048, 6144, 1 << 20}, ws[] = {1, 128, 129, 5000};
+  for (int m = 1; m <= 4100; m += 41)
+    for (int rank = 1; rank <= 128; rank += 7)
+      for (int k : ks) for (int w : ws) printf("%d %d %d\\n", m, rank, qtts::lora_splits(m, k, rank, w));
+}
+""")
+    L = _lib.load()
+    for m, rank, splits in {tuple(r) for r in rows}:
+        # a row's block: three 16-bit parts of the rank's entries (fp16: two and an exponent) in a multiple of 16 or 32
+        entries = 16 if rank <= 16 else -(-rank // 32) * 32
+        need = splits * m * entries * 6
+        assert L.qtts_workspace_bytes(_lib.OP_LORA, m, 1, rank, 0) >= need, (m, rank, splits)
