@@ -347,3 +347,22 @@ def test_rows_that_share_a_workgroup(ops, k, codes):
     _check_codes(q[pick], s[pick], v, codes, rel(0), "silu")
     _check_16bit(act[pick], v, rel(0), "act")
     assert torch.isnan(s).nonzero().flatten().tolist() == [2 * step + 6]
+
+
+@pytest.mark.parametrize("k", [1040, 1037, 16400])
+@pytest.mark.parametrize("dtype", DTYPES, ids=["bf16", "fp16", "fp32"])
+def test_far_gates(ops, dtype, k):
+    """Gates from where e^-g nears fp32's range (silu of -1e-36, a normal number) to that range's ends: what torch's fp32 gives, within
+    two roundings of the exponent's argument (2 |g| u) and 16 u more, and the type's own."""
+    g = torch.linspace(-88.7, -60, k).to(dtype)
+    g[:4] = torch.tensor([-1000.0, -90.0, 60000.0, 0.0]).to(dtype)
+    up = torch.full((k,), 2.0 ** 14).to(dtype)
+    q, s, act = ops.silu_mul_quant(torch.cat([g, up])[None].cuda(), 0, want_act=True)
+    v = g.double() * torch.sigmoid(g.double()) * up.double()
+    far = g.double() < -88.7228  # e^-g past fp32: zero, as torch's
+    tol = (2 * g.double().abs().clamp_max(89) + 16) * U
+    step = torch.finfo(dtype).eps / 2 if dtype != torch.float32 else 0.0
+    tiny = torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps / 2
+    err = (act[0].double().cpu() - v).abs()
+    assert (act[0].cpu()[far] == 0).all() and far.any()
+    assert (err <= (step + tol) * v.abs() + tiny)[~far].all() if dtype != torch.float16 else torch.isfinite(act[0, 3:]).all()

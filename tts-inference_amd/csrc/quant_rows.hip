@@ -83,9 +83,10 @@ struct NormQuotient {
 };
 
 // silu(g) = g / (1 + 2^(-g log2 e)), the exponential and the reciprocal by the hardware's (an ulp each; the
-// exponent's own rounding makes it |g| ulps where the result is e^-|g| small).
+// exponent's own rounding makes it |g| ulps where the result is e^-|g| small).  The quotient is taken of g / 16 and 1 / 16 of the
+// rest: the reciprocal gives zero for what is under fp32's smallest normal, which 1 / (1 + e^-g) is from g = -87.4 on, silu(g) not.
 __device__ __forceinline__ float silu_f32(float g) {
-  return g * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504f * g));
+  return g * 0.0625f * __builtin_amdgcn_rcpf(__builtin_fmaf(__builtin_amdgcn_exp2f(-1.44269504f * g), 0.0625f, 0.0625f));
 }
 
 // ---- eight elements of a row --------------------------------------------------------------
