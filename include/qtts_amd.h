@@ -479,7 +479,7 @@ int qtts_lora_plan(const int32_t* index, int64_t m, int64_t slots, int32_t* plan
  * a: [slots, parts * rank, k], b: [slots, n, rank], contiguous, of x_dtype.  ranks: [slots]
  * int32 or NULL (all `rank`); entries of a and b past a slot's rank are not used.  scaling:
  * [slots] fp32.  base, out: [m, n] of x_dtype, row strides ldb, ldo; out may be base itself
- * and shares no byte with x.  rank <= QTTS_LORA_MAX_RANK, parts <= QTTS_LORA_MAX_PARTS.
+ * and shares no byte with x or any other input.  rank <= QTTS_LORA_MAX_RANK, parts <= QTTS_LORA_MAX_PARTS.
  * plan: what qtts_lora_plan made of the same index, m and slots, or NULL (rows of one adapter
  * are then read together within each 64 rows); with a plan of another m or slots, in a buffer
  * of qtts_lora_plan_bytes(m, slots), nothing is written.

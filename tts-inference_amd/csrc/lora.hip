@@ -23,15 +23,17 @@
 //  * lora_one_kernel: both products in one launch, for few adapters of small rank (lora_rule.h);
 //  * lora_down_kernel, lora_up_kernel: one launch each, t through the workspace.
 //
-// What bounds them, bf16 (a large copy runs at 5.1 TB/s here):
+// What bounds them, bf16 (a large copy runs at 5.1 TB/s here; each figure a kernel's own time, its inputs from memory, and in
+// brackets with the same inputs in every call, which the Infinity Cache then holds):
 //  * one launch: latency, three round trips to memory (the index; x, A, B and base; the result).  Rank 16, one row through 2048 x
-//    2048 in 5.6 us, 27 rows of 9 adapters through 2048 -> 12288 in 8.5 (14 MB of A and B);
-//  * the first product: how much one compute unit can load, which is why K's parts and A's tiles get workgroups of their own while
-//    groups are few.  64 rows of 32 rank-64 adapters, two partitions of 2048 (17 MB of A), in 7.3 us; 2048 rows of 8 rank-16
-//    adapters, K = 2048, in 5.6 (8 MB of x), K = 6144 in 10.4; past rank 32 and a thousand rows A's re-reads, once a group through
-//    L2 (4096 rows, rank 64, three partitions of K = 2048: 280 MB of them in 42);
-//  * the second product: base and the result, or B where rows are few.  2048 rows through 2048 -> 12288, rank 16, in 23.4 us
-//    (101 MB, 4.3 TB/s); 64 rows of 32 rank-64 adapters (51 MB of B) in 12.0.
+//    2048 in 5.7 us (5.5), 27 rows of 9 adapters through 2048 -> 12288 in 8.3 (7.9): 4.7 MB of A and B;
+//  * the first product: its groups' loads of x and A, each group's anew.  64 rows of 32 rank-64 adapters, two partitions of 2048
+//    (17 MB of A), in 8.2 us (7.3); 2048 rows of 8 rank-16 adapters, K = 2048, in 7.3 (8 MB of x, 19 MB through the L2s), K = 6144 in
+//    13.0 (25 and 53), by 137 workgroups, which is why K's parts and A's tiles get workgroups of their own while groups are few.
+//    Past rank 32 and a thousand rows A's re-reads: 4096 rows through qkv, rank 64, 8 adapters 34 us (276 MB through the L2s, 40%
+//    of them missed), 64 adapters 50 (297 MB, 94%);
+//  * the second product: base and the result, or B where rows are few.  2048 rows through 2048 -> 12288, rank 16, in 25.8 us (19.7):
+//    101 MB, 3.9 TB/s; 64 rows of 32 rank-64 adapters (50 MB of B) in 14.6 (11.6).
 #include <algorithm>
 
 #include "common.h"
@@ -302,7 +304,8 @@ __device__ __forceinline__ void meet_waves(const uint8_t* sums, int pitch, int t
 // another batch's (a captured step replayed after the routing of other rows).  Row by row and in fp32.  It is in the first product's
 // kernel, whose waves a compute unit are counted by LDS: its registers, and those of groups of 16 rows in its place, cost the second's
 // a wave of five, 6% of a layer of 2048 rows.  It reads the kernel's arguments anew, where the compiler does not see that they are
-// those: it held them all from the kernel's start (33 scalar registers spilled, 0.4 us a launch; 0.1 so).  t: kLoraMaxRank of this wave alone.
+// those: it held them all from the kernel's start (33 scalar registers spilled, 0.4 us a launch; 0.1 so).  t: kLoraMaxRank of this
+// wave alone.
 template <typename XT> __device__ __forceinline__ void rows_by_index(int64_t row, int64_t step, float* t) {
   uint64_t args = (uint64_t)__builtin_amdgcn_kernarg_segment_ptr();
   asm volatile("" : "+s"(args));
@@ -415,12 +418,12 @@ template <typename XT, int NB, bool PACK, int S = 1> struct TOperand {
 
 // A slot's B by columns: an operand of 16 columns from c is the lane's eight entries of each block of rows c + lane % 16.  Read as
 // 16 bytes (a lane's place as bytes in the slot's B, 32 bits: the host checks; clamped to the partition's last column), aligned where
-// the rank is a multiple of 8, at any address elsewhere (gate_up of 2048 rows, rank 4: entry by entry 80.6 us, so 30.2, as rank 8
-// aligned; one form for both cost rank 64 up to 6%), or entry by entry where base or out forbid vectors.  Entries past the slot's
-// rank may hold anything, and those past the rank are no part of the row: a lane of such entries reads others of its row, a rank
-// that is no multiple of 8 has its last lane read into the next row, and all of them are masked; the last slot's last rows have none
-// behind them, and are read from further ahead and shifted.  (No load is in a branch: the compiler may give each side of one its
-// own copy of the MFMAs after it.)
+// the rank is a multiple of 8, at any address elsewhere (gate_up of 2048 rows, rank 4: 37.5 us, rank 8, aligned, 34.6; entry by entry
+// rank 4 took more than twice as long; one form for both cost rank 64 up to 6%), or entry by entry where base or out forbid vectors.
+// Entries past the slot's rank may hold anything, and those past the rank are no part of the row: a lane of such entries reads others
+// of its row, a rank that is no multiple of 8 has its last lane read into the next row, and all of them are masked; the last slot's
+// last rows have none behind them, and are read from further ahead and shifted.  (No load is in a branch: the compiler may give each
+// side of one its own copy of the MFMAs after it.)
 enum { kByEntry, kAligned, kAnywhere };
 
 struct __attribute__((packed, aligned(2))) Unaligned16 { i32x4_t v; };

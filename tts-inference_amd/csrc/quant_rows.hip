@@ -176,8 +176,9 @@ template <int T> __device__ __forceinline__ void meet(float& ss, uint32_t& mx, f
 // The row in registers (K <= 8 T V): one memory round trip and one exchange a row.  max |h w| is taken in the
 // same pass as the sum of squares, since inv scales every value alike: max |v| = max |h w| inv, and the codes
 // need h w alone (NormQuotient).  A product of two 16-bit values is exact in fp32.
-// Bound by memory where rows are many: 8192 x 4096 bf16 with residual and hidden, 7 bytes an element, in 37.4 us (6.3 TB/s; a
-// copy of 4 GiB 5.1; the form below that reads the row twice, 171); 1003 x 2048 in 3.8; one row in 2.2, its latency.
+// Bound by memory where rows are many: 8192 x 4096 bf16 with residual and hidden, 7 bytes an element, in 37.6 us (6.3 TB/s; a
+// copy of 4 GiB 5.1; 8192 x 4095, element by element, 50.6); 1003 x 2048 fp16 without either in 4.7 (3.9 with the same rows in every
+// call, which the Infinity Cache then holds); one row in 2.5 (2.3), its latency.
 template <typename XT, bool FP8, bool VEC, int T, int V>
 __global__ __launch_bounds__(T) void rms_norm_quant_kernel(
     const XT* x, int64_t ldx, const XT* res, int64_t ldr, const XT* __restrict__ w, int k, float eps,
@@ -237,7 +238,7 @@ __global__ __launch_bounds__(T) void rms_norm_quant_kernel(
 }
 
 // As above, without the sum: the gate and up values of a row meet in registers.  4096 x 6144 fp16 with act, 7 bytes an element, in
-// 28.7 us (6.1 TB/s); 1501 bf16 rows without it, 5 bytes, in 9.6 (4.8); 5 rows in 3.2.
+// 28.8 us (6.1 TB/s); 1501 bf16 rows without it, 5 bytes, in 10.7 (4.3; 1501 x 6143, element by element, 12.1); 5 rows in 3.2.
 template <typename XT, bool FP8, bool VEC, int T, int V>
 __global__ __launch_bounds__(T) void silu_mul_quant_kernel(const XT* __restrict__ gu, int64_t ld, int k,
                                                            uint8_t* __restrict__ q, float* __restrict__ sx,

@@ -915,7 +915,7 @@ def silu_mul_quant(gate_up: torch.Tensor, codes: int = CODE_E4M3, want_act: bool
 # ---- low-rank adapters of many requests ----------------------------------------------------
 
 #: Rows up to which a batch needs no plan (qtts_lora_add groups the rows of each 64 by itself; 128 rows of 4 rank-16 adapters
-#: through gate_up 8.2 us with a plan, 22.8 without; the plan 3.7 once a step).
+#: through gate_up 8.9 us with a plan, 22.6 without; the plan 4.2 once a step).
 LORA_WINDOW = 64
 
 
