@@ -104,6 +104,21 @@ def test_load_takes_a_training_modules_parameters():
     assert not any(t.requires_grad for t in bank.buffers()) and a.grad is None
 
 
+def test_load_from_the_bank_itself():
+    """Adapters taken from the bank's own tensors, the slot's own among them (another scaling, a swap of partitions)."""
+    bank = LinearAdapters(8, [6, 6], 3, 5, torch.float32, "cpu")
+    a0, a1, b0, b1 = torch.randn(5, 8), torch.randn(5, 8), torch.randn(6, 5), torch.randn(6, 5)
+    bank.load(1, [a0, a1], [b0, b1])
+    held = [bank.lora_a[1, :5], bank.lora_a[1, 8:13]], [bank.lora_b[1, :6, :5], bank.lora_b[1, 6:, :5]]
+    bank.load(1, *held, scaling=0.5)
+    assert torch.equal(bank.lora_a[1, :5], a0) and torch.equal(bank.lora_b[1, 6:, :5], b1) and bank.lora_scaling[1] == 0.5
+    bank.load(1, held[0][::-1], held[1][::-1])
+    assert torch.equal(bank.lora_a[1, :5], a1) and torch.equal(bank.lora_a[1, 8:13], a0)
+    assert torch.equal(bank.lora_b[1, :6, :5], b1) and torch.equal(bank.lora_b[1, 6:, :5], b0)
+    bank.load(2, bank.lora_a[1, :5], bank.lora_b[1, :, :5])
+    assert torch.equal(bank.lora_a[2, 8:13], a1) and torch.equal(bank.lora_b[2], bank.lora_b[1])
+
+
 def test_load_refusals_leave_the_slot():
     bank = LinearAdapters(8, [6, 4], 3, 5, torch.float32, "cpu")
     a, b0, b1 = torch.randn(5, 8), torch.randn(6, 5), torch.randn(4, 5)

@@ -114,6 +114,8 @@ class LinearAdapters(nn.Module):
                                    or ap.shape[0] > self.max_rank):
                 raise ValueError(f"A {tuple(ap.shape)} and B {tuple(bp.shape)} do not fit a [{width}, {self.in_features}] "
                                  f"partition with adapters of rank up to {self.max_rank}")
+        own = {t.untyped_storage().data_ptr() for t in (self.lora_a, self.lora_b)}  # the bank's own, which clear zeroes
+        a, b = ([t.clone() if t is not None and t.untyped_storage().data_ptr() in own else t for t in ts] for ts in (a, b))
         self.clear(slot)
         lo = 0
         for p, (ap, bp, width) in enumerate(zip(a, b, self.partitions)):
