@@ -79,7 +79,8 @@ typedef enum {
     QTTS_OP_FP8W = 5,
     QTTS_OP_W8A16_SILU = 6,
     QTTS_OP_W8A16_FUSED = 7,
-    QTTS_OP_LORA = 8 /* n: the linear's partitions, k: the rank */
+    QTTS_OP_LORA = 8, /* n: the linear's partitions, k: the rank */
+    QTTS_OP_PAGED_ATTENTION = 9 /* m: the largest count of a request, n: query heads, k: the head size */
 } qtts_op;
 
 /* What qtts_w8a16_fused_gemm_strips applies to its activations before the GEMM. */
@@ -497,6 +498,65 @@ int qtts_lora_add_fresh(const void* x, int x_dtype, int64_t m, int64_t k, int64_
                         const int32_t* ranks, const float* scaling, const int64_t* part_ends, int64_t parts,
                         const void* base, int64_t ldb, void* out, int64_t n, int64_t ldo, void* ws, int64_t ws_bytes,
                         void* stream);
+
+/* --- attention over a paged key-value cache ------------------------------------------ */
+
+/* The cache of a layer: `pages` pages of page_size tokens (a power of two, 16 to 1024),
+ *   k: [pages, kv_heads, page_size, d]      v: [pages, kv_heads, d, page_size]
+ * bf16 or fp16, 16-byte aligned, d a multiple of 16 up to 256.  A request r of a batch holds
+ * lengths[r] tokens, its tokens [j page_size, (j + 1) page_size) on page table[r, j]; a token's slot
+ * is page * page_size + its place on the page.  The table, the lengths, the pages not in use
+ * (free_pages[taken..pages)) live on the device and are shared by all layers, which each have a k
+ * and a v of their own.  The reference keeps a fixed slice of one tensor a request instead
+ * (qtts/models/talker.py:47-91).  At most 2048 requests. */
+
+/* What a step's new tokens need, in one launch: the rows of request r, added[r] of them (<= 0:
+ * none), lie behind those of the requests before it; its new pages come off the free list in the
+ * order of the requests.
+ *   starts [requests + 1]: each request's first row, and the end of the last one's
+ *   counts [requests]: rows that joined the request, added[r] or 0 (denied, below)
+ *   lengths_out [requests], taken_out [1]: the state after the step; may be lengths and taken
+ *   positions, slots [rows]: of each row; -1 for rows of no request or of a denied one
+ *   table: the columns of new pages are written
+ * A request is denied as a whole where added[r] > max_new, where its rows do not fit `rows` or its tokens the
+ * table, and where it needs pages while those that it and the requests before it need
+ * exceed what is left.  Workspace: the 64 KiB of counters that every workspace begins with. */
+int qtts_paged_step(const int32_t* added, int64_t requests, const int32_t* lengths, int32_t* table, int64_t cols,
+                    const int32_t* free_pages, int64_t pages, const int32_t* taken, int64_t page_size, int64_t rows,
+                    int64_t max_new, int32_t* starts, int32_t* counts, int32_t* lengths_out, int32_t* taken_out,
+                    int32_t* positions, int32_t* slots, void* ws, int64_t ws_bytes, void* stream);
+
+/* The pages of requests with which[r] != 0 back to the free list, in the order of the requests; their lengths are 0 then. */
+int qtts_paged_release(const int32_t* which, int64_t requests, int32_t* lengths, const int32_t* table, int64_t cols,
+                       int32_t* free_pages, int64_t pages, int32_t* taken, int64_t page_size, void* stream);
+
+/* The rows of a fused qkv projection (qtts/models/talker.py:116-136): [rows, (heads + 2 kv_heads) d],
+ * row stride ldqkv, query heads first, then key heads, then value heads.
+ *   h <- h / sqrt(mean h^2 + eps) * norm          query and key heads; norm [d] of dtype or NULL
+ *   (h_i, h_{i + d/2}) <- (h_i c_i - h_{i + d/2} s_i, h_{i + d/2} c_i + h_i s_i)      i < d / 2
+ * with c, s: cos, sin [rope_rows, d / 2] fp32 at the row's position (NULL: no rotation), in
+ * fp32 with one rounding at the end (the reference rounds to dtype after the norm, qtts/layers/norm.py:50-76).
+ * Queries go to q [rows, heads, d], keys and values to the row's slot.
+ * Rows with a slot outside the cache: q is zero, nothing else is written. */
+int qtts_qkv_to_cache(const void* qkv, int dtype, int64_t rows, int64_t ldqkv, int64_t heads, int64_t kv_heads, int64_t d,
+                      const int32_t* positions, const int32_t* slots, const void* q_norm, const void* k_norm, float eps,
+                      const float* cos, const float* sin, int64_t rope_rows, void* k, void* v, int64_t pages,
+                      int64_t page_size, void* q, void* stream);
+
+/* Attention of the step's rows over their requests' tokens (qtts/attention/torch_sdpa.py:31-39), the rows' own
+ * among them (qtts_qkv_to_cache first): row i of a request's counts[r] is at position
+ * p = lengths[r] - counts[r] + i and sees the keys j <= p with j > p - window or j < sinks (window 0: all).
+ *   out = sum_j w_j v_j / sum_j w_j,  w_j = exp(scale * q . k_j - max)
+ * q, out: [rows, heads, d] of dtype, row strides ldq, ldo; query head h reads key-value head
+ * h / (heads / kv_heads).  Rows of no request: zeros.  What a row does not see (keys
+ * and values behind it, outside the window, in places never written) does not reach it, whatever it holds.
+ * min_new, max_new: bounds of the counts; requests with more than max_new get zeros.
+ * Workspace: qtts_workspace_bytes(QTTS_OP_PAGED_ATTENTION, max_new, heads, d). */
+int qtts_paged_attention(const void* q, int dtype, int64_t rows, int64_t ldq, int64_t heads, int64_t kv_heads, int64_t d,
+                         const void* k, const void* v, int64_t pages, int64_t page_size, const int32_t* table, int64_t requests,
+                         int64_t cols, const int32_t* starts, const int32_t* counts, const int32_t* lengths,
+                         const int32_t* slots, int64_t min_new, int64_t max_new, int64_t window, int64_t sinks, float scale,
+                         void* out, int64_t ldo, void* ws, int64_t ws_bytes, void* stream);
 
 /* Kernel timer.  No counterpart in the reference: benchmark instrumentation.
  * Between qtts_kernel_timer_begin and qtts_kernel_timer_end, each kernel the

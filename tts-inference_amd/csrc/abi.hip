@@ -14,6 +14,7 @@
 #include "common.h"
 #include "layout.h"
 #include "lora.h"
+#include "paged.h"
 #include "qtts_amd.h"
 
 // Launchers implemented next to their kernels.
@@ -78,6 +79,11 @@ int qtts_launch_silu_mul_quant(const void* gu, int x_dtype, int64_t m, int64_t k
 int64_t qtts_lora_ws_bytes(int64_t m, int64_t parts, int64_t rank);
 int qtts_launch_lora_plan(const int32_t* index, int64_t m, int64_t slots, int32_t* plan, hipStream_t st);
 int qtts_launch_lora_add(const qtts::LoraArgs& args, int x_dtype, void* ws, hipStream_t st);
+int qtts_launch_paged_step(const qtts::PagedStepArgs& args, hipStream_t st);
+int qtts_launch_paged_release(const int32_t* which, int32_t* lengths, const int32_t* table, int requests, int cols,
+                              int32_t* free_pages, int pages, int32_t* taken, int page_shift, hipStream_t st);
+int qtts_launch_qkv_to_cache(const qtts::QkvCacheArgs& args, int dtype, hipStream_t st);
+int qtts_launch_paged_attention(const qtts::PagedAttentionArgs& args, int dtype, hipStream_t st);
 
 static thread_local char g_last_error[512] = "";
 
@@ -264,6 +270,8 @@ int64_t qtts_workspace_bytes(int op, int64_t m, int64_t n, int64_t k, int algo) 
       if (n > QTTS_LORA_MAX_PARTS || k > QTTS_LORA_MAX_RANK)
         return qtts_set_error(QTTS_ERR_INVALID_ARGUMENT, "bad workspace query");
       return qtts_lora_ws_bytes(m, n, k);
+    case QTTS_OP_PAGED_ATTENTION:  // n query heads of k
+      return qtts::kCounterBytes;
     default: return qtts_set_error(QTTS_ERR_INVALID_ARGUMENT, "unknown op %d", op);
   }
 }
@@ -914,6 +922,171 @@ int qtts_dequant_strips(const void* qs, int codes, int64_t n, int64_t k, const v
   QTTS_REQUIRE((uintptr_t)qs % 16 == 0, "dequant_strips: strip buffer must be 16-byte aligned");
   QTTS_TRY(current_device_check());
   return qtts_launch_dequant_strips(qs, codes, n, k, scale, scale_dtype, w, w_dtype, ldw, (hipStream_t)stream);
+}
+
+// ---- attention over a paged cache ---------------------------------------------------------
+
+// log2 of a page's tokens, or -1 for a size that no page has.
+static int page_shift_of(int64_t page_size) {
+  for (int s = qtts::kPagedMinShift; s <= qtts::kPagedMaxShift; ++s)
+    if (page_size == (1ll << s)) return s;
+  return -1;
+}
+
+// The checks that every call on a page table shares: sizes in 32 bits, slots and a request's capacity among them.
+static int paged_sizes(const char* what, int64_t requests, int64_t cols, int64_t pages, int64_t page_size) {
+  QTTS_REQUIRE(requests >= 0 && cols >= 0 && pages >= 0, "%s: negative size", what);
+  QTTS_REQUIRE(page_shift_of(page_size) >= 0, "%s: a page of %lld tokens is no power of two from 16 to 1024", what,
+               (long long)page_size);
+  QTTS_REQUIRE(requests <= qtts::kPagedMaxRequests, "%s: %lld requests, at most %d", what, (long long)requests,
+               qtts::kPagedMaxRequests);
+  QTTS_REQUIRE(pages < (1ll << 31) / page_size && cols < (1ll << 31) / page_size,
+               "%s: size too large (tokens of the cache or of a request past 32 bits)", what);
+  return QTTS_OK;
+}
+
+static int paged_cache(const char* what, qtts::PagedCache& c, const void* k, const void* v, int64_t pages, int64_t page_size,
+                       int64_t heads, int64_t kv_heads, int64_t d) {
+  QTTS_REQUIRE(heads >= 1 && kv_heads >= 1 && heads % kv_heads == 0 && heads <= 4096,
+               "%s: %lld query heads for %lld key-value heads", what, (long long)heads, (long long)kv_heads);
+  QTTS_REQUIRE(d >= 16 && d <= qtts::kPagedMaxDim && d % 16 == 0, "%s: heads of %lld, not a multiple of 16 up to %d", what,
+               (long long)d, qtts::kPagedMaxDim);
+  QTTS_REQUIRE(pages == 0 || (k && v), "%s: null pointer", what);
+  QTTS_REQUIRE(((uintptr_t)k | (uintptr_t)v) % 16 == 0, "%s: unaligned cache", what);
+  c.k = const_cast<void*>(k);
+  c.v = const_cast<void*>(v);
+  c.pages = (int32_t)pages;
+  c.page_shift = page_shift_of(page_size);
+  c.kv_heads = (int32_t)kv_heads;
+  c.d = (int32_t)d;
+  return QTTS_OK;
+}
+
+int qtts_paged_step(const int32_t* added, int64_t requests, const int32_t* lengths, int32_t* table, int64_t cols,
+                    const int32_t* free_pages, int64_t pages, const int32_t* taken, int64_t page_size, int64_t rows,
+                    int64_t max_new, int32_t* starts, int32_t* counts, int32_t* lengths_out, int32_t* taken_out,
+                    int32_t* positions, int32_t* slots, void* ws, int64_t ws_bytes, void* stream) {
+  QTTS_TRY(paged_sizes("paged_step", requests, cols, pages, page_size));
+  QTTS_REQUIRE(rows >= 0 && max_new >= 0, "paged_step: negative size");
+  QTTS_REQUIRE(rows < (1ll << 31) - 8192, "paged_step: size too large");
+  QTTS_REQUIRE(taken && starts && taken_out, "paged_step: null pointer");
+  QTTS_REQUIRE(requests == 0 || (added && lengths && counts && lengths_out && (cols == 0 || table)), "paged_step: null pointer");
+  QTTS_REQUIRE((pages == 0 || free_pages) && (rows == 0 || (positions && slots)), "paged_step: null pointer");
+  if (!ws || ws_bytes < qtts::kCounterBytes)
+    return qtts_set_error(QTTS_ERR_WORKSPACE, "paged_step: workspace of %lld bytes < %lld needed", (long long)ws_bytes,
+                          (long long)qtts::kCounterBytes);
+  QTTS_TRY(current_device_check());
+  qtts::PagedStepArgs a = {};
+  a.added = added;
+  a.lengths = lengths;
+  a.table = table;
+  a.free_pages = free_pages;
+  a.taken = taken;
+  a.starts = starts;
+  a.counts = counts;
+  a.lengths_out = lengths_out;
+  a.taken_out = taken_out;
+  a.positions = positions;
+  a.slots = slots;
+  a.ticket = (uint32_t*)ws;
+  a.requests = (int32_t)requests;
+  a.cols = (int32_t)cols;
+  a.pages = (int32_t)pages;
+  a.page_shift = page_shift_of(page_size);
+  a.rows = (int32_t)rows;
+  a.max_new = (int32_t)std::min<int64_t>(max_new, rows);
+  return qtts_launch_paged_step(a, (hipStream_t)stream);
+}
+
+int qtts_paged_release(const int32_t* which, int64_t requests, int32_t* lengths, const int32_t* table, int64_t cols,
+                       int32_t* free_pages, int64_t pages, int32_t* taken, int64_t page_size, void* stream) {
+  QTTS_TRY(paged_sizes("paged_release", requests, cols, pages, page_size));
+  if (requests == 0 || cols == 0 || pages == 0) return QTTS_OK;
+  QTTS_REQUIRE(which && lengths && table && free_pages && taken, "paged_release: null pointer");
+  QTTS_TRY(current_device_check());
+  return qtts_launch_paged_release(which, lengths, table, (int)requests, (int)cols, free_pages, (int)pages, taken,
+                                   page_shift_of(page_size), (hipStream_t)stream);
+}
+
+int qtts_qkv_to_cache(const void* qkv, int dtype, int64_t rows, int64_t ldqkv, int64_t heads, int64_t kv_heads, int64_t d,
+                      const int32_t* positions, const int32_t* slots, const void* q_norm, const void* k_norm, float eps,
+                      const float* cos, const float* sin, int64_t rope_rows, void* k, void* v, int64_t pages,
+                      int64_t page_size, void* q, void* stream) {
+  QTTS_TRY(paged_sizes("qkv_to_cache", 0, 0, pages, page_size));
+  QTTS_REQUIRE(dtype == QTTS_BF16 || dtype == QTTS_F16, "qkv_to_cache: activations must be bf16 or fp16");
+  qtts::QkvCacheArgs a = {};
+  QTTS_TRY(paged_cache("qkv_to_cache", a.cache, k, v, pages, page_size, heads, kv_heads, d));
+  const int64_t width = (heads + 2 * kv_heads) * d;
+  QTTS_REQUIRE(rows >= 0 && rope_rows >= 0, "qkv_to_cache: negative size");
+  QTTS_REQUIRE(rows < (1ll << 24) && rope_rows < (1ll << 31), "qkv_to_cache: size too large");
+  QTTS_REQUIRE(ldqkv >= width, "qkv_to_cache: leading dimension smaller than the row");
+  QTTS_REQUIRE((cos == nullptr) == (sin == nullptr) && (!cos || rope_rows > 0), "qkv_to_cache: half a rotation table");
+  if (rows == 0) return QTTS_OK;
+  QTTS_REQUIRE(qkv && slots && q && (!cos || positions), "qkv_to_cache: null pointer");
+  QTTS_REQUIRE(((uintptr_t)qkv | (uintptr_t)q | (uintptr_t)q_norm | (uintptr_t)k_norm | (uintptr_t)cos | (uintptr_t)sin) % 16 == 0 &&
+                   ldqkv % 8 == 0, "qkv_to_cache: rows, norm weights and angles must start on 16 bytes");
+  QTTS_REQUIRE(!spans_overlap(qkv, rows, ldqkv, width, 2, q, rows, heads * d, heads * d, 2), "qkv_to_cache: q overlaps qkv");
+  const int64_t held = pages * page_size * kv_heads * d;
+  for (const void* c : {(const void*)k, (const void*)v})
+    QTTS_REQUIRE(!spans_overlap(c, 1, held, held, 2, q, rows, heads * d, heads * d, 2) &&
+                     !spans_overlap(c, 1, held, held, 2, qkv, rows, ldqkv, width, 2), "qkv_to_cache: the cache overlaps q or qkv");
+  QTTS_TRY(current_device_check());
+  a.qkv = qkv;
+  a.ldqkv = ldqkv;
+  a.positions = positions;
+  a.slots = slots;
+  a.q_norm = q_norm;
+  a.k_norm = k_norm;
+  a.cos = cos;
+  a.sin = sin;
+  a.q = q;
+  a.rows = (int32_t)rows;
+  a.heads = (int32_t)heads;
+  a.rope_rows = (int32_t)rope_rows;
+  a.eps = eps;
+  return qtts_launch_qkv_to_cache(a, dtype, (hipStream_t)stream);
+}
+
+int qtts_paged_attention(const void* q, int dtype, int64_t rows, int64_t ldq, int64_t heads, int64_t kv_heads, int64_t d,
+                         const void* k, const void* v, int64_t pages, int64_t page_size, const int32_t* table, int64_t requests,
+                         int64_t cols, const int32_t* starts, const int32_t* counts, const int32_t* lengths,
+                         const int32_t* slots, int64_t min_new, int64_t max_new, int64_t window, int64_t sinks, float scale,
+                         void* out, int64_t ldo, void* ws, int64_t ws_bytes, void* stream) {
+  QTTS_TRY(paged_sizes("paged_attention", requests, cols, pages, page_size));
+  QTTS_REQUIRE(dtype == QTTS_BF16 || dtype == QTTS_F16, "paged_attention: activations must be bf16 or fp16");
+  qtts::PagedAttentionArgs a = {};
+  QTTS_TRY(paged_cache("paged_attention", a.cache, k, v, pages, page_size, heads, kv_heads, d));
+  QTTS_REQUIRE(rows >= 0 && min_new >= 0 && max_new >= 0 && window >= 0 && sinks >= 0, "paged_attention: negative size");
+  QTTS_REQUIRE(rows < (1ll << 24), "paged_attention: size too large");
+  QTTS_REQUIRE(ldq >= heads * d && ldo >= heads * d, "paged_attention: leading dimension smaller than the row");
+  if (rows == 0) return QTTS_OK;
+  QTTS_REQUIRE(q && out && slots && (requests == 0 || (starts && counts && lengths && (cols == 0 || table))),
+               "paged_attention: null pointer");
+  QTTS_REQUIRE(((uintptr_t)q | (uintptr_t)out) % 16 == 0 && ldq % 8 == 0 && ldo % 8 == 0,
+               "paged_attention: rows must start on 16 bytes");
+  QTTS_REQUIRE(!spans_overlap(q, rows, ldq, heads * d, 2, out, rows, ldo, heads * d, 2), "paged_attention: out overlaps q");
+  const int64_t held = pages * page_size * kv_heads * d;
+  for (const void* c : {k, v})
+    QTTS_REQUIRE(!spans_overlap(c, 1, held, held, 2, out, rows, ldo, heads * d, 2), "paged_attention: out overlaps the cache");
+  QTTS_TRY(current_device_check());
+  a.q = q;
+  a.ldq = ldq;
+  a.out = out;
+  a.ldo = ldo;
+  a.table = table;
+  a.starts = starts;
+  a.counts = counts;
+  a.lengths = lengths;
+  a.slots = slots;
+  a.rows = (int32_t)rows;
+  a.heads = (int32_t)heads;
+  a.requests = (int32_t)requests;
+  a.cols = (int32_t)cols;
+  a.max_new = (int32_t)std::min<int64_t>(max_new, rows);
+  a.window = (int32_t)std::min<int64_t>(window, INT32_MAX);
+  a.sinks = (int32_t)std::min<int64_t>(sinks, INT32_MAX);
+  a.scale = scale * 1.44269504088896340736f;  // exponentials of 2
+  return qtts_launch_paged_attention(a, dtype, (hipStream_t)stream);
 }
 
 int qtts_kernel_timer_begin(int max_launches) {

@@ -60,7 +60,7 @@ ALGO_SKINNY_HALF, ALGO_SKINNY_QUARTER = 3, 4
 #: (for weights read once a step and too large to stay cached between steps); same bits out.
 ALGO_STREAM = 0x80
 # qtts_op
-OP_W8A16, OP_W8A8_FP8, OP_FP8_LINEAR, OP_W8A8_INT8, OP_INT8_LINEAR, OP_FP8W, OP_W8A16_SILU, OP_W8A16_FUSED, OP_LORA = range(9)
+OP_W8A16, OP_W8A8_FP8, OP_FP8_LINEAR, OP_W8A8_INT8, OP_INT8_LINEAR, OP_FP8W, OP_W8A16_SILU, OP_W8A16_FUSED, OP_LORA, OP_PAGED_ATTENTION = range(10)
 # qtts_prologue
 PRO_NONE, PRO_SILU_MUL, PRO_RMS_NORM = 0, 1, 2
 # qtts_strip_kind
@@ -106,6 +106,10 @@ EXPORTS = (
     "qtts_lora_plan",
     "qtts_lora_add",
     "qtts_lora_add_fresh",
+    "qtts_paged_step",
+    "qtts_paged_release",
+    "qtts_qkv_to_cache",
+    "qtts_paged_attention",
     "qtts_kernel_timer_begin",
     "qtts_kernel_timer_end",
 )
@@ -211,6 +215,16 @@ def load() -> ctypes.CDLL:
         for add in (L.qtts_lora_add, L.qtts_lora_add_fresh):
             add.restype = i32
             add.argtypes = [p, i32, i64, i64, i64, p, p, i64, p, p, i64, p, p, p, i64, p, i64, p, i64, i64, p, i64, p]
+        L.qtts_paged_step.restype = i32
+        L.qtts_paged_step.argtypes = [p, i64, p, p, i64, p, i64, p, i64, i64, i64, p, p, p, p, p, p, p, i64, p]
+        L.qtts_paged_release.restype = i32
+        L.qtts_paged_release.argtypes = [p, i64, p, p, i64, p, i64, p, i64, p]
+        L.qtts_qkv_to_cache.restype = i32
+        L.qtts_qkv_to_cache.argtypes = [p, i32, i64, i64, i64, i64, i64, p, p, p, p, ctypes.c_float, p, p, i64, p, p, i64, i64,
+                                        p, p]
+        L.qtts_paged_attention.restype = i32
+        L.qtts_paged_attention.argtypes = [p, i32, i64, i64, i64, i64, i64, p, p, i64, i64, p, i64, i64, p, p, p, p, i64, i64,
+                                           i64, i64, ctypes.c_float, p, i64, p, i64, p]
         L.qtts_kernel_timer_begin.restype = i32
         L.qtts_kernel_timer_begin.argtypes = [i32]
         L.qtts_kernel_timer_end.restype = i32

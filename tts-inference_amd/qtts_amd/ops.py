@@ -16,7 +16,7 @@ import torch
 
 from . import _lib
 from ._lib import (ALGO_AUTO, ALGO_SKINNY_HALF, ALGO_SKINNY_QUARTER, ALGO_STREAM, DIV_DEVICE, DIV_IEEE,  # noqa: F401
-                   LORA_MAX_PARTS, LORA_MAX_RANK, OP_FP8_LINEAR, OP_FP8W, OP_INT8_LINEAR, OP_LORA, OP_W8A16, OP_W8A16_FUSED, OP_W8A16_SILU, OP_W8A8_FP8, OP_W8A8_INT8, PRO_NONE,
+                   LORA_MAX_PARTS, LORA_MAX_RANK, OP_FP8_LINEAR, OP_FP8W, OP_INT8_LINEAR, OP_LORA, OP_PAGED_ATTENTION, OP_W8A16, OP_W8A16_FUSED, OP_W8A16_SILU, OP_W8A8_FP8, OP_W8A8_INT8, PRO_NONE,
                    PRO_RMS_NORM, PRO_SILU_MUL, STRIP_FP8, STRIP_INT8, CODE_E4M3, CODE_INT8, TILE_READ_AHEAD, TILE_TWO_CHUNKS, algo_code,
                    tile_shape)
 
@@ -1046,6 +1046,209 @@ def lora_add(base: torch.Tensor, x: torch.Tensor, batch: LoraBatch, a: torch.Ten
     if out is not None:
         return out
     return y if base.dim() == 2 else y.view(base.shape)
+
+
+# ---- attention over a paged key-value cache ---------------------------------------------------
+
+class PagedBatch:
+    """A step's rows over a paged cache, as :func:`paged_step` makes it: request r's rows are ``starts[r]`` to
+    ``starts[r] + counts[r]``, its tokens (the rows among them) ``lengths[r]``, on the pages ``table[r]`` of ``page_size`` tokens;
+    ``positions`` and ``slots`` ``[rows]`` say where each row belongs (-1: to no request).  All contiguous int32 on one GPU.
+    ``min_new`` and ``max_new`` bound the counts of every step that these tensors will hold; ``taken`` ``[1]`` is the
+    free list's state after the step (None where the batch was made by hand)."""
+
+    __slots__ = ("table", "starts", "counts", "lengths", "positions", "slots", "page_size", "requests", "rows", "max_new", "min_new",
+                 "taken")
+
+    def __init__(self, table: torch.Tensor, starts: torch.Tensor, counts: torch.Tensor, lengths: torch.Tensor,
+                 positions: torch.Tensor, slots: torch.Tensor, page_size: int, max_new: int | None = None, min_new: int = 0,
+                 taken: torch.Tensor | None = None) -> None:
+        if table.dim() != 2:
+            raise ValueError(f"the page table must be [requests, columns], got {tuple(table.shape)}")
+        requests, rows, idx = table.shape[0], positions.shape[0], table.get_device()
+        for name, t, size in (("table", table, None), ("starts", starts, requests + 1), ("counts", counts, requests),
+                              ("lengths", lengths, requests), ("positions", positions, rows), ("slots", slots, rows),
+                              ("taken", taken, 1)):
+            if t is None:
+                continue
+            if t.dtype != torch.int32 or not t.is_contiguous() or (size is not None and t.shape != (size,)):
+                raise ValueError(f"{name} must be contiguous int32{'' if size is None else f' [{size}]'}, got {t.dtype} "
+                                 f"{tuple(t.shape)}")
+            if t.get_device() != idx:
+                raise ValueError(f"{name} is on {t.device}, the page table on {table.device}")
+        self.table, self.starts, self.counts, self.lengths, self.positions, self.slots = (table, starts, counts, lengths, positions,
+                                                                                          slots)
+        self.page_size, self.requests, self.rows, self.taken = int(page_size), requests, rows, taken
+        self.max_new, self.min_new = rows if max_new is None else int(max_new), int(min_new)
+
+
+def paged_step(new: torch.Tensor, lengths: torch.Tensor, table: torch.Tensor, free: torch.Tensor, taken: torch.Tensor,
+               page_size: int, rows: int, max_new: int | None = None, min_new: int = 0, out: PagedBatch | None = None) -> PagedBatch:
+    """The page tables, positions and cache slots of a step's new tokens, from the requests' lengths, in one kernel.
+
+    new ``[R]`` tokens join the requests that hold ``lengths`` ``[R]``; their rows lie one request behind the other in a batch of
+    ``rows``.  New pages are ``free[taken[0]:]`` in the requests' order; their columns of ``table`` ``[R, C]`` are written.
+    Everything is int32 on the GPU, so a captured step follows what the tensors hold at each replay.  A request whose rows
+    pass ``max_new`` (None: ``rows``) or the batch, whose tokens pass the table or whose pages are not left is denied as a whole:
+    ``counts`` 0, its rows at position and slot -1.  Returns a batch of fresh tensors on the same table, or ``out`` (of the
+    same sizes; its lengths and taken may be the ones given)."""
+    if table.dim() != 2:
+        raise ValueError(f"the page table must be [requests, columns], got {tuple(table.shape)}")
+    requests, cols = table.shape
+    rows = int(rows)
+    for name, t, size in (("new", new, requests), ("lengths", lengths, requests), ("free", free, None), ("taken", taken, 1),
+                          ("table", table, None)):
+        if t.dtype != torch.int32 or not t.is_contiguous() or (name != "table" and (t.dim() != 1 or size not in (None, t.shape[0]))):
+            raise ValueError(f"{name} must be contiguous int32{'' if size is None else f' [{size}]'}, got {t.dtype} {tuple(t.shape)}")
+    if rows < 0:
+        raise ValueError(f"a batch of {rows} rows")
+    idx = _gpu_index(table, new, lengths, free, taken)
+    if idx != _current_device():
+        with torch.cuda.device(idx):
+            return paged_step(new, lengths, table, free, taken, page_size, rows, max_new, min_new, out)
+    if out is None:
+        starts, counts, after, left, positions, slots = torch.empty(
+            3 * requests + 2 + 2 * rows, dtype=torch.int32, device=table.device).split(
+                [requests + 1, requests, requests, 1, rows, rows])
+        out = PagedBatch(table, starts, counts, after, positions, slots, page_size, max_new, min_new, left)
+    elif (out.requests != requests or out.rows != rows or out.page_size != page_size or out.taken is None
+          or out.table.data_ptr() != table.data_ptr()):
+        raise ValueError(f"out is no batch of {rows} rows and {requests} requests on this page table")
+    ws = _workspaces.get(idx)
+    if ws is None:
+        _ensure_workspace(table.device, 1, "paged_step")
+        ws = _workspaces[idx]
+    st = _lib.load().qtts_paged_step(
+        new.data_ptr(), requests, lengths.data_ptr(), table.data_ptr(), cols, free.data_ptr(), free.shape[0], taken.data_ptr(),
+        page_size, rows, out.max_new, out.starts.data_ptr(), out.counts.data_ptr(), out.lengths.data_ptr(), out.taken.data_ptr(),
+        out.positions.data_ptr(), out.slots.data_ptr(), ws.data_ptr(), ws.numel(), _raw_stream(idx))
+    if st:
+        _lib.check(st, "paged_step")
+    return out
+
+
+def paged_release(which: torch.Tensor, lengths: torch.Tensor, table: torch.Tensor, free: torch.Tensor, taken: torch.Tensor,
+                  page_size: int) -> None:
+    """The pages of the requests with a nonzero ``which`` ``[R]`` back to the free list; their lengths are 0 afterwards."""
+    if table.dim() != 2:
+        raise ValueError(f"the page table must be [requests, columns], got {tuple(table.shape)}")
+    requests, cols = table.shape
+    for name, t, size in (("which", which, requests), ("lengths", lengths, requests), ("free", free, None), ("taken", taken, 1),
+                          ("table", table, None)):
+        if t.dtype != torch.int32 or not t.is_contiguous() or (name != "table" and (t.dim() != 1 or size not in (None, t.shape[0]))):
+            raise ValueError(f"{name} must be contiguous int32{'' if size is None else f' [{size}]'}, got {t.dtype} {tuple(t.shape)}")
+    idx = _gpu_index(table, which, lengths, free, taken)
+    if idx != _current_device():
+        with torch.cuda.device(idx):
+            return paged_release(which, lengths, table, free, taken, page_size)
+    st = _lib.load().qtts_paged_release(which.data_ptr(), requests, lengths.data_ptr(), table.data_ptr(), cols, free.data_ptr(),
+                                        free.shape[0], taken.data_ptr(), page_size, _raw_stream(idx))
+    if st:
+        _lib.check(st, "paged_release")
+
+
+def _cache_sizes(k: torch.Tensor, v: torch.Tensor, batch: PagedBatch, dtype: torch.dtype) -> tuple[int, int, int]:
+    """Pages, key-value heads and head size of a cache that fits the batch."""
+    if k.dim() != 4 or v.dim() != 4:
+        raise ValueError(f"k and v must be [pages, kv heads, page size, head size] and [pages, kv heads, head size, page size], got "
+                         f"{tuple(k.shape)} and {tuple(v.shape)}")
+    pages, kv_heads, page_size, d = k.shape
+    if v.shape != (pages, kv_heads, d, page_size) or page_size != batch.page_size:
+        raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} are no cache of pages of {batch.page_size} tokens")
+    if k.dtype != dtype or v.dtype != dtype:
+        raise ValueError(f"the cache holds {k.dtype} and {v.dtype}, the rows are {dtype}")
+    if not k.is_contiguous() or not v.is_contiguous():
+        raise ValueError("k and v must be contiguous")
+    return pages, kv_heads, d
+
+
+def _aligned_rows(x: torch.Tensor) -> torch.Tensor:
+    """``[rows, n]`` with rows on 16 bytes (a copy where they are not)."""
+    if x.stride(1) != 1 or x.data_ptr() % 16 or (x.shape[0] > 1 and (x.stride(0) % 8 or x.stride(0) < x.shape[1])):
+        return x.clone(memory_format=torch.contiguous_format)
+    return x
+
+
+def qkv_to_cache(qkv: torch.Tensor, k: torch.Tensor, v: torch.Tensor, batch: PagedBatch, heads: int,
+                 q_norm: torch.Tensor | None = None, k_norm: torch.Tensor | None = None, eps: float = 1e-6,
+                 rope: tuple[torch.Tensor, torch.Tensor] | None = None) -> torch.Tensor:
+    """The rows of a fused qkv projection on their way to attention, in one kernel: RMSNorm of the query and key heads
+    (``q_norm``, ``k_norm`` ``[D]``, or None), rotation by the rows' positions, keys and values into the cache.
+
+    qkv ``[..., (Hq + 2 H) D]`` bf16 or fp16, ``batch.rows`` rows; k ``[pages, H, S, D]`` and v ``[pages, H, D, S]`` are written
+    at the batch's slots.  rope: fp32 ``(cos, sin)`` ``[positions, D / 2]``, for as many positions as the page table has
+    (None: no rotation); halves of a head rotate against each other.  In fp32 with one rounding.  Returns the queries
+    ``[rows, Hq, D]``, zeros in rows of no request."""
+    x = qkv.reshape(-1, qkv.shape[-1]) if qkv.dim() != 2 else qkv
+    dtype = x.dtype
+    pages, kv_heads, d = _cache_sizes(k, v, batch, dtype)
+    rows = x.shape[0]
+    if rows != batch.rows or x.shape[1] != (heads + 2 * kv_heads) * d:
+        raise ValueError(f"qkv is {tuple(qkv.shape)} for {batch.rows} rows of {heads} + 2 x {kv_heads} heads of {d}")
+    cos, sin = rope if rope is not None else (None, None)
+    if rope is not None:
+        need = batch.table.shape[1] * batch.page_size
+        for t in (cos, sin):
+            if t.dtype != torch.float32 or not t.is_contiguous() or t.dim() != 2 or t.shape[1] != d // 2 or t.shape[0] < need:
+                raise ValueError(f"rope must hold contiguous fp32 [{need} or more, {d // 2}] tables, got {t.dtype} {tuple(t.shape)}")
+        if cos.shape != sin.shape:
+            raise ValueError(f"rope's tables differ: {tuple(cos.shape)} and {tuple(sin.shape)}")
+    norms = []
+    for w in (q_norm, k_norm):
+        if w is not None:
+            if w.shape != (d,):
+                raise ValueError(f"norm weight {tuple(w.shape)} for heads of {d}")
+            w = w.to(dtype).contiguous()
+            w = w.clone() if w.data_ptr() % 16 else w
+        norms.append(w)
+    idx = _gpu_index(x, k, v, batch.table, cos, sin, *norms)
+    if idx != _current_device():
+        with torch.cuda.device(idx):
+            return qkv_to_cache(qkv, k, v, batch, heads, q_norm, k_norm, eps, rope)
+    x = _aligned_rows(x)
+    q = torch.empty(rows, heads, d, dtype=dtype, device=x.device)
+    st = _lib.load().qtts_qkv_to_cache(
+        x.data_ptr(), dtype_code(dtype), rows, x.stride(0) if rows > 1 else x.shape[1], heads, kv_heads, d, batch.positions.data_ptr(),
+        batch.slots.data_ptr(), _ptr(norms[0]), _ptr(norms[1]), eps, _ptr(cos), _ptr(sin), 0 if cos is None else cos.shape[0],
+        k.data_ptr(), v.data_ptr(), pages, batch.page_size, q.data_ptr(), _raw_stream(idx))
+    if st:
+        _lib.check(st, "qkv_to_cache")
+    return q
+
+
+def paged_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, batch: PagedBatch, window: int = 0, sinks: int = 0,
+                    scale: float | None = None) -> torch.Tensor:
+    """Attention of the batch's rows over their requests' tokens in a paged cache, the rows' own among them
+    (:func:`qkv_to_cache` comes first).
+
+    q ``[rows, Hq, D]`` bf16 or fp16 (any row stride), k ``[pages, H, S, D]``, v ``[pages, H, D, S]``; query head h reads key-value
+    head ``h // (Hq / H)``.  A row at position p sees the keys ``j <= p``, with a ``window`` those ``j > p - window`` and the first
+    ``sinks``.  scale: of the scores (None: ``D ** -0.5``).  Single tokens, prompts and chunks of prompts may share a batch;
+    long caches are split over the GPU and joined.  Returns ``[rows, Hq, D]``, zeros in rows of no request."""
+    if q.dim() != 3:
+        raise ValueError(f"q must be [rows, heads, head size], got {tuple(q.shape)}")
+    rows, heads, d = q.shape
+    pages, kv_heads, width = _cache_sizes(k, v, batch, q.dtype)
+    if rows != batch.rows or d != width:
+        raise ValueError(f"q is {tuple(q.shape)} for {batch.rows} rows of heads of {width}")
+    if window < 0 or sinks < 0:
+        raise ValueError(f"window {window} and sinks {sinks} must not be negative")
+    idx = _gpu_index(q, k, v, batch.table)
+    if idx != _current_device():
+        with torch.cuda.device(idx):
+            return paged_attention(q, k, v, batch, window, sinks, scale)
+    if q.stride(2) != 1 or q.stride(1) != d or q.data_ptr() % 16 or (rows > 1 and (q.stride(0) % 8 or q.stride(0) < heads * d)):
+        q = q.clone(memory_format=torch.contiguous_format)
+    out = torch.empty(rows, heads, d, dtype=q.dtype, device=q.device)
+    ws, ws_n = _ws_for(q.device)
+    st = _lib.load().qtts_paged_attention(
+        q.data_ptr(), dtype_code(q.dtype), rows, q.stride(0) if rows > 1 else heads * d, heads, kv_heads, d, k.data_ptr(), v.data_ptr(),
+        pages, batch.page_size, batch.table.data_ptr(), batch.requests, batch.table.shape[1], batch.starts.data_ptr(),
+        batch.counts.data_ptr(), batch.lengths.data_ptr(), batch.slots.data_ptr(), batch.min_new, batch.max_new, window, sinks,
+        d ** -0.5 if scale is None else scale, out.data_ptr(), heads * d, ws, ws_n, _raw_stream(idx))
+    if st:
+        _lib.check(st, "paged_attention")
+    return out
 
 
 class KernelTimer:
