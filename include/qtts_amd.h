@@ -80,7 +80,7 @@ typedef enum {
     QTTS_OP_W8A16_SILU = 6,
     QTTS_OP_W8A16_FUSED = 7,
     QTTS_OP_LORA = 8, /* n: the linear's partitions, k: the rank */
-    QTTS_OP_PAGED_ATTENTION = 9 /* m: the largest count of a request, n: query heads, k: the head size */
+    QTTS_OP_PAGED_ATTENTION = 16 /* m: the largest count of a request, n: query heads, k: the head size */
 } qtts_op;
 
 /* What qtts_w8a16_fused_gemm_strips applies to its activations before the GEMM. */

@@ -60,7 +60,8 @@ ALGO_SKINNY_HALF, ALGO_SKINNY_QUARTER = 3, 4
 #: (for weights read once a step and too large to stay cached between steps); same bits out.
 ALGO_STREAM = 0x80
 # qtts_op
-OP_W8A16, OP_W8A8_FP8, OP_FP8_LINEAR, OP_W8A8_INT8, OP_INT8_LINEAR, OP_FP8W, OP_W8A16_SILU, OP_W8A16_FUSED, OP_LORA, OP_PAGED_ATTENTION = range(10)
+OP_W8A16, OP_W8A8_FP8, OP_FP8_LINEAR, OP_W8A8_INT8, OP_INT8_LINEAR, OP_FP8W, OP_W8A16_SILU, OP_W8A16_FUSED, OP_LORA = range(9)
+OP_PAGED_ATTENTION = 16
 # qtts_prologue
 PRO_NONE, PRO_SILU_MUL, PRO_RMS_NORM = 0, 1, 2
 # qtts_strip_kind
