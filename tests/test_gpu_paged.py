@@ -391,3 +391,67 @@ def test_single_tokens(ops, held, page, heads, kv, d, window, sinks, dtype):
 def test_many_tokens(ops, requests, page, heads, kv, d, padding, window, sinks, dtype):
     q, k, v, batch = _inputs(ops, requests, page, heads, kv, d, dtype, seed=d + len(requests), padding=padding)
     _check(ops, q, k, v, batch, window, sinks)
+
+
+@DTYPES
+@pytest.mark.parametrize("heads,kv,d,page", [(16, 8, 128, 64), (16, 8, 128, 16), (8, 8, 64, 32), (16, 1, 256, 64), (28, 4, 80, 128)])
+@pytest.mark.parametrize("held,window,sinks", [([9000], 0, 0), ([20000, 3, 700], 0, 0), ([6000] * 5, 3000, 4), ([4095, 12345, 1], 0, 0),
+                                               ([8000, 100], 5000, 300)])
+def test_split_lengths(ops, held, window, sinks, heads, kv, d, page, dtype):
+    """Lengths that several workgroups share, next to short ones; again on the workspace that the first call left."""
+    q, k, v, batch = _inputs(ops, [(h, 1) for h in held], page, heads, kv, d, dtype, seed=len(held), padding=1)
+    first = _check(ops, q, k, v, batch, window, sinks)
+    for _ in range(2):
+        assert torch.equal(ops.paged_attention(q, k, v, batch, window, sinks), first)
+
+
+@DTYPES
+@pytest.mark.parametrize("requests,heads,kv", [([(50, 3), (0, 8), (1000, 1), (5000, 5)], 16, 8), ([(40, 4), (33, 2)], 4, 1), ([(100, 16)], 2, 2)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (20, 3)])
+def test_drafted_tokens(ops, requests, heads, kv, window, sinks, dtype):
+    """A few tokens a request (rows of a run at several positions), as when drafts are verified."""
+    q, k, v, batch = _inputs(ops, requests, 32, heads, kv, 128, dtype, seed=5)
+    _check(ops, q, k, v, batch, window, sinks)
+
+
+def _poison(k, v, batch, r, positions, value, where):
+    at = torch.tensor(positions, device="cuda")
+    slot = batch.table[r].long()[at // batch.page_size] * batch.page_size + at % batch.page_size
+    if "k" in where:
+        k[slot // batch.page_size, :, slot % batch.page_size] = value
+    if "v" in where:
+        v[slot // batch.page_size, :, :, slot % batch.page_size] = value
+
+
+@DTYPES
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), float("-inf")])
+@pytest.mark.parametrize("heads,kv,d", [(16, 8, 128), (4, 4, 64), (8, 1, 256), (4, 2, 80)])
+@pytest.mark.parametrize("count", [1, 2, 7, 60, 150])
+def test_what_a_row_does_not_see(ops, count, heads, kv, d, value, dtype):
+    """Infinities and NaN in tokens behind a row, or outside its window, do not reach it; those it sees do."""
+    requests = [(200, count), (3, 1)]
+    q, k, v, batch = _inputs(ops, requests, 16, heads, kv, d, dtype, seed=7)
+    clean = [_check(ops, q, k, v, batch, w, s) for w, s in ((0, 0), (50, 4))]
+    if count > 1:  # the last token's: the rows before it do not see it
+        kk, vv = k.clone(), v.clone()
+        _poison(kk, vv, batch, 0, [200 + count - 1], value, "kv")
+        for (w, s), want in zip(((0, 0), (50, 4)), clean):
+            out = ops.paged_attention(q, kk, vv, batch, w, s)
+            _check_rows(out, want, [r for r in range(count + 1) if r != count - 1])
+    kk, vv = k.clone(), v.clone()
+    _poison(kk, vv, batch, 0, list(range(4, 151)), value, "kv")  # outside the window, but of 50 keys in front of the first row
+    out = ops.paged_attention(q, kk, vv, batch, 50, 4)
+    _check_rows(out, clean[1], list(range(count + 1)))
+    kk, vv = k.clone(), v.clone()  # seen by all rows, values alone: infinities come out as they are
+    _poison(kk, vv, batch, 0, [199], value, "v")
+    out = ops.paged_attention(q, kk, vv, batch)
+    assert not out[:count].isfinite().any() and out[count:].isfinite().all()
+    if value == value:
+        assert (out[:count] == value).all()
+
+
+def _check_rows(out, want, rows):
+    """The rows as they are without the bad values (bit for bit up to the join of other tiles: within two steps)."""
+    fi = torch.finfo(out.dtype)
+    err = (out[rows].double() - want[rows].double()).abs()
+    assert (err <= 2 * fi.eps * want[rows].double().abs().amax(-1, keepdim=True) + fi.tiny).all()

@@ -83,7 +83,8 @@ int qtts_launch_paged_step(const qtts::PagedStepArgs& args, hipStream_t st);
 int qtts_launch_paged_release(const int32_t* which, int32_t* lengths, const int32_t* table, int requests, int cols,
                               int32_t* free_pages, int pages, int32_t* taken, int page_shift, hipStream_t st);
 int qtts_launch_qkv_to_cache(const qtts::QkvCacheArgs& args, int dtype, hipStream_t st);
-int qtts_launch_paged_attention(const qtts::PagedAttentionArgs& args, int dtype, hipStream_t st);
+int qtts_launch_paged_attention(const qtts::PagedAttentionArgs& args, int min_new, int dtype, void* ws, hipStream_t st);
+int64_t qtts_paged_attention_ws_bytes(int64_t d);
 
 static thread_local char g_last_error[512] = "";
 
@@ -271,7 +272,8 @@ int64_t qtts_workspace_bytes(int op, int64_t m, int64_t n, int64_t k, int algo) 
         return qtts_set_error(QTTS_ERR_INVALID_ARGUMENT, "bad workspace query");
       return qtts_lora_ws_bytes(m, n, k);
     case QTTS_OP_PAGED_ATTENTION:  // n query heads of k
-      return qtts::kCounterBytes;
+      if (k > qtts::kPagedMaxDim) return qtts_set_error(QTTS_ERR_INVALID_ARGUMENT, "bad workspace query");
+      return qtts_paged_attention_ws_bytes(k);
     default: return qtts_set_error(QTTS_ERR_INVALID_ARGUMENT, "unknown op %d", op);
   }
 }
@@ -1059,6 +1061,8 @@ int qtts_paged_attention(const void* q, int dtype, int64_t rows, int64_t ldq, in
   QTTS_REQUIRE(rows >= 0 && min_new >= 0 && max_new >= 0 && window >= 0 && sinks >= 0, "paged_attention: negative size");
   QTTS_REQUIRE(rows < (1ll << 24), "paged_attention: size too large");
   QTTS_REQUIRE(ldq >= heads * d && ldo >= heads * d, "paged_attention: leading dimension smaller than the row");
+  QTTS_REQUIRE(scale > 0 && scale <= 3.402823466e38f, "paged_attention: scale %g is not positive", (double)scale);
+  QTTS_REQUIRE(ws_bytes >= 0, "paged_attention: negative workspace size");
   if (rows == 0) return QTTS_OK;
   QTTS_REQUIRE(q && out && slots && (requests == 0 || (starts && counts && lengths && (cols == 0 || table))),
                "paged_attention: null pointer");
@@ -1068,6 +1072,10 @@ int qtts_paged_attention(const void* q, int dtype, int64_t rows, int64_t ldq, in
   const int64_t held = pages * page_size * kv_heads * d;
   for (const void* c : {k, v})
     QTTS_REQUIRE(!spans_overlap(c, 1, held, held, 2, out, rows, ldo, heads * d, 2), "paged_attention: out overlaps the cache");
+  const int64_t need = qtts_paged_attention_ws_bytes(d);
+  if (!ws || ws_bytes < need)
+    return qtts_set_error(QTTS_ERR_WORKSPACE, "paged_attention: workspace of %lld bytes < %lld needed", (long long)ws_bytes,
+                          (long long)need);
   QTTS_TRY(current_device_check());
   a.q = q;
   a.ldq = ldq;
@@ -1081,12 +1089,12 @@ int qtts_paged_attention(const void* q, int dtype, int64_t rows, int64_t ldq, in
   a.rows = (int32_t)rows;
   a.heads = (int32_t)heads;
   a.requests = (int32_t)requests;
-  a.cols = (int32_t)cols;
+  a.cols = pages ? (int32_t)cols : 0;  // no pages hold no tokens
   a.max_new = (int32_t)std::min<int64_t>(max_new, rows);
   a.window = (int32_t)std::min<int64_t>(window, INT32_MAX);
   a.sinks = (int32_t)std::min<int64_t>(sinks, INT32_MAX);
   a.scale = scale * 1.44269504088896340736f;  // exponentials of 2
-  return qtts_launch_paged_attention(a, dtype, (hipStream_t)stream);
+  return qtts_launch_paged_attention(a, (int)std::min<int64_t>(min_new, rows), dtype, ws, (hipStream_t)stream);
 }
 
 int qtts_kernel_timer_begin(int max_launches) {

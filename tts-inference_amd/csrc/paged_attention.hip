@@ -1,6 +1,6 @@
 // Attention of a step's new tokens over a paged key-value cache: the plain kernel, one wave a row and head.
 #include "common.h"
-#include "paged.h"
+#include "paged_attn.h"
 
 namespace qtts {
 
@@ -60,8 +60,38 @@ template <typename T> __global__ __launch_bounds__(64) void paged_attention_kern
 
 }  // namespace qtts
 
-int qtts_launch_paged_attention(const qtts::PagedAttentionArgs& a, int dtype, hipStream_t st) {
+int qtts_launch_paged_small(const qtts::PagedLaunch& p, int dtype, hipStream_t st);
+
+namespace qtts {
+
+constexpr int kSmallGroups = 1024;  // workgroups that the keys of few rows are cut for
+constexpr int kSmallRows = 16;
+
+static int64_t small_slot_floats(int rows, int d) { return ((int64_t)rows * (d + 2) + 63) & ~63ll; }
+
+}  // namespace qtts
+
+int64_t qtts_paged_attention_ws_bytes(int64_t d) {
   using namespace qtts;
+  return kCounterBytes + 2 * kSmallGroups * small_slot_floats(kSmallRows, (int)d) * 4;
+}
+
+int qtts_launch_paged_attention(const qtts::PagedAttentionArgs& a, int min_new, int dtype, void* ws, hipStream_t st) {
+  using namespace qtts;
+  const int64_t group = a.heads / a.cache.kv_heads;
+  if (a.max_new * group <= kSmallRows) {
+    PagedLaunch p = {};
+    p.a = a;
+    p.groups = kSmallGroups / a.cache.kv_heads;
+    p.least = 8;
+    p.max_rows = kSmallRows;
+    p.items = a.requests + p.groups;
+    p.fill = a.rows < 256 * 16 ? (a.rows + 15) / 16 : 256;
+    p.counters = (unsigned*)ws;
+    p.parts = (float*)((uint8_t*)ws + kCounterBytes);
+    p.slot_floats = small_slot_floats((int)(a.max_new * group), a.cache.d);
+    return qtts_launch_paged_small(p, dtype, st);
+  }
   const dim3 grid(a.rows, a.heads);
   if (dtype == QTTS_BF16) launch(paged_attention_kernel<bf16_t>, grid, dim3(64), 0u, st, a);
   else launch(paged_attention_kernel<f16_t>, grid, dim3(64), 0u, st, a);

@@ -1,0 +1,333 @@
+// Attention of few rows a request over a paged cache (single tokens; a count times the query heads of a key-value head up
+// to 16): bound by the cache's bytes.
+//
+// The mathematics: S^T = K Q^T and O^T = V^T P^T with 16x16x32 MFMAs, 32 keys a wave and step, the running maximum and sum
+// of the softmax per column (a row of Q).  The tile's keys are dealt to the rows of the two S^T products so that the eight
+// scores that a lane receives are those of eight consecutive keys, which are the lane's operand of the second product: P
+// never leaves its lane, and the values, d-major on their page, are 16-byte loads of that operand's other side.  Keys and
+// values go from memory to registers and nowhere else; LDS joins the four waves at the end.
+//
+// P goes to the second product in two 16-bit parts, whose products add up to P's in fp32's neighbourhood: the matrix cores
+// have the time (a wave's step is 32 MFMAs of 8 cycles to 16 KiB of cache), and sums that cancel keep their bits.
+//
+// Splits: the tiles of all requests are cut into pieces of one size, and a request's last workgroup to finish joins its
+// pieces (paged_attn.h).
+#include "paged_attn.h"
+
+namespace qtts {
+
+namespace {
+
+constexpr int kTile = 32, kRows = 16, kWaves = 4, kThreads = 64 * kWaves;
+
+// 16 bits a value: infinities and NaN have all exponent bits set.
+template <typename T> __device__ __forceinline__ bool not_finite(uint32_t two) {
+  constexpr uint32_t e = std::is_same<T, bf16_t>::value ? 0x7f80u : 0x7c00u;
+  return (two & e) == e || (two & (e << 16)) == (e << 16);  // of either
+}
+
+// Orders this wave's LDS writes before its reads, and the other way round (the wave's lanes run together).
+__device__ __forceinline__ void wave_lds_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+// DP: the head size rounded up to 64, 128 or 256.
+template <typename T, int DP> __global__ __launch_bounds__(kThreads, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) void paged_small_kernel(PagedLaunch p) {
+  typedef typename mfma16<T>::vec vec;
+  constexpr int NC = DP / 32, NB = DP / 16;
+  __shared__ float part[kWaves][kRows][DP + 4];
+  __shared__ float part_w[kWaves][kTile * kRows];
+  __shared__ float part_m[kWaves][kRows], part_l[kWaves][kRows];
+  __shared__ unsigned flag;
+  const PagedAttentionArgs& a = p.a;
+  const int kv_heads = a.cache.kv_heads, h = blockIdx.x % kv_heads, item = blockIdx.x / kv_heads;
+  if (item >= p.items) {
+    fill_rows<T>(p, blockIdx.x - p.items * kv_heads);
+    return;
+  }
+  PagedWork w;
+  if (!paged_work<kRows, kTile>(p, item, w)) return;
+  const int group = a.heads / kv_heads, d = a.cache.d, shift = a.cache.page_shift;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
+  const int rows = w.count * group;
+
+  const KeyTiles tiles = key_tiles<kTile>(w.position, w.length - 1, a.window, a.sinks);
+  const int begin = w.split * w.chunk, end = min(tiles.count, begin + w.chunk);
+  const int splits = (tiles.count + w.chunk - 1) / w.chunk;  // w.splits or fewer
+  if (w.split >= splits) return;
+
+  // this lane's column: row `col` of the run
+  const int token = col / group, query = h * group + col - token * group;
+  const bool live = col < rows;
+  const int hi = live ? w.position + token : -1, lo = a.window && live ? max(0, hi - a.window + 1) : 0;
+  const int32_t all_lo = a.window ? max(0, w.length - a.window) : 0;  // every row sees [all_lo, w.position]
+  const int32_t any_lo = a.window ? max(0, w.position - a.window + 1) : 0;  // and no row what is below any_lo and no sink
+  vec qf[NC];
+  {
+    const T* q = (const T*)a.q + (int64_t)(w.row + (live ? token : 0)) * a.ldq + (int64_t)(live ? query : 0) * d;
+    const i32x4_t zero = {0, 0, 0, 0};
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      const int dim = c * 32 + g * 8;
+      qf[c] = __builtin_bit_cast(vec, live && dim < d ? *(const i32x4_t*)(q + dim) : zero);
+    }
+  }
+
+  f32x4_t o[NB];
+  float m, l;
+
+  // Key of product t's row r: base + 8 (r / 4) + 4 t + r % 4; this lane's eight scores: keys base + 8 g + 0..7.
+  const int32_t* table = a.table + (int64_t)w.request * a.cols;
+  const int last = (w.length - 1) & ~7, mask = (1 << shift) - 1;
+  const int kgroup = (col >> 2) * 8, kin = col & 3;
+  auto tile_of = [&](int i) { return key_tile(tiles, min(i, end - 1)) * kTile; };
+  auto page_of = [&](int key) { return table[min(key, last) >> shift]; };
+  auto head_of = [&](int32_t page) {
+    return ((int64_t)paged_page(page, a.cache.pages) * kv_heads + h) * ((int64_t)d << shift);
+  };
+  i32x4_t kf[2][NC], vf[NB];
+  auto load_k = [&](int base, int32_t page) {
+    const T* k = (const T*)a.cache.k + head_of(page) + (int64_t)((min(base + kgroup, last) & mask) + kin) * d + g * 8;
+    const i32x4_t zero = {0, 0, 0, 0};
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+        kf[t][c] = c * 32 + g * 8 < d ? *(const i32x4_t*)(k + (int64_t)t * 4 * d + c * 32) : zero;
+  };
+  auto load_v = [&](int base, int32_t page) {
+    const T* v = (const T*)a.cache.v + head_of(page) + (min(base + g * 8, last) & mask) + ((int64_t)col << shift);
+#pragma unroll
+    for (int b = 0; b < NB; ++b) vf[b] = *(const i32x4_t*)(v + ((int64_t)min(b, d / 16 - 1) << (shift + 4)));
+  };
+
+  // One pass over the wave's tiles.  `careful`: values that are infinities or NaN do not go through the matrix cores, where a row
+  // that does not see them would take 0 * NaN from them and a weight's second part could turn an infinity's sign.
+  auto pass = [&](auto careful) {
+    m = kLowest;
+    l = 0.0f;
+#pragma unroll
+    for (int b = 0; b < NB; ++b) o[b] = f32x4_t{0, 0, 0, 0};
+    int i = begin + wave;
+    if (i >= end) return;
+    int base = tile_of(i), next = tile_of(i + kWaves);
+    load_k(base, page_of(base + kgroup));
+    load_v(base, page_of(base + g * 8));
+    int32_t page_k = page_of(next + kgroup), page_v = page_of(next + g * 8);
+    for (; i < end; i += kWaves) {
+      f32x4_t s[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) s[t] = mfma16<T>::mma(__builtin_bit_cast(vec, kf[t][c]), qf[c], s[t]);
+      const bool more = i + kWaves < end;
+      if (more) load_k(next, page_k);
+      const int key = base + g * 8;
+      // a tile that every row sees whole needs no mask
+      const bool whole = base + kTile - 1 <= w.position && (base >= all_lo || base + kTile <= a.sinks);
+      float x[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = s[j >> 2][j & 3];
+      if (!whole) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = key + j <= hi && (key + j >= lo || key + j < a.sinks) ? x[j] : -INFINITY;
+      }
+      float top = x[0];
+#pragma unroll
+      for (int j = 1; j < 8; ++j) top = fmaxf(top, x[j]);
+      top = max_16_32(top) * a.scale;
+      // The maximum moves only where a score passes it by 8 powers of two: weights stay under 256 and most steps keep O.
+      if (__any(top > m + 8.0f)) {
+        const float now = fmaxf(m, top), keep = exp2_hw(m - now);
+        m = now;
+        l *= keep;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) o[b] *= keep;
+      }
+      float w8[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        w8[j] = exp2_hw(__builtin_fmaf(x[j], a.scale, -m));
+        l += w8[j];
+      }
+      i32x4_t p1, p2;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t two = pack2_f32<T>(w8[2 * j], w8[2 * j + 1]);
+        p1[j] = (int)two;
+        p2[j] = (int)pack2_f32<T>(w8[2 * j] - to_f32(T{(uint16_t)two}), w8[2 * j + 1] - to_f32(T{(uint16_t)(two >> 16)}));
+      }
+      if (!whole) {  // values that no row sees, among them what lies behind the request's end and was never written: zero
+        uint32_t keep[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (key + j < w.length && (key + j >= any_lo || key + j < a.sinks)) keep[j >> 1] |= 0xffffu << (16 * (j & 1));
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) vf[b][j] = (int)((uint32_t)vf[b][j] & keep[j]);
+      }
+      if constexpr (decltype(careful)::value) {
+        // The tile and its weights through LDS: key by key, rows that see a value that is not finite add it; the others do not.
+        uint16_t* values = (uint16_t*)part[wave];  // [key][DP]
+        float* weights = part_w[wave];             // [key][row]
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          weights[(g * 8 + j) * kRows + col] = w8[j];
+#pragma unroll
+          for (int b = 0; b < NB; ++b)
+            values[(g * 8 + j) * DP + b * 16 + col] = (uint16_t)((uint32_t)vf[b][j >> 1] >> (16 * (j & 1)));
+        }
+        wave_lds_fence();
+#pragma unroll 1
+        for (int n = 0; n < kTile; ++n) {
+          const int at = base + n;
+          const bool seen = at <= hi && (at >= lo || at < a.sinks);
+          const float weight = weights[n * kRows + col];
+#pragma unroll
+          for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const uint16_t v = values[n * DP + b * 16 + g * 4 + e];
+              if (seen && not_finite<T>(v)) o[b][e] += weight * to_f32(T{v});
+            }
+        }
+        wave_lds_fence();
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const uint32_t two = (uint32_t)vf[b][j];
+            vf[b][j] = (int)((not_finite<T>(two & 0xffffu) ? 0u : two & 0xffffu) |
+                             (not_finite<T>(two & 0xffff0000u) ? 0u : two & 0xffff0000u));
+          }
+      }
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        o[b] = mfma16<T>::mma(__builtin_bit_cast(vec, vf[b]), __builtin_bit_cast(vec, p1), o[b]);
+        o[b] = mfma16<T>::mma(__builtin_bit_cast(vec, vf[b]), __builtin_bit_cast(vec, p2), o[b]);
+      }
+      if (more) {
+        load_v(next, page_v);
+        base = next;
+        next = tile_of(i + 2 * kWaves);
+        page_k = page_of(next + kgroup);
+        page_v = page_of(next + g * 8);
+      }
+    }
+  };
+  pass(std::false_type{});
+  bool odd = false;
+#pragma unroll
+  for (int b = 0; b < NB; ++b)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) odd |= !(fabsf(o[b][e]) <= -kLowest);
+  if (__any(odd)) pass(std::true_type{});
+
+  // the four waves' results
+  l = sum_16_32(l);
+  if (live) {
+    if (g == 0) {
+      part_m[wave][col] = m;
+      part_l[wave][col] = l;
+    }
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+      if (b * 16 < d) *(f32x4_t*)&part[wave][col][b * 16 + g * 4] = o[b];
+  }
+  __syncthreads();
+  auto joined = [&](int row, int dim, float& mm, float& ll) -> f32x4_t {
+    mm = part_m[0][row];
+#pragma unroll
+    for (int n = 1; n < kWaves; ++n) mm = fmaxf(mm, part_m[n][row]);
+    f32x4_t sum = {0, 0, 0, 0};
+    ll = 0.0f;
+#pragma unroll
+    for (int n = 0; n < kWaves; ++n) {
+      const float f = exp2_hw(part_m[n][row] - mm);
+      ll += f * part_l[n][row];
+      sum += f * *(const f32x4_t*)&part[n][row][dim];
+    }
+    return sum;
+  };
+  auto put = [&](int row, int dim, f32x4_t v, float ll) {
+    const int t = row / group;
+    T* out = (T*)a.out + (int64_t)(w.row + t) * a.ldo + (int64_t)(h * group + row - t * group) * d + dim;
+    const float inv = 1.0f / ll;
+    *(uint64_t*)out = (uint64_t)pack2_f32<T>(v[0] * inv, v[1] * inv) | ((uint64_t)pack2_f32<T>(v[2] * inv, v[3] * inv) << 32);
+  };
+  const int quads = rows * (d / 4);
+  if (splits == 1) {
+    for (int e = threadIdx.x; e < quads; e += kThreads) {
+      const int row = e / (d / 4), dim = (e - row * (d / 4)) * 4;
+      float mm, ll;
+      const f32x4_t v = joined(row, dim, mm, ll);
+      put(row, dim, v, ll);
+    }
+    return;
+  }
+  // a part: [rows][d] sums, then [rows] pairs of maximum and weight sum
+  float* parts = p.parts + ((int64_t)w.slot * kv_heads + h) * p.slot_floats;
+  const int64_t pitch = (int64_t)kv_heads * p.slot_floats;
+  float* mine = parts + w.split * pitch;
+  for (int e = threadIdx.x; e < quads; e += kThreads) {
+    const int row = e / (d / 4), dim = (e - row * (d / 4)) * 4;
+    float mm, ll;
+    const f32x4_t v = joined(row, dim, mm, ll);
+    store_pair(mine + row * d + dim, v[0], v[1]);
+    store_pair(mine + row * d + dim + 2, v[2], v[3]);
+    if (dim == 0) store_pair(mine + rows * d + 2 * row, mm, ll);
+  }
+  wait_vmem();
+  __syncthreads();
+  unsigned* counter = p.counters + (int64_t)w.slot * kv_heads + h;
+  if (threadIdx.x == 0) flag = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  __syncthreads();
+  if (flag != (unsigned)(splits - 1)) return;
+  if (threadIdx.x == 0) reset_counter(counter);
+  for (int e = threadIdx.x; e < quads; e += kThreads) {
+    const int row = e / (d / 4), dim = (e - row * (d / 4)) * 4;
+    float mm = kLowest, ll = 0.0f;
+    f32x4_t sum = {0, 0, 0, 0};
+    constexpr int AHEAD = 4;  // parts whose loads are out together
+    for (int s0 = 0; s0 < splits; s0 += AHEAD) {
+      f32x2_t ml[AHEAD], v0[AHEAD], v1[AHEAD];
+#pragma unroll
+      for (int n = 0; n < AHEAD; ++n) {
+        const float* src = parts + min(s0 + n, splits - 1) * pitch;
+        ml[n] = load_pair(src + rows * d + 2 * row);
+        v0[n] = load_pair(src + row * d + dim);
+        v1[n] = load_pair(src + row * d + dim + 2);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int n = 0; n < AHEAD; ++n) {
+        if (s0 + n >= splits) break;
+        const float now = fmaxf(mm, ml[n][0]), keep = exp2_hw(mm - now), f = exp2_hw(ml[n][0] - now);
+        mm = now;
+        ll = ll * keep + f * ml[n][1];
+        sum = sum * keep + f * f32x4_t{v0[n][0], v0[n][1], v1[n][0], v1[n][1]};
+      }
+    }
+    put(row, dim, sum, ll);
+  }
+}
+
+}  // namespace
+
+}  // namespace qtts
+
+int qtts_launch_paged_small(const qtts::PagedLaunch& p, int dtype, hipStream_t st) {
+  using namespace qtts;
+  const dim3 grid((uint32_t)((int64_t)p.items * p.a.cache.kv_heads + p.fill));
+  auto go = [&](auto type) {
+    typedef decltype(type) T;
+    if (p.a.cache.d <= 64) launch(paged_small_kernel<T, 64>, grid, dim3(kThreads), 0u, st, p);
+    else if (p.a.cache.d <= 128) launch(paged_small_kernel<T, 128>, grid, dim3(kThreads), 0u, st, p);
+    else launch(paged_small_kernel<T, 256>, grid, dim3(kThreads), 0u, st, p);
+  };
+  if (dtype == QTTS_BF16) go(bf16_t{});
+  else go(f16_t{});
+  return qtts_check_launch("paged_attention");
+}

@@ -1,0 +1,179 @@
+// What the paged attention kernels share: the work list that every workgroup makes for itself, the join of a run's splits
+// and the rows that no request has.
+#pragma once
+
+#include "common.h"
+#include "paged.h"
+#include "paged_rule.h"
+#include "splitk.h"
+
+namespace qtts {
+
+constexpr float kLowest = -3.402823466e38f;  // where a running maximum starts: below every score, and no infinity to subtract
+
+struct PagedLaunch {
+  PagedAttentionArgs a;
+  int32_t groups;       // workgroups a key-value head that the tiles are cut for; 0: never cut
+  int32_t least;        // tiles a split has at least
+  int32_t min_rows, max_rows;  // requests with more than min_rows and up to max_rows (counts times query heads a key-value head)
+  int32_t items;        // workgroups a key-value head in the grid
+  int32_t fill;         // workgroups behind them that write the rows without a request (0: another launch does)
+  unsigned* counters;   // one a split run, zero between calls
+  float* parts;         // results in parts: slot s of head h at (s * kv_heads + h) * slot_floats
+  int64_t slot_floats;
+};
+
+__device__ __forceinline__ PagedRequest load_request(const PagedAttentionArgs& a, int r) {
+  return paged_request(a.starts[r], a.counts[r], a.lengths[r], a.rows, (int64_t)a.cols << a.cache.page_shift, a.max_new);
+}
+
+__device__ __forceinline__ uint64_t wave_sum64(uint64_t v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+
+// One workgroup's share of a head: run `run` of a request whose rows begin at `row` and whose first token's position is
+// `position`, against split `split` of `splits` of its key tiles (`chunk` tiles each); `slot`: the run's first place among
+// the results in parts, and its counter.
+struct PagedWork {
+  int32_t request, row, position, count, length;
+  int32_t run, split, splits, chunk, slot;
+};
+
+// Item `item` of the list: requests in order, their runs of RUN rows (a token's query heads are rows that follow each
+// other), the last run first (it has the most keys), the splits of a run.  Each wave counts for itself, a lane a share of the requests: two passes over the requests' three numbers, the
+// second one from the cache.  False past the end.
+template <int RUN, int T>
+__device__ __forceinline__ bool paged_work(const PagedLaunch& p, int item, PagedWork& w) {
+  const PagedAttentionArgs& a = p.a;
+  const int lane = threadIdx.x & 63, per = (a.requests + 63) >> 6, group = a.heads / a.cache.kv_heads;
+  const int span = RUN / group + 2;  // tokens that a run's rows can touch
+  auto runs_of = [&](const PagedRequest& r, int32_t& tiles) -> int32_t {
+    const int64_t rows = (int64_t)r.count * group;
+    if (rows <= p.min_rows || rows > p.max_rows) {
+      tiles = 0;
+      return 0;
+    }
+    tiles = most_tiles<T>(r.length, r.count < span ? r.count : span, a.window, a.sinks);
+    return (int32_t)((rows + RUN - 1) / RUN);
+  };
+  PagedRequest mine = {0, 0, 0};
+  uint64_t total = 0;
+  for (int j = 0; j < per; ++j) {
+    const int r = lane * per + j;
+    if (r >= a.requests) break;
+    mine = load_request(a, r);
+    int32_t tiles;
+    const int32_t runs = runs_of(mine, tiles);
+    total += (uint64_t)runs * (uint32_t)tiles;
+  }
+  const int32_t chunk = p.groups ? tiles_a_split(wave_sum64(total), p.groups, p.least) : 0x7fffffff;
+  auto items_of = [&](const PagedRequest& r, int32_t& splits) -> int32_t {
+    int32_t tiles;
+    const int32_t runs = runs_of(r, tiles);
+    splits = runs ? (int32_t)(((int64_t)tiles + chunk - 1) / chunk) : 0;
+    return runs * splits;
+  };
+  int32_t items = 0, slots = 0;
+  for (int j = 0; j < per; ++j) {
+    const int r = lane * per + j;
+    if (r >= a.requests) break;
+    if (per > 1) mine = load_request(a, r);
+    int32_t splits;
+    const int32_t n = items_of(mine, splits);
+    items += n;
+    slots += splits > 1 ? n : 0;
+  }
+  int32_t upto = items, slot_upto = slots;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int32_t u = __shfl_up(upto, o, 64), s = __shfl_up(slot_upto, o, 64);
+    if (lane >= o) {
+      upto += u;
+      slot_upto += s;
+    }
+  }
+  const uint64_t past = __ballot(upto > item);
+  if (!past) return false;
+  const int owner = __ffsll((unsigned long long)past) - 1;
+  int32_t left = item - __builtin_amdgcn_readlane(upto - items, owner);
+  int32_t slot = __builtin_amdgcn_readlane(slot_upto - slots, owner);
+  for (int j = 0; j < per; ++j) {  // the owner's requests, every lane alike
+    const int r = owner * per + j;
+    PagedRequest q;
+    if (per > 1) q = load_request(a, r);
+    else q = {__builtin_amdgcn_readlane(mine.start, owner), __builtin_amdgcn_readlane(mine.count, owner),
+              __builtin_amdgcn_readlane(mine.length, owner)};
+    int32_t splits;
+    const int32_t n = items_of(q, splits);
+    if (left < n) {
+      const int32_t order = left / splits;
+      w.request = r;
+      w.row = q.start;
+      w.count = q.count;
+      w.length = q.length;
+      w.position = q.length - q.count;
+      w.run = n / splits - 1 - order;
+      w.split = left - order * splits;
+      w.splits = splits;
+      w.chunk = chunk;
+      w.slot = slot + order * splits;
+      return true;
+    }
+    left -= n;
+    slot += splits > 1 ? n : 0;
+  }
+  return false;
+}
+
+// Rows without a request, and those of requests that no run takes: zeros.  Group g of p.fill.
+template <typename T> __device__ __forceinline__ void fill_rows(const PagedLaunch& p, int g) {
+  const PagedAttentionArgs& a = p.a;
+  const int vecs = a.heads * a.cache.d / 8;
+  const i32x4_t zero = {0, 0, 0, 0};
+  for (int64_t row = g; row < a.rows; row += p.fill) {
+    if (a.slots[row] >= 0) continue;
+    T* out = (T*)a.out + row * a.ldo;
+    for (int i = threadIdx.x; i < vecs; i += blockDim.x) *(i32x4_t*)(out + 8 * i) = zero;
+  }
+  for (int r = g; r < a.requests; r += p.fill) {
+    if (a.counts[r] <= 0 || load_request(a, r).count) continue;
+    const int64_t lo = a.starts[r] > 0 ? a.starts[r] : 0, end = (int64_t)a.starts[r] + a.counts[r];
+    for (int64_t row = lo; row < end && row < a.rows; ++row) {
+      T* out = (T*)a.out + row * a.ldo;
+      for (int i = threadIdx.x; i < vecs; i += blockDim.x) *(i32x4_t*)(out + 8 * i) = zero;
+    }
+  }
+}
+
+// Maximum over the lanes that share a column: with lane ^ 32, and with lane ^ 16 where the column's four are 16 apart.
+__device__ __forceinline__ float max_32(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float max_16_32(float v) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return max_32(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
+}
+__device__ __forceinline__ float sum_32(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ float sum_16_32(float v) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return sum_32(__uint_as_float(r[0]) + __uint_as_float(r[1]));
+}
+
+// 2^x, the hardware's (2^-22 relative; results below 2^-126 are zero, as is 2^-inf).
+__device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// Two values of a result in parts, published and read past the caches that other dies do not see (splitk.h).
+__device__ __forceinline__ void store_pair(float* p, float a, float b) {
+  store_coherent((uint64_t*)p, (uint64_t)__float_as_uint(a) | ((uint64_t)__float_as_uint(b) << 32));
+}
+__device__ __forceinline__ f32x2_t load_pair(const float* p) {
+  return __builtin_bit_cast(f32x2_t, load_coherent((const uint64_t*)p));
+}
+
+}  // namespace qtts

@@ -1,0 +1,70 @@
+// Which keys a row of paged attention sees, and how the work is cut: plain arithmetic, shared by the kernels, their
+// launchers and the CPU tests.
+#pragma once
+
+#include <stdint.h>
+
+#ifdef __HIPCC__
+#define QTTS_RULE __host__ __device__ inline
+#else
+#define QTTS_RULE inline
+#endif
+
+namespace qtts {
+
+// ---- one request's rows ---------------------------------------------------------------------------
+
+// A request as its step left it; anything that no step makes (rows outside the batch, more rows than tokens, tokens past
+// the table, more rows than the call's bound) runs as a request of no rows.
+struct PagedRequest {
+  int32_t start, count, length;
+};
+QTTS_RULE PagedRequest paged_request(int32_t start, int32_t count, int32_t length, int32_t rows, int64_t capacity,
+                                     int32_t max_new) {
+  const bool sound = start >= 0 && count > 0 && count <= max_new && count <= length && length <= capacity &&
+                     (int64_t)start + count <= rows;
+  return sound ? PagedRequest{start, count, length} : PagedRequest{0, 0, 0};
+}
+
+QTTS_RULE uint32_t paged_page(int32_t page, int32_t pages) {
+  return (uint32_t)page < (uint32_t)pages ? (uint32_t)page : (uint32_t)pages - 1;
+}
+
+// ---- the keys of a run of rows, as tiles of T keys ---------------------------------------------------
+
+// Rows at positions lo..hi see keys from: the first `sinks` and those from lo - window + 1 on (no window: all), up to hi.
+// As tiles of T keys: `head` of them from key 0, then those from `first` on; `count` in all.
+struct KeyTiles {
+  int32_t head, first, count;
+};
+template <int T> QTTS_RULE KeyTiles key_tiles(int32_t lo, int32_t hi, int32_t window, int32_t sinks) {
+  const int32_t end = hi / T + 1;
+  const int32_t low = window ? lo - window + 1 : 0;
+  if (low <= 0) return {0, 0, end};
+  const int32_t first = low / T, kept = sinks < low ? sinks : low;
+  const int32_t reach = (kept + T - 1) / T, head = reach < first ? reach : first;
+  return {head, first, head + end - first};
+}
+QTTS_RULE int32_t key_tile(const KeyTiles& t, int32_t i) { return i < t.head ? i : t.first + i - t.head; }
+
+// At most so many tiles for `span` rows that follow each other, the last one at the request's last token.
+template <int T> QTTS_RULE int32_t most_tiles(int32_t length, int32_t span, int32_t window, int32_t sinks) {
+  const int64_t all = ((int64_t)length + T - 1) / T;
+  if (!window) return (int32_t)all;
+  const int64_t some = ((int64_t)(sinks < length ? sinks : length) + T - 1) / T + ((int64_t)span + window - 2) / T + 2;
+  return (int32_t)(some < all ? some : all);
+}
+
+// ---- splits of the keys over workgroups -----------------------------------------------------------------
+
+// Tiles of keys a workgroup takes, where `total` tiles (of all runs of rows of all requests, one key-value head) are
+// wanted in about `groups` workgroups a head, and no workgroup takes less than `least`.
+QTTS_RULE int32_t tiles_a_split(uint64_t total, int32_t groups, int32_t least) {
+  const uint64_t c = (total + groups - 1) / groups;
+  return c < (uint64_t)least ? least : c > 0x7fffffff ? 0x7fffffff : (int32_t)c;
+}
+// Runs that are split have fewer than 2 total / tiles_a_split <= 2 groups splits between them (n > 1 splits hold more than
+// n / 2 whole ones), so that many results in parts are ever held, a head.
+QTTS_RULE int64_t split_slots(int32_t groups) { return 2 * (int64_t)groups; }
+
+}  // namespace qtts

@@ -1216,6 +1216,12 @@ def qkv_to_cache(qkv: torch.Tensor, k: torch.Tensor, v: torch.Tensor, batch: Pag
     return q
 
 
+@functools.lru_cache(maxsize=1024)
+def _attention_bytes(max_new: int, heads: int, d: int) -> int:
+    """Workspace bytes of a :func:`paged_attention` call, a function of its sizes alone."""
+    return workspace_bytes(OP_PAGED_ATTENTION, max(1, max_new), heads, d)
+
+
 def paged_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, batch: PagedBatch, window: int = 0, sinks: int = 0,
                     scale: float | None = None) -> torch.Tensor:
     """Attention of the batch's rows over their requests' tokens in a paged cache, the rows' own among them
@@ -1240,12 +1246,17 @@ def paged_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, batch: Pa
     if q.stride(2) != 1 or q.stride(1) != d or q.data_ptr() % 16 or (rows > 1 and (q.stride(0) % 8 or q.stride(0) < heads * d)):
         q = q.clone(memory_format=torch.contiguous_format)
     out = torch.empty(rows, heads, d, dtype=q.dtype, device=q.device)
-    ws, ws_n = _ws_for(q.device)
+    if not rows:
+        return out
+    need, ws = _attention_bytes(batch.max_new, heads, d), _workspaces.get(idx)
+    if ws is None or ws.numel() < need:
+        _ensure_workspace(q.device, need, "paged_attention")
+        ws = _workspaces[idx]
     st = _lib.load().qtts_paged_attention(
         q.data_ptr(), dtype_code(q.dtype), rows, q.stride(0) if rows > 1 else heads * d, heads, kv_heads, d, k.data_ptr(), v.data_ptr(),
         pages, batch.page_size, batch.table.data_ptr(), batch.requests, batch.table.shape[1], batch.starts.data_ptr(),
         batch.counts.data_ptr(), batch.lengths.data_ptr(), batch.slots.data_ptr(), batch.min_new, batch.max_new, window, sinks,
-        d ** -0.5 if scale is None else scale, out.data_ptr(), heads * d, ws, ws_n, _raw_stream(idx))
+        d ** -0.5 if scale is None else scale, out.data_ptr(), heads * d, ws.data_ptr(), ws.numel(), _raw_stream(idx))
     if st:
         _lib.check(st, "paged_attention")
     return out
