@@ -1,0 +1,344 @@
+// Attention of many rows a request over a paged cache (prompts, chunks of prompts behind cached tokens): bound by the
+// matrix cores.
+//
+// The mathematics: S^T = K Q^T and O^T = V^T P^T with 32x32x16 MFMAs; a wave has 32 rows (a token's query heads of one
+// key-value head follow each other) as its columns, 64 keys a step, running maximum and sum per column.  The keys are dealt
+// to the rows of the S^T products so that the scores a lane receives are runs of eight keys, its operand of the second
+// product: P never leaves its lane.  The four waves of a workgroup share the tile's keys and values in LDS, which are
+// loaded there directly, one tile ahead; pieces of 16 bytes are placed so that the operand reads meet no bank twice
+// (swizzles below; ds_read_b128 serves the lanes as pipe.h says).
+//
+// P goes to the second product in 16 bits: a rounding of half a step of the weights, the size of the result's own.
+#include "paged_attn.h"
+#include "pipe.h"
+
+namespace qtts {
+
+namespace {
+
+constexpr int kTile = 64, kRun = 128, kWaves = 4, kThreads = 64 * kWaves, kWaveRows = kRun / kWaves;
+
+typedef __attribute__((ext_vector_type(16))) float f32x16_t;
+
+template <typename T> struct mfma32;
+template <> struct mfma32<bf16_t> {
+  static __device__ __forceinline__ f32x16_t mma(i32x4_t a, i32x4_t b, f32x16_t c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+  }
+};
+template <> struct mfma32<f16_t> {
+  static __device__ __forceinline__ f32x16_t mma(i32x4_t a, i32x4_t b, f32x16_t c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
+  }
+};
+
+// Position of piece `piece` in row `row`: rows of 128 bytes two to a bank cycle, longer ones one.
+template <int BYTES> __device__ __forceinline__ int place(int row, int piece) {
+  return BYTES == 128 ? piece ^ ((row >> 1) & 7) : piece ^ (row & 15);
+}
+
+// The key (of 64) whose scores are row `row` of the S^T products: a lane's rows 8 b + 4 h + c are keys 16 (b / 2) + 8 h + 4 (b % 2) + c.
+__device__ __forceinline__ int key_of_row(int row) {
+  const int b = (row >> 3) & 3, h = (row >> 2) & 1, c = row & 3;
+  return (row & 32) + 16 * (b >> 1) + 8 * h + 4 * (b & 1) + c;
+}
+
+// DP: the head size rounded up to 64, 128 or 256.  WIDE: pages of a tile or more.
+template <typename T, int DP, bool WIDE> __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void paged_many_kernel(PagedLaunch p) {
+  constexpr int NS = DP / 16, NB = DP / 32, KI = DP / 32;  // steps of Q K^T, blocks of O^T, 1 KiB loads a wave and operand
+  __shared__ __attribute__((aligned(16))) uint8_t keys[2][kTile * DP * 2], values[2][kTile * DP * 2];
+  __shared__ unsigned flag;
+  const PagedAttentionArgs& a = p.a;
+  const int kv_heads = a.cache.kv_heads, h = blockIdx.x % kv_heads, item = blockIdx.x / kv_heads;
+  if (item >= p.items) {
+    fill_rows<T>(p, blockIdx.x - p.items * kv_heads);
+    return;
+  }
+  PagedWork w;
+  if (!paged_work<kRun, kTile>(p, item, w)) return;
+  const int group = a.heads / kv_heads, d = a.cache.d, shift = a.cache.page_shift;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
+  const int64_t rows = (int64_t)w.count * group, first_row = (int64_t)w.run * kRun;
+
+  // tokens of the run, and of this wave's rows
+  const int run_lo = w.position + (int)(first_row / group);
+  const int run_hi = w.position + (int)(min(first_row + kRun, rows) - 1) / group;
+  const int64_t wave_row = first_row + wave * kWaveRows;
+  const bool busy = wave_row < rows;
+  const int wave_lo = w.position + (int)(wave_row / group);
+  const int wave_hi = busy ? w.position + (int)(min(wave_row + kWaveRows, rows) - 1) / group : -1;
+
+  const KeyTiles tiles = key_tiles<kTile>(run_lo, run_hi, a.window, a.sinks);
+  const int splits = (tiles.count + w.chunk - 1) / w.chunk;  // w.splits or fewer
+  if (w.split >= splits) return;
+  const int begin = w.split * w.chunk, end = min(tiles.count, begin + w.chunk);
+
+  const bool live = wave_row + col < rows;
+  const int token = live ? (int)((wave_row + col) / group) : 0;
+  const int query = h * group + (live ? (int)(wave_row + col - (int64_t)token * group) : 0);
+  const int hi = live ? w.position + token : -1, lo = a.window && live ? max(0, hi - a.window + 1) : 0;
+  const int all_lo = a.window ? max(0, wave_hi - a.window + 1) : 0;  // every row of the wave sees [all_lo, wave_lo]
+  const int any_lo = a.window ? max(0, wave_lo - a.window + 1) : 0;  // and none what is below any_lo and no sink
+
+  i32x4_t qf[NS];
+  {
+    const T* q = (const T*)a.q + (int64_t)(w.row + token) * a.ldq + (int64_t)query * d + half * 8;
+    const i32x4_t zero = {0, 0, 0, 0};
+#pragma unroll
+    for (int s = 0; s < NS; ++s) qf[s] = live && s * 16 < d ? *(const i32x4_t*)(q + s * 16) : zero;
+  }
+
+  // ---- the tile's way to LDS
+  const int32_t* table = a.table + (int64_t)w.request * a.cols;
+  const int last = w.length - 1, mask = (1 << shift) - 1;
+  const uint8_t *cache_k = (const uint8_t*)a.cache.k, *cache_v = (const uint8_t*)a.cache.v;
+  auto tile_of = [&](int i) { return key_tile(tiles, min(i, end - 1)) * kTile; };
+  auto head_of = [&](int32_t page) {  // bytes
+    return ((int64_t)paged_page(page, a.cache.pages) * kv_heads + h) * ((int64_t)d << (shift + 1));
+  };
+  // the page of this lane's key of the tile (all of them on one page where pages are wide)
+  auto pages_of = [&](int base) { return table[min(WIDE ? base : base + lane, last) >> shift]; };
+  uint32_t k_at[KI], v_at[KI];  // bytes from the tile's key 0 (k) and from its page's column (v), where pages are wide
+#pragma unroll
+  for (int n = 0; n < KI; ++n) {
+    const int unit = (wave * KI + n) * 64 + lane;
+    const int row = unit / (DP / 8), piece = min(place<DP * 2>(row, unit % (DP / 8)), d / 8 - 1);
+    k_at[n] = (uint32_t)(key_of_row(row) * d + piece * 8) * 2;
+    const int dim = unit / 8, run = place<128>(dim, unit % 8);
+    v_at[n] = ((uint32_t)min(dim, d - 1) << (shift + 1)) + run * 16;
+  }
+  auto stage = [&](int base, int32_t page, int buffer) {
+    uint8_t *kb = keys[buffer] + wave * KI * 1024, *vb = values[buffer] + wave * KI * 1024;
+    if constexpr (WIDE) {
+      const int64_t at = head_of(__builtin_amdgcn_readfirstlane(page));
+      const uint8_t *k = cache_k + at + (int64_t)(base & mask) * d * 2, *v = cache_v + at + (base & mask) * 2;
+#pragma unroll
+      for (int n = 0; n < KI; ++n) load_to_lds16(k + k_at[n], kb + n * 1024);
+#pragma unroll
+      for (int n = 0; n < KI; ++n) load_to_lds16(v + v_at[n], vb + n * 1024);
+    } else {
+#pragma unroll
+      for (int n = 0; n < KI; ++n) {
+        const int unit = (wave * KI + n) * 64 + lane;
+        const int row = unit / (DP / 8), piece = min(place<DP * 2>(row, unit % (DP / 8)), d / 8 - 1), key = key_of_row(row);
+        load_to_lds16(cache_k + head_of(__shfl(page, key, 64)) + ((int64_t)(min(base + key, last) & mask) * d + piece * 8) * 2,
+                      kb + n * 1024);
+      }
+#pragma unroll
+      for (int n = 0; n < KI; ++n) {
+        const int unit = (wave * KI + n) * 64 + lane;
+        const int dim = unit / 8, key = place<128>(dim, unit % 8) * 8;
+        load_to_lds16(cache_v + head_of(__shfl(page, key, 64)) + ((int64_t)min(dim, d - 1) << (shift + 1)) +
+                          (min(base + key, last & ~7) & mask) * 2, vb + n * 1024);
+      }
+    }
+  };
+
+  f32x16_t o[NB];
+  float m = kLowest, l = 0.0f;
+#pragma unroll
+  for (int b = 0; b < NB; ++b)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) o[b][e] = 0.0f;
+  int base = tile_of(begin), next = tile_of(begin + 1);
+  stage(base, pages_of(base), 0);
+  int32_t page = pages_of(next);
+  for (int i = begin; i < end; ++i) {
+    const int buffer = (i - begin) & 1;
+    wait_vmcnt<0>();   // this wave's share of the tile is in LDS
+    barrier_only();    // everyone's is, and the other buffer's readers are done
+    const int here = base;
+    if (i + 1 < end) {
+      stage(next, page, buffer ^ 1);
+      base = next;
+      next = tile_of(i + 2);
+      page = pages_of(next);
+    }
+    const bool out_of_sight = here > wave_hi || (here + kTile <= any_lo && here >= a.sinks);
+    if (out_of_sight) continue;
+    f32x16_t s[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s[t][e] = 0.0f;
+#pragma unroll
+    for (int n = 0; n < NS; ++n) {
+      if (n * 16 >= d) break;
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const int row = t * 32 + col;
+        s[t] = mfma32<T>::mma(*(const i32x4_t*)(keys[buffer] + row * DP * 2 + place<DP * 2>(row, 2 * n + half) * 16), qf[n], s[t]);
+      }
+    }
+    // score e of product t: key here + 32 t + 16 (e / 8) + 8 half + e % 8
+    const bool whole = here + kTile - 1 <= wave_lo && (here >= all_lo || here + kTile <= a.sinks);
+    if (!whole) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int key = here + 32 * t + 16 * (e >> 3) + 8 * half + (e & 7);
+          s[t][e] = key <= hi && (key >= lo || key < a.sinks) ? s[t][e] : -INFINITY;
+        }
+    }
+    float top = s[0][0];
+#pragma unroll
+    for (int e = 1; e < 32; ++e) top = fmaxf(top, s[e >> 4][e & 15]);
+    top = max_32(top) * a.scale;
+    // The maximum moves only where a score passes it by 8 powers of two: weights stay under 256 and most steps keep O.
+    if (__any(top > m + 8.0f)) {
+      const float now = fmaxf(m, top), keep = exp2_hw(m - now);
+      m = now;
+      l *= keep;
+#pragma unroll
+      for (int b = 0; b < NB; ++b) o[b] *= keep;
+    }
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        s[t][e] = exp2_hw(__builtin_fmaf(s[t][e], a.scale, -m));
+        l += s[t][e];
+      }
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) {
+      i32x4_t weights;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        weights[j] = (int)pack2_f32<T>(s[ks >> 1][8 * (ks & 1) + 2 * j], s[ks >> 1][8 * (ks & 1) + 2 * j + 1]);
+      uint32_t keep[4] = {~0u, ~0u, ~0u, ~0u};
+      if (!whole) {  // values that no row of the wave sees, among them what lies behind the request's end: zero
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int key = here + 16 * ks + 8 * half + 2 * j;
+          keep[j] = (key <= wave_hi && (key >= any_lo || key < a.sinks) ? 0xffffu : 0u) |
+                    (key + 1 <= wave_hi && (key + 1 >= any_lo || key + 1 < a.sinks) ? 0xffff0000u : 0u);
+        }
+      }
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        if (b * 32 >= d) break;
+        const int dim = b * 32 + col;
+        i32x4_t v = *(const i32x4_t*)(values[buffer] + dim * 128 + place<128>(dim, 2 * ks + half) * 16);
+        if (!whole) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) v[j] = (int)((uint32_t)v[j] & keep[j]);
+        }
+        o[b] = mfma32<T>::mma(v, weights, o[b]);
+      }
+    }
+  }
+  l = sum_32(l);
+
+  // rows whose sums are not finite though their weights are, one by one
+  bool odd = false;
+#pragma unroll
+  for (int b = 0; b < NB; ++b)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) odd |= b * 32 + 2 * (e & ~3) < d && !(fabsf(o[b][e]) <= -kLowest);
+  uint64_t again = __ballot(odd && live && l <= -kLowest);
+  again = (again | (again >> 32)) & 0xffffffff;
+  if (__syncthreads_or(again != 0)) {  // the tiles in LDS are done with
+    float* dst = (float*)keys[0] + wave * DP;
+    while (again) {
+      const int n = __builtin_ctzll(again);
+      again &= again - 1;
+      row_again<T, kTile>(a, w, tiles, begin, 1, end, h, w.row + __builtin_amdgcn_readlane(token, n),
+                          __builtin_amdgcn_readlane(query, n), __builtin_amdgcn_readlane(hi, n), __shfl(m, n, 64), dst);
+      wave_lds_fence();
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (col == n && b * 32 + 2 * (e & ~3) < d) o[b][e] = dst[b * 32 + 2 * (e & ~3) + 4 * half + (e & 3)];
+      wave_lds_fence();
+    }
+  }
+
+  // element e of block b: dimension 32 b + 8 (e / 4) + 4 half + e % 4 of this lane's row
+  auto put = [&](float inv) {
+    T* out = (T*)a.out + (int64_t)(w.row + token) * a.ldo + (int64_t)query * d + 4 * half;
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int e = 0; e < 16; e += 4)
+        if (live && b * 32 + 2 * e < d)
+          *(uint64_t*)(out + b * 32 + 2 * e) = (uint64_t)pack2_f32<T>(o[b][e] * inv, o[b][e + 1] * inv) |
+                                               ((uint64_t)pack2_f32<T>(o[b][e + 2] * inv, o[b][e + 3] * inv) << 32);
+  };
+  if (splits == 1) {
+    put(1.0f / l);
+    return;
+  }
+  // a part: [kRun][d] sums, then [kRun] pairs of maximum and weight sum
+  float* parts = p.parts + ((int64_t)w.slot * kv_heads + h) * p.slot_floats;
+  const int64_t pitch = (int64_t)kv_heads * p.slot_floats;
+  const int row = wave * kWaveRows + col;
+  if (live) {
+    float* mine = parts + w.split * pitch + row * d + 4 * half;
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int e = 0; e < 16; e += 4)
+        if (b * 32 + 2 * e < d) {
+          store_pair(mine + b * 32 + 2 * e, o[b][e], o[b][e + 1]);
+          store_pair(mine + b * 32 + 2 * e + 2, o[b][e + 2], o[b][e + 3]);
+        }
+    if (half == 0) store_pair(parts + w.split * pitch + kRun * d + 2 * row, m, l);
+  }
+  wait_vmem();
+  __syncthreads();
+  unsigned* counter = p.counters + (int64_t)w.slot * kv_heads + h;
+  if (threadIdx.x == 0) flag = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  __syncthreads();
+  if (flag != (unsigned)(splits - 1)) return;
+  if (threadIdx.x == 0) reset_counter(counter);
+  if (!live) return;
+  m = kLowest;
+  l = 0.0f;
+#pragma unroll
+  for (int b = 0; b < NB; ++b)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) o[b][e] = 0.0f;
+  for (int s = 0; s < splits; ++s) {
+    const float* src = parts + s * pitch;
+    const f32x2_t ml = load_pair(src + kRun * d + 2 * row);
+    const float now = fmaxf(m, ml[0]), keep = exp2_hw(m - now), f = exp2_hw(ml[0] - now);
+    m = now;
+    l = l * keep + f * ml[1];
+    src += row * d + 4 * half;
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int e = 0; e < 16; e += 2)
+        if (b * 32 + 2 * (e & ~3) < d) {
+          const f32x2_t v = load_pair(src + b * 32 + 2 * (e & ~3) + (e & 2));
+          o[b][e] = o[b][e] * keep + f * v[0];
+          o[b][e + 1] = o[b][e + 1] * keep + f * v[1];
+        }
+  }
+  put(1.0f / l);
+}
+
+}  // namespace
+
+}  // namespace qtts
+
+int qtts_launch_paged_many(const qtts::PagedLaunch& p, int dtype, hipStream_t st) {
+  using namespace qtts;
+  const dim3 grid((uint32_t)((int64_t)p.items * p.a.cache.kv_heads + p.fill));
+  auto go = [&](auto type, auto wide) {
+    typedef decltype(type) T;
+    constexpr bool W = decltype(wide)::value;
+    if (p.a.cache.d <= 64) launch(paged_many_kernel<T, 64, W>, grid, dim3(kThreads), 0u, st, p);
+    else if (p.a.cache.d <= 128) launch(paged_many_kernel<T, 128, W>, grid, dim3(kThreads), 0u, st, p);
+    else launch(paged_many_kernel<T, 256, W>, grid, dim3(kThreads), 0u, st, p);
+  };
+  auto pages = [&](auto type) {
+    if ((1 << p.a.cache.page_shift) >= kTile) go(type, std::true_type{});
+    else go(type, std::false_type{});
+  };
+  if (dtype == QTTS_BF16) pages(bf16_t{});
+  else pages(f16_t{});
+  return qtts_check_launch("paged_attention");
+}

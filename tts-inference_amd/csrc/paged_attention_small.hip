@@ -20,24 +20,11 @@ namespace {
 
 constexpr int kTile = 32, kRows = 16, kWaves = 4, kThreads = 64 * kWaves;
 
-// 16 bits a value: infinities and NaN have all exponent bits set.
-template <typename T> __device__ __forceinline__ bool not_finite(uint32_t two) {
-  constexpr uint32_t e = std::is_same<T, bf16_t>::value ? 0x7f80u : 0x7c00u;
-  return (two & e) == e || (two & (e << 16)) == (e << 16);  // of either
-}
-
-// Orders this wave's LDS writes before its reads, and the other way round (the wave's lanes run together).
-__device__ __forceinline__ void wave_lds_fence() {
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-}
-
 // DP: the head size rounded up to 64, 128 or 256.
 template <typename T, int DP> __global__ __launch_bounds__(kThreads, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) void paged_small_kernel(PagedLaunch p) {
   typedef typename mfma16<T>::vec vec;
   constexpr int NC = DP / 32, NB = DP / 16;
   __shared__ float part[kWaves][kRows][DP + 4];
-  __shared__ float part_w[kWaves][kTile * kRows];
   __shared__ float part_m[kWaves][kRows], part_l[kWaves][kRows];
   __shared__ unsigned flag;
   const PagedAttentionArgs& a = p.a;
@@ -75,7 +62,9 @@ template <typename T, int DP> __global__ __launch_bounds__(kThreads, DP <= 64 ? 
   }
 
   f32x4_t o[NB];
-  float m, l;
+#pragma unroll
+  for (int b = 0; b < NB; ++b) o[b] = f32x4_t{0, 0, 0, 0};
+  float m = kLowest, l = 0.0f;
 
   // Key of product t's row r: base + 8 (r / 4) + 4 t + r % 4; this lane's eight scores: keys base + 8 g + 0..7.
   const int32_t* table = a.table + (int64_t)w.request * a.cols;
@@ -102,15 +91,8 @@ template <typename T, int DP> __global__ __launch_bounds__(kThreads, DP <= 64 ? 
     for (int b = 0; b < NB; ++b) vf[b] = *(const i32x4_t*)(v + ((int64_t)min(b, d / 16 - 1) << (shift + 4)));
   };
 
-  // One pass over the wave's tiles.  `careful`: values that are infinities or NaN do not go through the matrix cores, where a row
-  // that does not see them would take 0 * NaN from them and a weight's second part could turn an infinity's sign.
-  auto pass = [&](auto careful) {
-    m = kLowest;
-    l = 0.0f;
-#pragma unroll
-    for (int b = 0; b < NB; ++b) o[b] = f32x4_t{0, 0, 0, 0};
-    int i = begin + wave;
-    if (i >= end) return;
+  int i = begin + wave;
+  if (i < end) {
     int base = tile_of(i), next = tile_of(i + kWaves);
     load_k(base, page_of(base + kgroup));
     load_v(base, page_of(base + g * 8));
@@ -168,41 +150,6 @@ template <typename T, int DP> __global__ __launch_bounds__(kThreads, DP <= 64 ? 
 #pragma unroll
           for (int j = 0; j < 4; ++j) vf[b][j] = (int)((uint32_t)vf[b][j] & keep[j]);
       }
-      if constexpr (decltype(careful)::value) {
-        // The tile and its weights through LDS: key by key, rows that see a value that is not finite add it; the others do not.
-        uint16_t* values = (uint16_t*)part[wave];  // [key][DP]
-        float* weights = part_w[wave];             // [key][row]
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          weights[(g * 8 + j) * kRows + col] = w8[j];
-#pragma unroll
-          for (int b = 0; b < NB; ++b)
-            values[(g * 8 + j) * DP + b * 16 + col] = (uint16_t)((uint32_t)vf[b][j >> 1] >> (16 * (j & 1)));
-        }
-        wave_lds_fence();
-#pragma unroll 1
-        for (int n = 0; n < kTile; ++n) {
-          const int at = base + n;
-          const bool seen = at <= hi && (at >= lo || at < a.sinks);
-          const float weight = weights[n * kRows + col];
-#pragma unroll
-          for (int b = 0; b < NB; ++b)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const uint16_t v = values[n * DP + b * 16 + g * 4 + e];
-              if (seen && not_finite<T>(v)) o[b][e] += weight * to_f32(T{v});
-            }
-        }
-        wave_lds_fence();
-#pragma unroll
-        for (int b = 0; b < NB; ++b)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const uint32_t two = (uint32_t)vf[b][j];
-            vf[b][j] = (int)((not_finite<T>(two & 0xffffu) ? 0u : two & 0xffffu) |
-                             (not_finite<T>(two & 0xffff0000u) ? 0u : two & 0xffff0000u));
-          }
-      }
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
         o[b] = mfma16<T>::mma(__builtin_bit_cast(vec, vf[b]), __builtin_bit_cast(vec, p1), o[b]);
@@ -216,17 +163,31 @@ template <typename T, int DP> __global__ __launch_bounds__(kThreads, DP <= 64 ? 
         page_v = page_of(next + g * 8);
       }
     }
-  };
-  pass(std::false_type{});
+  }
+
+  // rows whose sums are not finite though their weights are, one by one
+  l = sum_16_32(l);
   bool odd = false;
 #pragma unroll
   for (int b = 0; b < NB; ++b)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) odd |= !(fabsf(o[b][e]) <= -kLowest);
-  if (__any(odd)) pass(std::true_type{});
+    for (int e = 0; e < 4; ++e) odd |= b * 16 < d && !(fabsf(o[b][e]) <= -kLowest);
+  uint64_t again = __ballot(odd && live && l <= -kLowest);
+  again = (again | (again >> 16) | (again >> 32) | (again >> 48)) & 0xffff;
+  while (again) {
+    const int n = __builtin_ctzll(again);
+    again &= again - 1;
+    const int t = n / group;
+    row_again<T, kTile>(a, w, tiles, begin + wave, kWaves, end, h, w.row + t, h * group + n - t * group, w.position + t,
+                        __shfl(m, n, 64), &part[wave][0][0]);
+    wave_lds_fence();
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+      if (col == n && b * 16 < d) o[b] = *(const f32x4_t*)(&part[wave][0][0] + b * 16 + g * 4);
+    wave_lds_fence();
+  }
 
   // the four waves' results
-  l = sum_16_32(l);
   if (live) {
     if (g == 0) {
       part_m[wave][col] = m;

@@ -68,11 +68,10 @@ __device__ __forceinline__ bool paged_work(const PagedLaunch& p, int item, Paged
     const int32_t runs = runs_of(mine, tiles);
     total += (uint64_t)runs * (uint32_t)tiles;
   }
-  const int32_t chunk = p.groups ? tiles_a_split(wave_sum64(total), p.groups, p.least) : 0x7fffffff;
-  auto items_of = [&](const PagedRequest& r, int32_t& splits) -> int32_t {
-    int32_t tiles;
+  const uint32_t share = p.groups ? tiles_a_split(wave_sum64(total), p.groups, p.least) : 0;
+  auto items_of = [&](const PagedRequest& r, int32_t& tiles, int32_t& splits) -> int32_t {
     const int32_t runs = runs_of(r, tiles);
-    splits = runs ? (int32_t)(((int64_t)tiles + chunk - 1) / chunk) : 0;
+    splits = p.groups ? splits_of(tiles, share) : 1;
     return runs * splits;
   };
   int32_t items = 0, slots = 0;
@@ -80,8 +79,8 @@ __device__ __forceinline__ bool paged_work(const PagedLaunch& p, int item, Paged
     const int r = lane * per + j;
     if (r >= a.requests) break;
     if (per > 1) mine = load_request(a, r);
-    int32_t splits;
-    const int32_t n = items_of(mine, splits);
+    int32_t tiles, splits;
+    const int32_t n = items_of(mine, tiles, splits);
     items += n;
     slots += splits > 1 ? n : 0;
   }
@@ -105,8 +104,8 @@ __device__ __forceinline__ bool paged_work(const PagedLaunch& p, int item, Paged
     if (per > 1) q = load_request(a, r);
     else q = {__builtin_amdgcn_readlane(mine.start, owner), __builtin_amdgcn_readlane(mine.count, owner),
               __builtin_amdgcn_readlane(mine.length, owner)};
-    int32_t splits;
-    const int32_t n = items_of(q, splits);
+    int32_t tiles, splits;
+    const int32_t n = items_of(q, tiles, splits);
     if (left < n) {
       const int32_t order = left / splits;
       w.request = r;
@@ -117,7 +116,7 @@ __device__ __forceinline__ bool paged_work(const PagedLaunch& p, int item, Paged
       w.run = n / splits - 1 - order;
       w.split = left - order * splits;
       w.splits = splits;
-      w.chunk = chunk;
+      w.chunk = (tiles + splits - 1) / splits;
       w.slot = slot + order * splits;
       return true;
     }
@@ -174,6 +173,59 @@ __device__ __forceinline__ void store_pair(float* p, float a, float b) {
 }
 __device__ __forceinline__ f32x2_t load_pair(const float* p) {
   return __builtin_bit_cast(f32x2_t, load_coherent((const uint64_t*)p));
+}
+
+// 16 bits a value: infinities and NaN have all exponent bits set (of either half of `two`).
+template <typename T> __device__ __forceinline__ bool not_finite(uint32_t two) {
+  constexpr uint32_t e = std::is_same<T, bf16_t>::value ? 0x7f80u : 0x7c00u;
+  return (two & e) == e || (two & (e << 16)) == (e << 16);
+}
+
+// One row's sums over tiles first, first + step, ... < end again, by one wave and without the matrix cores: a value that
+// the row does not see cannot reach it, where a product of tiles has 0 * NaN.  For rows whose weights are sound (l finite) and
+// whose sums came out infinite or NaN.  m: the maximum that the sums stand at; dst [d], in LDS.
+template <typename T, int TILE>
+__device__ __forceinline__ void row_again(const PagedAttentionArgs& a, const PagedWork& w, const KeyTiles& tiles, int first,
+                                          int step, int end, int kv_head, int row, int query, int hi, float m, float* dst) {
+  const int lane = threadIdx.x & 63, d = a.cache.d, shift = a.cache.page_shift, mask = (1 << shift) - 1;
+  const int lo = a.window ? max(0, hi - a.window + 1) : 0;
+  const int32_t* table = a.table + (int64_t)w.request * a.cols;
+  const T* q = (const T*)a.q + (int64_t)row * a.ldq + (int64_t)query * d;
+  float sum[kPagedMaxDim / 64] = {};
+#pragma unroll 1
+  for (int i = first; i < end; i += step) {
+    const int key = key_tile(tiles, i) * TILE + lane;
+    const bool seen = lane < TILE && key <= hi && (key >= lo || key < a.sinks);
+    const int64_t page = seen ? paged_page(table[key >> shift], a.cache.pages) : 0;
+    const int64_t at = (page * a.cache.kv_heads + kv_head) * ((int64_t)d << shift);
+    const T* k = (const T*)a.cache.k + at + (int64_t)(key & mask) * d;
+    float s = 0.0f;
+    if (seen) {
+#pragma unroll 1
+      for (int c = 0; c < d; ++c) s += to_f32(q[c]) * to_f32(k[c]);
+    }
+    const float weight = seen ? exp2_hw(__builtin_fmaf(s, a.scale, -m)) : 0.0f;
+    const uint64_t seen_by = __ballot(seen);
+#pragma unroll 1
+    for (int j = 0; j < TILE; ++j) {
+      if (!((seen_by >> j) & 1)) continue;
+      const float wj = __shfl(weight, j, 64);
+      const int64_t pj = __shfl((int)page, j, 64);
+      const T* v = (const T*)a.cache.v + (pj * a.cache.kv_heads + kv_head) * ((int64_t)d << shift) + ((key - lane + j) & mask);
+#pragma unroll
+      for (int c = 0; c < kPagedMaxDim / 64; ++c)
+        if (lane + 64 * c < d) sum[c] += wj * to_f32(v[(int64_t)(lane + 64 * c) << shift]);
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < kPagedMaxDim / 64; ++c)
+    if (lane + 64 * c < d) dst[lane + 64 * c] = sum[c];
+}
+
+// Orders this wave's LDS writes before its reads, and the other way round (the wave's lanes run together).
+__device__ __forceinline__ void wave_lds_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
 }
 
 }  // namespace qtts

@@ -59,12 +59,18 @@ template <int T> QTTS_RULE int32_t most_tiles(int32_t length, int32_t span, int3
 
 // Tiles of keys a workgroup takes, where `total` tiles (of all runs of rows of all requests, one key-value head) are
 // wanted in about `groups` workgroups a head, and no workgroup takes less than `least`.
-QTTS_RULE int32_t tiles_a_split(uint64_t total, int32_t groups, int32_t least) {
+QTTS_RULE uint32_t tiles_a_split(uint64_t total, int32_t groups, int32_t least) {
   const uint64_t c = (total + groups - 1) / groups;
-  return c < (uint64_t)least ? least : c > 0x7fffffff ? 0x7fffffff : (int32_t)c;
+  return c < (uint64_t)least ? (uint32_t)least : c > 0x40000000 ? 0x40000000u : (uint32_t)c;
 }
-// Runs that are split have fewer than 2 total / tiles_a_split <= 2 groups splits between them (n > 1 splits hold more than
-// n / 2 whole ones), so that many results in parts are ever held, a head.
-QTTS_RULE int64_t split_slots(int32_t groups) { return 2 * (int64_t)groups; }
+// Splits of a run of up to `tiles` tiles, equal ones: tiles / share rounded to the nearest, so that a run a little longer
+// than a share stays whole.
+QTTS_RULE int32_t splits_of(int32_t tiles, uint32_t share) {
+  const int32_t n = (int32_t)(((uint64_t)2 * tiles + share) / (2 * (uint64_t)share));
+  return n > 1 ? n : 1;
+}
+// n > 1 splits hold n - 1/2 shares or more, so that the runs that are split have at most 4/3 groups splits between them a
+// head: the results in parts that are ever held.
+QTTS_RULE int64_t split_slots(int64_t groups) { return groups + groups / 3; }
 
 }  // namespace qtts
