@@ -80,7 +80,7 @@ typedef enum {
     QTTS_OP_W8A16_SILU = 6,
     QTTS_OP_W8A16_FUSED = 7,
     QTTS_OP_LORA = 8, /* n: the linear's partitions, k: the rank */
-    QTTS_OP_PAGED_ATTENTION = 16 /* m: the largest count of a request, n: query heads, k: the head size */
+    QTTS_OP_PAGED_ATTENTION = 16 /* m: rows a request has at most, times heads / kv_heads; n: 1; k: the head size */
 } qtts_op;
 
 /* What qtts_w8a16_fused_gemm_strips applies to its activations before the GEMM. */
@@ -551,7 +551,7 @@ int qtts_qkv_to_cache(const void* qkv, int dtype, int64_t rows, int64_t ldqkv, i
  * h / (heads / kv_heads).  Rows of no request: zeros.  What a row does not see (keys
  * and values behind it, outside the window, in places never written) does not reach it, whatever it holds.
  * min_new, max_new: bounds of the counts; requests with more than max_new get zeros.
- * Workspace: qtts_workspace_bytes(QTTS_OP_PAGED_ATTENTION, max_new, heads, d). */
+ * Workspace: qtts_workspace_bytes(QTTS_OP_PAGED_ATTENTION, max_new * heads / kv_heads, 1, d, 0). */
 int qtts_paged_attention(const void* q, int dtype, int64_t rows, int64_t ldq, int64_t heads, int64_t kv_heads, int64_t d,
                          const void* k, const void* v, int64_t pages, int64_t page_size, const int32_t* table, int64_t requests,
                          int64_t cols, const int32_t* starts, const int32_t* counts, const int32_t* lengths,

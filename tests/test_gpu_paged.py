@@ -125,9 +125,11 @@ def test_step_edges(ops):
     _check_step(ops, [1, 1], [32, 31], [[1, 2], [3, 0]], [1, 2, 3, 0, 4], 4, 16, 2)
     for left in (2, 3, 4):  # requests that need none pass even behind one that is denied
         _check_step(ops, [40, 20, 3, 17], [0, 0, 5, 0], [[-1] * 3, [-1] * 3, [0, 0, 0], [-1] * 3], list(range(left + 1)), 1, 16, 90)
-    # lengths, a count of taken pages and pages that no step makes: denied, and no slot outside the cache
-    b = ops.paged_step(_i32([1, 1]), _i32([-5, 3]), _i32([[0], [77]]), _i32([0, 1]), _i32([0]), 16, 2)
-    assert b.counts.tolist() == [0, 1] and b.slots.tolist() == [-1, -1] and b.positions.tolist() == [-1, 3]
+    # lengths, a count of taken pages and pages that no step makes: denied, and no slot that int32 does not hold
+    b = ops.paged_step(_i32([1, 1, 1]), _i32([-5, 3, 3]), _i32([[0], [-1], [1 << 27]]), _i32([0, 1]), _i32([0]), 16, 3)
+    assert b.counts.tolist() == [0, 1, 1] and b.slots.tolist() == [-1, -1, -1] and b.positions.tolist() == [-1, 3, 3]
+    # a free list shorter than the cache
+    _check_step(ops, [20, 3], [0, 0], [[-1, -1], [-1, -1]], [900, 70, 5], 0, 16, 23)
     for taken in (-1, 3):
         assert ops.paged_step(_i32([1]), _i32([0]), _i32([[0]]), _i32([0, 1]), _i32([taken]), 16, 1).counts.tolist() == [0]
 

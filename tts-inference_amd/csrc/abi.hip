@@ -84,7 +84,7 @@ int qtts_launch_paged_release(const int32_t* which, int32_t* lengths, const int3
                               int32_t* free_pages, int pages, int32_t* taken, int page_shift, hipStream_t st);
 int qtts_launch_qkv_to_cache(const qtts::QkvCacheArgs& args, int dtype, hipStream_t st);
 int qtts_launch_paged_attention(const qtts::PagedAttentionArgs& args, int min_new, int dtype, void* ws, hipStream_t st);
-int64_t qtts_paged_attention_ws_bytes(int64_t d);
+int64_t qtts_paged_attention_ws_bytes(int64_t m, int64_t d);
 
 static thread_local char g_last_error[512] = "";
 
@@ -271,9 +271,9 @@ int64_t qtts_workspace_bytes(int op, int64_t m, int64_t n, int64_t k, int algo) 
       if (n > QTTS_LORA_MAX_PARTS || k > QTTS_LORA_MAX_RANK)
         return qtts_set_error(QTTS_ERR_INVALID_ARGUMENT, "bad workspace query");
       return qtts_lora_ws_bytes(m, n, k);
-    case QTTS_OP_PAGED_ATTENTION:  // n query heads of k
+    case QTTS_OP_PAGED_ATTENTION:  // m rows a key-value head of k
       if (k > qtts::kPagedMaxDim) return qtts_set_error(QTTS_ERR_INVALID_ARGUMENT, "bad workspace query");
-      return qtts_paged_attention_ws_bytes(k);
+      return qtts_paged_attention_ws_bytes(m, k);
     default: return qtts_set_error(QTTS_ERR_INVALID_ARGUMENT, "unknown op %d", op);
   }
 }
@@ -1072,7 +1072,7 @@ int qtts_paged_attention(const void* q, int dtype, int64_t rows, int64_t ldq, in
   const int64_t held = pages * page_size * kv_heads * d;
   for (const void* c : {k, v})
     QTTS_REQUIRE(!spans_overlap(c, 1, held, held, 2, out, rows, ldo, heads * d, 2), "paged_attention: out overlaps the cache");
-  const int64_t need = qtts_paged_attention_ws_bytes(d);
+  const int64_t need = qtts_paged_attention_ws_bytes(std::min(max_new, rows) * (heads / kv_heads), d);
   if (!ws || ws_bytes < need)
     return qtts_set_error(QTTS_ERR_WORKSPACE, "paged_attention: workspace of %lld bytes < %lld needed", (long long)ws_bytes,
                           (long long)need);

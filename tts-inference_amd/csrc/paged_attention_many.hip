@@ -43,8 +43,8 @@ __device__ __forceinline__ int key_of_row(int row) {
   return (row & 32) + 16 * (b >> 1) + 8 * h + 4 * (b & 1) + c;
 }
 
-// DP: the head size rounded up to 64, 128 or 256.  WIDE: pages of a tile or more.
-template <typename T, int DP, bool WIDE> __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void paged_many_kernel(PagedLaunch p) {
+// DP: the head size (EXACT) or what it is rounded up to, 64, 128 or 256.  WIDE: pages of a tile or more.
+template <typename T, int DP, bool EXACT, bool WIDE> __global__ __launch_bounds__(kThreads, DP == 64 || (DP == 128 && EXACT) ? 2 : 1) void paged_many_kernel(PagedLaunch p) {
   constexpr int NS = DP / 16, NB = DP / 32, KI = DP / 32;  // steps of Q K^T, blocks of O^T, 1 KiB loads a wave and operand
   __shared__ __attribute__((aligned(16))) uint8_t keys[2][kTile * DP * 2], values[2][kTile * DP * 2];
   __shared__ unsigned flag;
@@ -56,7 +56,7 @@ template <typename T, int DP, bool WIDE> __global__ __launch_bounds__(kThreads, 
   }
   PagedWork w;
   if (!paged_work<kRun, kTile>(p, item, w)) return;
-  const int group = a.heads / kv_heads, d = a.cache.d, shift = a.cache.page_shift;
+  const int group = a.heads / kv_heads, d = EXACT ? DP : a.cache.d, shift = a.cache.page_shift;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
   const int64_t rows = (int64_t)w.count * group, first_row = (int64_t)w.run * kRun;
 
@@ -163,9 +163,9 @@ template <typename T, int DP, bool WIDE> __global__ __launch_bounds__(kThreads, 
       for (int e = 0; e < 16; ++e) s[t][e] = 0.0f;
 #pragma unroll
     for (int n = 0; n < NS; ++n) {
-      if (n * 16 >= d) break;
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
+        if (!EXACT && n * 16 >= d) continue;
         const int row = t * 32 + col;
         s[t] = mfma32<T>::mma(*(const i32x4_t*)(keys[buffer] + row * DP * 2 + place<DP * 2>(row, 2 * n + half) * 16), qf[n], s[t]);
       }
@@ -205,7 +205,7 @@ template <typename T, int DP, bool WIDE> __global__ __launch_bounds__(kThreads, 
       i32x4_t weights;
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        weights[j] = (int)pack2_f32<T>(s[ks >> 1][8 * (ks & 1) + 2 * j], s[ks >> 1][8 * (ks & 1) + 2 * j + 1]);
+        weights[j] = (int)pack2<T>(s[ks >> 1][8 * (ks & 1) + 2 * j], s[ks >> 1][8 * (ks & 1) + 2 * j + 1]);
       uint32_t keep[4] = {~0u, ~0u, ~0u, ~0u};
       if (!whole) {  // values that no row of the wave sees, among them what lies behind the request's end: zero
 #pragma unroll
@@ -217,7 +217,7 @@ template <typename T, int DP, bool WIDE> __global__ __launch_bounds__(kThreads, 
       }
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
-        if (b * 32 >= d) break;
+        if (!EXACT && b * 32 >= d) continue;
         const int dim = b * 32 + col;
         i32x4_t v = *(const i32x4_t*)(values[buffer] + dim * 128 + place<128>(dim, 2 * ks + half) * 16);
         if (!whole) {
@@ -263,8 +263,8 @@ template <typename T, int DP, bool WIDE> __global__ __launch_bounds__(kThreads, 
 #pragma unroll
       for (int e = 0; e < 16; e += 4)
         if (live && b * 32 + 2 * e < d)
-          *(uint64_t*)(out + b * 32 + 2 * e) = (uint64_t)pack2_f32<T>(o[b][e] * inv, o[b][e + 1] * inv) |
-                                               ((uint64_t)pack2_f32<T>(o[b][e + 2] * inv, o[b][e + 3] * inv) << 32);
+          *(uint64_t*)(out + b * 32 + 2 * e) = (uint64_t)pack2<T>(o[b][e] * inv, o[b][e + 1] * inv) |
+                                               ((uint64_t)pack2<T>(o[b][e + 2] * inv, o[b][e + 3] * inv) << 32);
   };
   if (splits == 1) {
     put(1.0f / l);
@@ -330,9 +330,13 @@ int qtts_launch_paged_many(const qtts::PagedLaunch& p, int dtype, hipStream_t st
   auto go = [&](auto type, auto wide) {
     typedef decltype(type) T;
     constexpr bool W = decltype(wide)::value;
-    if (p.a.cache.d <= 64) launch(paged_many_kernel<T, 64, W>, grid, dim3(kThreads), 0u, st, p);
-    else if (p.a.cache.d <= 128) launch(paged_many_kernel<T, 128, W>, grid, dim3(kThreads), 0u, st, p);
-    else launch(paged_many_kernel<T, 256, W>, grid, dim3(kThreads), 0u, st, p);
+    const int d = p.a.cache.d;
+    if (d == 64) launch(paged_many_kernel<T, 64, true, W>, grid, dim3(kThreads), 0u, st, p);
+    else if (d == 128) launch(paged_many_kernel<T, 128, true, W>, grid, dim3(kThreads), 0u, st, p);
+    else if (d == 256) launch(paged_many_kernel<T, 256, true, W>, grid, dim3(kThreads), 0u, st, p);
+    else if (d < 64) launch(paged_many_kernel<T, 64, false, W>, grid, dim3(kThreads), 0u, st, p);
+    else if (d < 128) launch(paged_many_kernel<T, 128, false, W>, grid, dim3(kThreads), 0u, st, p);
+    else launch(paged_many_kernel<T, 256, false, W>, grid, dim3(kThreads), 0u, st, p);
   };
   auto pages = [&](auto type) {
     if ((1 << p.a.cache.page_shift) >= kTile) go(type, std::true_type{});

@@ -20,8 +20,10 @@ namespace {
 
 constexpr int kTile = 32, kRows = 16, kWaves = 4, kThreads = 64 * kWaves;
 
-// DP: the head size rounded up to 64, 128 or 256.
-template <typename T, int DP> __global__ __launch_bounds__(kThreads, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) void paged_small_kernel(PagedLaunch p) {
+// DP: the head size (EXACT) or what it is rounded up to, 64, 128 or 256.
+template <typename T, int DP, bool EXACT>
+__global__ __launch_bounds__(kThreads, DP == 64 || (DP == 128 && EXACT) ? 3 : DP == 128 ? 2 : 1)
+void paged_small_kernel(PagedLaunch p) {
   typedef typename mfma16<T>::vec vec;
   constexpr int NC = DP / 32, NB = DP / 16;
   __shared__ float part[kWaves][kRows][DP + 4];
@@ -35,7 +37,7 @@ template <typename T, int DP> __global__ __launch_bounds__(kThreads, DP <= 64 ? 
   }
   PagedWork w;
   if (!paged_work<kRows, kTile>(p, item, w)) return;
-  const int group = a.heads / kv_heads, d = a.cache.d, shift = a.cache.page_shift;
+  const int group = a.heads / kv_heads, d = EXACT ? DP : a.cache.d, shift = a.cache.page_shift;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
   const int rows = w.count * group;
 
@@ -83,12 +85,12 @@ template <typename T, int DP> __global__ __launch_bounds__(kThreads, DP <= 64 ? 
     for (int t = 0; t < 2; ++t)
 #pragma unroll
       for (int c = 0; c < NC; ++c)
-        kf[t][c] = c * 32 + g * 8 < d ? *(const i32x4_t*)(k + (int64_t)t * 4 * d + c * 32) : zero;
+        kf[t][c] = EXACT || c * 32 + g * 8 < d ? *(const i32x4_t*)(k + (int64_t)t * 4 * d + c * 32) : zero;
   };
   auto load_v = [&](int base, int32_t page) {
     const T* v = (const T*)a.cache.v + head_of(page) + (min(base + g * 8, last) & mask) + ((int64_t)col << shift);
 #pragma unroll
-    for (int b = 0; b < NB; ++b) vf[b] = *(const i32x4_t*)(v + ((int64_t)min(b, d / 16 - 1) << (shift + 4)));
+    for (int b = 0; b < NB; ++b) vf[b] = *(const i32x4_t*)(v + ((int64_t)(EXACT ? b : min(b, d / 16 - 1)) << (shift + 4)));
   };
 
   int i = begin + wave;
@@ -127,18 +129,14 @@ template <typename T, int DP> __global__ __launch_bounds__(kThreads, DP <= 64 ? 
 #pragma unroll
         for (int b = 0; b < NB; ++b) o[b] *= keep;
       }
-      float w8[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        w8[j] = exp2_hw(__builtin_fmaf(x[j], a.scale, -m));
-        l += w8[j];
-      }
       i32x4_t p1, p2;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const uint32_t two = pack2_f32<T>(w8[2 * j], w8[2 * j + 1]);
+        const float w0 = exp2_hw(__builtin_fmaf(x[2 * j], a.scale, -m)), w1 = exp2_hw(__builtin_fmaf(x[2 * j + 1], a.scale, -m));
+        l += w0 + w1;
+        const uint32_t two = pack2<T>(w0, w1);
         p1[j] = (int)two;
-        p2[j] = (int)pack2_f32<T>(w8[2 * j] - to_f32(T{(uint16_t)two}), w8[2 * j + 1] - to_f32(T{(uint16_t)(two >> 16)}));
+        p2[j] = (int)pack2<T>(w0 - to_f32(T{(uint16_t)two}), w1 - to_f32(T{(uint16_t)(two >> 16)}));
       }
       if (!whole) {  // values that no row sees, among them what lies behind the request's end and was never written: zero
         uint32_t keep[4] = {0, 0, 0, 0};
@@ -187,7 +185,7 @@ template <typename T, int DP> __global__ __launch_bounds__(kThreads, DP <= 64 ? 
     wave_lds_fence();
   }
 
-  // the four waves' results
+  // the waves' results
   if (live) {
     if (g == 0) {
       part_m[wave][col] = m;
@@ -216,7 +214,7 @@ template <typename T, int DP> __global__ __launch_bounds__(kThreads, DP <= 64 ? 
     const int t = row / group;
     T* out = (T*)a.out + (int64_t)(w.row + t) * a.ldo + (int64_t)(h * group + row - t * group) * d + dim;
     const float inv = 1.0f / ll;
-    *(uint64_t*)out = (uint64_t)pack2_f32<T>(v[0] * inv, v[1] * inv) | ((uint64_t)pack2_f32<T>(v[2] * inv, v[3] * inv) << 32);
+    *(uint64_t*)out = (uint64_t)pack2<T>(v[0] * inv, v[1] * inv) | ((uint64_t)pack2<T>(v[2] * inv, v[3] * inv) << 32);
   };
   const int quads = rows * (d / 4);
   if (splits == 1) {
@@ -247,16 +245,21 @@ template <typename T, int DP> __global__ __launch_bounds__(kThreads, DP <= 64 ? 
   __syncthreads();
   if (flag != (unsigned)(splits - 1)) return;
   if (threadIdx.x == 0) reset_counter(counter);
-  for (int e = threadIdx.x; e < quads; e += kThreads) {
+  // Threads beyond one a quad take further parts: team `team` of `teams` those at its place of every `teams`.
+  const int teams = max(1, kThreads / quads);
+  f32x4_t* sums = (f32x4_t*)&part[0][0][0];
+  f32x2_t* heads = (f32x2_t*)(sums + kThreads);
+  for (int e0 = threadIdx.x; e0 < max(quads, kThreads); e0 += kThreads) {
+    const int team = e0 / quads, e = e0 - team * quads;
     const int row = e / (d / 4), dim = (e - row * (d / 4)) * 4;
     float mm = kLowest, ll = 0.0f;
     f32x4_t sum = {0, 0, 0, 0};
-    constexpr int AHEAD = 4;  // parts whose loads are out together
-    for (int s0 = 0; s0 < splits; s0 += AHEAD) {
+    constexpr int AHEAD = 8;  // parts whose loads are out together
+    for (int s0 = team; s0 < splits && team < teams; s0 += AHEAD * teams) {
       f32x2_t ml[AHEAD], v0[AHEAD], v1[AHEAD];
 #pragma unroll
       for (int n = 0; n < AHEAD; ++n) {
-        const float* src = parts + min(s0 + n, splits - 1) * pitch;
+        const float* src = parts + min(s0 + n * teams, splits - 1) * pitch;
         ml[n] = load_pair(src + rows * d + 2 * row);
         v0[n] = load_pair(src + row * d + dim);
         v1[n] = load_pair(src + row * d + dim + 2);
@@ -264,14 +267,27 @@ template <typename T, int DP> __global__ __launch_bounds__(kThreads, DP <= 64 ? 
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int n = 0; n < AHEAD; ++n) {
-        if (s0 + n >= splits) break;
+        if (s0 + n * teams >= splits) break;
         const float now = fmaxf(mm, ml[n][0]), keep = exp2_hw(mm - now), f = exp2_hw(ml[n][0] - now);
         mm = now;
         ll = ll * keep + f * ml[n][1];
         sum = sum * keep + f * f32x4_t{v0[n][0], v0[n][1], v1[n][0], v1[n][1]};
       }
     }
-    put(row, dim, sum, ll);
+    if (teams > 1) {
+      sums[threadIdx.x] = sum;
+      heads[threadIdx.x] = f32x2_t{mm, ll};
+      __syncthreads();
+      if (team) continue;
+      for (int n = 1; n < teams; ++n) {
+        const f32x2_t ml = heads[n * quads + e];
+        const float now = fmaxf(mm, ml[0]), keep = exp2_hw(mm - now), f = exp2_hw(ml[0] - now);
+        mm = now;
+        ll = ll * keep + f * ml[1];
+        sum = sum * keep + f * sums[n * quads + e];
+      }
+    }
+    if (team == 0) put(row, dim, sum, ll);
   }
 }
 
@@ -284,9 +300,13 @@ int qtts_launch_paged_small(const qtts::PagedLaunch& p, int dtype, hipStream_t s
   const dim3 grid((uint32_t)((int64_t)p.items * p.a.cache.kv_heads + p.fill));
   auto go = [&](auto type) {
     typedef decltype(type) T;
-    if (p.a.cache.d <= 64) launch(paged_small_kernel<T, 64>, grid, dim3(kThreads), 0u, st, p);
-    else if (p.a.cache.d <= 128) launch(paged_small_kernel<T, 128>, grid, dim3(kThreads), 0u, st, p);
-    else launch(paged_small_kernel<T, 256>, grid, dim3(kThreads), 0u, st, p);
+    const int d = p.a.cache.d;
+    if (d == 64) launch(paged_small_kernel<T, 64, true>, grid, dim3(kThreads), 0u, st, p);
+    else if (d == 128) launch(paged_small_kernel<T, 128, true>, grid, dim3(kThreads), 0u, st, p);
+    else if (d == 256) launch(paged_small_kernel<T, 256, true>, grid, dim3(kThreads), 0u, st, p);
+    else if (d < 64) launch(paged_small_kernel<T, 64, false>, grid, dim3(kThreads), 0u, st, p);
+    else if (d < 128) launch(paged_small_kernel<T, 128, false>, grid, dim3(kThreads), 0u, st, p);
+    else launch(paged_small_kernel<T, 256, false>, grid, dim3(kThreads), 0u, st, p);
   };
   if (dtype == QTTS_BF16) go(bf16_t{});
   else go(f16_t{});

@@ -13,8 +13,6 @@ constexpr float kLowest = -3.402823466e38f;  // where a running maximum starts: 
 
 struct PagedLaunch {
   PagedAttentionArgs a;
-  int32_t groups;       // workgroups a key-value head that the tiles are cut for; 0: never cut
-  int32_t least;        // tiles a split has at least
   int32_t min_rows, max_rows;  // requests with more than min_rows and up to max_rows (counts times query heads a key-value head)
   int32_t items;        // workgroups a key-value head in the grid
   int32_t fill;         // workgroups behind them that write the rows without a request (0: another launch does)
@@ -27,10 +25,25 @@ __device__ __forceinline__ PagedRequest load_request(const PagedAttentionArgs& a
   return paged_request(a.starts[r], a.counts[r], a.lengths[r], a.rows, (int64_t)a.cols << a.cache.page_shift, a.max_new);
 }
 
-__device__ __forceinline__ uint64_t wave_sum64(uint64_t v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+// Inclusive sum over the lanes up to each, by DPP (no LDS round trips): within rows of 16 lanes by shifts, then each row's
+// total into the rows behind it.
+template <int CTRL, int ROWS> __device__ __forceinline__ uint32_t dpp_moved(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, true);
+}
+__device__ __forceinline__ uint32_t wave_upto(uint32_t v) {
+  v += dpp_moved<0x111, 0xF>(v);  // row_shr 1, 2, 4, 8: zeros come in
+  v += dpp_moved<0x112, 0xF>(v);
+  v += dpp_moved<0x114, 0xF>(v);
+  v += dpp_moved<0x118, 0xF>(v);
+  v += dpp_moved<0x142, 0xA>(v);  // lane 15 of rows 0 and 2 to rows 1 and 3
+  v += dpp_moved<0x143, 0xC>(v);  // lane 31 to rows 2 and 3
   return v;
+}
+// The wave's sum of 64-bit values under 2^52: the low 26 bits' sum and the rest's.
+__device__ __forceinline__ uint64_t wave_sum64(uint64_t v) {
+  const uint32_t lo = __builtin_amdgcn_readlane(wave_upto((uint32_t)v & 0x3ffffff), 63);
+  const uint32_t hi = __builtin_amdgcn_readlane(wave_upto((uint32_t)(v >> 26)), 63);
+  return ((uint64_t)hi << 26) + lo;
 }
 
 // One workgroup's share of a head: run `run` of a request whose rows begin at `row` and whose first token's position is
@@ -60,6 +73,7 @@ __device__ __forceinline__ bool paged_work(const PagedLaunch& p, int item, Paged
   };
   PagedRequest mine = {0, 0, 0};
   uint64_t total = 0;
+  uint32_t all_runs = 0;
   for (int j = 0; j < per; ++j) {
     const int r = lane * per + j;
     if (r >= a.requests) break;
@@ -67,11 +81,15 @@ __device__ __forceinline__ bool paged_work(const PagedLaunch& p, int item, Paged
     int32_t tiles;
     const int32_t runs = runs_of(mine, tiles);
     total += (uint64_t)runs * (uint32_t)tiles;
+    all_runs += runs;
   }
-  const uint32_t share = p.groups ? tiles_a_split(wave_sum64(total), p.groups, p.least) : 0;
+  const int64_t pairs = (int64_t)__builtin_amdgcn_readlane(wave_upto(all_runs), 63) * a.cache.kv_heads;
+  const PagedCut cut = RUN == 16 ? small_cut(pairs) : many_cut(pairs);
+  const int32_t groups = cut.groups / a.cache.kv_heads;  // a head; 0: so many heads that nothing is cut
+  const uint32_t share = groups ? tiles_a_split(wave_sum64(total), groups, cut.least) : 0;
   auto items_of = [&](const PagedRequest& r, int32_t& tiles, int32_t& splits) -> int32_t {
     const int32_t runs = runs_of(r, tiles);
-    splits = p.groups ? splits_of(tiles, share) : 1;
+    splits = groups ? splits_of(tiles, share) : 1;
     return runs * splits;
   };
   int32_t items = 0, slots = 0;
@@ -84,15 +102,7 @@ __device__ __forceinline__ bool paged_work(const PagedLaunch& p, int item, Paged
     items += n;
     slots += splits > 1 ? n : 0;
   }
-  int32_t upto = items, slot_upto = slots;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int32_t u = __shfl_up(upto, o, 64), s = __shfl_up(slot_upto, o, 64);
-    if (lane >= o) {
-      upto += u;
-      slot_upto += s;
-    }
-  }
+  const int32_t upto = wave_upto(items), slot_upto = wave_upto(slots);
   const uint64_t past = __ballot(upto > item);
   if (!past) return false;
   const int owner = __ffsll((unsigned long long)past) - 1;
@@ -162,6 +172,14 @@ __device__ __forceinline__ float sum_32(float v) {
 __device__ __forceinline__ float sum_16_32(float v) {
   const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   return sum_32(__uint_as_float(r[0]) + __uint_as_float(r[1]));
+}
+
+// Two values rounded to T, the first in the low half, by conversions that the compiler schedules: it keeps the wait that an
+// exponential's reader needs (with from_f32's v_cvt_f16_f32 in inline asm right behind v_exp_f32, fp16 weights came out wrong).
+template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b) {
+  typedef __attribute__((ext_vector_type(2))) _Float16 f16x2_t;
+  if constexpr (std::is_same<T, bf16_t>::value) return pack2_f32<T>(a, b);
+  else return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2_t{a, b}), f16x2_t));
 }
 
 // 2^x, the hardware's (2^-22 relative; results below 2^-126 are zero, as is 2^-inf).

@@ -57,8 +57,26 @@ template <int T> QTTS_RULE int32_t most_tiles(int32_t length, int32_t span, int3
 
 // ---- splits of the keys over workgroups -----------------------------------------------------------------
 
-// Tiles of keys a workgroup takes, where `total` tiles (of all runs of rows of all requests, one key-value head) are
-// wanted in about `groups` workgroups a head, and no workgroup takes less than `least`.
+// How the tiles of a call are cut, by its runs of rows times key-value heads (`pairs`): so many workgroups in all are
+// wanted, none with fewer tiles than `least`.
+struct PagedCut {
+  int32_t groups, least;
+};
+constexpr int32_t kCutGroups = 4096;  // at most
+
+// Runs of up to 16 rows (tiles of 32 keys, four waves a workgroup, three workgroups a compute unit).  Few pairs: one round
+// of workgroups, two a unit (lengths of 4 x 16000, 16 x 4000 and 1 x 65536 tokens: 44.6, 29.2 and 47.2 us captured;
+// 1024 workgroups: 54.4, 36.8 and 50.8).  A workgroup's start costs about what 8 tiles do and a join as much again, so
+// that 8 are the least while compute units are idle (1 x 1000: 11.3, with 16: 14.6) and 16 where half of them are busy
+// (27 windows of 512: 15.3, with 8: 17.5).  Many pairs: pieces small enough to even out ragged lengths (64 x up to 8192: 221,
+// in 1024 workgroups 246).
+constexpr QTTS_RULE PagedCut small_cut(int64_t pairs) {
+  return pairs < 128 ? PagedCut{512, 8} : pairs < 256 ? PagedCut{512, 16} : PagedCut{kCutGroups, 16};
+}
+// Runs of up to 128 rows (tiles of 64 keys).
+constexpr QTTS_RULE PagedCut many_cut(int64_t pairs) { return PagedCut{512, 8}; }
+
+// Tiles a split, where `total` tiles (of all runs, one head) are wanted in about `groups` workgroups a head.
 QTTS_RULE uint32_t tiles_a_split(uint64_t total, int32_t groups, int32_t least) {
   const uint64_t c = (total + groups - 1) / groups;
   return c < (uint64_t)least ? (uint32_t)least : c > 0x40000000 ? 0x40000000u : (uint32_t)c;

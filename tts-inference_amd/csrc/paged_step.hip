@@ -104,7 +104,7 @@ __global__ __launch_bounds__(kStepThreads) void paged_step_kernel(PagedStepArgs 
         page = a.free_pages[base[lo] + column];
         if ((position & round) == 0) *entry = page;  // a new page has one first token, among the new ones
       }
-      if ((uint32_t)page < (uint32_t)a.pages) slot = (page << a.page_shift) + (position & round);
+      if (page >= 0 && page <= INT32_MAX >> a.page_shift) slot = (page << a.page_shift) + (position & round);
     }
     a.positions[t] = position;
     a.slots[t] = slot;

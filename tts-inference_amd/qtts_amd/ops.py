@@ -1217,9 +1217,10 @@ def qkv_to_cache(qkv: torch.Tensor, k: torch.Tensor, v: torch.Tensor, batch: Pag
 
 
 @functools.lru_cache(maxsize=1024)
-def _attention_bytes(max_new: int, heads: int, d: int) -> int:
-    """Workspace bytes of a :func:`paged_attention` call, a function of its sizes alone."""
-    return workspace_bytes(OP_PAGED_ATTENTION, max(1, max_new), heads, d)
+def attention_bytes(rows: int, d: int) -> int:
+    """Workspace bytes of a :func:`paged_attention` call: ``rows`` a request has at most (its new tokens times the query heads
+    of a key-value head), heads of ``d``."""
+    return workspace_bytes(OP_PAGED_ATTENTION, max(1, rows), 1, d)
 
 
 def paged_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, batch: PagedBatch, window: int = 0, sinks: int = 0,
@@ -1235,8 +1236,8 @@ def paged_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, batch: Pa
         raise ValueError(f"q must be [rows, heads, head size], got {tuple(q.shape)}")
     rows, heads, d = q.shape
     pages, kv_heads, width = _cache_sizes(k, v, batch, q.dtype)
-    if rows != batch.rows or d != width:
-        raise ValueError(f"q is {tuple(q.shape)} for {batch.rows} rows of heads of {width}")
+    if rows != batch.rows or d != width or not kv_heads or heads % kv_heads:
+        raise ValueError(f"q is {tuple(q.shape)} for {batch.rows} rows and {kv_heads} key-value heads of {width}")
     if window < 0 or sinks < 0:
         raise ValueError(f"window {window} and sinks {sinks} must not be negative")
     idx = _gpu_index(q, k, v, batch.table)
@@ -1248,7 +1249,7 @@ def paged_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, batch: Pa
     out = torch.empty(rows, heads, d, dtype=q.dtype, device=q.device)
     if not rows:
         return out
-    need, ws = _attention_bytes(batch.max_new, heads, d), _workspaces.get(idx)
+    need, ws = attention_bytes(min(batch.max_new, rows) * (heads // kv_heads), d), _workspaces.get(idx)
     if ws is None or ws.numel() < need:
         _ensure_workspace(q.device, need, "paged_attention")
         ws = _workspaces[idx]
