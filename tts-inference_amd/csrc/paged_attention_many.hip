@@ -32,6 +32,15 @@ template <> struct mfma32<f16_t> {
   }
 };
 
+// sum + lo + hi of two packed values, in one dot product with ones: the weights' sum is of what the second product takes.
+template <typename T> __device__ __forceinline__ float add2(uint32_t two, float sum) {
+  typedef __attribute__((ext_vector_type(2))) _Float16 f16x2_t;
+  if constexpr (std::is_same<T, bf16_t>::value)
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, two), __builtin_bit_cast(bf16x2_t, 0x3f803f80u), sum, false);
+  else
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2_t, two), __builtin_bit_cast(f16x2_t, 0x3c003c00u), sum, false);
+}
+
 // Position of piece `piece` in row `row`: rows of 128 bytes two to a bank cycle, longer ones one.
 template <int BYTES> __device__ __forceinline__ int place(int row, int piece) {
   return BYTES == 128 ? piece ^ ((row >> 1) & 7) : piece ^ (row & 15);
@@ -44,7 +53,7 @@ __device__ __forceinline__ int key_of_row(int row) {
 }
 
 // DP: the head size (EXACT) or what it is rounded up to, 64, 128 or 256.  WIDE: pages of a tile or more.
-template <typename T, int DP, bool EXACT, bool WIDE> __global__ __launch_bounds__(kThreads, DP == 64 || (DP == 128 && EXACT) ? 2 : 1) void paged_many_kernel(PagedLaunch p) {
+template <typename T, int DP, bool EXACT, bool WIDE> __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void paged_many_kernel(PagedLaunch p) {
   constexpr int NS = DP / 16, NB = DP / 32, KI = DP / 32;  // steps of Q K^T, blocks of O^T, 1 KiB loads a wave and operand
   __shared__ __attribute__((aligned(16))) uint8_t keys[2][kTile * DP * 2], values[2][kTile * DP * 2];
   __shared__ unsigned flag;
@@ -57,7 +66,7 @@ template <typename T, int DP, bool EXACT, bool WIDE> __global__ __launch_bounds_
   PagedWork w;
   if (!paged_work<kRun, kTile>(p, item, w)) return;
   const int group = a.heads / kv_heads, d = EXACT ? DP : a.cache.d, shift = a.cache.page_shift;
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
   const int64_t rows = (int64_t)w.count * group, first_row = (int64_t)w.run * kRun;
 
   // tokens of the run, and of this wave's rows
@@ -77,8 +86,8 @@ template <typename T, int DP, bool EXACT, bool WIDE> __global__ __launch_bounds_
   const int token = live ? (int)((wave_row + col) / group) : 0;
   const int query = h * group + (live ? (int)(wave_row + col - (int64_t)token * group) : 0);
   const int hi = live ? w.position + token : -1, lo = a.window && live ? max(0, hi - a.window + 1) : 0;
-  const int all_lo = a.window ? max(0, wave_hi - a.window + 1) : 0;  // every row of the wave sees [all_lo, wave_lo]
-  const int any_lo = a.window ? max(0, wave_lo - a.window + 1) : 0;  // and none what is below any_lo and no sink
+  const int wave_all_lo = a.window ? max(0, wave_hi - a.window + 1) : 0;  // every row of the wave sees [wave_all_lo, wave_lo]
+  const int any_lo = a.window ? max(0, wave_lo - a.window + 1) : 0;       // and none what is below any_lo and no sink
 
   i32x4_t qf[NS];
   {
@@ -98,12 +107,19 @@ template <typename T, int DP, bool EXACT, bool WIDE> __global__ __launch_bounds_
   };
   // the page of this lane's key of the tile (all of them on one page where pages are wide)
   auto pages_of = [&](int base) { return table[min(WIDE ? base : base + lane, last) >> shift]; };
+  if constexpr (!EXACT) {  // the columns of a key past its d are zero in both buffers and stay so
+    for (int i = threadIdx.x; i < 2 * kTile * DP / 8; i += kThreads) {
+      const i32x4_t zero = {0, 0, 0, 0};
+      *(i32x4_t*)(&keys[0][0] + 16 * i) = zero;
+    }
+    __syncthreads();
+  }
+  auto piece_of = [&](int unit) { return place<DP * 2>(unit / (DP / 8), unit % (DP / 8)); };
   uint32_t k_at[KI], v_at[KI];  // bytes from the tile's key 0 (k) and from its page's column (v), where pages are wide
 #pragma unroll
   for (int n = 0; n < KI; ++n) {
     const int unit = (wave * KI + n) * 64 + lane;
-    const int row = unit / (DP / 8), piece = min(place<DP * 2>(row, unit % (DP / 8)), d / 8 - 1);
-    k_at[n] = (uint32_t)(key_of_row(row) * d + piece * 8) * 2;
+    k_at[n] = (uint32_t)(key_of_row(unit / (DP / 8)) * d + piece_of(unit) * 8) * 2;
     const int dim = unit / 8, run = place<128>(dim, unit % 8);
     v_at[n] = ((uint32_t)min(dim, d - 1) << (shift + 1)) + run * 16;
   }
@@ -113,18 +129,20 @@ template <typename T, int DP, bool EXACT, bool WIDE> __global__ __launch_bounds_
       const int64_t at = head_of(__builtin_amdgcn_readfirstlane(page));
       const uint8_t *k = cache_k + at + (int64_t)(base & mask) * d * 2, *v = cache_v + at + (base & mask) * 2;
 #pragma unroll
-      for (int n = 0; n < KI; ++n) load_to_lds16(k + k_at[n], kb + n * 1024);
+      for (int n = 0; n < KI; ++n)
+        if (EXACT || piece_of((wave * KI + n) * 64 + lane) * 8 < d) load_to_lds16(k + k_at[n], kb + n * 1024);
 #pragma unroll
       for (int n = 0; n < KI; ++n) load_to_lds16(v + v_at[n], vb + n * 1024);
     } else {
-#pragma unroll
+      constexpr int UNROLL = DP == 256 ? 1 : KI;  // 16 addresses at once are more than there are registers
+#pragma unroll UNROLL
       for (int n = 0; n < KI; ++n) {
         const int unit = (wave * KI + n) * 64 + lane;
-        const int row = unit / (DP / 8), piece = min(place<DP * 2>(row, unit % (DP / 8)), d / 8 - 1), key = key_of_row(row);
-        load_to_lds16(cache_k + head_of(__shfl(page, key, 64)) + ((int64_t)(min(base + key, last) & mask) * d + piece * 8) * 2,
-                      kb + n * 1024);
+        const int piece = piece_of(unit), key = key_of_row(unit / (DP / 8));
+        const int64_t at = head_of(__shfl(page, key, 64)) + ((int64_t)(min(base + key, last) & mask) * d + piece * 8) * 2;
+        if (EXACT || piece * 8 < d) load_to_lds16(cache_k + at, kb + n * 1024);
       }
-#pragma unroll
+#pragma unroll UNROLL
       for (int n = 0; n < KI; ++n) {
         const int unit = (wave * KI + n) * 64 + lane;
         const int dim = unit / 8, key = place<128>(dim, unit % 8) * 8;
@@ -140,45 +158,53 @@ template <typename T, int DP, bool EXACT, bool WIDE> __global__ __launch_bounds_
   for (int b = 0; b < NB; ++b)
 #pragma unroll
     for (int e = 0; e < 16; ++e) o[b][e] = 0.0f;
-  int base = tile_of(begin), next = tile_of(begin + 1);
-  stage(base, pages_of(base), 0);
-  int32_t page = pages_of(next);
-  for (int i = begin; i < end; ++i) {
-    const int buffer = (i - begin) & 1;
-    wait_vmcnt<0>();   // this wave's share of the tile is in LDS
-    barrier_only();    // everyone's is, and the other buffer's readers are done
-    const int here = base;
-    if (i + 1 < end) {
-      stage(next, page, buffer ^ 1);
-      base = next;
-      next = tile_of(i + 2);
-      page = pages_of(next);
-    }
-    const bool out_of_sight = here > wave_hi || (here + kTile <= any_lo && here >= a.sinks);
-    if (out_of_sight) continue;
+
+  // One tile in LDS.
+  auto tile = [&](int here, const uint8_t* kb, const uint8_t* vb) {
+    // Operands leave LDS some products before theirs: the barriers keep the compiler from gathering loads and uses.
     f32x16_t s[2];
-#pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) s[t][e] = 0.0f;
-#pragma unroll
-    for (int n = 0; n < NS; ++n) {
+    constexpr int KP = 2;
+    i32x4_t k[KP][2];
+    auto load_k = [&](int n) {
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
-        if (!EXACT && n * 16 >= d) continue;
         const int row = t * 32 + col;
-        s[t] = mfma32<T>::mma(*(const i32x4_t*)(keys[buffer] + row * DP * 2 + place<DP * 2>(row, 2 * n + half) * 16), qf[n], s[t]);
+        k[n % KP][t] = *(const i32x4_t*)(kb + row * DP * 2 + place<DP * 2>(row, 2 * n + half) * 16);
+      }
+    };
+#pragma unroll
+    for (int n = 0; n < KP - 1; ++n) load_k(n);
+#pragma unroll
+    for (int n = 0; n < NS; ++n) {
+      if (n + KP - 1 < NS) load_k(n + KP - 1);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        if (n) s[t] = mfma32<T>::mma(k[n % KP][t], qf[n], s[t]);
+        else s[t] = mfma32<T>::mma(k[n % KP][t], qf[n], f32x16_t{});
       }
     }
-    // score e of product t: key here + 32 t + 16 (e / 8) + 8 half + e % 8
-    const bool whole = here + kTile - 1 <= wave_lo && (here >= all_lo || here + kTile <= a.sinks);
-    if (!whole) {
+    constexpr int VP = 4;  // values' operands that are out together; operand n: keys 16 (n / NB), columns 32 (n % NB)
+    i32x4_t v[VP];
+    auto load_v = [&](int n) {
+      const int dim = n % NB * 32 + col;
+      v[n % VP] = *(const i32x4_t*)(vb + dim * 128 + place<128>(dim, 2 * (n / NB) + half) * 16);
+    };
+#pragma unroll
+    for (int n = 0; n < VP; ++n) load_v(n);
+    __builtin_amdgcn_sched_barrier(0);
+    // Score e of product t: key here + 32 t + 16 (e / 8) + 8 half + e % 8.  Where some row does not see some key of the tile: a
+    // bit a key, set for those that this lane's row sees, makes each score's upper bound (infinite, or -infinite).
+    if (here + kTile - 1 > wave_lo || (here < wave_all_lo && here + kTile > a.sinks)) {
+      auto below = [&](int n) { return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1; };  // keys here .. here + n - 1
+      const uint64_t seen = (below(hi + 1 - here) & (~below(lo - here) | below(a.sinks - here))) >> (8 * half);
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          const int key = here + 32 * t + 16 * (e >> 3) + 8 * half + (e & 7);
-          s[t][e] = key <= hi && (key >= lo || key < a.sinks) ? s[t][e] : -INFINITY;
+          const uint32_t hidden = ~(uint32_t)(seen >> (32 * t));
+          const uint32_t sign = (hidden << (31 - 16 * (e >> 3) - (e & 7))) & 0x80000000u;
+          s[t][e] = fminf(s[t][e], __uint_as_float(sign | 0x7f800000u));
         }
     }
     float top = s[0][0];
@@ -194,39 +220,53 @@ template <typename T, int DP, bool EXACT, bool WIDE> __global__ __launch_bounds_
       for (int b = 0; b < NB; ++b) o[b] *= keep;
     }
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        s[t][e] = exp2_hw(__builtin_fmaf(s[t][e], a.scale, -m));
-        l += s[t][e];
-      }
-#pragma unroll
     for (int ks = 0; ks < 4; ++ks) {
       i32x4_t weights;
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        weights[j] = (int)pack2<T>(s[ks >> 1][8 * (ks & 1) + 2 * j], s[ks >> 1][8 * (ks & 1) + 2 * j + 1]);
-      uint32_t keep[4] = {~0u, ~0u, ~0u, ~0u};
-      if (!whole) {  // values that no row of the wave sees, among them what lies behind the request's end: zero
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int key = here + 16 * ks + 8 * half + 2 * j;
-          keep[j] = (key <= wave_hi && (key >= any_lo || key < a.sinks) ? 0xffffu : 0u) |
-                    (key + 1 <= wave_hi && (key + 1 >= any_lo || key + 1 < a.sinks) ? 0xffff0000u : 0u);
-        }
+      for (int j = 0; j < 4; ++j) {
+        const float w0 = exp2_hw(__builtin_fmaf(s[ks >> 1][8 * (ks & 1) + 2 * j], a.scale, -m));
+        const float w1 = exp2_hw(__builtin_fmaf(s[ks >> 1][8 * (ks & 1) + 2 * j + 1], a.scale, -m));
+        weights[j] = (int)pack2<T>(w0, w1);
+        l = add2<T>((uint32_t)weights[j], l);
       }
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
-        if (!EXACT && b * 32 >= d) continue;
-        const int dim = b * 32 + col;
-        i32x4_t v = *(const i32x4_t*)(values[buffer] + dim * 128 + place<128>(dim, 2 * ks + half) * 16);
-        if (!whole) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) v[j] = (int)((uint32_t)v[j] & keep[j]);
-        }
-        o[b] = mfma32<T>::mma(v, weights, o[b]);
+        const int n = ks * NB + b;
+        o[b] = mfma32<T>::mma(v[n % VP], weights, o[b]);
+        if (n + VP < 4 * NB) load_v(n + VP);
       }
     }
+  };
+
+  int base = tile_of(begin), next = tile_of(begin + 1);
+  stage(base, pages_of(base), 0);
+  int32_t page = pages_of(next);
+  for (int i = begin; i < end; ++i) {
+    const int buffer = (i - begin) & 1, here = base;
+    wait_vmcnt<0>();   // this wave's share of the tile is in LDS
+    barrier_only();    // everyone's is, and the other buffer's readers are done
+    if (i + 1 < end) {
+      stage(next, page, buffer ^ 1);
+      base = next;
+      next = tile_of(i + 2);
+      page = pages_of(next);
+    }
+    if (here + kTile > w.length) {  // values behind the request's end were never written: zero
+      for (int u = threadIdx.x; u < DP * 8; u += kThreads) {
+        const int past = w.length - here - 8 * place<128>(u / 8, u % 8);  // values of the piece that are the request's
+        i32x4_t* piece = (i32x4_t*)(values[buffer] + 16 * u);
+        if (past < 8) {
+          i32x4_t kept = *piece;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) kept[j] &= past <= 2 * j ? 0 : past == 2 * j + 1 ? 0xffff : -1;
+          *piece = kept;
+        }
+      }
+      wait_lgkmcnt0();
+      barrier_only();
+    }
+    if (here > wave_hi || (here + kTile <= any_lo && here >= a.sinks)) continue;  // out of the wave's sight
+    tile(here, keys[buffer], values[buffer]);
   }
   l = sum_32(l);
 

@@ -38,7 +38,7 @@ void paged_small_kernel(PagedLaunch p) {
   PagedWork w;
   if (!paged_work<kRows, kTile>(p, item, w)) return;
   const int group = a.heads / kv_heads, d = EXACT ? DP : a.cache.d, shift = a.cache.page_shift;
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
   const int rows = w.count * group;
 
   const KeyTiles tiles = key_tiles<kTile>(w.position, w.length - 1, a.window, a.sinks);

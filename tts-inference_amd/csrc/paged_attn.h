@@ -111,8 +111,10 @@ __device__ __forceinline__ bool paged_work(const PagedLaunch& p, int item, Paged
   for (int j = 0; j < per; ++j) {  // the owner's requests, every lane alike
     const int r = owner * per + j;
     PagedRequest q;
-    if (per > 1) q = load_request(a, r);
-    else q = {__builtin_amdgcn_readlane(mine.start, owner), __builtin_amdgcn_readlane(mine.count, owner),
+    if (per > 1) {
+      q = load_request(a, r);
+      q = {__builtin_amdgcn_readfirstlane(q.start), __builtin_amdgcn_readfirstlane(q.count), __builtin_amdgcn_readfirstlane(q.length)};
+    } else q = {__builtin_amdgcn_readlane(mine.start, owner), __builtin_amdgcn_readlane(mine.count, owner),
               __builtin_amdgcn_readlane(mine.length, owner)};
     int32_t tiles, splits;
     const int32_t n = items_of(q, tiles, splits);
