@@ -15,7 +15,7 @@ namespace qtts {
 namespace {
 
 constexpr int kStepThreads = 1024;
-constexpr int kStepRows = 4 * kStepThreads;  // rows a workgroup
+constexpr int kStepRows = kStepThreads;  // rows a workgroup
 
 __device__ __forceinline__ int64_t wave_scan(int64_t v) {
 #pragma unroll

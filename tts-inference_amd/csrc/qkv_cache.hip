@@ -4,7 +4,7 @@
 // The mathematics, in fp32 with one rounding at the end: x <- x / sqrt(mean x^2 + eps) * w, then for i < d / 2
 // (x_i, x_{i + d/2}) <- (x_i cos_i - x_{i + d/2} sin_i, x_{i + d/2} cos_i + x_i sin_i).  A group of lanes takes a head of
 // a row, each lane 8 columns of either half (16-byte loads), so that a rotation's pair is in one lane and the norm's sum
-// is a few lane exchanges.
+// is a few lane exchanges; workgroups of their own take the values.
 #include "common.h"
 #include "paged.h"
 
@@ -13,6 +13,9 @@ namespace qtts {
 namespace {
 
 constexpr int kThreads = 256;
+// Heads of rows from which a thread takes four, which share the row's angles, and values go 64 rows a workgroup instead of 8
+// (2048 rows of 16 + 8 heads: 9.3 us captured, one head and 8 rows 9.8; 512 rows 6.9 and 4.9, 64 single tokens 9.5 and 4.2).
+constexpr int64_t kManyHeads = 32768;
 
 template <typename T> __device__ __forceinline__ void unpack8(i32x4_t v, float (&x)[8]) {
 #pragma unroll
@@ -29,28 +32,43 @@ template <typename T> __device__ __forceinline__ i32x4_t pack8(const float (&x)[
   return v;
 }
 
-// L lanes a head: the least power of two with 16 L >= d.
-template <typename T, int L> __global__ __launch_bounds__(kThreads) void qkv_cache_kernel(QkvCacheArgs a) {
-  const int heads = a.heads + 2 * a.cache.kv_heads, d = a.cache.d, half = d / 2;
-  const int64_t unit = ((int64_t)blockIdx.x * kThreads + threadIdx.x) / L;
+// Queries and keys: L lanes a head (the least power of two with 16 L >= d), PER heads of a row one after the other.
+template <typename T, int L, int PER> __device__ __forceinline__ void qk_heads(const QkvCacheArgs& a, int block) {
+  const int heads = a.heads + a.cache.kv_heads, d = a.cache.d, half = d / 2, parts = (heads + PER - 1) / PER;
+  const int64_t unit = ((int64_t)block * kThreads + threadIdx.x) / L;
   const int lane = threadIdx.x & (L - 1), col = lane * 8;
-  const int64_t row = unit / heads;
-  const int head = (int)(unit - row * heads);
-  const bool live = row < a.rows;
-  const bool mine = live && col < half;
+  const int64_t row = unit / parts;
+  const int first = (int)(unit - row * parts) * PER;
+  const bool live = row < a.rows, mine = live && col < half;
   const int32_t slot = live ? a.slots[row] : -1;
   const bool kept = slot >= 0 && (slot >> a.cache.page_shift) < a.cache.pages;
-  const T* src = (const T*)a.qkv + row * a.ldqkv + (int64_t)head * d;
-  i32x4_t lo = {0, 0, 0, 0}, hi = {0, 0, 0, 0};
-  if (mine && kept) {
-    lo = *(const i32x4_t*)(src + col);
-    hi = *(const i32x4_t*)(src + half + col);
+  const T* src = (const T*)a.qkv + row * a.ldqkv + (int64_t)first * d;
+  i32x4_t lo[PER], hi[PER];
+#pragma unroll
+  for (int n = 0; n < PER; ++n) {
+    lo[n] = hi[n] = i32x4_t{0, 0, 0, 0};
+    if (mine && kept && first + n < heads) {
+      lo[n] = *(const i32x4_t*)(src + n * d + col);
+      hi[n] = *(const i32x4_t*)(src + n * d + half + col);
+    }
   }
-  const bool is_q = head < a.heads, is_v = head >= a.heads + a.cache.kv_heads;
-  if (!is_v) {
+  float c[8], s[8];
+  if (mine && kept && a.cos) {
+    int32_t position = a.positions[row];
+    position = position < 0 ? 0 : position < a.rope_rows ? position : a.rope_rows - 1;
+#pragma unroll
+    for (int i = 0; i < 8; i += 4) {
+      *(f32x4_t*)(c + i) = *(const f32x4_t*)(a.cos + (int64_t)position * half + col + i);
+      *(f32x4_t*)(s + i) = *(const f32x4_t*)(a.sin + (int64_t)position * half + col + i);
+    }
+  }
+#pragma unroll
+  for (int n = 0; n < PER; ++n) {
+    const int head = first + n;
+    const bool is_q = head < a.heads;
     float x[8], y[8];
-    unpack8<T>(lo, x);
-    unpack8<T>(hi, y);
+    unpack8<T>(lo[n], x);
+    unpack8<T>(hi[n], y);
     const T* weight = (const T*)(is_q ? a.q_norm : a.k_norm);
     float sum = 0.0f;
 #pragma unroll
@@ -69,58 +87,111 @@ template <typename T, int L> __global__ __launch_bounds__(kThreads) void qkv_cac
       }
     }
     if (mine && kept && a.cos) {
-      int32_t position = a.positions[row];
-      position = position < 0 ? 0 : position < a.rope_rows ? position : a.rope_rows - 1;
-      const float* cos = a.cos + (int64_t)position * half + col;
-      const float* sin = a.sin + (int64_t)position * half + col;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float c = cos[i], s = sin[i], u = x[i], v = y[i];
-        x[i] = u * c - v * s;
-        y[i] = v * c + u * s;
+        const float u = x[i], v = y[i];
+        x[i] = u * c[i] - v * s[i];
+        y[i] = v * c[i] + u * s[i];
       }
     }
-    lo = pack8<T>(x);
-    hi = pack8<T>(y);
-  }
-  if (!mine) return;
-  if (is_q) {  // a row of no request: zeros
-    T* q = (T*)a.q + (row * a.heads + head) * d;
-    *(i32x4_t*)(q + col) = lo;
-    *(i32x4_t*)(q + half + col) = hi;
-    return;
-  }
-  if (!kept) return;
-  const int kvh = head - a.heads - (is_v ? a.cache.kv_heads : 0);
-  const int64_t page = slot >> a.cache.page_shift, off = slot & ((1 << a.cache.page_shift) - 1);
-  const int64_t at = ((page * a.cache.kv_heads + kvh) * d) << a.cache.page_shift;
-  if (!is_v) {
-    T* k = (T*)a.cache.k + at + off * d;
-    *(i32x4_t*)(k + col) = lo;
-    *(i32x4_t*)(k + half + col) = hi;
-    return;
-  }
-  T* v = (T*)a.cache.v + at + off;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int sh = 16 * (i & 1);
-    v[(int64_t)(col + i) << a.cache.page_shift] = T{(uint16_t)((uint32_t)lo[i >> 1] >> sh)};
-    v[(int64_t)(half + col + i) << a.cache.page_shift] = T{(uint16_t)((uint32_t)hi[i >> 1] >> sh)};
+    if (!mine || head >= heads || !(is_q || kept)) continue;
+    T* out;
+    if (is_q) {  // a row of no request: zeros
+      out = (T*)a.q + (row * a.heads + head) * d;
+    } else {
+      const int64_t page = slot >> a.cache.page_shift, off = slot & ((1 << a.cache.page_shift) - 1);
+      out = (T*)a.cache.k + (((page * a.cache.kv_heads + head - a.heads) * d) << a.cache.page_shift) + off * d;
+    }
+    *(i32x4_t*)(out + col) = pack8<T>(x);
+    *(i32x4_t*)(out + half + col) = pack8<T>(y);
   }
 }
 
+// Values: a workgroup takes ROWS rows of one head through LDS, since they lie d-major on their page.  Eight rows whose slots are
+// eight tokens in a row from a multiple of eight go out together, 16 bytes a dimension (eight such groups fill lines of
+// 128 bytes); the group belongs to the workgroup of its first row, which reads up to 7 rows past its own.  Other rows
+// (a request's ends) go out by themselves, 2 bytes a dimension.
+template <typename T, int ROWS> __device__ __forceinline__ void value_rows(const QkvCacheArgs& a, int tile, int h) {
+  constexpr int kReach = ROWS + 8, GROUPS = ROWS / 8;
+  __shared__ uint16_t rows[kReach][kPagedMaxDim + 2];
+  __shared__ int32_t slot_of[kReach + 8];  // of rows first - 8 .. first + kReach - 1
+  const int d = a.cache.d, wave = threadIdx.x >> 6, lane = threadIdx.x & 63, shift = a.cache.page_shift;
+  const int64_t first = (int64_t)tile * ROWS;
+  if (threadIdx.x < kReach + 8) {
+    const int64_t row = first - 8 + threadIdx.x;
+    int32_t slot = row >= 0 && row < a.rows ? a.slots[row] : -1;
+    if (slot >= 0 && (slot >> shift) >= a.cache.pages) slot = -1;
+    slot_of[threadIdx.x] = slot;
+  }
+  const uint16_t* src = (const uint16_t*)a.qkv + first * a.ldqkv + (int64_t)(a.heads + a.cache.kv_heads + h) * d;
+  for (int u = threadIdx.x; u < kReach * (d / 8); u += kThreads) {
+    const int r = u / (d / 8), col = (u - r * (d / 8)) * 8;
+    if (first + r >= a.rows) break;
+    const i32x4_t v = *(const i32x4_t*)(src + r * a.ldqkv + col);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) *(int32_t*)&rows[r][col + 2 * i] = v[i];
+  }
+  __syncthreads();
+  auto leads = [&](int t) {  // row first + t, t >= -7: the first of a group
+    const int32_t slot = slot_of[8 + t];
+    bool all = slot >= 0 && (slot & 7) == 0;
+#pragma unroll
+    for (int i = 1; i < 8; ++i) all = all && slot_of[8 + t + i] == slot + i;
+    return all;
+  };
+  const int row = lane & (ROWS - 1);  // the lane's row of the tile, for the two questions asked of each
+  const int32_t mine = slot_of[8 + row];
+  const uint64_t leaders = __ballot(lane < ROWS && leads(row));
+  uint64_t alone = __ballot(lane < ROWS && mine >= 0 && !leads(row - (mine & 7)));
+  T* cache = (T*)a.cache.v;
+  auto base_of = [&](int32_t slot) {
+    return ((((int64_t)(slot >> shift)) * a.cache.kv_heads + h) * d << shift) + (slot & ((1 << shift) - 1));
+  };
+  uint64_t left = leaders;  // at most GROUPS
+  for (int n = lane & (GROUPS - 1); n && left; --n) left &= left - 1;
+  if (left) {
+    const int t = __builtin_ctzll(left);
+    T* to = cache + base_of(slot_of[8 + t]);
+    for (int dim = threadIdx.x / GROUPS; dim < d; dim += kThreads / GROUPS) {
+      i32x4_t v;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = (int)(rows[t + 2 * i][dim] | ((uint32_t)rows[t + 2 * i + 1][dim] << 16));
+      *(i32x4_t*)(to + ((int64_t)dim << shift)) = v;
+    }
+  }
+  for (int n = 0; alone; ++n) {
+    const int t = __builtin_ctzll(alone);
+    alone &= alone - 1;
+    if ((n & 3) != wave) continue;
+    T* to = cache + base_of(slot_of[8 + t]);
+    for (int dim = lane; dim < d; dim += 64) to[(int64_t)dim << shift] = T{rows[t][dim]};
+  }
+}
+
+template <typename T, int L, int PER, int ROWS> __global__ __launch_bounds__(kThreads) void qkv_cache_kernel(QkvCacheArgs a, int value_groups) {
+  if ((int)blockIdx.x < value_groups) value_rows<T, ROWS>(a, blockIdx.x / a.cache.kv_heads, blockIdx.x % a.cache.kv_heads);
+  else qk_heads<T, L, PER>(a, blockIdx.x - value_groups);
+}
+
 template <typename T> void launch_qkv(const QkvCacheArgs& a, hipStream_t st) {
-  const int64_t units = (int64_t)a.rows * (a.heads + 2 * a.cache.kv_heads);
-  auto go = [&](auto lanes) {
-    constexpr int L = decltype(lanes)::value;
-    launch(qkv_cache_kernel<T, L>, dim3((uint32_t)((units * L + kThreads - 1) / kThreads)), dim3(kThreads), 0u, st, a);
+  const int heads = a.heads + a.cache.kv_heads;
+  auto go = [&](auto lanes, auto per, auto rows) {
+    constexpr int L = decltype(lanes)::value, PER = decltype(per)::value, ROWS = decltype(rows)::value;
+    const int64_t values = ((int64_t)a.rows + ROWS - 1) / ROWS * a.cache.kv_heads;
+    const int64_t units = (int64_t)a.rows * ((heads + PER - 1) / PER);
+    launch(qkv_cache_kernel<T, L, PER, ROWS>, dim3((uint32_t)(values + (units * L + kThreads - 1) / kThreads)), dim3(kThreads), 0u, st,
+           a, (int)values);
+  };
+  auto by_rows = [&](auto lanes) {
+    if ((int64_t)a.rows * heads >= kManyHeads) go(lanes, std::integral_constant<int, 4>{}, std::integral_constant<int, 64>{});
+    else go(lanes, std::integral_constant<int, 1>{}, std::integral_constant<int, 8>{});
   };
   const int need = a.cache.d / 16;
-  if (need <= 1) go(std::integral_constant<int, 1>{});
-  else if (need <= 2) go(std::integral_constant<int, 2>{});
-  else if (need <= 4) go(std::integral_constant<int, 4>{});
-  else if (need <= 8) go(std::integral_constant<int, 8>{});
-  else go(std::integral_constant<int, 16>{});
+  if (need <= 1) by_rows(std::integral_constant<int, 1>{});
+  else if (need <= 2) by_rows(std::integral_constant<int, 2>{});
+  else if (need <= 4) by_rows(std::integral_constant<int, 4>{});
+  else if (need <= 8) by_rows(std::integral_constant<int, 8>{});
+  else by_rows(std::integral_constant<int, 16>{});
 }
 
 }  // namespace
