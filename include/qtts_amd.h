@@ -516,14 +516,15 @@ int qtts_lora_add_fresh(const void* x, int x_dtype, int64_t m, int64_t k, int64_
  *   starts [requests + 1]: each request's first row, and the end of the last one's
  *   counts [requests]: rows that joined the request, added[r] or 0 (denied, below)
  *   lengths_out [requests], taken_out [1]: the state after the step; may be lengths and taken
- *   positions, slots [rows]: of each row; -1 for rows of no request or of a denied one
+ *   positions, slots [room], room >= rows: of each row; -1 for rows of no request or of a denied one
+ *     and for what lies behind the batch's rows (another captured step's may)
  *   table: the columns of new pages are written
  * A request is denied as a whole where added[r] > max_new, where its rows do not fit `rows` or its tokens the
  * table, and where it needs pages while those that it and the requests before it need
  * exceed what is left.  Workspace: the 64 KiB of counters that every workspace begins with. */
 int qtts_paged_step(const int32_t* added, int64_t requests, const int32_t* lengths, int32_t* table, int64_t cols,
                     const int32_t* free_pages, int64_t pages, const int32_t* taken, int64_t page_size, int64_t rows,
-                    int64_t max_new, int32_t* starts, int32_t* counts, int32_t* lengths_out, int32_t* taken_out,
+                    int64_t room, int64_t max_new, int32_t* starts, int32_t* counts, int32_t* lengths_out, int32_t* taken_out,
                     int32_t* positions, int32_t* slots, void* ws, int64_t ws_bytes, void* stream);
 
 /* The pages of requests with which[r] != 0 back to the free list, in the order of the requests; their lengths are 0 then. */

@@ -457,3 +457,124 @@ def _check_rows(out, want, rows):
     fi = torch.finfo(out.dtype)
     err = (out[rows].double() - want[rows].double()).abs()
     assert (err <= 2 * fi.eps * want[rows].double().abs().amax(-1, keepdim=True) + fi.tiny).all()
+
+
+@DTYPES
+@pytest.mark.parametrize("count,most,mixed", [(64, 40, False), (65, 200, False), (130, 90, True), (500, 300, False), (2048, 40, True)])
+def test_many_requests(ops, count, most, mixed, dtype):
+    """More requests than a wave has lanes: single tokens alone, and between prompts and drafts; a few denied ones."""
+    rng = random.Random(count)
+    requests = [None if rng.random() < 0.03 else (rng.randint(0, most), rng.choice([1, 1, 1, 3, 9, rng.randint(1, 40)]) if mixed else 1)
+                for _ in range(count)]
+    q, k, v, batch = _inputs(ops, requests, 16, 4, 2, 64, dtype, seed=count, padding=5)
+    _check(ops, q, k, v, batch)
+    _check(ops, q, k, v, batch, 20, 3)
+
+
+@DTYPES
+def test_one_long_among_short(ops, dtype):
+    """A chunk behind a long cache, whose keys are split, next to prompts, drafts and single tokens."""
+    requests = [(9000, 70), (0, 5), (100, 1), (3000, 1), (40, 200), (0, 1), (12000, 1)]
+    q, k, v, batch = _inputs(ops, requests, 64, 8, 4, 128, dtype, seed=2, padding=2)
+    first = _check(ops, q, k, v, batch)
+    _check(ops, q, k, v, batch, 4000, 5)
+    for _ in range(2):
+        assert torch.equal(ops.paged_attention(q, k, v, batch), first)
+
+
+def test_rows_apart_and_bounds(ops):
+    """Query rows out of a wider tensor, off 16 bytes too; requests past max_new and lengths that no step makes get zeros."""
+    requests = [(40, 1), (0, 30), (5, 2), (100, 1)]
+    q, k, v, batch = _inputs(ops, requests, 16, 4, 2, 64, torch.bfloat16, seed=3, padding=3)
+    want = _check(ops, q, k, v, batch)
+    for width, lead in ((4 * 64 + 128, 64), (4 * 64 + 5, 3)):
+        wide = torch.full((batch.rows, width), float("nan"), dtype=q.dtype, device="cuda")
+        wide[:, lead:lead + 256] = q.view(batch.rows, 256)
+        view = wide[:, lead:lead + 256].unflatten(1, (4, 64))
+        assert torch.equal(ops.paged_attention(view, k, v, batch), want)
+    assert torch.equal(ops.paged_attention(q.transpose(0, 1).contiguous().transpose(0, 1), k, v, batch), want)
+    few = ops.PagedBatch(batch.table, batch.starts, batch.counts, batch.lengths, batch.positions, batch.slots, 16, max_new=2)
+    out = ops.paged_attention(q, k, v, few)
+    kept = [0, *range(31, 34)]
+    assert not out[1:31].any() and torch.equal(out[34:], want[34:])
+    _check_rows(out, want, kept)
+    for field, value in (("lengths", 1 << 20), ("lengths", 0), ("lengths", -7), ("counts", 500), ("starts", -3), ("starts", 1 << 30)):
+        parts = {n: getattr(batch, n).clone() for n in ("table", "starts", "counts", "lengths", "positions", "slots")}
+        parts[field][1] = value
+        odd = ops.PagedBatch(**parts, page_size=16, max_new=30)
+        out = ops.paged_attention(q, k, v, odd)
+        _check_rows(out, want, [0, 31, 32, 33] if field != "starts" else [31, 32, 33])
+        if field == "lengths":
+            assert not out[1:31].any()
+    parts = {n: getattr(batch, n).clone() for n in ("table", "starts", "counts", "lengths", "positions", "slots")}
+    parts["table"][1] = torch.tensor([-1, 2 ** 31 - 1, 10 ** 6], device="cuda")[torch.arange(parts["table"].shape[1], device="cuda") % 3]
+    out = ops.paged_attention(q, k, v, ops.PagedBatch(**parts, page_size=16, max_new=30))  # entries that are no page: a page all the same
+    _check_rows(out, want, [0, 31, 32, 33])
+    slots = batch.slots.clone()
+    slots[2], slots[5], slots[7] = 2 ** 31 - 1, -2 ** 31, k.shape[0] * 16  # slots outside the cache: nothing is written
+    kc, vc = torch.zeros_like(k), torch.zeros_like(v)
+    qkv = _rand((batch.rows, 8 * 64), torch.bfloat16, 4)
+    out = ops.qkv_to_cache(qkv, kc, vc, ops.PagedBatch(batch.table, batch.starts, batch.counts, batch.lengths, batch.positions, slots, 16), 4)
+    live = [i for i in range(34) if i not in (2, 5, 7)]
+    assert not out[[2, 5, 7, 34, 35, 36]].any() and (out[live] != 0).any(-1).all()
+    assert int((kc != 0).any(-1).sum()) == 2 * len(live)
+
+
+@pytest.mark.parametrize("new", [1, 80])
+def test_caches_past_32_bits(ops, new):
+    """Pages whose bytes and elements pass 2^32, on either side of those offsets."""
+    pages, kv, d, page = 70000, 8, 128, 64
+    k, v = (torch.empty(shape, dtype=torch.bfloat16, device="cuda") for shape in ((pages, kv, page, d), (pages, kv, d, page)))
+    assert k.numel() > 1 << 32
+    used = [0, 32767, 32768, 65535, 65536, pages - 1, 1, 16384, 49152]
+    table = _i32([used[:5], used[5:] + [7]])
+    lengths = [5 * 64 - 3, 4 * 64]
+    for i, p in enumerate(used + [7]):
+        k[p], v[p] = _rand((kv, page, d), torch.bfloat16, i), _rand((kv, d, page), torch.bfloat16, 50 + i)
+    at = [list(range(n - new, n)) for n in lengths]
+    slots = [[table.tolist()[r][p // page] * page + p % page for p in at[r]] for r in range(2)]
+    batch = ops.PagedBatch(table, _i32([0, new, 2 * new]), _i32([new, new]), _i32(lengths), _i32(at[0] + at[1]), _i32(slots[0] + slots[1]), page,
+                           max_new=new)
+    qkv = _rand((2 * new, 32 * d), torch.bfloat16, 3)
+    q = ops.qkv_to_cache(qkv, k, v, batch, 16)
+    slot = batch.slots.long()
+    assert torch.equal(k[slot // page, :, slot % page], qkv.view(2 * new, 32, d)[:, 16:24])
+    assert torch.equal(v[slot // page, :, :, slot % page], qkv.view(2 * new, 32, d)[:, 24:])
+    _check(ops, q, k, v, batch)
+    _check(ops, q, k, v, batch, 100, 70)
+
+
+def test_first_calls_of_a_process(ops, monkeypatch):
+    """Without a workspace yet: a call of no rows needs none, any other reserves its own; a captured one says what is missing."""
+    monkeypatch.setattr(ops, "_workspaces", {})
+    q, k, v, batch = _inputs(ops, [(0, 0)], 16, 4, 2, 64, torch.bfloat16)
+    assert ops.paged_attention(q, k, v, batch).shape == (0, 4, 64)
+    assert ops.qkv_to_cache(torch.empty(0, 8 * 64, dtype=torch.bfloat16, device="cuda"), k, v, batch, 4).shape == (0, 4, 64)
+    assert not ops._workspaces
+    q, k, v, batch = _inputs(ops, [(30, 1)], 16, 4, 2, 64, torch.bfloat16)
+    _check(ops, q, k, v, batch)
+    assert len(ops._workspaces) == 1
+    monkeypatch.setattr(ops, "_workspaces", {})
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(ValueError, match="reserve_workspace"):
+        with torch.cuda.graph(graph):
+            ops.paged_attention(q, k, v, batch)
+
+
+def test_large_scores(ops):
+    """Scores of hundreds, rising and falling along the keys (the running maximum moves on every tile), and one that
+    leaves all others without weight."""
+    for dtype in (torch.bfloat16, torch.float16):
+        for requests in ([(700, 1), (2000, 1)], [(100, 150), (1500, 70)]):
+            q, k, v, batch = _inputs(ops, requests, 64, 8, 4, 128, dtype, seed=6)
+            for ramp in (0.02, -0.02):
+                kk = k.clone()
+                for r in range(2):
+                    at = torch.arange(int(batch.lengths[r]), device="cuda")
+                    slot = batch.table[r].long()[at // 64] * 64 + at % 64
+                    kk[slot // 64, :, slot % 64] = (kk[slot // 64, :, slot % 64].float() + ramp * at[:, None, None]).to(dtype)
+                qq = (q.float() + 1).to(dtype)
+                _check(ops, qq, kk, v, batch)
+                _check(ops, qq, kk, v, batch, 130, 4)
+            _check(ops, q, k, v, batch, scale=2.0)
+            _check(ops, q, k, v, batch, scale=1e-3)

@@ -966,14 +966,15 @@ static int paged_cache(const char* what, qtts::PagedCache& c, const void* k, con
 
 int qtts_paged_step(const int32_t* added, int64_t requests, const int32_t* lengths, int32_t* table, int64_t cols,
                     const int32_t* free_pages, int64_t pages, const int32_t* taken, int64_t page_size, int64_t rows,
-                    int64_t max_new, int32_t* starts, int32_t* counts, int32_t* lengths_out, int32_t* taken_out,
+                    int64_t room, int64_t max_new, int32_t* starts, int32_t* counts, int32_t* lengths_out, int32_t* taken_out,
                     int32_t* positions, int32_t* slots, void* ws, int64_t ws_bytes, void* stream) {
   QTTS_TRY(paged_sizes("paged_step", requests, cols, pages, page_size));
   QTTS_REQUIRE(rows >= 0 && max_new >= 0, "paged_step: negative size");
-  QTTS_REQUIRE(rows < (1ll << 31) - 8192, "paged_step: size too large");
+  QTTS_REQUIRE(room >= rows, "paged_step: room for %lld of %lld rows", (long long)room, (long long)rows);
+  QTTS_REQUIRE(room < (1ll << 31) - 8192, "paged_step: size too large");
   QTTS_REQUIRE(taken && starts && taken_out, "paged_step: null pointer");
   QTTS_REQUIRE(requests == 0 || (added && lengths && counts && lengths_out && (cols == 0 || table)), "paged_step: null pointer");
-  QTTS_REQUIRE((pages == 0 || free_pages) && (rows == 0 || (positions && slots)), "paged_step: null pointer");
+  QTTS_REQUIRE((pages == 0 || free_pages) && (room == 0 || (positions && slots)), "paged_step: null pointer");
   if (!ws || ws_bytes < qtts::kCounterBytes)
     return qtts_set_error(QTTS_ERR_WORKSPACE, "paged_step: workspace of %lld bytes < %lld needed", (long long)ws_bytes,
                           (long long)qtts::kCounterBytes);
@@ -996,6 +997,7 @@ int qtts_paged_step(const int32_t* added, int64_t requests, const int32_t* lengt
   a.pages = (int32_t)pages;
   a.page_shift = page_shift_of(page_size);
   a.rows = (int32_t)rows;
+  a.room = (int32_t)room;
   a.max_new = (int32_t)std::min<int64_t>(max_new, rows);
   return qtts_launch_paged_step(a, (hipStream_t)stream);
 }
@@ -1022,6 +1024,7 @@ int qtts_qkv_to_cache(const void* qkv, int dtype, int64_t rows, int64_t ldqkv, i
   QTTS_REQUIRE(rows >= 0 && rope_rows >= 0, "qkv_to_cache: negative size");
   QTTS_REQUIRE(rows < (1ll << 24) && rope_rows < (1ll << 31), "qkv_to_cache: size too large");
   QTTS_REQUIRE(ldqkv >= width, "qkv_to_cache: leading dimension smaller than the row");
+  QTTS_REQUIRE(ldqkv < (1ll << 36), "qkv_to_cache: size too large");
   QTTS_REQUIRE((cos == nullptr) == (sin == nullptr) && (!cos || rope_rows > 0), "qkv_to_cache: half a rotation table");
   if (rows == 0) return QTTS_OK;
   QTTS_REQUIRE(qkv && slots && q && (!cos || positions), "qkv_to_cache: null pointer");
@@ -1061,6 +1064,7 @@ int qtts_paged_attention(const void* q, int dtype, int64_t rows, int64_t ldq, in
   QTTS_REQUIRE(rows >= 0 && min_new >= 0 && max_new >= 0 && window >= 0 && sinks >= 0, "paged_attention: negative size");
   QTTS_REQUIRE(rows < (1ll << 24), "paged_attention: size too large");
   QTTS_REQUIRE(ldq >= heads * d && ldo >= heads * d, "paged_attention: leading dimension smaller than the row");
+  QTTS_REQUIRE(ldq < (1ll << 36) && ldo < (1ll << 36), "paged_attention: size too large");
   QTTS_REQUIRE(scale > 0 && scale <= 3.402823466e38f, "paged_attention: scale %g is not positive", (double)scale);
   QTTS_REQUIRE(ws_bytes >= 0, "paged_attention: negative workspace size");
   if (rows == 0) return QTTS_OK;

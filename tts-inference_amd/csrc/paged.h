@@ -32,7 +32,7 @@ struct PagedStepArgs {
   int32_t* positions;    // [rows]
   int32_t* slots;
   uint32_t* ticket;  // a zero counter, left at zero; used by grids of several workgroups
-  int32_t requests, cols, pages, page_shift, rows, max_new;
+  int32_t requests, cols, pages, page_shift, rows, room, max_new;
 };
 
 struct QkvCacheArgs {

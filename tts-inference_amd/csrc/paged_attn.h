@@ -150,7 +150,7 @@ template <typename T> __device__ __forceinline__ void fill_rows(const PagedLaunc
   }
   for (int r = g; r < a.requests; r += p.fill) {
     if (a.counts[r] <= 0 || load_request(a, r).count) continue;
-    const int64_t lo = a.starts[r] > 0 ? a.starts[r] : 0, end = (int64_t)a.starts[r] + a.counts[r];
+    const int64_t lo = a.starts[r] > 0 ? a.starts[r] : 0, end = min((int64_t)a.starts[r] + a.counts[r], (int64_t)a.starts[r + 1]);
     for (int64_t row = lo; row < end && row < a.rows; ++row) {
       T* out = (T*)a.out + row * a.ldo;
       for (int i = threadIdx.x; i < vecs; i += blockDim.x) *(i32x4_t*)(out + 8 * i) = zero;

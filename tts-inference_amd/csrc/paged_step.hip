@@ -85,7 +85,7 @@ __global__ __launch_bounds__(kStepThreads) void paged_step_kernel(PagedStepArgs 
   }
   const int64_t total = block_scan(got, sums);  // of the threads up to this one; its barriers make the LDS arrays readable
 
-  for (int t = blockIdx.x * kStepRows + threadIdx.x; t < a.rows && t < (int)(blockIdx.x + 1) * kStepRows; t += blockDim.x) {
+  for (int t = blockIdx.x * kStepRows + threadIdx.x; t < a.room && t < (int)(blockIdx.x + 1) * kStepRows; t += blockDim.x) {
     int lo = 0, hi = a.requests;  // the first request that ends past t
     while (lo < hi) {
       const int mid = (lo + hi) >> 1;
@@ -93,7 +93,7 @@ __global__ __launch_bounds__(kStepThreads) void paged_step_kernel(PagedStepArgs 
       else lo = mid + 1;
     }
     int32_t position = -1, slot = -1;
-    if (lo < a.requests && base[lo] != kDenied) {
+    if (t < a.rows && lo < a.requests && base[lo] != kDenied) {
       position = length[lo] + t - (lo ? end[lo - 1] : 0);
       const int32_t column = position >> a.page_shift;
       int32_t* entry = a.table + (int64_t)lo * a.cols + column;
@@ -172,9 +172,9 @@ __global__ __launch_bounds__(kStepThreads) void paged_release_kernel(const int32
 
 int qtts_launch_paged_step(const qtts::PagedStepArgs& a, hipStream_t st) {
   using namespace qtts;
-  const int groups = a.rows > kStepRows ? (a.rows + kStepRows - 1) / kStepRows : 1;
+  const int groups = a.room > kStepRows ? (a.room + kStepRows - 1) / kStepRows : 1;
   // one wave is enough for the prefix sums of 64 requests and as many rows; 16 waves' barriers are not
-  const int most = a.rows > a.requests ? a.rows : a.requests;
+  const int most = a.room > a.requests ? a.room : a.requests;
   const int threads = most <= 64 ? 64 : most <= 256 ? 256 : kStepThreads;
   launch(paged_step_kernel, dim3(groups), dim3(threads), (uint32_t)(16 * a.requests), st, a);
   return qtts_check_launch("paged_step");

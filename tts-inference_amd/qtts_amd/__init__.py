@@ -10,6 +10,7 @@ from .config import QuantConfig
 from .layers.linear import LinearBase, MergedLinear, iter_linears
 from .quant import apply_quantization, build_method, fp8_supported, quantize_module
 from .layers.adapters import AdapterRouting, attach_adapters  # after quant, which the layers' modules import
+from .layers.attention import PagedCache, attend
 
 __all__ = ["ops", "torch_ops", "QuantConfig", "LinearBase", "MergedLinear", "iter_linears", "apply_quantization",
-           "build_method", "fp8_supported", "quantize_module", "AdapterRouting", "attach_adapters"]
+           "build_method", "fp8_supported", "quantize_module", "AdapterRouting", "attach_adapters", "PagedCache", "attend"]

@@ -70,6 +70,8 @@ STRIP_INT8, STRIP_FP8 = 0, 1
 CODE_INT8, CODE_E4M3 = 0, 1
 #: the largest rank and partition count of qtts_lora_add
 LORA_MAX_RANK, LORA_MAX_PARTS = 128, 8
+#: the most requests of a paged cache
+PAGED_MAX_REQUESTS = 2048
 
 EXPORTS = (
     "qtts_abi_version",
@@ -217,7 +219,7 @@ def load() -> ctypes.CDLL:
             add.restype = i32
             add.argtypes = [p, i32, i64, i64, i64, p, p, i64, p, p, i64, p, p, p, i64, p, i64, p, i64, i64, p, i64, p]
         L.qtts_paged_step.restype = i32
-        L.qtts_paged_step.argtypes = [p, i64, p, p, i64, p, i64, p, i64, i64, i64, p, p, p, p, p, p, p, i64, p]
+        L.qtts_paged_step.argtypes = [p, i64, p, p, i64, p, i64, p, i64, i64, i64, i64, p, p, p, p, p, p, p, i64, p]
         L.qtts_paged_release.restype = i32
         L.qtts_paged_release.argtypes = [p, i64, p, p, i64, p, i64, p, i64, p]
         L.qtts_qkv_to_cache.restype = i32

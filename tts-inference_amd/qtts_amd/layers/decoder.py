@@ -22,6 +22,9 @@ normalizes the sum and quantizes the result::
     qkv, hidden = add_norm_linear(layer.input_layernorm, attn.qkv_proj, delta, hidden)
     ...attention...
     delta, hidden = add_norm_mlp(layer.post_attention_layernorm, layer.mlp, attn.o_proj(out), hidden)
+
+``...attention...`` is ``out = attend(attn, qkv, cache, layer_index)`` over a :class:`~.attention.PagedCache`; :func:`paged_layer`
+and :func:`paged_layer_w8a8` are a whole layer with it.
 """
 
 from __future__ import annotations
@@ -33,6 +36,7 @@ from torch import nn
 from .. import ops, torch_ops  # noqa: F401  (torch_ops registers torch.ops.qtts)
 from ..quant.base import weight_flags
 from .adapters import AdapterMethod
+from .attention import PagedCache, attend
 from .norm import is_rms_norm, norm_eps
 
 
@@ -164,3 +168,19 @@ def add_norm_mlp(norm: nn.Module, mlp: nn.Module, x: torch.Tensor, residual: tor
             return y, hidden
     hidden = x if residual is None else residual + x
     return mlp(norm(hidden)), hidden
+
+
+def paged_layer(layer: nn.Module, hidden: torch.Tensor, cache: PagedCache, index: int, window: int = 0, sinks: int = 0) -> torch.Tensor:
+    """One decoder layer (talker.py:246-271) of the cache's step: ``layer.input_layernorm``, ``layer.attn`` (qkv_proj, q_norm, k_norm,
+    o_proj), ``layer.post_attention_layernorm`` and ``layer.mlp``, with the neighbours inside int8 weight-only linears."""
+    attn = layer.attn
+    out = attend(attn, norm_linear(layer.input_layernorm, attn.qkv_proj, hidden), cache, index, window, sinks)
+    return norm_mlp_residual(layer.post_attention_layernorm, layer.mlp, linear_residual(attn.o_proj, out, hidden))
+
+
+def paged_layer_w8a8(layer: nn.Module, delta: torch.Tensor, hidden: torch.Tensor | None, cache: PagedCache, index: int, window: int = 0,
+                     sinks: int = 0):
+    """The same as ``(delta, hidden)`` for W8A8 linears, the residual beside the hidden state as in :func:`add_norm_linear`."""
+    attn = layer.attn
+    qkv, hidden = add_norm_linear(layer.input_layernorm, attn.qkv_proj, delta, hidden)
+    return add_norm_mlp(layer.post_attention_layernorm, layer.mlp, attn.o_proj(attend(attn, qkv, cache, index, window, sinks)), hidden)

@@ -16,7 +16,7 @@ import torch
 
 from . import _lib
 from ._lib import (ALGO_AUTO, ALGO_SKINNY_HALF, ALGO_SKINNY_QUARTER, ALGO_STREAM, DIV_DEVICE, DIV_IEEE,  # noqa: F401
-                   LORA_MAX_PARTS, LORA_MAX_RANK, OP_FP8_LINEAR, OP_FP8W, OP_INT8_LINEAR, OP_LORA, OP_PAGED_ATTENTION, OP_W8A16, OP_W8A16_FUSED, OP_W8A16_SILU, OP_W8A8_FP8, OP_W8A8_INT8, PRO_NONE,
+                   LORA_MAX_PARTS, LORA_MAX_RANK, PAGED_MAX_REQUESTS, OP_FP8_LINEAR, OP_FP8W, OP_INT8_LINEAR, OP_LORA, OP_PAGED_ATTENTION, OP_W8A16, OP_W8A16_FUSED, OP_W8A16_SILU, OP_W8A8_FP8, OP_W8A8_INT8, PRO_NONE,
                    PRO_RMS_NORM, PRO_SILU_MUL, STRIP_FP8, STRIP_INT8, CODE_E4M3, CODE_INT8, TILE_READ_AHEAD, TILE_TWO_CHUNKS, algo_code,
                    tile_shape)
 
@@ -1057,33 +1057,50 @@ class PagedBatch:
     ``min_new`` and ``max_new`` bound the counts of every step that these tensors will hold; ``taken`` ``[1]`` is the
     free list's state after the step (None where the batch was made by hand)."""
 
-    __slots__ = ("table", "starts", "counts", "lengths", "positions", "slots", "page_size", "requests", "rows", "max_new", "min_new",
-                 "taken")
+    __slots__ = ("table", "starts", "counts", "lengths", "positions", "slots", "page_size", "requests", "cols", "rows", "max_new",
+                 "min_new", "taken")
 
     def __init__(self, table: torch.Tensor, starts: torch.Tensor, counts: torch.Tensor, lengths: torch.Tensor,
                  positions: torch.Tensor, slots: torch.Tensor, page_size: int, max_new: int | None = None, min_new: int = 0,
                  taken: torch.Tensor | None = None) -> None:
-        if table.dim() != 2:
-            raise ValueError(f"the page table must be [requests, columns], got {tuple(table.shape)}")
-        requests, rows, idx = table.shape[0], positions.shape[0], table.get_device()
-        for name, t, size in (("table", table, None), ("starts", starts, requests + 1), ("counts", counts, requests),
-                              ("lengths", lengths, requests), ("positions", positions, rows), ("slots", slots, rows),
-                              ("taken", taken, 1)):
-            if t is None:
-                continue
-            if t.dtype != torch.int32 or not t.is_contiguous() or (size is not None and t.shape != (size,)):
-                raise ValueError(f"{name} must be contiguous int32{'' if size is None else f' [{size}]'}, got {t.dtype} "
-                                 f"{tuple(t.shape)}")
-            if t.get_device() != idx:
-                raise ValueError(f"{name} is on {t.device}, the page table on {table.device}")
+        if table.dim() != 2 or table.dtype is not torch.int32 or not table.is_contiguous():
+            raise ValueError(f"the page table must be contiguous int32 [requests, columns], got {table.dtype} {tuple(table.shape)}")
+        requests, rows, idx = table.size(0), positions.numel(), table.get_device()
+        _check_int32("starts", starts, requests + 1, idx)
+        _check_int32("counts", counts, requests, idx)
+        _check_int32("lengths", lengths, requests, idx)
+        _check_int32("positions", positions, rows, idx)
+        _check_int32("slots", slots, rows, idx)
+        if taken is not None:
+            _check_int32("taken", taken, 1, idx)
         self.table, self.starts, self.counts, self.lengths, self.positions, self.slots = (table, starts, counts, lengths, positions,
                                                                                           slots)
-        self.page_size, self.requests, self.rows, self.taken = int(page_size), requests, rows, taken
+        self.page_size, self.requests, self.cols, self.rows, self.taken = int(page_size), requests, table.size(1), rows, taken
         self.max_new, self.min_new = rows if max_new is None else int(max_new), int(min_new)
 
 
+def _check_int32(name: str, t: torch.Tensor, size: int, idx: int) -> None:
+    """A contiguous 1-D int32 tensor of ``size`` entries (-1: any) on the GPU of this index."""
+    if t.dtype is not torch.int32 or not t.is_contiguous() or t.dim() != 1 or (size >= 0 and t.numel() != size):
+        raise ValueError(f"{name} must be contiguous int32{'' if size < 0 else f' [{size}]'}, got {t.dtype} {tuple(t.shape)}")
+    if t.get_device() != idx:
+        raise ValueError(f"{name} is on {t.device}, the page table on another device")
+
+
+def _check_state(table: torch.Tensor, lengths: torch.Tensor, free: torch.Tensor, taken: torch.Tensor) -> int:
+    """The GPU of a cache's state."""
+    if table.dim() != 2 or table.dtype is not torch.int32 or not table.is_contiguous():
+        raise ValueError(f"the page table must be contiguous int32 [requests, columns], got {table.dtype} {tuple(table.shape)}")
+    idx = _gpu_index(table)
+    _check_int32("lengths", lengths, table.size(0), idx)
+    _check_int32("free", free, -1, idx)
+    _check_int32("taken", taken, 1, idx)
+    return idx
+
+
 def paged_step(new: torch.Tensor, lengths: torch.Tensor, table: torch.Tensor, free: torch.Tensor, taken: torch.Tensor,
-               page_size: int, rows: int, max_new: int | None = None, min_new: int = 0, out: PagedBatch | None = None) -> PagedBatch:
+               page_size: int, rows: int, max_new: int | None = None, min_new: int = 0, out: PagedBatch | None = None,
+               room: int | None = None) -> PagedBatch:
     """The page tables, positions and cache slots of a step's new tokens, from the requests' lengths, in one kernel.
 
     new ``[R]`` tokens join the requests that hold ``lengths`` ``[R]``; their rows lie one request behind the other in a batch of
@@ -1091,21 +1108,17 @@ def paged_step(new: torch.Tensor, lengths: torch.Tensor, table: torch.Tensor, fr
     Everything is int32 on the GPU, so a captured step follows what the tensors hold at each replay.  A request whose rows
     pass ``max_new`` (None: ``rows``) or the batch, whose tokens pass the table or whose pages are not left is denied as a whole:
     ``counts`` 0, its rows at position and slot -1.  Returns a batch of fresh tensors on the same table, or ``out`` (of the
-    same sizes; its lengths and taken may be the ones given)."""
-    if table.dim() != 2:
-        raise ValueError(f"the page table must be [requests, columns], got {tuple(table.shape)}")
-    requests, cols = table.shape
+    same sizes; its lengths and taken may be the ones given).  room: entries that lie behind ``out``'s positions and slots in
+    their buffers, rows among them; those past the batch get -1 (a step captured with more rows reads them)."""
     rows = int(rows)
-    for name, t, size in (("new", new, requests), ("lengths", lengths, requests), ("free", free, None), ("taken", taken, 1),
-                          ("table", table, None)):
-        if t.dtype != torch.int32 or not t.is_contiguous() or (name != "table" and (t.dim() != 1 or size not in (None, t.shape[0]))):
-            raise ValueError(f"{name} must be contiguous int32{'' if size is None else f' [{size}]'}, got {t.dtype} {tuple(t.shape)}")
     if rows < 0:
         raise ValueError(f"a batch of {rows} rows")
-    idx = _gpu_index(table, new, lengths, free, taken)
+    idx = _check_state(table, lengths, free, taken)
+    requests = table.size(0)
+    _check_int32("new", new, requests, idx)
     if idx != _current_device():
         with torch.cuda.device(idx):
-            return paged_step(new, lengths, table, free, taken, page_size, rows, max_new, min_new, out)
+            return paged_step(new, lengths, table, free, taken, page_size, rows, max_new, min_new, out, room)
     if out is None:
         starts, counts, after, left, positions, slots = torch.empty(
             3 * requests + 2 + 2 * rows, dtype=torch.int32, device=table.device).split(
@@ -1114,14 +1127,21 @@ def paged_step(new: torch.Tensor, lengths: torch.Tensor, table: torch.Tensor, fr
     elif (out.requests != requests or out.rows != rows or out.page_size != page_size or out.taken is None
           or out.table.data_ptr() != table.data_ptr()):
         raise ValueError(f"out is no batch of {rows} rows and {requests} requests on this page table")
+    room, positions, slots = rows if room is None else int(room), out.positions.data_ptr(), out.slots.data_ptr()
+    if room > rows:
+        for t in (out.positions, out.slots):
+            if t.storage_offset() + room > t.untyped_storage().nbytes() // 4:
+                raise ValueError(f"out has no room for {room} rows")
+        # (a tensor of no rows has no address of its own)
+        positions, slots = (t.untyped_storage().data_ptr() + 4 * t.storage_offset() for t in (out.positions, out.slots))
     ws = _workspaces.get(idx)
     if ws is None:
         _ensure_workspace(table.device, 1, "paged_step")
         ws = _workspaces[idx]
     st = _lib.load().qtts_paged_step(
-        new.data_ptr(), requests, lengths.data_ptr(), table.data_ptr(), cols, free.data_ptr(), free.shape[0], taken.data_ptr(),
-        page_size, rows, out.max_new, out.starts.data_ptr(), out.counts.data_ptr(), out.lengths.data_ptr(), out.taken.data_ptr(),
-        out.positions.data_ptr(), out.slots.data_ptr(), ws.data_ptr(), ws.numel(), _raw_stream(idx))
+        new.data_ptr(), requests, lengths.data_ptr(), table.data_ptr(), out.cols, free.data_ptr(), free.numel(), taken.data_ptr(),
+        page_size, rows, room, out.max_new, out.starts.data_ptr(), out.counts.data_ptr(), out.lengths.data_ptr(), out.taken.data_ptr(),
+        positions, slots, ws.data_ptr(), ws.numel(), _raw_stream(idx))
     if st:
         _lib.check(st, "paged_step")
     return out
@@ -1130,36 +1150,35 @@ def paged_step(new: torch.Tensor, lengths: torch.Tensor, table: torch.Tensor, fr
 def paged_release(which: torch.Tensor, lengths: torch.Tensor, table: torch.Tensor, free: torch.Tensor, taken: torch.Tensor,
                   page_size: int) -> None:
     """The pages of the requests with a nonzero ``which`` ``[R]`` back to the free list; their lengths are 0 afterwards."""
-    if table.dim() != 2:
-        raise ValueError(f"the page table must be [requests, columns], got {tuple(table.shape)}")
-    requests, cols = table.shape
-    for name, t, size in (("which", which, requests), ("lengths", lengths, requests), ("free", free, None), ("taken", taken, 1),
-                          ("table", table, None)):
-        if t.dtype != torch.int32 or not t.is_contiguous() or (name != "table" and (t.dim() != 1 or size not in (None, t.shape[0]))):
-            raise ValueError(f"{name} must be contiguous int32{'' if size is None else f' [{size}]'}, got {t.dtype} {tuple(t.shape)}")
-    idx = _gpu_index(table, which, lengths, free, taken)
+    idx = _check_state(table, lengths, free, taken)
+    _check_int32("which", which, table.size(0), idx)
     if idx != _current_device():
         with torch.cuda.device(idx):
             return paged_release(which, lengths, table, free, taken, page_size)
+    requests, cols = table.shape
     st = _lib.load().qtts_paged_release(which.data_ptr(), requests, lengths.data_ptr(), table.data_ptr(), cols, free.data_ptr(),
-                                        free.shape[0], taken.data_ptr(), page_size, _raw_stream(idx))
+                                        free.numel(), taken.data_ptr(), page_size, _raw_stream(idx))
     if st:
         _lib.check(st, "paged_release")
 
 
+@functools.lru_cache(maxsize=1024)
+def _cache_shape(k: torch.Size, v: torch.Size, page_size: int) -> tuple[int, int, int]:
+    """Pages, key-value heads and head size of a cache of these shapes."""
+    if len(k) != 4 or len(v) != 4 or k[2] != page_size or v != (k[0], k[1], k[3], k[2]):
+        raise ValueError(f"k and v must be [pages, kv heads, page size, head size] and [pages, kv heads, head size, page size] with "
+                         f"pages of {page_size} tokens, got {tuple(k)} and {tuple(v)}")
+    return k[0], k[1], k[3]
+
+
 def _cache_sizes(k: torch.Tensor, v: torch.Tensor, batch: PagedBatch, dtype: torch.dtype) -> tuple[int, int, int]:
     """Pages, key-value heads and head size of a cache that fits the batch."""
-    if k.dim() != 4 or v.dim() != 4:
-        raise ValueError(f"k and v must be [pages, kv heads, page size, head size] and [pages, kv heads, head size, page size], got "
-                         f"{tuple(k.shape)} and {tuple(v.shape)}")
-    pages, kv_heads, page_size, d = k.shape
-    if v.shape != (pages, kv_heads, d, page_size) or page_size != batch.page_size:
-        raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} are no cache of pages of {batch.page_size} tokens")
-    if k.dtype != dtype or v.dtype != dtype:
+    sizes = _cache_shape(k.shape, v.shape, batch.page_size)
+    if k.dtype is not dtype or v.dtype is not dtype:
         raise ValueError(f"the cache holds {k.dtype} and {v.dtype}, the rows are {dtype}")
     if not k.is_contiguous() or not v.is_contiguous():
         raise ValueError("k and v must be contiguous")
-    return pages, kv_heads, d
+    return sizes
 
 
 def _aligned_rows(x: torch.Tensor) -> torch.Tensor:
@@ -1167,6 +1186,17 @@ def _aligned_rows(x: torch.Tensor) -> torch.Tensor:
     if x.stride(1) != 1 or x.data_ptr() % 16 or (x.shape[0] > 1 and (x.stride(0) % 8 or x.stride(0) < x.shape[1])):
         return x.clone(memory_format=torch.contiguous_format)
     return x
+
+
+def _head_norm(w: torch.Tensor | None, d: int, dtype: torch.dtype) -> torch.Tensor | None:
+    """A head's norm weight as the kernel reads it."""
+    if w is None:
+        return None
+    if w.dim() != 1 or w.numel() != d:
+        raise ValueError(f"norm weight {tuple(w.shape)} for heads of {d}")
+    if w.dtype is not dtype or not w.is_contiguous() or w.data_ptr() % 16:
+        w = w.to(dtype).clone(memory_format=torch.contiguous_format)
+    return w
 
 
 def qkv_to_cache(qkv: torch.Tensor, k: torch.Tensor, v: torch.Tensor, batch: PagedBatch, heads: int,
@@ -1185,23 +1215,17 @@ def qkv_to_cache(qkv: torch.Tensor, k: torch.Tensor, v: torch.Tensor, batch: Pag
     rows = x.shape[0]
     if rows != batch.rows or x.shape[1] != (heads + 2 * kv_heads) * d:
         raise ValueError(f"qkv is {tuple(qkv.shape)} for {batch.rows} rows of {heads} + 2 x {kv_heads} heads of {d}")
-    cos, sin = rope if rope is not None else (None, None)
+    cos = sin = None
     if rope is not None:
-        need = batch.table.shape[1] * batch.page_size
-        for t in (cos, sin):
-            if t.dtype != torch.float32 or not t.is_contiguous() or t.dim() != 2 or t.shape[1] != d // 2 or t.shape[0] < need:
-                raise ValueError(f"rope must hold contiguous fp32 [{need} or more, {d // 2}] tables, got {t.dtype} {tuple(t.shape)}")
-        if cos.shape != sin.shape:
-            raise ValueError(f"rope's tables differ: {tuple(cos.shape)} and {tuple(sin.shape)}")
-    norms = []
-    for w in (q_norm, k_norm):
-        if w is not None:
-            if w.shape != (d,):
-                raise ValueError(f"norm weight {tuple(w.shape)} for heads of {d}")
-            w = w.to(dtype).contiguous()
-            w = w.clone() if w.data_ptr() % 16 else w
-        norms.append(w)
-    idx = _gpu_index(x, k, v, batch.table, cos, sin, *norms)
+        cos, sin = rope
+        need = batch.cols * batch.page_size
+        for t in rope:
+            if (t.dtype is not torch.float32 or not t.is_contiguous() or t.dim() != 2 or t.size(1) != d // 2 or t.size(0) < need
+                    or t.size(0) != cos.size(0) or t.data_ptr() % 16):
+                raise ValueError(f"rope must hold two contiguous fp32 [{need} or more, {d // 2}] tables on 16 bytes, got {t.dtype} "
+                                 f"{tuple(t.shape)}")
+    q_norm, k_norm = _head_norm(q_norm, d, dtype), _head_norm(k_norm, d, dtype)
+    idx = _gpu_index(x, k, v, batch.table, cos, sin, q_norm, k_norm)
     if idx != _current_device():
         with torch.cuda.device(idx):
             return qkv_to_cache(qkv, k, v, batch, heads, q_norm, k_norm, eps, rope)
@@ -1209,7 +1233,7 @@ def qkv_to_cache(qkv: torch.Tensor, k: torch.Tensor, v: torch.Tensor, batch: Pag
     q = torch.empty(rows, heads, d, dtype=dtype, device=x.device)
     st = _lib.load().qtts_qkv_to_cache(
         x.data_ptr(), dtype_code(dtype), rows, x.stride(0) if rows > 1 else x.shape[1], heads, kv_heads, d, batch.positions.data_ptr(),
-        batch.slots.data_ptr(), _ptr(norms[0]), _ptr(norms[1]), eps, _ptr(cos), _ptr(sin), 0 if cos is None else cos.shape[0],
+        batch.slots.data_ptr(), _ptr(q_norm), _ptr(k_norm), eps, _ptr(cos), _ptr(sin), 0 if cos is None else cos.shape[0],
         k.data_ptr(), v.data_ptr(), pages, batch.page_size, q.data_ptr(), _raw_stream(idx))
     if st:
         _lib.check(st, "qkv_to_cache")
@@ -1255,7 +1279,7 @@ def paged_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, batch: Pa
         ws = _workspaces[idx]
     st = _lib.load().qtts_paged_attention(
         q.data_ptr(), dtype_code(q.dtype), rows, q.stride(0) if rows > 1 else heads * d, heads, kv_heads, d, k.data_ptr(), v.data_ptr(),
-        pages, batch.page_size, batch.table.data_ptr(), batch.requests, batch.table.shape[1], batch.starts.data_ptr(),
+        pages, batch.page_size, batch.table.data_ptr(), batch.requests, batch.cols, batch.starts.data_ptr(),
         batch.counts.data_ptr(), batch.lengths.data_ptr(), batch.slots.data_ptr(), batch.min_new, batch.max_new, window, sinks,
         d ** -0.5 if scale is None else scale, out.data_ptr(), heads * d, ws.data_ptr(), ws.numel(), _raw_stream(idx))
     if st:

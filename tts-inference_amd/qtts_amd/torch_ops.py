@@ -271,8 +271,38 @@ def _(base, x, index, plan, slots, a, b, scaling, ranks, partitions):
     return base.new_empty(base.shape)
 
 
+# ---- attention over a paged cache (layers/attention.py) ---------------------------------------
+
+def _batch(state: list[torch.Tensor], bounds: list[int]) -> "ops.PagedBatch":
+    """A step's batch from its tensors (table, starts, counts, lengths, positions, slots) and page size, max_new and min_new."""
+    return ops.PagedBatch(*state, bounds[0], max_new=bounds[1], min_new=bounds[2])
+
+
+@torch.library.custom_op(f"{_LIB}::qkv_to_cache", mutates_args=("k", "v"))
+def qkv_to_cache(qkv: torch.Tensor, k: torch.Tensor, v: torch.Tensor, state: list[torch.Tensor], bounds: list[int], heads: int,
+                 q_norm: Optional[torch.Tensor], k_norm: Optional[torch.Tensor], eps: float, cos: Optional[torch.Tensor],
+                 sin: Optional[torch.Tensor]) -> torch.Tensor:
+    return ops.qkv_to_cache(qkv, k, v, _batch(state, bounds), heads, q_norm, k_norm, eps, None if cos is None else (cos, sin))
+
+
+@qkv_to_cache.register_fake
+def _(qkv, k, v, state, bounds, heads, q_norm, k_norm, eps, cos, sin):
+    return qkv.new_empty((state[4].shape[0], heads, k.shape[3]))
+
+
+@torch.library.custom_op(f"{_LIB}::paged_attention", mutates_args=())
+def paged_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, state: list[torch.Tensor], bounds: list[int], window: int,
+                    sinks: int, scale: float) -> torch.Tensor:
+    return ops.paged_attention(q, k, v, _batch(state, bounds), window, sinks, scale)
+
+
+@paged_attention.register_fake
+def _(q, k, v, state, bounds, window, sinks, scale):
+    return q.new_empty(q.shape)
+
+
 #: Every op this module registers, by name (``torch.ops.qtts.<name>``).
 OPS = ("w8a16_gemm", "w8a16_gemm_strips", "fp8_linear", "fp8_linear_strips", "int8_linear", "int8_linear_strips",
        "fp8w_gemm_strips", "dequant_linear", "rms_norm", "silu_mul", "w8a16_silu_mul_gemm_strips",
        "w8a16_fused_gemm_strips", "w8a16_gate_up_silu_strips", "w8a8_fp8_gemm_strips", "w8a8_int8_gemm_strips",
-       "rms_norm_quant", "silu_mul_quant", "lora_add")
+       "rms_norm_quant", "silu_mul_quant", "lora_add", "qkv_to_cache", "paged_attention")
