@@ -114,41 +114,38 @@ template <typename T, int DP, bool EXACT, bool WIDE> __global__ __launch_bounds_
     }
     __syncthreads();
   }
-  auto piece_of = [&](int unit) { return place<DP * 2>(unit / (DP / 8), unit % (DP / 8)); };
-  uint32_t k_at[KI], v_at[KI];  // bytes from the tile's key 0 (k) and from its page's column (v), where pages are wide
+  // Load n of this wave: units of 16 bytes (wave KI + n) 64 + lane, of keys' rows and of values' dimensions.  Its keys are of one
+  // page of 16 tokens or more; its values' keys are this lane's piece of n's parity.
+  auto unit_of = [&](int n) { return (wave * KI + n) * 64 + lane; };
+  auto piece_of = [&](int n) { return place<DP * 2>(unit_of(n) / (DP / 8), unit_of(n) % (DP / 8)); };
+  uint32_t k_at[KI], v_at[KI];  // bytes from the tile's place on its page, or from a load's page where pages are narrow
 #pragma unroll
   for (int n = 0; n < KI; ++n) {
-    const int unit = (wave * KI + n) * 64 + lane;
-    k_at[n] = (uint32_t)(key_of_row(unit / (DP / 8)) * d + piece_of(unit) * 8) * 2;
-    const int dim = unit / 8, run = place<128>(dim, unit % 8);
-    v_at[n] = ((uint32_t)min(dim, d - 1) << (shift + 1)) + run * 16;
+    const int key = key_of_row(unit_of(n) / (DP / 8)), dim = unit_of(n) / 8, run = place<128>(dim, unit_of(n) % 8);
+    k_at[n] = (uint32_t)((WIDE ? key : key & mask) * d + piece_of(n) * 8) * 2;
+    v_at[n] = ((uint32_t)min(dim, d - 1) << (shift + 1)) + (WIDE ? run * 8 : (run * 8) & mask) * 2;
   }
   auto stage = [&](int base, int32_t page, int buffer) {
     uint8_t *kb = keys[buffer] + wave * KI * 1024, *vb = values[buffer] + wave * KI * 1024;
+    auto load_k = [&](const uint8_t* k, int n) {
+      if (EXACT || piece_of(n) * 8 < d) load_to_lds16(k + k_at[n], kb + n * 1024);
+    };
     if constexpr (WIDE) {
       const int64_t at = head_of(__builtin_amdgcn_readfirstlane(page));
       const uint8_t *k = cache_k + at + (int64_t)(base & mask) * d * 2, *v = cache_v + at + (base & mask) * 2;
 #pragma unroll
-      for (int n = 0; n < KI; ++n)
-        if (EXACT || piece_of((wave * KI + n) * 64 + lane) * 8 < d) load_to_lds16(k + k_at[n], kb + n * 1024);
+      for (int n = 0; n < KI; ++n) load_k(k, n);
 #pragma unroll
       for (int n = 0; n < KI; ++n) load_to_lds16(v + v_at[n], vb + n * 1024);
     } else {
-      constexpr int UNROLL = DP == 256 ? 1 : KI;  // 16 addresses at once are more than there are registers
-#pragma unroll UNROLL
-      for (int n = 0; n < KI; ++n) {
-        const int unit = (wave * KI + n) * 64 + lane;
-        const int piece = piece_of(unit), key = key_of_row(unit / (DP / 8));
-        const int64_t at = head_of(__shfl(page, key, 64)) + ((int64_t)(min(base + key, last) & mask) * d + piece * 8) * 2;
-        if (EXACT || piece * 8 < d) load_to_lds16(cache_k + at, kb + n * 1024);
-      }
-#pragma unroll UNROLL
-      for (int n = 0; n < KI; ++n) {
-        const int unit = (wave * KI + n) * 64 + lane;
-        const int dim = unit / 8, key = place<128>(dim, unit % 8) * 8;
-        load_to_lds16(cache_v + head_of(__shfl(page, key, 64)) + ((int64_t)min(dim, d - 1) << (shift + 1)) +
-                          (min(base + key, last & ~7) & mask) * 2, vb + n * 1024);
-      }
+#pragma unroll
+      for (int n = 0; n < KI; ++n)
+        load_k(cache_k + head_of(__builtin_amdgcn_readlane(page, key_of_row((wave * KI + n) * 64 / (DP / 8)))), n);
+      const uint8_t* v[2];
+#pragma unroll
+      for (int n = 0; n < 2; ++n) v[n] = cache_v + head_of(__shfl(page, place<128>(unit_of(n) / 8, lane % 8) * 8, 64));
+#pragma unroll
+      for (int n = 0; n < KI; ++n) load_to_lds16(v[n & 1] + v_at[n], vb + n * 1024);
     }
   };
 
