@@ -508,7 +508,7 @@ int qtts_lora_add_fresh(const void* x, int x_dtype, int64_t m, int64_t k, int64_
  * is page * page_size + its place on the page.  The table, the lengths, the pages not in use
  * (free_pages[taken..pages)) live on the device and are shared by all layers, which each have a k
  * and a v of their own.  The reference keeps a fixed slice of one tensor a request instead
- * (qtts/models/talker.py:47-91).  At most 2048 requests. */
+ * (qtts/models/talker.py:47-91).  At most 2048 requests of up to 2^30 tokens, fewer than 2^31 tokens of pages. */
 
 /* What a step's new tokens need, in one launch: the rows of request r, added[r] of them (<= 0:
  * none), lie behind those of the requests before it; its new pages come off the free list in the

@@ -578,3 +578,18 @@ def test_large_scores(ops):
                 _check(ops, qq, kk, v, batch, 130, 4)
             _check(ops, q, k, v, batch, scale=2.0)
             _check(ops, q, k, v, batch, scale=1e-3)
+
+
+@DTYPES
+@pytest.mark.parametrize("count", [1, 5, 70])
+def test_unwritten_memory_of_any_bits(ops, count, dtype):
+    """What lies behind a request's tokens on its last page may hold any bits, signalling NaN among them."""
+    q, k, v, batch = _inputs(ops, [(33, count), (0, count)], 64, 8, 4, 128, dtype, seed=count)
+    want = _check(ops, q, k, v, batch, 30, 2)
+    exponent = 0x7f80 if dtype == torch.bfloat16 else 0x7c00
+    for bits in (exponent + 1, exponent + 0x8001 - 0x10000, exponent, exponent + 0x8000 - 0x10000):
+        for t in (k, v):
+            t.view(torch.int16)[t.isnan()] = bits
+        assert torch.equal(ops.paged_attention(q, k, v, batch, 30, 2), want)
+        for t in (k, v):
+            t[~t.isfinite()] = float("nan")

@@ -233,6 +233,12 @@ def test_counts_on_the_gpu(ops):
         assert int(cache.taken) == sum(-(-w // 16) for w in want)
     with pytest.raises(ValueError, match="rows must be given"):
         cache.step(new)
+    cache.release(torch.tensor([1, 900, -3, 1, 2 ** 40], device="cuda"))  # the same twice, and numbers of no request
+    want[1] = 0
+    assert cache.lengths.tolist() == want and int(cache.taken) == sum(-(-w // 16) for w in want)
+    cache.release([3, 3])
+    want[3] = 0
+    assert cache.lengths.tolist() == want
 
 
 def test_attend_with_other_norms(ops):

@@ -93,6 +93,17 @@ int main() {
     }
     if (slots > split_slots(groups) || slots * kv > split_slots(cut.groups) || items > (long long)runs + groups) abort();
   }
+  // totals past 32 bits and the largest sizes
+  for (unsigned long long total : {0ull, 1ull, 4294967295ull, 4294967296ull, 1ull << 40, 1ull << 60})
+    for (int groups : {1, 7, 512, 4096}) {
+      const unsigned long long c = (total + groups - 1) / groups, want = c < 8 ? 8 : c > 0x40000000 ? 0x40000000 : c;
+      if (tiles_a_split(total, groups, 8) != want) abort();
+    }
+  for (int tiles : {0, 1, (1 << 27) - 1})
+    for (unsigned share : {8u, 9u, 1u << 27, 0x40000000u}) {
+      const long long n = (2ll * tiles + share) / (2ll * share);
+      if (splits_of(tiles, share) != (n > 1 ? n : 1)) abort();
+    }
   printf("fine");
 }
 """) == "fine"

@@ -942,8 +942,8 @@ static int paged_sizes(const char* what, int64_t requests, int64_t cols, int64_t
                (long long)page_size);
   QTTS_REQUIRE(requests <= qtts::kPagedMaxRequests, "%s: %lld requests, at most %d", what, (long long)requests,
                qtts::kPagedMaxRequests);
-  QTTS_REQUIRE(pages < (1ll << 31) / page_size && cols < (1ll << 31) / page_size,
-               "%s: size too large (tokens of the cache or of a request past 32 bits)", what);
+  QTTS_REQUIRE(pages < (1ll << 31) / page_size && cols <= (1ll << 30) / page_size,
+               "%s: size too large (2^31 tokens of the cache or more than 2^30 of a request)", what);
   return QTTS_OK;
 }
 

@@ -78,13 +78,15 @@ constexpr QTTS_RULE PagedCut many_cut(int64_t pairs) { return PagedCut{512, 8}; 
 
 // Tiles a split, where `total` tiles (of all runs, one head) are wanted in about `groups` workgroups a head.
 QTTS_RULE uint32_t tiles_a_split(uint64_t total, int32_t groups, int32_t least) {
-  const uint64_t c = (total + groups - 1) / groups;
-  return c < (uint64_t)least ? (uint32_t)least : c > 0x40000000 ? 0x40000000u : (uint32_t)c;
+  const uint64_t most = 0x40000000, wide = total + (uint32_t)groups - 1;
+  // (a division of 64 bits is a long way on the GPU, and no total of an ordinary call needs one)
+  const uint64_t c = wide >> 32 ? wide / (uint32_t)groups : (uint32_t)wide / (uint32_t)groups;
+  return c < (uint64_t)least ? (uint32_t)least : (uint32_t)(c > most ? most : c);
 }
 // Splits of a run of up to `tiles` tiles, equal ones: tiles / share rounded to the nearest, so that a run a little longer
 // than a share stays whole.
 QTTS_RULE int32_t splits_of(int32_t tiles, uint32_t share) {
-  const int32_t n = (int32_t)(((uint64_t)2 * tiles + share) / (2 * (uint64_t)share));
+  const int32_t n = (int32_t)((2 * (uint32_t)tiles + share) / (2 * share));  // tiles < 2^27, share <= 2^30
   return n > 1 ? n : 1;
 }
 // n > 1 splits hold n - 1/2 shares or more, so that the runs that are split have at most 4/3 groups splits between them a

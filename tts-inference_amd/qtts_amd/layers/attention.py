@@ -67,7 +67,7 @@ class PagedCache:
         kw = {"dtype": torch.int32, "device": device}
         self.lengths, self.table = torch.zeros(requests, **kw), torch.zeros(requests, cols, **kw)
         self.free, self.taken = torch.arange(pages, **kw), torch.zeros(1, **kw)
-        self._new, self._which = torch.zeros(requests, **kw), torch.zeros(requests, **kw)
+        self._new, self._which, self._numbers = torch.zeros(requests, **kw), torch.zeros(requests, **kw), torch.arange(requests, **kw)
         self._starts, self._counts = torch.zeros(requests + 1, **kw), torch.zeros(requests, **kw)
         self._positions, self._slots = torch.full((self.max_rows,), -1, **kw), torch.full((self.max_rows,), -1, **kw)
         self.rope = None if rope_theta is None else rope_tables(cols * page_size, head_dim, rope_theta, device)
@@ -77,8 +77,8 @@ class PagedCache:
 
     def _whole(self, values, name: str) -> torch.Tensor:
         values = torch.as_tensor(values)
-        if values.dim() != 1 or values.shape[0] > self.requests:
-            raise ValueError(f"{name} must be 1-D with up to {self.requests} entries, got shape {tuple(values.shape)}")
+        if values.dim() != 1:
+            raise ValueError(f"{name} must be 1-D, got shape {tuple(values.shape)}")
         if values.numel() and (values.dtype == torch.bool or values.is_floating_point() or values.is_complex()):
             raise ValueError(f"{name} must hold whole numbers, got {values.dtype}")
         return values
@@ -90,6 +90,8 @@ class PagedCache:
         ``max_new`` bounds its entries (None: ``rows``), and what does not fit is denied (``batch.counts`` 0).  Requests whose pages are not left
         are denied in either case."""
         new = self._whole(new, "new")
+        if new.shape[0] > self.requests:
+            raise ValueError(f"new must have up to {self.requests} entries, got {new.shape[0]}")
         if new.device.type == "cpu":
             given = new.tolist()
             if any(n < 0 for n in given):
@@ -123,14 +125,15 @@ class PagedCache:
         return batch
 
     def release(self, requests: torch.Tensor | Sequence[int]) -> None:
-        """The requests (their numbers) hold nothing from here on; their pages are free again."""
+        """The requests (their numbers; on the GPU, others than the cache's are left aside) hold nothing from here on; their
+        pages are free again."""
         requests = self._whole(requests, "requests")
         if requests.device.type == "cpu" and any(not 0 <= r < self.requests for r in requests.tolist()):
             raise ValueError(f"requests {requests.tolist()} of {self.requests}")
         if not requests.numel():
             return
-        self._which.zero_()
-        self._which.index_fill_(0, requests.to(device=self._which.device, dtype=torch.int64), 1)
+        requests = requests.to(device=self._which.device, dtype=torch.int64)
+        self._which.copy_((self._numbers[:, None] == requests).any(1))  # (an index out of range would end the process)
         ops.paged_release(self._which, self.lengths, self.table, self.free, self.taken, self.page_size)
 
     def batch_for(self, rows: int) -> ops.PagedBatch:
