@@ -1065,7 +1065,8 @@ int qtts_paged_attention(const void* q, int dtype, int64_t rows, int64_t ldq, in
   QTTS_REQUIRE(rows < (1ll << 24), "paged_attention: size too large");
   QTTS_REQUIRE(ldq >= heads * d && ldo >= heads * d, "paged_attention: leading dimension smaller than the row");
   QTTS_REQUIRE(ldq < (1ll << 36) && ldo < (1ll << 36), "paged_attention: size too large");
-  QTTS_REQUIRE(scale > 0 && scale <= 3.402823466e38f, "paged_attention: scale %g is not positive", (double)scale);
+  // (up to where the scale of exponentials of 2 is finite)
+  QTTS_REQUIRE(scale > 0 && scale <= 2e38f, "paged_attention: scale %g is not in (0, 2e38]", (double)scale);
   QTTS_REQUIRE(ws_bytes >= 0, "paged_attention: negative workspace size");
   if (rows == 0) return QTTS_OK;
   QTTS_REQUIRE(q && out && slots && (requests == 0 || (starts && counts && lengths && (cols == 0 || table))),

@@ -5,6 +5,10 @@
 // (x_i, x_{i + d/2}) <- (x_i cos_i - x_{i + d/2} sin_i, x_{i + d/2} cos_i + x_i sin_i).  A group of lanes takes a head of
 // a row, each lane 8 columns of either half (16-byte loads), so that a rotation's pair is in one lane and the norm's sum
 // is a few lane exchanges; workgroups of their own take the values.
+//
+// Memory bounds many rows: 2048 rows of 16 + 2 x 8 heads of 128 (34 MB in and out) take 9.1 us captured, 3.7 TB/s, of which
+// 2.5 are an empty launch; the norm and the rotation hide behind the loads.  With values written as they come, 2 bytes a
+// dimension into lines of other rows, it took 17.6.  One row is latency: 3.0 us.
 #include "common.h"
 #include "paged.h"
 
