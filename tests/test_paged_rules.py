@@ -86,7 +86,10 @@ int main() {
     const unsigned share = tiles_a_split(total, groups, cut.least);
     long long slots = 0, items = 0;
     for (int r = 0; r < runs; ++r) {
-      const int tiles = 1 + rnd(longest), n = splits_of(tiles, share), chunk = (tiles + n - 1) / n;
+      const int tiles = 1 + rnd(longest);
+      const unsigned mine = joined_share(tiles, share, many ? 1.0f : (1 + r * 97 % 4096) * kPartCost);
+      const int n = splits_of(tiles, mine), chunk = (tiles + n - 1) / n;
+      if (mine < share) abort();
       if ((tiles + chunk - 1) / chunk > n || n > splits_of(longest, cut.least)) abort();
       items += n;
       if (n > 1) slots += n;
@@ -250,7 +253,7 @@ def test_attention_entry():
     _refused(call(ldq=63), "leading dimension")
     _refused(call(ldo=56), "leading dimension")
     _refused(call(ldo=1 << 40), "too large")
-    for scale in (0.0, -1.0, float("nan"), float("inf")):
+    for scale in (0.0, -1.0, float("nan"), float("inf"), 3e38):
         _refused(call(scale=scale), "scale")
     for null in ("q", "out", "slots", "table", "starts", "counts", "lengths", "k", "v"):
         _refused(call(**{null: None}), "null pointer")

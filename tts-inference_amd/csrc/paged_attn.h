@@ -89,7 +89,8 @@ __device__ __forceinline__ bool paged_work(const PagedLaunch& p, int item, Paged
   const uint32_t share = groups ? tiles_a_split(wave_sum64(total), groups, cut.least) : 0;
   auto items_of = [&](const PagedRequest& r, int32_t& tiles, int32_t& splits) -> int32_t {
     const int32_t runs = runs_of(r, tiles);
-    splits = groups ? splits_of(tiles, share) : 1;
+    const float part = RUN == 16 ? (float)(r.count * group * a.cache.d) * kPartCost : 1.0f;
+    splits = groups ? splits_of(tiles, joined_share(tiles, share, part)) : 1;
     return runs * splits;
   };
   int32_t items = 0, slots = 0;

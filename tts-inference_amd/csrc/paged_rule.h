@@ -73,8 +73,10 @@ constexpr int32_t kCutGroups = 4096;  // at most
 constexpr QTTS_RULE PagedCut small_cut(int64_t pairs) {
   return pairs < 128 ? PagedCut{512, 8} : pairs < 256 ? PagedCut{512, 16} : PagedCut{kCutGroups, 16};
 }
-// Runs of up to 128 rows (tiles of 64 keys).
-constexpr QTTS_RULE PagedCut many_cut(int64_t pairs) { return PagedCut{512, 8}; }
+// Runs of up to 128 rows (tiles of 64 keys, two workgroups a compute unit): one round of them (512 rows behind 30000 tokens:
+// 132 us captured, in 256 workgroups 170, in 1024 172; 4 x 1003 behind 2500: 100, 100, 113), and whole runs sooner where each
+// unit has one (8 x 300 behind 1000 under a window of 512: 26.9, with 8 tiles as the least 31.4; 1 x 1000: 22.1, with 16: 27.0).
+constexpr QTTS_RULE PagedCut many_cut(int64_t pairs) { return PagedCut{512, pairs < 256 ? 8 : 16}; }
 
 // Tiles a split, where `total` tiles (of all runs, one head) are wanted in about `groups` workgroups a head.
 QTTS_RULE uint32_t tiles_a_split(uint64_t total, int32_t groups, int32_t least) {
@@ -88,6 +90,20 @@ QTTS_RULE uint32_t tiles_a_split(uint64_t total, int32_t groups, int32_t least) 
 QTTS_RULE int32_t splits_of(int32_t tiles, uint32_t share) {
   const int32_t n = (int32_t)((2 * (uint32_t)tiles + share) / (2 * share));  // tiles < 2^27, share <= 2^30
   return n > 1 ? n : 1;
+}
+// The share of a run whose parts cost the one workgroup that joins them `part` tiles' time each: the time, share + part
+// tiles / share, is least at a share of sqrt(part tiles).
+// Up to 128 rows: a part costs what a tile does, about 1 us either (100 rows behind 20000 tokens, 314 tiles: 47 us in 17
+// parts, 58 in 9, 72 in 39).  Up to 16 rows: by the part's numbers (1 x 65536 tokens, 16 query heads of 128 on one: 36 us in 91
+// parts, 38 in 64 or 128, 64 in 256).
+constexpr float kPartCost = 1.0f / 4096;
+QTTS_RULE uint32_t joined_share(int32_t tiles, uint32_t share, float part) {
+#ifdef __HIP_DEVICE_COMPILE__
+  const uint32_t least = (uint32_t)__builtin_amdgcn_sqrtf((float)tiles * part);  // (the precise one is a long way)
+#else
+  const uint32_t least = (uint32_t)__builtin_sqrtf((float)tiles * part);
+#endif
+  return share < least ? least : share;
 }
 // n > 1 splits hold n - 1/2 shares or more, so that the runs that are split have at most 4/3 groups splits between them a
 // head: the results in parts that are ever held.
