@@ -15,7 +15,8 @@
 // the cycles and the vector units 41%, the softmax's 5.1e7 instructions to 8.5e6 MFMAs; LDS reads meet no bank twice
 // (0 conflicts).  Without the softmax it took 252 us, without the loads 241, without the second product 224: no one of them
 // is what is waited for, the two waves a SIMD just do not fill each other's gaps.  Operands further ahead, wave
-// priorities and loads that the compiler does not count gave nothing.  16384 tokens under a window of 1024: 177 us, 756
+// priorities and loads that the compiler does not count gave nothing; waves of 64 rows, one a SIMD, 373 us; the next tile's
+// scores beside this one's softmax in a wave spilled 63 registers (554 us).  16384 tokens under a window of 1024: 177 us, 756
 // TFLOP/s of what the rows see (every run of 64 tokens has two or three masked tiles of 18); 4 x 1003 tokens behind 2500 on
 // pages of 32: 100 us, 699.
 #include "paged_attn.h"
