@@ -408,6 +408,18 @@ def test_split_lengths(ops, held, window, sinks, heads, kv, d, page, dtype):
 
 
 @DTYPES
+@pytest.mark.parametrize("heads,kv,d,page", [(16, 8, 128, 64), (16, 8, 128, 16), (8, 8, 64, 32), (16, 1, 256, 64), (28, 4, 80, 128), (6, 2, 16, 16)])
+@pytest.mark.parametrize("requests,window,sinks", [([(9000, 20)], 0, 0), ([(20000, 100), (3, 5), (700, 40)], 0, 0), ([(6000, 30)] * 3, 3000, 4),
+                                                   ([(4095, 300), (1, 1)], 0, 0), ([(8000, 129)], 5000, 300)])
+def test_split_runs(ops, requests, window, sinks, heads, kv, d, page, dtype):
+    """Runs of many rows whose keys several workgroups share."""
+    q, k, v, batch = _inputs(ops, requests, page, heads, kv, d, dtype, seed=len(requests), padding=1)
+    first = _check(ops, q, k, v, batch, window, sinks)
+    for _ in range(2):
+        assert torch.equal(ops.paged_attention(q, k, v, batch, window, sinks), first)
+
+
+@DTYPES
 @pytest.mark.parametrize("requests,heads,kv", [([(50, 3), (0, 8), (1000, 1), (5000, 5)], 16, 8), ([(40, 4), (33, 2)], 4, 1), ([(100, 16)], 2, 2)])
 @pytest.mark.parametrize("window,sinks", [(0, 0), (20, 3)])
 def test_drafted_tokens(ops, requests, heads, kv, window, sinks, dtype):
