@@ -1,0 +1,141 @@
+"""The softmax's weights on their way through ops.paged_attention: what they keep of their bits where sums cancel, in long tails
+far below the largest weight, and at scores whose own steps pass the weights' range.
+
+Scores are exact here: a query has one nonzero entry, so a score is one product of two 16-bit numbers.  Tolerances, with
+u = 2^-24 and e = eps / 2 of the type, for out = sum w_j v_j / sum w_j and A = sum w_j |v_j| / sum w_j:
+
+* a weight's exponent is off by 4 u (|s_j| + |max|) and the exponential by 2^-22: with the largest of these, r, 2 r A;
+* a weight goes to the second product in two parts of the type, the second one the first one's error: e^2 A;
+* fp16 holds nothing under 2^-25; of a tile's keys (64, the larger of the kernels') the largest weight is 1 or more
+  before it is cut off, so that each key loses at most 2^-25 of the tile's largest weight;
+* n terms summed in fp32 in any order, and rescaled: 4 (n + 64) u A;
+* the result is rounded once: e |out|.
+"""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from test_gpu_paged import U, _batch, _inputs, _near
+from test_gpu_paged import _exact as _exact_rounded
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from qtts_amd import ops as _ops
+    assert _ops.device_supported(), "GPU is not a gfx950"
+    _ops.reserve_workspace(torch.device("cuda"), 64 << 20)
+    return _ops
+
+
+def _call(ops, keys, values, count, dtype, heads=1, kv=1, page=64, window=0, sinks=0, scale=1.0, query=1.0):
+    """One request whose key j has entry keys[j] and value values[j] ([n, d]), its last `count` tokens the rows, each of whose
+    queries has one entry.  Returns the output [count, heads, d] and the batch."""
+    n, d = values.shape
+    batch, pages = _batch(ops, [(n - count, count)], page, seed=n)
+    at = torch.arange(n, device="cuda")
+    slot = batch.table[0].long()[at // page] * page + at % page
+    k = torch.zeros(pages, kv, page, d, dtype=dtype, device="cuda")
+    v = torch.zeros(pages, kv, d, page, dtype=dtype, device="cuda")
+    k[slot // page, :, slot % page, 5] = keys.to(dtype)[:, None]
+    v[slot // page, :, :, slot % page] = values.to(dtype)[:, None]
+    q = torch.zeros(count, heads, d, dtype=dtype, device="cuda")
+    q[:, :, 5] = query
+    return ops.paged_attention(q, k, v, batch, window, sinks, scale)
+
+
+def _exact(keys, values, count, dtype, window=0, sinks=0):
+    """(result [count, d], bound without its rounding) in 64 bits, a row at a time."""
+    n = values.shape[0]
+    s, v = keys.to(dtype).double(), values.to(dtype).double()
+    key = torch.arange(n, device="cuda")
+    e = torch.finfo(dtype).eps / 2
+    out, off = [], []
+    for p in range(n - count, n):
+        seen = key <= p
+        if window:
+            seen &= (key > p - window) | (key < sinks)
+        top = s[seen].max()
+        w = torch.where(seen, (s - top).exp(), 0.0)
+        total = w.sum()
+        y, mags = w @ v / total, w @ v.abs() / total
+        rel = 4 * U * (s[seen].abs().max() + top.abs()) + 2.0 ** -22
+        bound = mags * (2 * rel + e * e + 4 * (n + 64) * U)
+        if dtype == torch.float16:
+            tail = -n % 64
+            tops = torch.nn.functional.pad(w, (0, tail)).view(-1, 64).amax(1).repeat_interleave(64)[:n]
+            bound = bound + 2.0 ** -25 * ((tops * seen) @ v.abs()) / total
+        out.append(y)
+        off.append(bound)
+    return torch.stack(out), torch.stack(off)
+
+
+def _check(ops, keys, values, count, dtype, heads=1, what="", window=0, sinks=0, **kw):
+    out = _call(ops, keys, values, count, dtype, heads, window=window, sinks=sinks, **kw)
+    want, off = _exact(keys, values, count, dtype, window, sinks)
+    _near(out, want[:, None].expand_as(out), off[:, None].expand_as(out), what)
+
+
+@DTYPES
+@pytest.mark.parametrize("held,count,heads", [(63, 1, 1), (60, 1, 16), (0, 40, 1), (20, 44, 1), (0, 24, 8), (40, 17, 2), (100, 30, 4)])
+@pytest.mark.parametrize("d", [16, 64, 128, 256])
+def test_sums_that_cancel(ops, held, count, heads, d, dtype):
+    """Values of both signs: the sum is far smaller than its terms, and no term loses what its rounding to 16 bits would take."""
+    g = torch.Generator(device="cuda").manual_seed(held + count)
+    n = held + count
+    for spread in (128, 512):  # weights down to e^-1 and e^-4, in steps of 2^-7
+        keys = -torch.randint(0, spread, (n,), generator=g, device="cuda") / 128.0
+        keys = keys.to(dtype).float()
+        values = torch.randn(n, d, generator=g, device="cuda")
+        _check(ops, keys, values, count, dtype, heads)
+        _check(ops, keys, values, count, dtype, heads, window=25, sinks=3)
+
+
+@DTYPES
+def test_a_chunk_whose_keys_are_split(ops, dtype):
+    """The same where several workgroups share the keys: the chunk's rows see few of them but the first tokens."""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    n, count = 3000, 70
+    keys = (-torch.randint(0, 128, (n,), generator=g, device="cuda") / 128.0).to(dtype).float()
+    keys[64:2900] -= 16  # (hardly any weight)
+    values = torch.randn(n, 64, generator=g, device="cuda")
+    _check(ops, keys, values, count, dtype)
+
+
+@DTYPES
+@pytest.mark.parametrize("heads,kv,d,page", [(16, 8, 128, 64), (4, 4, 64, 16), (4, 1, 256, 32), (12, 4, 80, 128)])
+@pytest.mark.parametrize("requests,window,sinks", [([(0, 37), (300, 130), (9, 1)], 0, 0), ([(40, 1), (5000, 60), (0, 200)], 0, 0),
+                                                   ([(500, 150), None, (3, 2)], 70, 4)])
+def test_weights_of_16_bits(ops, requests, window, sinks, heads, kv, d, page, dtype):
+    """Where a caller asks for them: prompts within half a step of each weight, requests of up to 16 rows as without."""
+    q, k, v, batch = _inputs(ops, requests, page, heads, kv, d, dtype, seed=d, padding=2)
+    full = ops.paged_attention(q, k, v, batch, window, sinks)
+    out = ops.paged_attention(q, k, v, batch, window, sinks, weights16=True)
+    want, off = _exact_rounded(q, k, v, batch, window, sinks, d ** -0.5)
+    _near(out, want, off, "16 bits")
+    at = 0
+    for r in requests:
+        new = 3 if r is None else r[1]
+        same = torch.equal(out[at:at + new], full[at:at + new])
+        assert same == (r is None or new * heads // kv <= 16)
+        at += new
+    assert not out[batch.slots < 0].any()
+
+
+def test_weights_of_16_bits_in_a_layer(ops):
+    """The switch's way through the cache's layer."""
+    from qtts_amd import PagedCache, attend
+    cache = PagedCache(1, 2, 8, 4, 2, 64, max_rows=64, rope_theta=1e4)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    qkv = torch.randn(50, 8 * 64, generator=g, device="cuda").to(torch.bfloat16)
+    cache.step([50])
+    attn = torch.nn.Module()
+    outs = [attend(attn, qkv, cache, 0, weights16=w) for w in (False, True, False)]
+    assert torch.equal(outs[0], outs[2]) and not torch.equal(outs[0], outs[1])
+    # half a step of each weight, and of either result
+    assert (outs[1].double() - outs[0].double()).abs().max() < 2.0 ** -6 * qkv.abs().max()

@@ -1,0 +1,58 @@
+"""Calls over a paged cache without a GPU: what the entries and the cache refuse and how they pass on what they are given."""
+
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
+
+import qtts_amd  # noqa: F401
+from qtts_amd import _lib, ops
+
+BUF = ctypes.create_string_buffer(1 << 20)
+AT = (ctypes.addressof(BUF) + 255) & ~255
+
+
+def _at(v):
+    return None if v is None else AT + v
+
+
+def _passes(status):
+    """Past every check: no device here, or the call ran nothing."""
+    assert status == 0 or (status == -2 and not torch.cuda.is_available()), _lib.last_error()
+
+
+def _i32(*shape):
+    return torch.zeros(*shape, dtype=torch.int32)
+
+
+def _attention(entry, q=0, dt=1, rows=2, ldq=64, heads=4, kv=2, d=16, k=65536, v=131072, pages=8, page=16, table=4096, requests=2, cols=3,
+               starts=5120, counts=5184, lengths=5248, slots=5312, least=1, most=1, window=0, sinks=0, scale=0.25, out=8192, ldo=64,
+               ws=262144, ws_n=1 << 62):
+    return entry(_at(q), dt, rows, ldq, heads, kv, d, _at(k), _at(v), pages, page, _at(table), requests, cols, _at(starts), _at(counts),
+                 _at(lengths), _at(slots), least, most, window, sinks, scale, _at(out), ldo, _at(ws), ws_n, None)
+
+
+def test_attention_with_weights_of_16_bits():
+    """Its entry checks what the other one checks, and the op has it as its last argument."""
+    entry = _lib.load().qtts_paged_attention_w16
+    for kw, text in (({"dt": 0}, "bf16 or fp16"), ({"rows": -1}, "negative size"), ({"heads": 5}, "query heads"), ({"ldo": 56}, "leading dimension"),
+                     ({"scale": 0.0}, "scale"), ({"out": 64}, "out overlaps q"), ({"ws": None}, "workspace"), ({"table": None}, "null pointer")):
+        status = _attention(entry, **kw)
+        assert status in (-1, -5) and text in _lib.last_error(), (kw, status, _lib.last_error())
+    assert _attention(entry, rows=0) == 0
+    if not torch.cuda.is_available():
+        _passes(_attention(entry))
+    with FakeTensorMode():
+        bf = torch.bfloat16
+        k, v = torch.empty(9, 2, 16, 32, dtype=bf, device="cuda"), torch.empty(9, 2, 32, 16, dtype=bf, device="cuda")
+        state = [torch.empty(*s, dtype=torch.int32, device="cuda") for s in ((3, 4), (4,), (3,), (3,), (5,), (5,))]
+        q = torch.empty(5, 4, 32, dtype=bf, device="cuda")
+        assert torch.ops.qtts.paged_attention(q, k, v, state, [16, 5, 0], 0, 0, 0.1, True).shape == (5, 4, 32)
+    batch = ops.PagedBatch(_i32(3, 4), _i32(4), _i32(3), _i32(3), _i32(5), _i32(5), 16)
+    bf = torch.bfloat16
+    with pytest.raises(ValueError, match="GPU tensor"):
+        ops.paged_attention(torch.zeros(5, 4, 32, dtype=bf), torch.zeros(9, 2, 16, 32, dtype=bf), torch.zeros(9, 2, 32, 16, dtype=bf), batch,
+                            weights16=True)

@@ -1052,11 +1052,11 @@ int qtts_qkv_to_cache(const void* qkv, int dtype, int64_t rows, int64_t ldqkv, i
   return qtts_launch_qkv_to_cache(a, dtype, (hipStream_t)stream);
 }
 
-int qtts_paged_attention(const void* q, int dtype, int64_t rows, int64_t ldq, int64_t heads, int64_t kv_heads, int64_t d,
-                         const void* k, const void* v, int64_t pages, int64_t page_size, const int32_t* table, int64_t requests,
-                         int64_t cols, const int32_t* starts, const int32_t* counts, const int32_t* lengths,
-                         const int32_t* slots, int64_t min_new, int64_t max_new, int64_t window, int64_t sinks, float scale,
-                         void* out, int64_t ldo, void* ws, int64_t ws_bytes, void* stream) {
+static int paged_attention(bool weights16, const void* q, int dtype, int64_t rows, int64_t ldq, int64_t heads, int64_t kv_heads,
+                           int64_t d, const void* k, const void* v, int64_t pages, int64_t page_size, const int32_t* table,
+                           int64_t requests, int64_t cols, const int32_t* starts, const int32_t* counts, const int32_t* lengths,
+                           const int32_t* slots, int64_t min_new, int64_t max_new, int64_t window, int64_t sinks, float scale,
+                           void* out, int64_t ldo, void* ws, int64_t ws_bytes, void* stream) {
   QTTS_TRY(paged_sizes("paged_attention", requests, cols, pages, page_size));
   QTTS_REQUIRE(dtype == QTTS_BF16 || dtype == QTTS_F16, "paged_attention: activations must be bf16 or fp16");
   qtts::PagedAttentionArgs a = {};
@@ -1099,7 +1099,26 @@ int qtts_paged_attention(const void* q, int dtype, int64_t rows, int64_t ldq, in
   a.window = (int32_t)std::min<int64_t>(window, INT32_MAX);
   a.sinks = (int32_t)std::min<int64_t>(sinks, INT32_MAX);
   a.scale = scale * 1.44269504088896340736f;  // exponentials of 2
+  a.weights16 = weights16;
   return qtts_launch_paged_attention(a, (int)std::min<int64_t>(min_new, rows), dtype, ws, (hipStream_t)stream);
+}
+
+int qtts_paged_attention(const void* q, int dtype, int64_t rows, int64_t ldq, int64_t heads, int64_t kv_heads, int64_t d,
+                         const void* k, const void* v, int64_t pages, int64_t page_size, const int32_t* table, int64_t requests,
+                         int64_t cols, const int32_t* starts, const int32_t* counts, const int32_t* lengths,
+                         const int32_t* slots, int64_t min_new, int64_t max_new, int64_t window, int64_t sinks, float scale,
+                         void* out, int64_t ldo, void* ws, int64_t ws_bytes, void* stream) {
+  return paged_attention(false, q, dtype, rows, ldq, heads, kv_heads, d, k, v, pages, page_size, table, requests, cols, starts, counts,
+                         lengths, slots, min_new, max_new, window, sinks, scale, out, ldo, ws, ws_bytes, stream);
+}
+
+int qtts_paged_attention_w16(const void* q, int dtype, int64_t rows, int64_t ldq, int64_t heads, int64_t kv_heads, int64_t d,
+                             const void* k, const void* v, int64_t pages, int64_t page_size, const int32_t* table, int64_t requests,
+                             int64_t cols, const int32_t* starts, const int32_t* counts, const int32_t* lengths,
+                             const int32_t* slots, int64_t min_new, int64_t max_new, int64_t window, int64_t sinks, float scale,
+                             void* out, int64_t ldo, void* ws, int64_t ws_bytes, void* stream) {
+  return paged_attention(true, q, dtype, rows, ldq, heads, kv_heads, d, k, v, pages, page_size, table, requests, cols, starts, counts,
+                         lengths, slots, min_new, max_new, window, sinks, scale, out, ldo, ws, ws_bytes, stream);
 }
 
 int qtts_kernel_timer_begin(int max_launches) {

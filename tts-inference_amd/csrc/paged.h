@@ -63,6 +63,7 @@ struct PagedAttentionArgs {
   PagedCache cache;
   int32_t rows, heads, requests, cols, max_new, window, sinks;
   float scale;  // times log2 e
+  bool weights16;  // the weights of runs of more than 16 rows in 16 bits
 };
 
 }  // namespace qtts

@@ -113,6 +113,7 @@ EXPORTS = (
     "qtts_paged_release",
     "qtts_qkv_to_cache",
     "qtts_paged_attention",
+    "qtts_paged_attention_w16",
     "qtts_kernel_timer_begin",
     "qtts_kernel_timer_end",
 )
@@ -225,9 +226,10 @@ def load() -> ctypes.CDLL:
         L.qtts_qkv_to_cache.restype = i32
         L.qtts_qkv_to_cache.argtypes = [p, i32, i64, i64, i64, i64, i64, p, p, p, p, ctypes.c_float, p, p, i64, p, p, i64, i64,
                                         p, p]
-        L.qtts_paged_attention.restype = i32
-        L.qtts_paged_attention.argtypes = [p, i32, i64, i64, i64, i64, i64, p, p, i64, i64, p, i64, i64, p, p, p, p, i64, i64,
-                                           i64, i64, ctypes.c_float, p, i64, p, i64, p]
+        for attention in (L.qtts_paged_attention, L.qtts_paged_attention_w16):
+            attention.restype = i32
+            attention.argtypes = [p, i32, i64, i64, i64, i64, i64, p, p, i64, i64, p, i64, i64, p, p, p, p, i64, i64, i64, i64,
+                                  ctypes.c_float, p, i64, p, i64, p]
         L.qtts_kernel_timer_begin.restype = i32
         L.qtts_kernel_timer_begin.argtypes = [i32]
         L.qtts_kernel_timer_end.restype = i32

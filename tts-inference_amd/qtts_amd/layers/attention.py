@@ -144,11 +144,12 @@ class PagedCache:
 
 
 def attend(attn: nn.Module, qkv: torch.Tensor, cache: PagedCache, layer: int, window: int = 0, sinks: int = 0,
-           scale: float | None = None) -> torch.Tensor:
+           scale: float | None = None, weights16: bool = False) -> torch.Tensor:
     """The attention between qkv_proj and o_proj (talker.py:249-270) for the rows of the cache's step: head norms
     (``attn.q_norm``, ``attn.k_norm``, None or missing: none), rotation, this layer's cache, attention.  qkv
     ``[..., (Hq + 2 H) D]`` is qkv_proj's output; returns ``[..., Hq D]``, o_proj's input.  Norms that are no RMSNorm of one weight
-    run as the modules they are."""
+    run as the modules they are.  weights16: :func:`~qtts_amd.ops.paged_attention`'s, for prompts whose time counts more than their
+    last bits."""
     d, kv = cache.head_dim, cache.kv_heads
     shape, width = qkv.shape, (cache.heads + 2 * kv) * d
     rows = qkv.numel() // width
@@ -171,5 +172,5 @@ def attend(attn: nn.Module, qkv: torch.Tensor, cache: PagedCache, layer: int, wi
     q = torch.ops.qtts.qkv_to_cache(qkv.reshape(rows, width), cache.k[layer], cache.v[layer], state, bounds, cache.heads, weights[0],
                                     weights[1], eps, cos, sin)
     out = torch.ops.qtts.paged_attention(q, cache.k[layer], cache.v[layer], state, bounds, window, sinks,
-                                         d ** -0.5 if scale is None else scale)
+                                         d ** -0.5 if scale is None else scale, weights16)
     return out.view(*shape[:-1], cache.heads * d)

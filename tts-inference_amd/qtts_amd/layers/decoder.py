@@ -170,17 +170,20 @@ def add_norm_mlp(norm: nn.Module, mlp: nn.Module, x: torch.Tensor, residual: tor
     return mlp(norm(hidden)), hidden
 
 
-def paged_layer(layer: nn.Module, hidden: torch.Tensor, cache: PagedCache, index: int, window: int = 0, sinks: int = 0) -> torch.Tensor:
+def paged_layer(layer: nn.Module, hidden: torch.Tensor, cache: PagedCache, index: int, window: int = 0, sinks: int = 0,
+                weights16: bool = False) -> torch.Tensor:
     """One decoder layer (talker.py:246-271) of the cache's step: ``layer.input_layernorm``, ``layer.attn`` (qkv_proj, q_norm, k_norm,
-    o_proj), ``layer.post_attention_layernorm`` and ``layer.mlp``, with the neighbours inside int8 weight-only linears."""
+    o_proj), ``layer.post_attention_layernorm`` and ``layer.mlp``, with the neighbours inside int8 weight-only linears.  weights16:
+    as in :func:`attend`."""
     attn = layer.attn
-    out = attend(attn, norm_linear(layer.input_layernorm, attn.qkv_proj, hidden), cache, index, window, sinks)
+    out = attend(attn, norm_linear(layer.input_layernorm, attn.qkv_proj, hidden), cache, index, window, sinks, weights16=weights16)
     return norm_mlp_residual(layer.post_attention_layernorm, layer.mlp, linear_residual(attn.o_proj, out, hidden))
 
 
 def paged_layer_w8a8(layer: nn.Module, delta: torch.Tensor, hidden: torch.Tensor | None, cache: PagedCache, index: int, window: int = 0,
-                     sinks: int = 0):
+                     sinks: int = 0, weights16: bool = False):
     """The same as ``(delta, hidden)`` for W8A8 linears, the residual beside the hidden state as in :func:`add_norm_linear`."""
     attn = layer.attn
     qkv, hidden = add_norm_linear(layer.input_layernorm, attn.qkv_proj, delta, hidden)
-    return add_norm_mlp(layer.post_attention_layernorm, layer.mlp, attn.o_proj(attend(attn, qkv, cache, index, window, sinks)), hidden)
+    out = attend(attn, qkv, cache, index, window, sinks, weights16=weights16)
+    return add_norm_mlp(layer.post_attention_layernorm, layer.mlp, attn.o_proj(out), hidden)

@@ -1248,14 +1248,18 @@ def attention_bytes(rows: int, d: int) -> int:
 
 
 def paged_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, batch: PagedBatch, window: int = 0, sinks: int = 0,
-                    scale: float | None = None) -> torch.Tensor:
+                    scale: float | None = None, weights16: bool = False) -> torch.Tensor:
     """Attention of the batch's rows over their requests' tokens in a paged cache, the rows' own among them
     (:func:`qkv_to_cache` comes first).
 
     q ``[rows, Hq, D]`` bf16 or fp16 (any row stride), k ``[pages, H, S, D]``, v ``[pages, H, D, S]``; query head h reads key-value
     head ``h // (Hq / H)``.  A row at position p sees the keys ``j <= p``, with a ``window`` those ``j > p - window`` and the first
     ``sinks``.  scale: of the scores (None: ``D ** -0.5``).  Single tokens, prompts and chunks of prompts may share a batch;
-    long caches are split over the GPU and joined.  Returns ``[rows, Hq, D]``, zeros in rows of no request."""
+    long caches are split over the GPU and joined.  Returns ``[rows, Hq, D]``, zeros in rows of no request.
+
+    weights16: round the softmax's weights to q's type on their way to the values, for requests of more than 16 rows a key-value
+    head (new tokens times ``Hq / H``).  A long prompt takes 0.7 of the time; its result is off by up to half a step of the type
+    times ``sum w |v| / sum w``, where it is otherwise rounded once."""
     if q.dim() != 3:
         raise ValueError(f"q must be [rows, heads, head size], got {tuple(q.shape)}")
     rows, heads, d = q.shape
@@ -1267,7 +1271,7 @@ def paged_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, batch: Pa
     idx = _gpu_index(q, k, v, batch.table)
     if idx != _current_device():
         with torch.cuda.device(idx):
-            return paged_attention(q, k, v, batch, window, sinks, scale)
+            return paged_attention(q, k, v, batch, window, sinks, scale, weights16)
     if q.stride(2) != 1 or q.stride(1) != d or q.data_ptr() % 16 or (rows > 1 and (q.stride(0) % 8 or q.stride(0) < heads * d)):
         q = q.clone(memory_format=torch.contiguous_format)
     out = torch.empty(rows, heads, d, dtype=q.dtype, device=q.device)
@@ -1277,7 +1281,8 @@ def paged_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, batch: Pa
     if ws is None or ws.numel() < need:
         _ensure_workspace(q.device, need, "paged_attention")
         ws = _workspaces[idx]
-    st = _lib.load().qtts_paged_attention(
+    lib = _lib.load()
+    st = (lib.qtts_paged_attention_w16 if weights16 else lib.qtts_paged_attention)(
         q.data_ptr(), dtype_code(q.dtype), rows, q.stride(0) if rows > 1 else heads * d, heads, kv_heads, d, k.data_ptr(), v.data_ptr(),
         pages, batch.page_size, batch.table.data_ptr(), batch.requests, batch.cols, batch.starts.data_ptr(),
         batch.counts.data_ptr(), batch.lengths.data_ptr(), batch.slots.data_ptr(), batch.min_new, batch.max_new, window, sinks,

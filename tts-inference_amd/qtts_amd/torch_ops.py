@@ -292,12 +292,12 @@ def _(qkv, k, v, state, bounds, heads, q_norm, k_norm, eps, cos, sin):
 
 @torch.library.custom_op(f"{_LIB}::paged_attention", mutates_args=())
 def paged_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, state: list[torch.Tensor], bounds: list[int], window: int,
-                    sinks: int, scale: float) -> torch.Tensor:
-    return ops.paged_attention(q, k, v, _batch(state, bounds), window, sinks, scale)
+                    sinks: int, scale: float, weights16: bool = False) -> torch.Tensor:
+    return ops.paged_attention(q, k, v, _batch(state, bounds), window, sinks, scale, weights16)
 
 
 @paged_attention.register_fake
-def _(q, k, v, state, bounds, window, sinks, scale):
+def _(q, k, v, state, bounds, window, sinks, scale, weights16=False):
     return q.new_empty(q.shape)
 
 
