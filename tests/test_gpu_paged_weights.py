@@ -139,3 +139,24 @@ def test_weights_of_16_bits_in_a_layer(ops):
     assert torch.equal(outs[0], outs[2]) and not torch.equal(outs[0], outs[1])
     # half a step of each weight, and of either result
     assert (outs[1].double() - outs[0].double()).abs().max() < 2.0 ** -6 * qkv.abs().max()
+
+
+@DTYPES
+@pytest.mark.parametrize("count", [1, 5, 40])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_scores_past_the_weights_range(ops, count, sign, dtype):
+    """Scores whose own fp32 steps are many powers of two: the largest one's key has all the weight (the next one is a
+    thousand steps below), and rounding the maximum makes no weight infinite.  The result is that key's value, up to its weight's
+    two parts (e^2), the sum's and the quotient's roundings (4 u) and its own."""
+    g = torch.Generator(device="cuda").manual_seed(11)
+    n, e = 100, torch.finfo(dtype).eps / 2
+    for case in range(12):
+        keys = sign * (1 + torch.randperm(n, generator=g, device="cuda") / 128.0)
+        values = torch.randn(n, 64, generator=g, device="cuda").to(dtype)
+        for power in (20, 24, 26, 27, 28, 30, 33, 36, 50, 100):
+            out = _call(ops, keys, values, count, dtype, scale=2.0 ** power, query=1 + case / 16)
+            for i in range(count):
+                best = int(keys[:n - count + i + 1].argmax())
+                v = values[best].double()
+                err = (out[i, 0].double() - v).abs()
+                assert (err <= (e + e * e + 4 * U) * v.abs()).all(), (case, power, i, float(err.max()))

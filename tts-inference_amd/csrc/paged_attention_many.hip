@@ -163,7 +163,8 @@ template <typename T, int DP, bool EXACT, bool WIDE, bool W16> __global__ __laun
   };
 
   f32x16_t o[NB];
-  float m = kLowest, l = 0.0f;
+  float ref = -INFINITY, bias = 0.0f, l = 0.0f;
+  bool far = false;  // some row of the wave
 #pragma unroll
   for (int b = 0; b < NB; ++b)
 #pragma unroll
@@ -220,22 +221,32 @@ template <typename T, int DP, bool EXACT, bool WIDE, bool W16> __global__ __laun
     float top = s[0][0];
 #pragma unroll
     for (int e = 1; e < 32; ++e) top = fmaxf(top, s[e >> 4][e & 15]);
-    top = max_32(top) * a.scale;
-    // The maximum moves only where a score passes it by 8 powers of two: weights stay under 256 and most steps keep O.
-    if (__any(top > m + 8.0f)) {
-      const float now = fmaxf(m, top), keep = exp2_hw(m - now);
-      m = now;
+    top = max_32(top);
+    const bool up = reach_of(top, ref, a.scale) > kLag;
+    if (__any(up)) {
+      const float keep = up ? exp2_hw(reach_of(ref, top, a.scale)) : 1.0f;
+      ref = up ? top : ref;
+      bias = up ? -top * a.scale : bias;
+      far = __any(fabsf(bias) > kFar);
       l *= keep;
 #pragma unroll
       for (int b = 0; b < NB; ++b) o[b] *= keep;
     }
+    if (far) {
+      const float off = fmaxf(ref, kLowest);
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[t][e] -= off;
+    }
+    const float add = far ? 0.0f : bias;
 #pragma unroll
     for (int ks = 0; ks < 4; ++ks) {
       i32x4_t p1, p2;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const float w0 = exp2_hw(__builtin_fmaf(s[ks >> 1][8 * (ks & 1) + 2 * j], a.scale, -m));
-        const float w1 = exp2_hw(__builtin_fmaf(s[ks >> 1][8 * (ks & 1) + 2 * j + 1], a.scale, -m));
+        const float w0 = exp2_hw(__builtin_fmaf(s[ks >> 1][8 * (ks & 1) + 2 * j], a.scale, add));
+        const float w1 = exp2_hw(__builtin_fmaf(s[ks >> 1][8 * (ks & 1) + 2 * j + 1], a.scale, add));
         const uint32_t two = pack2<T>(w0, w1);
         p1[j] = (int)two;
         if constexpr (W16) {
@@ -286,6 +297,7 @@ template <typename T, int DP, bool EXACT, bool WIDE, bool W16> __global__ __laun
     tile(here, keys[buffer], values[buffer]);
   }
   l = sum_32(l);
+  ref = fmaxf(ref, kLowest);
 
   // rows whose sums are not finite though their weights are, one by one
   bool odd = false;
@@ -301,7 +313,7 @@ template <typename T, int DP, bool EXACT, bool WIDE, bool W16> __global__ __laun
       const int n = __builtin_ctzll(again);
       again &= again - 1;
       row_again<T, kTile>(a, w, tiles, begin, 1, end, h, w.row + __builtin_amdgcn_readlane(token, n),
-                          __builtin_amdgcn_readlane(query, n), __builtin_amdgcn_readlane(hi, n), __shfl(m, n, 64), dst);
+                          __builtin_amdgcn_readlane(query, n), __builtin_amdgcn_readlane(hi, n), __shfl(ref, n, 64), dst);
       wave_lds_fence();
 #pragma unroll
       for (int b = 0; b < NB; ++b)
@@ -328,7 +340,7 @@ template <typename T, int DP, bool EXACT, bool WIDE, bool W16> __global__ __laun
     return;
   }
   // A part: d / 4 pairs of sums a thread, pair j of thread t at j kThreads + t, so that a wave's accesses are whole lines, then
-  // [kRun] pairs of maximum and weight sum.
+  // [kRun] pairs of reference and weight sum.
   float* parts = p.parts + ((int64_t)w.slot * kv_heads + h) * p.slot_floats;
   const int64_t pitch = (int64_t)kv_heads * p.slot_floats;
   const int row = wave * kWaveRows + col;
@@ -339,7 +351,7 @@ template <typename T, int DP, bool EXACT, bool WIDE, bool W16> __global__ __laun
 #pragma unroll
       for (int e = 0; e < 16; e += 2)
         if (b * 32 + 2 * (e & ~3) < d) store_pair(mine + (8 * b + e / 2) * 2 * kThreads, o[b][e], o[b][e + 1]);
-    if (half == 0) store_pair(parts + w.split * pitch + kRun * d + 2 * row, m, l);
+    if (half == 0) store_pair(parts + w.split * pitch + kRun * d + 2 * row, ref, l);
   }
   wait_vmem();
   __syncthreads();
@@ -349,7 +361,7 @@ template <typename T, int DP, bool EXACT, bool WIDE, bool W16> __global__ __laun
   if (flag != (unsigned)(splits - 1)) return;
   if (threadIdx.x == 0) reset_counter(counter);
   if (!live) return;
-  m = kLowest;
+  ref = kLowest;
   l = 0.0f;
 #pragma unroll
   for (int b = 0; b < NB; ++b)
@@ -357,10 +369,10 @@ template <typename T, int DP, bool EXACT, bool WIDE, bool W16> __global__ __laun
     for (int e = 0; e < 16; ++e) o[b][e] = 0.0f;
   for (int s = 0; s < splits; ++s) {
     const float* src = parts + s * pitch;
-    const f32x2_t ml = load_pair(src + kRun * d + 2 * row);
-    const float now = fmaxf(m, ml[0]), keep = exp2_hw(m - now), f = exp2_hw(ml[0] - now);
-    m = now;
-    l = l * keep + f * ml[1];
+    const f32x2_t rl = load_pair(src + kRun * d + 2 * row);
+    const float now = fmaxf(ref, rl[0]), keep = exp2_hw(reach_of(ref, now, a.scale)), f = exp2_hw(reach_of(rl[0], now, a.scale));
+    ref = now;
+    l = l * keep + f * rl[1];
     src += 2 * threadIdx.x;
 #pragma unroll
     for (int b = 0; b < NB; ++b)

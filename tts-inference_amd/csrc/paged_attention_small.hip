@@ -34,7 +34,7 @@ void paged_small_kernel(PagedLaunch p) {
   typedef typename mfma16<T>::vec vec;
   constexpr int NC = DP / 32, NB = DP / 16;
   __shared__ float part[kWaves][kRows][DP + 4];
-  __shared__ float part_m[kWaves][kRows], part_l[kWaves][kRows];
+  __shared__ float part_r[kWaves][kRows], part_l[kWaves][kRows];
   __shared__ unsigned flag;
   const PagedAttentionArgs& a = p.a;
   const int kv_heads = a.cache.kv_heads, h = blockIdx.x % kv_heads, item = blockIdx.x / kv_heads;
@@ -73,7 +73,8 @@ void paged_small_kernel(PagedLaunch p) {
   f32x4_t o[NB];
 #pragma unroll
   for (int b = 0; b < NB; ++b) o[b] = f32x4_t{0, 0, 0, 0};
-  float m = kLowest, l = 0.0f;
+  float ref = -INFINITY, bias = 0.0f, l = 0.0f;
+  bool far = false;  // some row of the run
 
   // Key of product t's row r: base + 8 (r / 4) + 4 t + r % 4; this lane's eight scores: keys base + 8 g + 0..7.
   const int32_t* table = a.table + (int64_t)w.request * a.cols;
@@ -127,19 +128,27 @@ void paged_small_kernel(PagedLaunch p) {
       float top = x[0];
 #pragma unroll
       for (int j = 1; j < 8; ++j) top = fmaxf(top, x[j]);
-      top = max_16_32(top) * a.scale;
-      // The maximum moves only where a score passes it by 8 powers of two: weights stay under 256 and most steps keep O.
-      if (__any(top > m + 8.0f)) {
-        const float now = fmaxf(m, top), keep = exp2_hw(m - now);
-        m = now;
+      top = max_16_32(top);
+      const bool up = reach_of(top, ref, a.scale) > kLag;
+      if (__any(up)) {
+        const float keep = up ? exp2_hw(reach_of(ref, top, a.scale)) : 1.0f;
+        ref = up ? top : ref;
+        bias = up ? -top * a.scale : bias;
+        far = __any(fabsf(bias) > kFar);
         l *= keep;
 #pragma unroll
         for (int b = 0; b < NB; ++b) o[b] *= keep;
       }
+      if (far) {
+        const float off = fmaxf(ref, kLowest);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] -= off;
+      }
+      const float add = far ? 0.0f : bias;
       i32x4_t p1, p2;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const float w0 = exp2_hw(__builtin_fmaf(x[2 * j], a.scale, -m)), w1 = exp2_hw(__builtin_fmaf(x[2 * j + 1], a.scale, -m));
+        const float w0 = exp2_hw(__builtin_fmaf(x[2 * j], a.scale, add)), w1 = exp2_hw(__builtin_fmaf(x[2 * j + 1], a.scale, add));
         l += w0 + w1;
         const uint32_t two = pack2<T>(w0, w1);
         p1[j] = (int)two;
@@ -172,6 +181,7 @@ void paged_small_kernel(PagedLaunch p) {
 
   // rows whose sums are not finite though their weights are, one by one
   l = sum_16_32(l);
+  ref = fmaxf(ref, kLowest);
   bool odd = false;
 #pragma unroll
   for (int b = 0; b < NB; ++b)
@@ -184,7 +194,7 @@ void paged_small_kernel(PagedLaunch p) {
     again &= again - 1;
     const int t = n / group;
     row_again<T, kTile>(a, w, tiles, begin + wave, kWaves, end, h, w.row + t, h * group + n - t * group, w.position + t,
-                        __shfl(m, n, 64), &part[wave][0][0]);
+                        __shfl(ref, n, 64), &part[wave][0][0]);
     wave_lds_fence();
 #pragma unroll
     for (int b = 0; b < NB; ++b)
@@ -195,7 +205,7 @@ void paged_small_kernel(PagedLaunch p) {
   // the waves' results
   if (live) {
     if (g == 0) {
-      part_m[wave][col] = m;
+      part_r[wave][col] = ref;
       part_l[wave][col] = l;
     }
 #pragma unroll
@@ -203,15 +213,15 @@ void paged_small_kernel(PagedLaunch p) {
       if (b * 16 < d) *(f32x4_t*)&part[wave][col][b * 16 + g * 4] = o[b];
   }
   __syncthreads();
-  auto joined = [&](int row, int dim, float& mm, float& ll) -> f32x4_t {
-    mm = part_m[0][row];
+  auto joined = [&](int row, int dim, float& rr, float& ll) -> f32x4_t {
+    rr = part_r[0][row];
 #pragma unroll
-    for (int n = 1; n < kWaves; ++n) mm = fmaxf(mm, part_m[n][row]);
+    for (int n = 1; n < kWaves; ++n) rr = fmaxf(rr, part_r[n][row]);
     f32x4_t sum = {0, 0, 0, 0};
     ll = 0.0f;
 #pragma unroll
     for (int n = 0; n < kWaves; ++n) {
-      const float f = exp2_hw(part_m[n][row] - mm);
+      const float f = exp2_hw(reach_of(part_r[n][row], rr, a.scale));
       ll += f * part_l[n][row];
       sum += f * *(const f32x4_t*)&part[n][row][dim];
     }
@@ -227,23 +237,23 @@ void paged_small_kernel(PagedLaunch p) {
   if (splits == 1) {
     for (int e = threadIdx.x; e < quads; e += kThreads) {
       const int row = e / (d / 4), dim = (e - row * (d / 4)) * 4;
-      float mm, ll;
-      const f32x4_t v = joined(row, dim, mm, ll);
+      float rr, ll;
+      const f32x4_t v = joined(row, dim, rr, ll);
       put(row, dim, v, ll);
     }
     return;
   }
-  // a part: [rows][d] sums, then [rows] pairs of maximum and weight sum
+  // a part: [rows][d] sums, then [rows] pairs of reference and weight sum
   float* parts = p.parts + ((int64_t)w.slot * kv_heads + h) * p.slot_floats;
   const int64_t pitch = (int64_t)kv_heads * p.slot_floats;
   float* mine = parts + w.split * pitch;
   for (int e = threadIdx.x; e < quads; e += kThreads) {
     const int row = e / (d / 4), dim = (e - row * (d / 4)) * 4;
-    float mm, ll;
-    const f32x4_t v = joined(row, dim, mm, ll);
+    float rr, ll;
+    const f32x4_t v = joined(row, dim, rr, ll);
     store_pair(mine + row * d + dim, v[0], v[1]);
     store_pair(mine + row * d + dim + 2, v[2], v[3]);
-    if (dim == 0) store_pair(mine + rows * d + 2 * row, mm, ll);
+    if (dim == 0) store_pair(mine + rows * d + 2 * row, rr, ll);
   }
   wait_vmem();
   __syncthreads();
@@ -259,15 +269,15 @@ void paged_small_kernel(PagedLaunch p) {
   for (int e0 = threadIdx.x; e0 < max(quads, kThreads); e0 += kThreads) {
     const int team = e0 / quads, e = e0 - team * quads;
     const int row = e / (d / 4), dim = (e - row * (d / 4)) * 4;
-    float mm = kLowest, ll = 0.0f;
+    float rr = kLowest, ll = 0.0f;
     f32x4_t sum = {0, 0, 0, 0};
     constexpr int AHEAD = 8;  // parts whose loads are out together
     for (int s0 = team; s0 < splits && team < teams; s0 += AHEAD * teams) {
-      f32x2_t ml[AHEAD], v0[AHEAD], v1[AHEAD];
+      f32x2_t rl[AHEAD], v0[AHEAD], v1[AHEAD];
 #pragma unroll
       for (int n = 0; n < AHEAD; ++n) {
         const float* src = parts + min(s0 + n * teams, splits - 1) * pitch;
-        ml[n] = load_pair(src + rows * d + 2 * row);
+        rl[n] = load_pair(src + rows * d + 2 * row);
         v0[n] = load_pair(src + row * d + dim);
         v1[n] = load_pair(src + row * d + dim + 2);
       }
@@ -275,22 +285,22 @@ void paged_small_kernel(PagedLaunch p) {
 #pragma unroll
       for (int n = 0; n < AHEAD; ++n) {
         if (s0 + n * teams >= splits) break;
-        const float now = fmaxf(mm, ml[n][0]), keep = exp2_hw(mm - now), f = exp2_hw(ml[n][0] - now);
-        mm = now;
-        ll = ll * keep + f * ml[n][1];
+        const float now = fmaxf(rr, rl[n][0]), keep = exp2_hw(reach_of(rr, now, a.scale)), f = exp2_hw(reach_of(rl[n][0], now, a.scale));
+        rr = now;
+        ll = ll * keep + f * rl[n][1];
         sum = sum * keep + f * f32x4_t{v0[n][0], v0[n][1], v1[n][0], v1[n][1]};
       }
     }
     if (teams > 1) {
       sums[threadIdx.x] = sum;
-      heads[threadIdx.x] = f32x2_t{mm, ll};
+      heads[threadIdx.x] = f32x2_t{rr, ll};
       __syncthreads();
       if (team) continue;
       for (int n = 1; n < teams; ++n) {
-        const f32x2_t ml = heads[n * quads + e];
-        const float now = fmaxf(mm, ml[0]), keep = exp2_hw(mm - now), f = exp2_hw(ml[0] - now);
-        mm = now;
-        ll = ll * keep + f * ml[1];
+        const f32x2_t rl = heads[n * quads + e];
+        const float now = fmaxf(rr, rl[0]), keep = exp2_hw(reach_of(rr, now, a.scale)), f = exp2_hw(reach_of(rl[0], now, a.scale));
+        rr = now;
+        ll = ll * keep + f * rl[1];
         sum = sum * keep + f * sums[n * quads + e];
       }
     }

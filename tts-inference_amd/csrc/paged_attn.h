@@ -9,7 +9,7 @@
 
 namespace qtts {
 
-constexpr float kLowest = -3.402823466e38f;  // where a running maximum starts: below every score, and no infinity to subtract
+constexpr float kLowest = -3.402823466e38f;  // a reference (below) that nothing has set, as one to subtract
 
 struct PagedLaunch {
   PagedAttentionArgs a;
@@ -196,6 +196,13 @@ __device__ __forceinline__ f32x2_t load_pair(const float* p) {
   return __builtin_bit_cast(f32x2_t, load_coherent((const uint64_t*)p));
 }
 
+// Weights are 2^(scale (s - r)) about a score r, the reference, that moves up to a tile's largest one only where that leads by more
+// than kLag powers of two: weights stay under 2^kLag and most tiles leave O as it is.  An exponent is one fma with
+// -scale r, rounded; where that is past kFar its steps would be the weights' own (from 2^27 on they passed every range), and r is
+// taken off the scores themselves, which are near each other wherever a weight is left.
+constexpr float kLag = 8.0f, kFar = 1024.0f;
+__device__ __forceinline__ float reach_of(float s, float r, float scale) { return (s - r) * scale; }
+
 // 16 bits a value: infinities and NaN have all exponent bits set (of either half of `two`).
 template <typename T> __device__ __forceinline__ bool not_finite(uint32_t two) {
   constexpr uint32_t e = std::is_same<T, bf16_t>::value ? 0x7f80u : 0x7c00u;
@@ -204,10 +211,11 @@ template <typename T> __device__ __forceinline__ bool not_finite(uint32_t two) {
 
 // One row's sums over tiles first, first + step, ... < end again, by one wave and without the matrix cores: a value that
 // the row does not see cannot reach it, where a product of tiles has 0 * NaN.  For rows whose weights are sound (l finite) and
-// whose sums came out infinite or NaN.  m: the maximum that the sums stand at; dst [d], in LDS.
+// whose sums came out infinite or NaN.  r: their reference (scores summed in another order may pass it further: to kLag, as theirs);
+// dst [d], in LDS.
 template <typename T, int TILE>
 __device__ __forceinline__ void row_again(const PagedAttentionArgs& a, const PagedWork& w, const KeyTiles& tiles, int first,
-                                          int step, int end, int kv_head, int row, int query, int hi, float m, float* dst) {
+                                          int step, int end, int kv_head, int row, int query, int hi, float r, float* dst) {
   const int lane = threadIdx.x & 63, d = a.cache.d, shift = a.cache.page_shift, mask = (1 << shift) - 1;
   const int lo = a.window ? max(0, hi - a.window + 1) : 0;
   const int32_t* table = a.table + (int64_t)w.request * a.cols;
@@ -225,7 +233,7 @@ __device__ __forceinline__ void row_again(const PagedAttentionArgs& a, const Pag
 #pragma unroll 1
       for (int c = 0; c < d; ++c) s += to_f32(q[c]) * to_f32(k[c]);
     }
-    const float weight = seen ? exp2_hw(__builtin_fmaf(s, a.scale, -m)) : 0.0f;
+    const float weight = seen ? exp2_hw(fminf(reach_of(s, r, a.scale), kLag)) : 0.0f;
     const uint64_t seen_by = __ballot(seen);
 #pragma unroll 1
     for (int j = 0; j < TILE; ++j) {
