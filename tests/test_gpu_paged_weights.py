@@ -5,9 +5,11 @@ Scores are exact here: a query has one nonzero entry, so a score is one product 
 u = 2^-24 and e = eps / 2 of the type, for out = sum w_j v_j / sum w_j and A = sum w_j |v_j| / sum w_j:
 
 * a weight's exponent is off by 4 u (|s_j| + |max|) and the exponential by 2^-22: with the largest of these, r, 2 r A;
-* a weight goes to the second product in two parts of the type, the second one the first one's error: e^2 A;
+* a weight goes to the second product in two parts of the type, the second one the first one's error: e^2 A (in one part, e A);
 * fp16 holds nothing under 2^-25; of a tile's keys (64, the larger of the kernels') the largest weight is 1 or more
   before it is cut off, so that each key loses at most 2^-25 of the tile's largest weight;
+* fp32's normal numbers end at 2^-126: a weight that is smaller beside the row's largest is zero (the exponential's, and the factor of
+  a part that is joined), 2^-125 for both;
 * n terms summed in fp32 in any order, and rescaled: 4 (n + 64) u A;
 * the result is rounded once: e |out|.
 """
@@ -33,7 +35,7 @@ def ops():
     return _ops
 
 
-def _call(ops, keys, values, count, dtype, heads=1, kv=1, page=64, window=0, sinks=0, scale=1.0, query=1.0):
+def _call(ops, keys, values, count, dtype, heads=1, kv=1, page=64, window=0, sinks=0, scale=1.0, query=1.0, weights16=False):
     """One request whose key j has entry keys[j] and value values[j] ([n, d]), its last `count` tokens the rows, each of whose
     queries has one entry.  Returns the output [count, heads, d] and the batch."""
     n, d = values.shape
@@ -46,10 +48,10 @@ def _call(ops, keys, values, count, dtype, heads=1, kv=1, page=64, window=0, sin
     v[slot // page, :, :, slot % page] = values.to(dtype)[:, None]
     q = torch.zeros(count, heads, d, dtype=dtype, device="cuda")
     q[:, :, 5] = query
-    return ops.paged_attention(q, k, v, batch, window, sinks, scale)
+    return ops.paged_attention(q, k, v, batch, window, sinks, scale, weights16)
 
 
-def _exact(keys, values, count, dtype, window=0, sinks=0):
+def _exact(keys, values, count, dtype, window=0, sinks=0, weights16=False):
     """(result [count, d], bound without its rounding) in 64 bits, a row at a time."""
     n = values.shape[0]
     s, v = keys.to(dtype).double(), values.to(dtype).double()
@@ -65,7 +67,7 @@ def _exact(keys, values, count, dtype, window=0, sinks=0):
         total = w.sum()
         y, mags = w @ v / total, w @ v.abs() / total
         rel = 4 * U * (s[seen].abs().max() + top.abs()) + 2.0 ** -22
-        bound = mags * (2 * rel + e * e + 4 * (n + 64) * U)
+        bound = mags * (2 * rel + (e if weights16 else e * e) + 4 * (n + 64) * U) + 2.0 ** -125 * (seen.double() @ v.abs()) / total
         if dtype == torch.float16:
             tail = -n % 64
             tops = torch.nn.functional.pad(w, (0, tail)).view(-1, 64).amax(1).repeat_interleave(64)[:n]
@@ -75,9 +77,9 @@ def _exact(keys, values, count, dtype, window=0, sinks=0):
     return torch.stack(out), torch.stack(off)
 
 
-def _check(ops, keys, values, count, dtype, heads=1, what="", window=0, sinks=0, **kw):
-    out = _call(ops, keys, values, count, dtype, heads, window=window, sinks=sinks, **kw)
-    want, off = _exact(keys, values, count, dtype, window, sinks)
+def _check(ops, keys, values, count, dtype, heads=1, what="", window=0, sinks=0, weights16=False, **kw):
+    out = _call(ops, keys, values, count, dtype, heads, window=window, sinks=sinks, weights16=weights16, **kw)
+    want, off = _exact(keys, values, count, dtype, window, sinks, weights16)
     _near(out, want[:, None].expand_as(out), off[:, None].expand_as(out), what)
 
 
@@ -160,3 +162,76 @@ def test_scores_past_the_weights_range(ops, count, sign, dtype):
                 v = values[best].double()
                 err = (out[i, 0].double() - v).abs()
                 assert (err <= (e + e * e + 4 * U) * v.abs()).all(), (case, power, i, float(err.max()))
+
+
+def _tail(n, where, far, spread, g):
+    """Scores of one key at 0 and the others `far` below it, give or take; values: 0 and 1, and the other way round."""
+    keys = -far - torch.rand(n, generator=g, device="cuda") * spread
+    at = {"first": 0, "middle": n // 2 + 3, "last": n - 41}[where]
+    keys[at] = 0.0
+    values = torch.ones(n, 16, device="cuda")
+    values[:, 8:] = 0.0
+    values[at] = 1 - values[at]
+    return keys, values
+
+
+@DTYPES
+@pytest.mark.parametrize("count", [1, 40])
+@pytest.mark.parametrize("where", ["first", "middle", "last"])
+@pytest.mark.parametrize("far,spread", [(11.0, 0.0), (15.5, 3.0), (17.5, 0.0), (17.5, 4.0), (24.0, 0.0), (40.0, 0.0)])
+def test_long_tails(ops, far, spread, where, count, dtype):
+    """One key far above tens of thousands of others: their share of the result is theirs, however small each one's weight."""
+    g = torch.Generator(device="cuda").manual_seed(7)
+    keys, values = _tail(65536, where, far, spread, g)
+    _check(ops, keys, values, count, dtype)
+    if count > 1:
+        _check(ops, keys, values, count, dtype, weights16=True)
+
+
+@pytest.mark.parametrize("count", [1, 17])
+def test_a_million_keys_behind_one(ops, count):
+    """Lengths at which weights of 2^-25 outweigh the key that stands out."""
+    for far in (14.0, 17.375, 19.0):
+        keys, values = _tail(1 << 20, "first", far, 0.0, torch.Generator(device="cuda").manual_seed(1))
+        _check(ops, keys, values, count, torch.float16, page=1024)
+
+
+@DTYPES
+@pytest.mark.parametrize("count", [1, 30])
+def test_falling_and_rising_scores(ops, count, dtype):
+    """Scores along a slope of hundreds of powers of two either way, and up and down again: the tiles' largest weights are anywhere
+    below the row's."""
+    n = 4000
+    at = torch.arange(n, device="cuda")
+    for keys in (-at / 32.0, (at - n) / 32.0, -(at - n / 2).abs() / 64.0, (at - n / 2).abs() / 64.0 - 40, -(at % 700) / 8.0):
+        keys = keys.to(dtype).float()
+        for low in (-3.0, -12.0, -25.0):
+            below = keys - keys.max() < low  # of the sum, what lies under e^low alone
+            values = below.float()[:, None].expand(n, 16)
+            _check(ops, keys, values, count, dtype)
+            _check(ops, keys, values, count, dtype, window=1000, sinks=70)
+
+
+@DTYPES
+@pytest.mark.parametrize("n,heads", [(20000, 1), (4096, 1024)])
+@pytest.mark.parametrize("count", [1, 3, 20])
+@pytest.mark.parametrize("value", [0.0, float("inf"), float("nan")])
+def test_tails_around_a_value_that_is_not_finite(ops, value, count, n, heads, dtype):
+    """Sums that are formed key by key keep the tail and the key before it as well: of the rows before the last one, which alone sees an
+    infinity or NaN."""
+    keys, v = _tail(n, "first", 17.5, 0.0, torch.Generator(device="cuda").manual_seed(2))
+    v[n - 1] = value
+    out = _call(ops, keys, v, count, dtype, heads=heads, kv=heads)
+    want, off = _exact(keys, torch.nan_to_num(v, 0.0, 0.0, 0.0), count, dtype)
+    last = count if value == 0.0 else count - 1
+    _near(out[:last], want[:last, None].expand(last, heads, 16), off[:last, None].expand(last, heads, 16), "rows")
+    if last < count:
+        assert not out[-1].isfinite().any()
+
+
+@DTYPES
+@pytest.mark.parametrize("count", [1, 20])
+def test_tails_of_many_heads(ops, count, dtype):
+    """So many heads that each one's keys stay with a few waves, whose own keys are a tail behind the one that stands out."""
+    keys, values = _tail(4096, "first", 17.5, 0.0, torch.Generator(device="cuda").manual_seed(5))
+    _check(ops, keys, values, count, dtype, heads=1024, kv=1024)

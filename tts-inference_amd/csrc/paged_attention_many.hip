@@ -163,8 +163,8 @@ template <typename T, int DP, bool EXACT, bool WIDE, bool W16> __global__ __laun
   };
 
   f32x16_t o[NB];
-  float ref = -INFINITY, bias = 0.0f, l = 0.0f;
-  bool far = false;  // some row of the wave
+  Reference<T> ref;
+  float l = 0.0f;
 #pragma unroll
   for (int b = 0; b < NB; ++b)
 #pragma unroll
@@ -222,24 +222,21 @@ template <typename T, int DP, bool EXACT, bool WIDE, bool W16> __global__ __laun
 #pragma unroll
     for (int e = 1; e < 32; ++e) top = fmaxf(top, s[e >> 4][e & 15]);
     top = max_32(top);
-    const bool up = reach_of(top, ref, a.scale) > kLag;
-    if (__any(up)) {
-      const float keep = up ? exp2_hw(reach_of(ref, top, a.scale)) : 1.0f;
-      ref = up ? top : ref;
-      bias = up ? -top * a.scale : bias;
-      far = __any(fabsf(bias) > kFar);
+    const bool now = ref.moves(top, a.scale);
+    if (__any(now)) {
+      const float keep = ref.move(now, top, a.scale);
       l *= keep;
 #pragma unroll
       for (int b = 0; b < NB; ++b) o[b] *= keep;
     }
-    if (far) {
-      const float off = fmaxf(ref, kLowest);
+    if (ref.far) {
+      const float off = fmaxf(ref.r, kLowest);
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int e = 0; e < 16; ++e) s[t][e] -= off;
     }
-    const float add = far ? 0.0f : bias;
+    const float add = ref.far ? kAim<T> : ref.bias;
 #pragma unroll
     for (int ks = 0; ks < 4; ++ks) {
       i32x4_t p1, p2;
@@ -297,7 +294,7 @@ template <typename T, int DP, bool EXACT, bool WIDE, bool W16> __global__ __laun
     tile(here, keys[buffer], values[buffer]);
   }
   l = sum_32(l);
-  ref = fmaxf(ref, kLowest);
+  ref.r = fmaxf(ref.r, kLowest);
 
   // rows whose sums are not finite though their weights are, one by one
   bool odd = false;
@@ -313,7 +310,7 @@ template <typename T, int DP, bool EXACT, bool WIDE, bool W16> __global__ __laun
       const int n = __builtin_ctzll(again);
       again &= again - 1;
       row_again<T, kTile>(a, w, tiles, begin, 1, end, h, w.row + __builtin_amdgcn_readlane(token, n),
-                          __builtin_amdgcn_readlane(query, n), __builtin_amdgcn_readlane(hi, n), __shfl(ref, n, 64), dst);
+                          __builtin_amdgcn_readlane(query, n), __builtin_amdgcn_readlane(hi, n), __shfl(ref.r, n, 64), dst);
       wave_lds_fence();
 #pragma unroll
       for (int b = 0; b < NB; ++b)
@@ -351,7 +348,7 @@ template <typename T, int DP, bool EXACT, bool WIDE, bool W16> __global__ __laun
 #pragma unroll
       for (int e = 0; e < 16; e += 2)
         if (b * 32 + 2 * (e & ~3) < d) store_pair(mine + (8 * b + e / 2) * 2 * kThreads, o[b][e], o[b][e + 1]);
-    if (half == 0) store_pair(parts + w.split * pitch + kRun * d + 2 * row, ref, l);
+    if (half == 0) store_pair(parts + w.split * pitch + kRun * d + 2 * row, ref.r, l);
   }
   wait_vmem();
   __syncthreads();
@@ -361,7 +358,7 @@ template <typename T, int DP, bool EXACT, bool WIDE, bool W16> __global__ __laun
   if (flag != (unsigned)(splits - 1)) return;
   if (threadIdx.x == 0) reset_counter(counter);
   if (!live) return;
-  ref = kLowest;
+  float r = kLowest;
   l = 0.0f;
 #pragma unroll
   for (int b = 0; b < NB; ++b)
@@ -370,8 +367,8 @@ template <typename T, int DP, bool EXACT, bool WIDE, bool W16> __global__ __laun
   for (int s = 0; s < splits; ++s) {
     const float* src = parts + s * pitch;
     const f32x2_t rl = load_pair(src + kRun * d + 2 * row);
-    const float now = fmaxf(ref, rl[0]), keep = exp2_hw(reach_of(ref, now, a.scale)), f = exp2_hw(reach_of(rl[0], now, a.scale));
-    ref = now;
+    const float now = fmaxf(r, rl[0]), keep = exp2_hw(reach_of(r, now, a.scale)), f = exp2_hw(reach_of(rl[0], now, a.scale));
+    r = now;
     l = l * keep + f * rl[1];
     src += 2 * threadIdx.x;
 #pragma unroll

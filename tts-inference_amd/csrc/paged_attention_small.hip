@@ -7,8 +7,9 @@
 // never leaves its lane, and the values, d-major on their page, are 16-byte loads of that operand's other side.  Keys and
 // values go from memory to registers and nowhere else; LDS joins the four waves at the end.
 //
-// P goes to the second product in two 16-bit parts, whose products add up to P's in fp32's neighbourhood: the matrix cores
-// have the time (a wave's step at d = 128 is 24 MFMAs to 16 KiB of cache), and sums that cancel keep their bits.
+// P goes to the second product in two 16-bit parts, whose products add up to P's in 16 bits (bf16) or 22 (fp16): the matrix cores
+// have the time (a wave's step at d = 128 is 24 MFMAs to 16 KiB of cache), and sums that cancel keep their bits.  Where fp16's
+// parts end, and what keeps a long tail above that: paged_attn.h.
 //
 // Splits: the tiles of all requests are cut into pieces of one size, and a request's last workgroup to finish joins its
 // pieces (paged_attn.h).
@@ -73,8 +74,8 @@ void paged_small_kernel(PagedLaunch p) {
   f32x4_t o[NB];
 #pragma unroll
   for (int b = 0; b < NB; ++b) o[b] = f32x4_t{0, 0, 0, 0};
-  float ref = -INFINITY, bias = 0.0f, l = 0.0f;
-  bool far = false;  // some row of the run
+  Reference<T> ref;
+  float l = 0.0f;
 
   // Key of product t's row r: base + 8 (r / 4) + 4 t + r % 4; this lane's eight scores: keys base + 8 g + 0..7.
   const int32_t* table = a.table + (int64_t)w.request * a.cols;
@@ -129,22 +130,19 @@ void paged_small_kernel(PagedLaunch p) {
 #pragma unroll
       for (int j = 1; j < 8; ++j) top = fmaxf(top, x[j]);
       top = max_16_32(top);
-      const bool up = reach_of(top, ref, a.scale) > kLag;
-      if (__any(up)) {
-        const float keep = up ? exp2_hw(reach_of(ref, top, a.scale)) : 1.0f;
-        ref = up ? top : ref;
-        bias = up ? -top * a.scale : bias;
-        far = __any(fabsf(bias) > kFar);
+      const bool now = ref.moves(top, a.scale);
+      if (__any(now)) {
+        const float keep = ref.move(now, top, a.scale);
         l *= keep;
 #pragma unroll
         for (int b = 0; b < NB; ++b) o[b] *= keep;
       }
-      if (far) {
-        const float off = fmaxf(ref, kLowest);
+      if (ref.far) {
+        const float off = fmaxf(ref.r, kLowest);
 #pragma unroll
         for (int j = 0; j < 8; ++j) x[j] -= off;
       }
-      const float add = far ? 0.0f : bias;
+      const float add = ref.far ? kAim<T> : ref.bias;
       i32x4_t p1, p2;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -181,7 +179,7 @@ void paged_small_kernel(PagedLaunch p) {
 
   // rows whose sums are not finite though their weights are, one by one
   l = sum_16_32(l);
-  ref = fmaxf(ref, kLowest);
+  ref.r = fmaxf(ref.r, kLowest);
   bool odd = false;
 #pragma unroll
   for (int b = 0; b < NB; ++b)
@@ -194,7 +192,7 @@ void paged_small_kernel(PagedLaunch p) {
     again &= again - 1;
     const int t = n / group;
     row_again<T, kTile>(a, w, tiles, begin + wave, kWaves, end, h, w.row + t, h * group + n - t * group, w.position + t,
-                        __shfl(ref, n, 64), &part[wave][0][0]);
+                        __shfl(ref.r, n, 64), &part[wave][0][0]);
     wave_lds_fence();
 #pragma unroll
     for (int b = 0; b < NB; ++b)
@@ -205,7 +203,7 @@ void paged_small_kernel(PagedLaunch p) {
   // the waves' results
   if (live) {
     if (g == 0) {
-      part_r[wave][col] = ref;
+      part_r[wave][col] = ref.r;
       part_l[wave][col] = l;
     }
 #pragma unroll

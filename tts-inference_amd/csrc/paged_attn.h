@@ -196,12 +196,41 @@ __device__ __forceinline__ f32x2_t load_pair(const float* p) {
   return __builtin_bit_cast(f32x2_t, load_coherent((const uint64_t*)p));
 }
 
-// Weights are 2^(scale (s - r)) about a score r, the reference, that moves up to a tile's largest one only where that leads by more
-// than kLag powers of two: weights stay under 2^kLag and most tiles leave O as it is.  An exponent is one fma with
-// -scale r, rounded; where that is past kFar its steps would be the weights' own (from 2^27 on they passed every range), and r is
-// taken off the scores themselves, which are near each other wherever a weight is left.
-constexpr float kLag = 8.0f, kFar = 1024.0f;
+// Weights are 2^(scale (s - r) + kAim) about a score r, the reference, that moves to a tile's largest one only where that leads by
+// more than kLag powers of two: most tiles leave O as it is.  An exponent is one fma with kAim - scale r, rounded; where that is past
+// kFar its steps would be the weights' own (from 2^27 on they passed every range), and r is taken off the scores
+// themselves, which are near each other wherever a weight is left.
+//
+// fp16 holds weights from 2^-24 to 2^15 alone.  kAim uses the range above 1, and the reference moves down as well, where a tile's
+// largest weight would be under 1: what falls off is 2^-25 of its tile's largest weight or less, however far that lies below the
+// row's, so that a long tail keeps its share.  It stays within kDeep of the largest one so far: O stays
+// under 2^117 with 2^30 keys, and as many keys in tiles below that are worth 2^-26 of the result.
+constexpr float kLag = 8.0f, kFar = 1024.0f, kDeep = 56.0f;
+template <typename T> constexpr float kAim = std::is_same<T, f16_t>::value ? 7.0f : 0.0f;
+template <typename T> constexpr float kMost = std::is_same<T, f16_t>::value ? kDeep + kLag : kLag;  // powers of two that a key passes r by
 __device__ __forceinline__ float reach_of(float s, float r, float scale) { return (s - r) * scale; }
+
+// A column's reference, its rounded negative with kAim, and the largest reference so far.
+template <typename T> struct Reference {
+  float r = -INFINITY, bias = kAim<T>, peak = -INFINITY;
+  bool far = false;  // some column of the wave
+
+  // A tile's largest score: whether the reference moves to it.
+  __device__ __forceinline__ bool moves(float top, float scale) const {
+    const float lead = reach_of(top, r, scale);
+    if constexpr (std::is_same<T, f16_t>::value) return lead > kLag || (lead < -kAim<T> && reach_of(top, peak, scale) >= -kDeep);
+    else return lead > kLag;
+  }
+  // It does, where `now`; the factor of what was summed so far.  For whole waves.
+  __device__ __forceinline__ float move(bool now, float top, float scale) {
+    const float keep = now ? exp2_hw(reach_of(r, top, scale)) : 1.0f;
+    r = now ? top : r;
+    peak = fmaxf(peak, r);
+    bias = now ? __builtin_fmaf(-top, scale, kAim<T>) : bias;
+    far = __any(fabsf(bias) > kFar);
+    return keep;
+  }
+};
 
 // 16 bits a value: infinities and NaN have all exponent bits set (of either half of `two`).
 template <typename T> __device__ __forceinline__ bool not_finite(uint32_t two) {
@@ -211,7 +240,7 @@ template <typename T> __device__ __forceinline__ bool not_finite(uint32_t two) {
 
 // One row's sums over tiles first, first + step, ... < end again, by one wave and without the matrix cores: a value that
 // the row does not see cannot reach it, where a product of tiles has 0 * NaN.  For rows whose weights are sound (l finite) and
-// whose sums came out infinite or NaN.  r: their reference (scores summed in another order may pass it further: to kLag, as theirs);
+// whose sums came out infinite or NaN.  r: their reference (scores summed in another order may pass it further: to kMost, as theirs);
 // dst [d], in LDS.
 template <typename T, int TILE>
 __device__ __forceinline__ void row_again(const PagedAttentionArgs& a, const PagedWork& w, const KeyTiles& tiles, int first,
@@ -233,7 +262,7 @@ __device__ __forceinline__ void row_again(const PagedAttentionArgs& a, const Pag
 #pragma unroll 1
       for (int c = 0; c < d; ++c) s += to_f32(q[c]) * to_f32(k[c]);
     }
-    const float weight = seen ? exp2_hw(fminf(reach_of(s, r, a.scale), kLag)) : 0.0f;
+    const float weight = seen ? exp2_hw(fminf(reach_of(s, r, a.scale), kMost<T>) + kAim<T>) : 0.0f;
     const uint64_t seen_by = __ballot(seen);
 #pragma unroll 1
     for (int j = 0; j < TILE; ++j) {
