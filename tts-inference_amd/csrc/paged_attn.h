@@ -232,12 +232,6 @@ template <typename T> struct Reference {
   }
 };
 
-// 16 bits a value: infinities and NaN have all exponent bits set (of either half of `two`).
-template <typename T> __device__ __forceinline__ bool not_finite(uint32_t two) {
-  constexpr uint32_t e = std::is_same<T, bf16_t>::value ? 0x7f80u : 0x7c00u;
-  return (two & e) == e || (two & (e << 16)) == (e << 16);
-}
-
 // One row's sums over tiles first, first + step, ... < end again, by one wave and without the matrix cores: a value that
 // the row does not see cannot reach it, where a product of tiles has 0 * NaN.  For rows whose weights are sound (l finite) and
 // whose sums came out infinite or NaN.  r: their reference (scores summed in another order may pass it further: to kMost, as theirs);
