@@ -57,7 +57,8 @@ def _exact(keys, values, count, dtype, window=0, sinks=0, weights16=False):
     s, v = keys.to(dtype).double(), values.to(dtype).double()
     key = torch.arange(n, device="cuda")
     e = torch.finfo(dtype).eps / 2
-    out, off = [], []
+    out, off, size = [], [], v.abs()
+    dot = lambda x, y: (x[:, None] * y).sum(0)  # noqa: E731
     for p in range(n - count, n):
         seen = key <= p
         if window:
@@ -65,13 +66,13 @@ def _exact(keys, values, count, dtype, window=0, sinks=0, weights16=False):
         top = s[seen].max()
         w = torch.where(seen, (s - top).exp(), 0.0)
         total = w.sum()
-        y, mags = w @ v / total, w @ v.abs() / total
+        y, mags = dot(w, v) / total, dot(w, size) / total
         rel = 4 * U * (s[seen].abs().max() + top.abs()) + 2.0 ** -22
-        bound = mags * (2 * rel + (e if weights16 else e * e) + 4 * (n + 64) * U) + 2.0 ** -125 * (seen.double() @ v.abs()) / total
+        bound = mags * (2 * rel + (e if weights16 else e * e) + 4 * (n + 64) * U) + 2.0 ** -125 * dot(seen, size) / total
         if dtype == torch.float16:
             tail = -n % 64
             tops = torch.nn.functional.pad(w, (0, tail)).view(-1, 64).amax(1).repeat_interleave(64)[:n]
-            bound = bound + 2.0 ** -25 * ((tops * seen) @ v.abs()) / total
+            bound = bound + 2.0 ** -25 * dot(tops * seen, size) / total
         out.append(y)
         off.append(bound)
     return torch.stack(out), torch.stack(off)
