@@ -79,7 +79,7 @@ template <typename T, int L, int PER> __device__ __forceinline__ void qk_heads(c
     for (int i = 0; i < 8; ++i) sum += x[i] * x[i] + y[i] * y[i];
 #pragma unroll
     for (int o = 1; o < L; o <<= 1) sum += __shfl_xor(sum, o, 64);
-    if (mine && weight) {
+    if (mine && kept && weight) {  // (a norm of zeros need not be zeros)
       const float inv = 1.0f / sqrtf(sum / (float)d + a.eps);
       float wx[8], wy[8];
       unpack8<T>(*(const i32x4_t*)(weight + col), wx);
