@@ -533,7 +533,7 @@ int qtts_paged_release(const int32_t* which, int64_t requests, int32_t* lengths,
 
 /* The rows of a fused qkv projection (qtts/models/talker.py:116-136): [rows, (heads + 2 kv_heads) d],
  * row stride ldqkv, query heads first, then key heads, then value heads.
- *   h <- h / sqrt(mean h^2 + eps) * norm          query and key heads; norm [d] of dtype or NULL
+ *   h <- h / sqrt(mean h^2 + eps) * norm          query and key heads; norm [d] of dtype or NULL, eps >= 0
  *   (h_i, h_{i + d/2}) <- (h_i c_i - h_{i + d/2} s_i, h_{i + d/2} c_i + h_i s_i)      i < d / 2
  * with c, s: cos, sin [rope_rows, d / 2] fp32 at the row's position (NULL: no rotation), in
  * fp32 with one rounding at the end (the reference rounds to dtype after the norm, qtts/layers/norm.py:50-76).

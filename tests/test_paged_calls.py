@@ -56,3 +56,19 @@ def test_attention_with_weights_of_16_bits():
     with pytest.raises(ValueError, match="GPU tensor"):
         ops.paged_attention(torch.zeros(5, 4, 32, dtype=bf), torch.zeros(9, 2, 16, 32, dtype=bf), torch.zeros(9, 2, 32, 16, dtype=bf), batch,
                             weights16=True)
+
+
+def test_an_eps_that_no_norm_has():
+    entry = _lib.load().qtts_qkv_to_cache
+
+    def call(eps, qn=8320, kn=8384):
+        return entry(_at(0), 1, 2, 128, 4, 2, 16, _at(8192), _at(8256), _at(qn), _at(kn), eps, _at(8448), _at(12544), 32, _at(65536),
+                     _at(131072), 8, 16, _at(16384), None)
+
+    for eps in (-1e-6, float("nan"), float("inf"), -float("inf")):
+        for norms in ({}, {"qn": None}, {"kn": None}):
+            assert call(eps, **norms) == -1 and "eps" in _lib.last_error(), (eps, norms)
+    if not torch.cuda.is_available():
+        for eps in (0.0, 1e-6, 1.0):
+            _passes(call(eps))
+        _passes(call(-1.0, qn=None, kn=None))  # no norm, no eps

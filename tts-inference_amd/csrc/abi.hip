@@ -1026,6 +1026,7 @@ int qtts_qkv_to_cache(const void* qkv, int dtype, int64_t rows, int64_t ldqkv, i
   QTTS_REQUIRE(ldqkv >= width, "qkv_to_cache: leading dimension smaller than the row");
   QTTS_REQUIRE(ldqkv < (1ll << 36), "qkv_to_cache: size too large");
   QTTS_REQUIRE((cos == nullptr) == (sin == nullptr) && (!cos || rope_rows > 0), "qkv_to_cache: half a rotation table");
+  QTTS_REQUIRE(!(q_norm || k_norm) || (eps >= 0 && eps < INFINITY), "qkv_to_cache: an eps of %g", (double)eps);
   if (rows == 0) return QTTS_OK;
   QTTS_REQUIRE(qkv && slots && q && (!cos || positions), "qkv_to_cache: null pointer");
   QTTS_REQUIRE(((uintptr_t)qkv | (uintptr_t)q | (uintptr_t)q_norm | (uintptr_t)k_norm | (uintptr_t)cos | (uintptr_t)sin) % 16 == 0 &&
