@@ -549,7 +549,8 @@ int qtts_qkv_to_cache(const void* qkv, int dtype, int64_t rows, int64_t ldqkv, i
  * p = lengths[r] - counts[r] + i and sees the keys j <= p with j > p - window or j < sinks (window 0: all).
  *   out = sum_j w_j v_j / sum_j w_j,  w_j = exp(scale * q . k_j - max)
  * q, out: [rows, heads, d] of dtype, row strides ldq, ldo; query head h reads key-value head
- * h / (heads / kv_heads).  Rows of no request: zeros.  What a row does not see (keys
+ * h / (heads / kv_heads).  Rows of no request: zeros; whose a row is goes by starts and counts (of requests that share no row),
+ * whatever its slot, which is checked for being there alone.  What a row does not see (keys
  * and values behind it, outside the window, in places never written) does not reach it, whatever it holds.
  * min_new, max_new: bounds of the counts; requests with more than max_new get zeros.
  * Workspace: qtts_workspace_bytes(QTTS_OP_PAGED_ATTENTION, max_new * heads / kv_heads, 1, d, 0). */

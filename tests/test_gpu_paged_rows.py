@@ -6,7 +6,7 @@ from __future__ import annotations
 import pytest
 import torch
 
-from test_gpu_paged import U, _batch, _near
+from test_gpu_paged import U, _batch, _exact, _i32, _inputs, _near
 
 pytestmark = pytest.mark.gpu
 
@@ -40,3 +40,50 @@ def test_padding_rows_are_zeros_whatever_the_norm(ops, weight, eps, rope, dtype)
             x = qkv[:rows].double().view(rows, -1, d)[:, :heads]
             want = x / x.square().mean(-1, keepdim=True).sqrt()
             _near(q[:rows], want, want.abs() * U * (d / 2 + 11), "q")
+
+
+def _poisoned(shape, dtype):
+    """What the next tensor of this size is likely to find in its memory."""
+    torch.full(shape, float("nan"), dtype=dtype, device="cuda")
+
+
+@DTYPES
+@pytest.mark.parametrize("counts,heads,kv", [([1] * 9, 16, 8), ([1, 3, 60, 1, 0, 200], 8, 4)])
+def test_rows_go_by_starts_and_counts(ops, counts, heads, kv, dtype):
+    """Slots that disagree: every row of a request is computed and every other one zero, once each."""
+    q, k, v, batch = _inputs(ops, [(30 + 7 * i, n) for i, n in enumerate(counts)], 16, heads, kv, 64, dtype, seed=4, padding=6)
+    want = ops.paged_attention(q, k, v, batch)
+    off, slots = torch.full_like(batch.slots, -1), batch.slots.clone()
+    slots[-6:] = 5  # rows of no request
+    slots[0] = -1
+    for other in (off, slots, torch.zeros_like(off)):
+        odd = ops.PagedBatch(batch.table, batch.starts, batch.counts, batch.lengths, batch.positions, other, 16, max_new=batch.max_new)
+        for _ in range(3):
+            _poisoned(q.shape, dtype)
+            assert torch.equal(ops.paged_attention(q, k, v, odd), want)
+
+
+@DTYPES
+def test_gaps_between_requests(ops, dtype):
+    """Requests with rows of none between and behind them, more than a workgroup's share of rows (its span of 1024 several times)."""
+    at, counts = [3, 1030, 1100, 2047, 250000, 300000 - 41], [1, 70, 0, 2, 40, 41]
+    rows, n = 300000, 100
+    table = _i32([[i * 7 + j for j in range(7)] for i in range(6)])
+    lengths = [n if c else 0 for c in counts]
+    batch = ops.PagedBatch(table, _i32(at + [rows]), _i32(counts), _i32(lengths), _i32([-1] * rows), _i32([-1] * rows), 16, max_new=70)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    q, k, v = (torch.randn(s, generator=g, device="cuda").to(dtype) for s in ((rows, 1, 16), (42, 1, 16, 16), (42, 1, 16, 16)))
+    _poisoned(q.shape, dtype)
+    out = ops.paged_attention(q, k, v, batch)
+    live = torch.zeros(rows, dtype=torch.bool, device="cuda")
+    for a, c in zip(at, counts):
+        live[a:a + c] = True
+    assert not out[~live].any()
+    want, off = _exact(q, k, v, batch, 0, 0, 0.25)
+    _near(out[live], want[live], off[live], "rows of requests")
+    bad = [a if i != 1 else -5 for i, a in enumerate(at)]  # and where one of them is nothing that a step makes
+    odd = ops.PagedBatch(table, _i32(bad + [rows]), batch.counts, batch.lengths, batch.positions, batch.slots, 16, max_new=70)
+    _poisoned(q.shape, dtype)
+    again = ops.paged_attention(q, k, v, odd)
+    out[at[1]:at[1] + counts[1]] = 0
+    assert torch.equal(again, out)

@@ -1091,7 +1091,6 @@ static int paged_attention(bool weights16, const void* q, int dtype, int64_t row
   a.starts = starts;
   a.counts = counts;
   a.lengths = lengths;
-  a.slots = slots;
   a.rows = (int32_t)rows;
   a.heads = (int32_t)heads;
   a.requests = (int32_t)requests;

@@ -59,7 +59,6 @@ struct PagedAttentionArgs {
   const int32_t* starts;
   const int32_t* counts;
   const int32_t* lengths;
-  const int32_t* slots;  // [rows], -1 where no request has the row
   PagedCache cache;
   int32_t rows, heads, requests, cols, max_new, window, sinks;
   float scale;  // times log2 e

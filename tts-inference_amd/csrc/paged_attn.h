@@ -139,23 +139,35 @@ __device__ __forceinline__ bool paged_work(const PagedLaunch& p, int item, Paged
   return false;
 }
 
-// Rows without a request, and those of requests that no run takes: zeros.  Group g of p.fill.
+// Rows that no run writes: zeros.  Which those are goes by the requests alone, as the runs do (a slot may say otherwise: -1 where a
+// table's entry is no page, or none of a request's), so that every row is written once.  Group g of p.fill takes a share of the
+// rows, kFillSpan at a time, and marks in LDS what the requests cover of them.
+constexpr int kFillSpan = 1024;
 template <typename T> __device__ __forceinline__ void fill_rows(const PagedLaunch& p, int g) {
+  __shared__ uint32_t covered[kFillSpan / 32];
   const PagedAttentionArgs& a = p.a;
-  const int vecs = a.heads * a.cache.d / 8;
+  const int vecs = a.heads * a.cache.d / 8, share = (a.rows + p.fill - 1) / p.fill;
+  const int end = min(a.rows, (g + 1) * share);
   const i32x4_t zero = {0, 0, 0, 0};
-  for (int64_t row = g; row < a.rows; row += p.fill) {
-    if (a.slots[row] >= 0) continue;
-    T* out = (T*)a.out + row * a.ldo;
-    for (int i = threadIdx.x; i < vecs; i += blockDim.x) *(i32x4_t*)(out + 8 * i) = zero;
-  }
-  for (int r = g; r < a.requests; r += p.fill) {
-    if (a.counts[r] <= 0 || load_request(a, r).count) continue;
-    const int64_t lo = a.starts[r] > 0 ? a.starts[r] : 0, end = min((int64_t)a.starts[r] + a.counts[r], (int64_t)a.starts[r + 1]);
-    for (int64_t row = lo; row < end && row < a.rows; ++row) {
-      T* out = (T*)a.out + row * a.ldo;
+  for (int first = g * share; first < end; first += kFillSpan) {
+    const int rows = min(kFillSpan, end - first);
+    if (threadIdx.x < kFillSpan / 32) covered[threadIdx.x] = 0;
+    __syncthreads();
+    for (int r = threadIdx.x; r < a.requests; r += blockDim.x) {
+      const PagedRequest q = load_request(a, r);
+      const int stop = min(q.start + q.count - first, rows);
+      for (int at = max(q.start - first, 0), next; at < stop; at = next) {
+        next = min((at | 31) + 1, stop);
+        atomicOr(&covered[at >> 5], (uint32_t)(((1ull << (next - at)) - 1) << (at & 31)));
+      }
+    }
+    __syncthreads();
+    for (int t = 0; t < rows; ++t) {
+      if ((covered[t >> 5] >> (t & 31)) & 1) continue;
+      T* out = (T*)a.out + (int64_t)(first + t) * a.ldo;
       for (int i = threadIdx.x; i < vecs; i += blockDim.x) *(i32x4_t*)(out + 8 * i) = zero;
     }
+    __syncthreads();
   }
 }
 
