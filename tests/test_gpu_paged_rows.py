@@ -87,3 +87,43 @@ def test_gaps_between_requests(ops, dtype):
     again = ops.paged_attention(q, k, v, odd)
     out[at[1]:at[1] + counts[1]] = 0
     assert torch.equal(again, out)
+
+
+@DTYPES
+@pytest.mark.parametrize("captured,later", [([1, 1], [3, 4]), ([0, 0, 0], [5, 0, 1]), ([2, 1], [1, 0, 7]), ([1] * 8, [8])])
+def test_a_graph_of_a_step_without_max_new(ops, captured, later, dtype):
+    """A step's own largest count bounds that step alone: a graph captured after it replays for counts up to its rows."""
+    from qtts_amd import PagedCache, attend
+    g = torch.Generator(device="cuda").manual_seed(3)
+    attn = torch.nn.Module()
+    caches = [PagedCache(1, 9, 40, 4, 1, 64, page_size=16, max_rows=64, dtype=dtype, rope_theta=1e4) for _ in range(2)]
+    prompt = torch.randn(40, 6 * 64, generator=g, device="cuda").to(dtype)
+    for c in caches:
+        c.k[0].zero_(), c.v[0].zero_()
+        c.step([20, 15, 5])
+        attend(attn, prompt, c, 0)
+    x = torch.randn(8, 6 * 64, generator=g, device="cuda").to(dtype)
+    for c in caches:
+        c.step(captured, rows=8)
+        attend(attn, x, c, 0)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = attend(attn, x, caches[1], 0)
+    for n, new in enumerate((later, captured, later, [1, 2, 3])):
+        x.copy_(torch.randn(8, 6 * 64, generator=g, device="cuda").to(dtype))
+        for c in caches:
+            c.step(new, rows=8)
+        want = attend(attn, x, caches[0], 0)
+        graph.replay()
+        # of runs of one kernel or the other: within two steps of the largest value
+        assert ((out.double() - want.double()).abs() <= 2 * torch.finfo(dtype).eps * x.abs().max()).all(), n
+        assert torch.equal(out.any(1), want.any(1)) and int(want.any(1).sum()) == sum(new)
+    # a bound that the caller gives stands for the graph as well: more tokens than it are zeros
+    for c in caches:
+        c.step([1, 1], rows=8, max_new=1)
+    tight = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(tight):
+        out = attend(attn, x, caches[1], 0)
+    caches[1].step([1, 3], rows=8)
+    tight.replay()
+    assert out[0].any() and not out[1:].any()

@@ -11,8 +11,8 @@ Per step, a serving loop says how many tokens join each request, then runs the m
     cache = PagedCache(layers=28, requests=64, pages=4096, heads=16, kv_heads=8, head_dim=128, rope_theta=1e6)
     cache.step([37, 12])                     # two prompts, 49 rows
     ...
-    cache.step([1, 1, 0, 1], rows=8)         # decode: requests 0, 1 and 3, padded to the captured batch of 8
-    graph.replay()                           # reads the cache's buffers
+    cache.step([1, 1, 0, 1], rows=8, max_new=1)   # decode: requests 0, 1 and 3, padded to the captured batch of 8
+    graph.replay()                           # captured after such a step; reads the cache's buffers
     cache.release([1])                       # its pages are free again
 
 A request is a row of the table; its number is the caller's.  Rows of the batch lie in the order of the requests.
@@ -41,7 +41,8 @@ def rope_tables(length: int, head_dim: int, theta: float = 1e6, device: torch.de
 class PagedCache:
     """Keys and values of up to ``requests`` requests in ``pages`` pages of ``page_size`` tokens, for ``layers`` layers, in
     buffers that keep their addresses: a graph captured after one :meth:`step` reads, on every replay, what the last one
-    wrote (positions -1, and no attention, for rows that it does not have).
+    wrote (positions -1, and no attention, for rows that it does not have).  The graph has that step's ``rows`` and, where it was
+    given, its ``max_new``: requests with more new tokens, or rows past those, get zeros.
 
     ``max_length``: tokens a request can have (None: as many as the pool holds); ``max_rows``: rows of a step.  ``rope_theta``:
     the base of the rotation's angles (None: no rotation; ``rope`` takes tables of the caller's own)."""
@@ -88,15 +89,18 @@ class PagedCache:
         """``new[r]`` tokens join request r (requests past the end of ``new``: none), in a batch of ``rows`` rows with padding
         rows behind.  Numbers on the host are checked here.  A tensor on the GPU is not read: ``rows`` is then required,
         ``max_new`` bounds its entries (None: ``rows``), and what does not fit is denied (``batch.counts`` 0).  Requests whose pages are not left
-        are denied in either case."""
-        new = self._whole(new, "new")
+        are denied in either case.
+
+        A captured call keeps ``max_new`` (1: the decode step's kernel alone); without it, it is made for up to ``rows`` tokens a request,
+        whatever this step's are."""
+        new, this_step = self._whole(new, "new"), False
         if new.shape[0] > self.requests:
             raise ValueError(f"new must have up to {self.requests} entries, got {new.shape[0]}")
         if new.device.type == "cpu":
             given = new.tolist()
             if any(n < 0 for n in given):
                 raise ValueError(f"new must not be negative: {given}")
-            total, most = sum(given), max(given, default=0)
+            total, most, this_step = sum(given), max(given, default=0), max_new is None
             rows = total if rows is None else int(rows)
             if total > rows:
                 raise ValueError(f"{total} new tokens do not fit a batch of {rows} rows")
@@ -119,7 +123,7 @@ class PagedCache:
         if given < self.requests:
             self._new[given:].zero_()
         batch = ops.PagedBatch(self.table, self._starts, self._counts, self.lengths, self._positions[:rows], self._slots[:rows],
-                               self.page_size, max_new, min_new, self.taken)
+                               self.page_size, max_new, min_new, self.taken, this_step)
         ops.paged_step(self._new, self.lengths, self.table, self.free, self.taken, self.page_size, rows, out=batch, room=self.max_rows)
         self.batch = batch
         return batch
@@ -168,7 +172,7 @@ def attend(attn: nn.Module, qkv: torch.Tensor, cache: PagedCache, layer: int, wi
         qkv, weights, eps = torch.cat([q, k, v], 1), [None, None], 1e-6
     cos, sin = cache.rope if cache.rope is not None else (None, None)
     state = [batch.table, batch.starts, batch.counts, batch.lengths, batch.positions, batch.slots]
-    bounds = [batch.page_size, batch.max_new, batch.min_new]
+    bounds = [batch.page_size, batch.max_new, batch.min_new, int(batch.this_step)]
     q = torch.ops.qtts.qkv_to_cache(qkv.reshape(rows, width), cache.k[layer], cache.v[layer], state, bounds, cache.heads, weights[0],
                                     weights[1], eps, cos, sin)
     out = torch.ops.qtts.paged_attention(q, cache.k[layer], cache.v[layer], state, bounds, window, sinks,

@@ -1055,14 +1055,15 @@ class PagedBatch:
     ``starts[r] + counts[r]``, its tokens (the rows among them) ``lengths[r]``, on the pages ``table[r]`` of ``page_size`` tokens;
     ``positions`` and ``slots`` ``[rows]`` say where each row belongs (-1: to no request).  All contiguous int32 on one GPU.
     ``min_new`` and ``max_new`` bound the counts of every step that these tensors will hold; ``taken`` ``[1]`` is the
-    free list's state after the step (None where the batch was made by hand)."""
+    free list's state after the step (None where the batch was made by hand).  ``this_step``: ``max_new`` is of the step at hand
+    alone, and a call that a graph captures takes ``rows`` in its place."""
 
     __slots__ = ("table", "starts", "counts", "lengths", "positions", "slots", "page_size", "requests", "cols", "rows", "max_new",
-                 "min_new", "taken")
+                 "min_new", "taken", "this_step")
 
     def __init__(self, table: torch.Tensor, starts: torch.Tensor, counts: torch.Tensor, lengths: torch.Tensor,
                  positions: torch.Tensor, slots: torch.Tensor, page_size: int, max_new: int | None = None, min_new: int = 0,
-                 taken: torch.Tensor | None = None) -> None:
+                 taken: torch.Tensor | None = None, this_step: bool = False) -> None:
         if table.dim() != 2 or table.dtype is not torch.int32 or not table.is_contiguous():
             raise ValueError(f"the page table must be contiguous int32 [requests, columns], got {table.dtype} {tuple(table.shape)}")
         requests, rows, idx = table.size(0), positions.numel(), table.get_device()
@@ -1077,6 +1078,7 @@ class PagedBatch:
                                                                                           slots)
         self.page_size, self.requests, self.cols, self.rows, self.taken = int(page_size), requests, table.size(1), rows, taken
         self.max_new, self.min_new = rows if max_new is None else int(max_new), int(min_new)
+        self.this_step = bool(this_step)
 
 
 def _check_int32(name: str, t: torch.Tensor, size: int, idx: int) -> None:
@@ -1277,7 +1279,8 @@ def paged_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, batch: Pa
     out = torch.empty(rows, heads, d, dtype=q.dtype, device=q.device)
     if not rows:
         return out
-    need, ws = attention_bytes(min(batch.max_new, rows) * (heads // kv_heads), d), _workspaces.get(idx)
+    max_new = rows if batch.this_step and torch.cuda.is_current_stream_capturing() else batch.max_new
+    need, ws = attention_bytes(min(max_new, rows) * (heads // kv_heads), d), _workspaces.get(idx)
     if ws is None or ws.numel() < need:
         _ensure_workspace(q.device, need, "paged_attention")
         ws = _workspaces[idx]
@@ -1285,7 +1288,7 @@ def paged_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, batch: Pa
     st = (lib.qtts_paged_attention_w16 if weights16 else lib.qtts_paged_attention)(
         q.data_ptr(), dtype_code(q.dtype), rows, q.stride(0) if rows > 1 else heads * d, heads, kv_heads, d, k.data_ptr(), v.data_ptr(),
         pages, batch.page_size, batch.table.data_ptr(), batch.requests, batch.cols, batch.starts.data_ptr(),
-        batch.counts.data_ptr(), batch.lengths.data_ptr(), batch.slots.data_ptr(), batch.min_new, batch.max_new, window, sinks,
+        batch.counts.data_ptr(), batch.lengths.data_ptr(), batch.slots.data_ptr(), batch.min_new, max_new, window, sinks,
         d ** -0.5 if scale is None else scale, out.data_ptr(), heads * d, ws.data_ptr(), ws.numel(), _raw_stream(idx))
     if st:
         _lib.check(st, "paged_attention")

@@ -274,8 +274,9 @@ def _(base, x, index, plan, slots, a, b, scaling, ranks, partitions):
 # ---- attention over a paged cache (layers/attention.py) ---------------------------------------
 
 def _batch(state: list[torch.Tensor], bounds: list[int]) -> "ops.PagedBatch":
-    """A step's batch from its tensors (table, starts, counts, lengths, positions, slots) and page size, max_new and min_new."""
-    return ops.PagedBatch(*state, bounds[0], max_new=bounds[1], min_new=bounds[2])
+    """A step's batch from its tensors (table, starts, counts, lengths, positions, slots) and page size, max_new, min_new and
+    whether max_new is of this step alone (no, where it is left out)."""
+    return ops.PagedBatch(*state, bounds[0], max_new=bounds[1], min_new=bounds[2], this_step=any(bounds[3:]))
 
 
 @torch.library.custom_op(f"{_LIB}::qkv_to_cache", mutates_args=("k", "v"))
