@@ -552,7 +552,7 @@ int qtts_qkv_to_cache(const void* qkv, int dtype, int64_t rows, int64_t ldqkv, i
  * h / (heads / kv_heads).  Rows of no request: zeros; whose a row is goes by starts and counts (of requests that share no row),
  * whatever its slot, which is checked for being there alone.  What a row does not see (keys
  * and values behind it, outside the window, in places never written) does not reach it, whatever it holds.
- * min_new, max_new: bounds of the counts; requests with more than max_new get zeros.
+ * min_new, max_new: bounds of the counts; requests with more than max_new get zeros.  Fewer than 2^31 rows times heads.
  * Workspace: qtts_workspace_bytes(QTTS_OP_PAGED_ATTENTION, max_new * heads / kv_heads, 1, d, 0). */
 int qtts_paged_attention(const void* q, int dtype, int64_t rows, int64_t ldq, int64_t heads, int64_t kv_heads, int64_t d,
                          const void* k, const void* v, int64_t pages, int64_t page_size, const int32_t* table, int64_t requests,

@@ -72,3 +72,14 @@ def test_an_eps_that_no_norm_has():
         for eps in (0.0, 1e-6, 1.0):
             _passes(call(eps))
         _passes(call(-1.0, qn=None, kn=None))  # no norm, no eps
+
+
+def test_rows_times_heads_past_32_bits():
+    """A request's rows of one key-value head are counted in 32 bits and make a grid of fewer than 2^32 threads."""
+    for entry in (_lib.load().qtts_paged_attention, _lib.load().qtts_paged_attention_w16):
+        for rows, heads, kv in ((1 << 20, 2048, 1), ((1 << 24) - 1, 4096, 4), ((1 << 24) - 1, 129, 129)):
+            # (q and out: any addresses that do not overlap; nothing is read)
+            status = _attention(entry, rows=rows, heads=heads, kv=kv, ldq=heads * 16, ldo=heads * 16, q=0, out=1 << 45, k=1 << 50, v=1 << 51)
+            assert status == -1 and "too large" in _lib.last_error(), (rows, heads, status, _lib.last_error())
+        if not torch.cuda.is_available():
+            _passes(_attention(entry, rows=(1 << 20) - 1, heads=2048, kv=1, ldq=2048 * 16, ldo=2048 * 16, q=0, out=1 << 45, k=1 << 50, v=1 << 51))

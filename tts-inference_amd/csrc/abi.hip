@@ -1063,7 +1063,7 @@ static int paged_attention(bool weights16, const void* q, int dtype, int64_t row
   qtts::PagedAttentionArgs a = {};
   QTTS_TRY(paged_cache("paged_attention", a.cache, k, v, pages, page_size, heads, kv_heads, d));
   QTTS_REQUIRE(rows >= 0 && min_new >= 0 && max_new >= 0 && window >= 0 && sinks >= 0, "paged_attention: negative size");
-  QTTS_REQUIRE(rows < (1ll << 24), "paged_attention: size too large");
+  QTTS_REQUIRE(rows < (1ll << 24) && rows * heads < (1ll << 31), "paged_attention: size too large");
   QTTS_REQUIRE(ldq >= heads * d && ldo >= heads * d, "paged_attention: leading dimension smaller than the row");
   QTTS_REQUIRE(ldq < (1ll << 36) && ldo < (1ll << 36), "paged_attention: size too large");
   // (up to where the scale of exponentials of 2 is finite)

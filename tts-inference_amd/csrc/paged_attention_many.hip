@@ -84,11 +84,11 @@ template <typename T, int DP, bool EXACT, bool WIDE, bool W16> __global__ __laun
 
   // tokens of the run, and of this wave's rows
   const int run_lo = w.position + (int)(first_row / group);
-  const int run_hi = w.position + (int)(min(first_row + kRun, rows) - 1) / group;
+  const int run_hi = w.position + (int)((min(first_row + kRun, rows) - 1) / group);
   const int64_t wave_row = first_row + wave * kWaveRows;
   const bool busy = wave_row < rows;
   const int wave_lo = w.position + (int)(wave_row / group);
-  const int wave_hi = busy ? w.position + (int)(min(wave_row + kWaveRows, rows) - 1) / group : -1;
+  const int wave_hi = busy ? w.position + (int)((min(wave_row + kWaveRows, rows) - 1) / group) : -1;
 
   const KeyTiles tiles = key_tiles<kTile>(run_lo, run_hi, a.window, a.sinks);
   const int splits = (tiles.count + w.chunk - 1) / w.chunk;  // w.splits or fewer
