@@ -127,3 +127,15 @@ def test_a_graph_of_a_step_without_max_new(ops, captured, later, dtype):
     caches[1].step([1, 3], rows=8)
     tight.replay()
     assert out[0].any() and not out[1:].any()
+
+
+def test_bounds_that_out_does_not_have(ops):
+    """A step into a batch takes the batch's bounds: other ones beside it are refused, not left aside."""
+    table, lengths, free, taken = _i32([[-1] * 4] * 2), _i32([0, 0]), _i32(list(range(8))), _i32([0])
+    out = ops.paged_step(_i32([0, 0]), lengths, table, free, taken, 16, 9, max_new=5, min_new=1)
+    args = (_i32([4, 2]), lengths, table, free, taken, 16, 9)
+    for kw in ({"max_new": 3}, {"max_new": 9}, {"min_new": 2}):
+        with pytest.raises(ValueError, match="new"):
+            ops.paged_step(*args, out=out, **kw)
+    for kw in ({}, {"max_new": 5}, {"min_new": 1}, {"max_new": 5, "min_new": 1}):
+        assert ops.paged_step(*args, out=out, **kw).counts.tolist() == [4, 2]

@@ -1110,7 +1110,7 @@ def paged_step(new: torch.Tensor, lengths: torch.Tensor, table: torch.Tensor, fr
     Everything is int32 on the GPU, so a captured step follows what the tensors hold at each replay.  A request whose rows
     pass ``max_new`` (None: ``rows``) or the batch, whose tokens pass the table or whose pages are not left is denied as a whole:
     ``counts`` 0, its rows at position and slot -1.  Returns a batch of fresh tensors on the same table, or ``out`` (of the
-    same sizes; its lengths and taken may be the ones given).  room: entries that lie behind ``out``'s positions and slots in
+    same sizes and bounds; its lengths and taken may be the ones given).  room: entries that lie behind ``out``'s positions and slots in
     their buffers, rows among them; those past the batch get -1 (a step captured with more rows reads them)."""
     rows = int(rows)
     if rows < 0:
@@ -1129,6 +1129,8 @@ def paged_step(new: torch.Tensor, lengths: torch.Tensor, table: torch.Tensor, fr
     elif (out.requests != requests or out.rows != rows or out.page_size != page_size or out.taken is None
           or out.table.data_ptr() != table.data_ptr()):
         raise ValueError(f"out is no batch of {rows} rows and {requests} requests on this page table")
+    elif (max_new is not None and int(max_new) != out.max_new) or (min_new and int(min_new) != out.min_new):
+        raise ValueError(f"out is a batch of {out.min_new} to {out.max_new} new tokens a request, not of {min_new} to {max_new}")
     room, positions, slots = rows if room is None else int(room), out.positions.data_ptr(), out.slots.data_ptr()
     if room > rows:
         for t in (out.positions, out.slots):
