@@ -139,3 +139,31 @@ def test_bounds_that_out_does_not_have(ops):
             ops.paged_step(*args, out=out, **kw)
     for kw in ({}, {"max_new": 5}, {"min_new": 1}, {"max_new": 5, "min_new": 1}):
         assert ops.paged_step(*args, out=out, **kw).counts.tolist() == [4, 2]
+
+
+@DTYPES
+def test_head_norms_of_another_type(ops, dtype):
+    """A norm whose weight is in 32 bits runs as the module it is (in 16 its weight would be rounded), and so does one that
+    returns 32 bits."""
+    from qtts_amd import PagedCache, attend
+    from test_gpu_w8a8_layer import Norm
+    d, heads, kv, rows = 64, 4, 2, 40
+
+    class Wide(Norm):
+        def forward(self, x):
+            return super().forward(x.float())
+
+    g = torch.Generator(device="cuda").manual_seed(6)
+    qkv = torch.randn(rows, (heads + 2 * kv) * d, generator=g, device="cuda").to(dtype)
+    attn = torch.nn.Module()
+    for kind, weight in ((Norm, torch.float32), (Wide, torch.float32), (Wide, dtype), (Norm, dtype)):
+        attn.q_norm, attn.k_norm = kind(d, weight), kind(d, weight)
+        cache = PagedCache(1, 1, 4, heads, kv, d, page_size=16, max_rows=rows, dtype=dtype)
+        batch = cache.step([rows])
+        attend(attn, qkv, cache, 0)
+        slot = batch.slots.long()
+        got = cache.k[0][slot // 16, :, slot % 16]
+        x = qkv.view(rows, -1, d)[:, heads:heads + kv].double()
+        want = x / (x.square().mean(-1, keepdim=True) + 1e-6).sqrt() * attn.k_norm.weight.double()
+        # the module in fp32: half of the sum's relative error, then a root, a division, two products
+        _near(got, want, want.abs() * U * (d / 2 + 11), kind.__name__)

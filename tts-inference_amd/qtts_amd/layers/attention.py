@@ -152,7 +152,7 @@ def attend(attn: nn.Module, qkv: torch.Tensor, cache: PagedCache, layer: int, wi
     """The attention between qkv_proj and o_proj (talker.py:249-270) for the rows of the cache's step: head norms
     (``attn.q_norm``, ``attn.k_norm``, None or missing: none), rotation, this layer's cache, attention.  qkv
     ``[..., (Hq + 2 H) D]`` is qkv_proj's output; returns ``[..., Hq D]``, o_proj's input.  Norms that are no RMSNorm of one weight
-    run as the modules they are.  weights16: :func:`~qtts_amd.ops.paged_attention`'s, for prompts whose time counts more than their
+    in qkv's type run as the modules they are.  weights16: :func:`~qtts_amd.ops.paged_attention`'s, for prompts whose time counts more than their
     last bits."""
     d, kv = cache.head_dim, cache.kv_heads
     shape, width = qkv.shape, (cache.heads + 2 * kv) * d
@@ -162,13 +162,13 @@ def attend(attn: nn.Module, qkv: torch.Tensor, cache: PagedCache, layer: int, wi
     batch = cache.batch_for(rows)
     norms = [getattr(attn, name, None) for name in ("q_norm", "k_norm")]
     eps = {norm_eps(n) for n in norms if n is not None}
-    if all(n is None or (is_rms_norm(n) and n.weight.dim() == 1 and n.weight.shape[0] == d) for n in norms) and len(eps) <= 1:
+    if all(n is None or (is_rms_norm(n) and n.weight.shape == (d,) and n.weight.dtype == qkv.dtype) for n in norms) and len(eps) <= 1:
         weights = [None if n is None else n.weight for n in norms]
         eps = next(iter(eps), 1e-6)
     else:
         x = qkv.reshape(rows, cache.heads + 2 * kv, d)
         q, k, v = x.split([cache.heads, kv, kv], 1)
-        q, k = (t if n is None else n(t) for n, t in zip(norms, (q, k)))
+        q, k = (t if n is None else n(t).to(qkv.dtype) for n, t in zip(norms, (q, k)))
         qkv, weights, eps = torch.cat([q, k, v], 1), [None, None], 1e-6
     cos, sin = cache.rope if cache.rope is not None else (None, None)
     state = [batch.table, batch.starts, batch.counts, batch.lengths, batch.positions, batch.slots]
