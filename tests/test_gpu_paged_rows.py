@@ -167,3 +167,13 @@ def test_head_norms_of_another_type(ops, dtype):
         want = x / (x.square().mean(-1, keepdim=True) + 1e-6).sqrt() * attn.k_norm.weight.double()
         # the module in fp32: half of the sum's relative error, then a root, a division, two products
         _near(got, want, want.abs() * U * (d / 2 + 11), kind.__name__)
+
+
+@DTYPES
+@pytest.mark.parametrize("heads,kv,d", [(200, 1, 16), (512, 2, 64), (129, 1, 128), (1024, 1024, 16), (1000, 8, 32)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (20, 3)])
+def test_many_query_heads(ops, heads, kv, d, window, sinks, dtype):
+    """A token's query heads past a run's rows, and so many key-value heads that nothing is cut."""
+    q, k, v, batch = _inputs(ops, [(70, 1), (0, 3), (33, 2), None], 16, heads, kv, d, dtype, seed=heads, padding=2)
+    want, off = _exact(q, k, v, batch, window, sinks, d ** -0.5)
+    _near(ops.paged_attention(q, k, v, batch, window, sinks), want, off, "rows")

@@ -236,3 +236,22 @@ def test_tails_of_many_heads(ops, count, dtype):
     """So many heads that each one's keys stay with a few waves, whose own keys are a tail behind the one that stands out."""
     keys, values = _tail(4096, "first", 17.5, 0.0, torch.Generator(device="cuda").manual_seed(5))
     _check(ops, keys, values, count, dtype, heads=1024, kv=1024)
+
+
+@pytest.mark.parametrize("method", ["none", "fp8"])
+def test_weights_of_16_bits_in_whole_layers(ops, method):
+    from qtts_amd.layers.decoder import paged_layer, paged_layer_w8a8
+    from test_gpu_paged_layer import _cache, _model, _rows
+    dtype = torch.bfloat16
+    layer, x = _model(method, dtype, layers=1)[0], _rows(50, torch.bfloat16, 1)
+    outs = []
+    for w in (False, True, False):
+        cache = _cache(dtype, layers=1)
+        cache.step([50])
+        if method == "none":
+            outs.append(paged_layer(layer, x, cache, 0, weights16=w))
+        else:
+            delta, hidden = paged_layer_w8a8(layer, x, None, cache, 0, weights16=w)
+            outs.append(hidden + delta)
+    assert torch.equal(outs[0], outs[2]) and not torch.equal(outs[0], outs[1])
+    assert outs[1].isfinite().all()
