@@ -561,7 +561,8 @@ int qtts_paged_attention(const void* q, int dtype, int64_t rows, int64_t ldq, in
                          void* out, int64_t ldo, void* ws, int64_t ws_bytes, void* stream);
 
 /* The same with the softmax's weights rounded to dtype (half a step of each, the size of the result's own rounding) for requests of
- * more than 16 rows a key-value head: 0.7 of the time of a long prompt.  Requests of fewer rows are computed as above. */
+ * more than 16 rows a key-value head: 280 us instead of 398 for
+ * one of 8192 tokens, 16 query and 8 key-value heads of 128.  Requests of fewer rows are computed as above. */
 int qtts_paged_attention_w16(const void* q, int dtype, int64_t rows, int64_t ldq, int64_t heads, int64_t kv_heads, int64_t d,
                              const void* k, const void* v, int64_t pages, int64_t page_size, const int32_t* table, int64_t requests,
                              int64_t cols, const int32_t* starts, const int32_t* counts, const int32_t* lengths,

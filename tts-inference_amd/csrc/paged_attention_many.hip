@@ -9,18 +9,18 @@
 // (swizzles below; ds_read_b128 serves the lanes as pipe.h says).
 //
 // P goes to the second product in two 16-bit parts, whose products add up to P's in 16 bits (bf16) or 22 (fp16), so that sums that
-// cancel keep their bits.  In one part (W16, where the caller asks for it) a weight is rounded by half a step of the type, and its sum
-// with it: the 8192 tokens below 277 us instead of 399, the 16384 180 instead of 222, the 4 x 1003 102 instead of 133.
+// cancel keep their bits; where fp16's parts end, and what keeps a long tail above that: paged_attn.h.  In one part (W16, where the
+// caller asks for it) a weight is rounded by half a step of the type: two products of three, half of the softmax's instructions.
 //
-// One prompt of 8192 tokens, 16 query and 8 key-value heads of 128 in bf16 (275 GFLOP): 271 us, 1016 TFLOP/s, where
-// a large library product reaches 1530 (2250 on zeros: the card's power bounds its clock).  The matrix cores are busy 46% of
-// the cycles and the vector units 41%, the softmax's 5.1e7 instructions to 8.5e6 MFMAs; LDS reads meet no bank twice
-// (0 conflicts).  Without the softmax it took 252 us, without the loads 241, without the second product 224: no one of them
-// is what is waited for, the two waves a SIMD just do not fill each other's gaps.  Operands further ahead, wave
+// One prompt of 8192 tokens, 16 query and 8 key-value heads of 128 in bf16 (275 GFLOP): 398 us, 691 TFLOP/s (W16: 280 us, 980), where
+// a large library product reaches 1530 (2250 on zeros: the card's power bounds its clock, 2.0 GHz here).  The matrix cores are
+// busy 49% of the cycles and the vector units 44%, 8.3e7 instructions to 1.27e7 MFMAs (W16: 46, 41, 5.1e7, 8.5e6); LDS reads meet
+// no bank twice.  With W16 it takes 252 us without the softmax, 241 without the loads, 224 without the second product: no one of
+// them is what is waited for, the two waves a SIMD do not fill each other's gaps.  Operands further ahead, wave
 // priorities and loads that the compiler does not count gave nothing; waves of 64 rows, one a SIMD, 373 us; the next tile's
-// scores beside this one's softmax in a wave spilled 63 registers (554 us).  16384 tokens under a window of 1024: 177 us, 756
-// TFLOP/s of what the rows see (every run of 64 tokens has two or three masked tiles of 18); 4 x 1003 tokens behind 2500 on
-// pages of 32: 100 us, 699.
+// scores beside this one's softmax in a wave spilled 63 registers (554 us).  Both parts' products by groups of operands instead of
+// one after the other: 396 us.  16384 tokens under a window of 1024: 223 us, 598 TFLOP/s of what the rows see (W16: 177, 755; every
+// run of 64 tokens has two or three masked tiles of 18); 4 x 1003 tokens behind 2500 on pages of 32: 136 us, 512 (W16: 105, 660).
 #include "paged_attn.h"
 #include "pipe.h"
 

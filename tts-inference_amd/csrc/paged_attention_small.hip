@@ -14,9 +14,10 @@
 // Splits: the tiles of all requests are cut into pieces of one size, and a request's last workgroup to finish joins its
 // pieces (paged_attn.h).
 //
-// The cache's bytes bound it: 64 requests of up to 8192 tokens, 16 query and 8 key-value heads of 128 in fp16 (1.20 GB): 221 us,
+// The cache's bytes bound it: 64 requests of up to 8192 tokens, 16 query and 8 key-value heads of 128 in fp16 (1.20 GB): 222 us,
 // 5.4 TB/s, as fast as the card reads (a sum over a large tensor: 5.2); one request of 65536 tokens (268 MB): 47 us,
-// 5.7 TB/s with part of it left in the Infinity Cache; 27 windows of 512 tokens on pages of 16 (57 MB): 15 us.  Short
+// 5.7 TB/s with part of it left in the Infinity Cache; 27 windows of 512 tokens on pages of 16 (57 MB): 15 us, 18
+// where the pages come from memory.  Short
 // ones are latency: 1 x 300 tokens 9.9 us captured, of which the empty launch 2.5, the work list 1.2, the page table 1.3,
 // the first tile's keys and values 3.6 and the join of the waves and splits 1.3.  Three workgroups a compute unit with
 // a tile's keys and values in registers ahead of their use keep the loads out; 64 keys a step or 8 waves gave nothing.

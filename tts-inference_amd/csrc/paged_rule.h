@@ -74,8 +74,8 @@ constexpr QTTS_RULE PagedCut small_cut(int64_t pairs) {
   return pairs < 128 ? PagedCut{512, 8} : pairs < 256 ? PagedCut{512, 16} : PagedCut{kCutGroups, 16};
 }
 // Runs of up to 128 rows (tiles of 64 keys, two workgroups a compute unit): one round of them (512 rows behind 30000 tokens:
-// 132 us captured, in 256 workgroups 170, in 1024 172; 4 x 1003 behind 2500: 100, 100, 113), and whole runs sooner where each
-// unit has one (8 x 300 behind 1000 under a window of 512: 26.9, with 8 tiles as the least 31.4; 1 x 1000: 22.1, with 16: 27.0).
+// 176 us captured, in 256 workgroups 204, in 1024 210; 4 x 1003 behind 2500: 136, 136, 149), and whole runs sooner where each
+// unit has one (8 x 300 behind 1000 under a window of 512: 31.1, with 8 tiles as the least 33.3; 1 x 1000: 24.7, with 16: 32.0).
 constexpr QTTS_RULE PagedCut many_cut(int64_t pairs) { return PagedCut{512, pairs < 256 ? 8 : 16}; }
 
 // Tiles a split, where `total` tiles (of all runs, one head) are wanted in about `groups` workgroups a head.
@@ -93,8 +93,8 @@ QTTS_RULE int32_t splits_of(int32_t tiles, uint32_t share) {
 }
 // The share of a run whose parts cost the one workgroup that joins them `part` tiles' time each: the time, share + part
 // tiles / share, is least at a share of sqrt(part tiles).
-// Up to 128 rows: a part costs what a tile does, about 1 us either (100 rows behind 20000 tokens, 314 tiles: 47 us in 17
-// parts, 58 in 9, 72 in 39).  Up to 16 rows: by the part's numbers (1 x 65536 tokens, 16 query heads of 128 on one: 36 us in 91
+// Up to 128 rows: a part costs what a tile does, about 1 us either (100 rows behind 20000 tokens, 314 tiles: 51 us in 17
+// parts, 66 in 9, 76 in 39).  Up to 16 rows: by the part's numbers (1 x 65536 tokens, 16 query heads of 128 on one: 36 us in 91
 // parts, 38 in 64 or 128, 64 in 256).
 constexpr float kPartCost = 1.0f / 4096;
 QTTS_RULE uint32_t joined_share(int32_t tiles, uint32_t share, float part) {

@@ -134,6 +134,8 @@ __global__ __launch_bounds__(kStepThreads) void paged_step_kernel(PagedStepArgs 
   if (threadIdx.x == blockDim.x - 1) *a.taken_out = (int32_t)(taken + total);
 }
 
+// Latency bounds it: 64 requests of 64 pages 5.4 us captured, 2048 of 7 (16 waves, each 128 requests in turn) 34.
+//
 // Requests' pages back: request r's page j to free[taken - (all returned) + (returned by requests before r) + j].  One
 // workgroup, a wave a request.
 __global__ __launch_bounds__(kStepThreads) void paged_release_kernel(const int32_t* which, int32_t* lengths,

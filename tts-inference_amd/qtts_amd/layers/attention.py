@@ -91,6 +91,7 @@ class PagedCache:
         ``max_new`` bounds its entries (None: ``rows``), and what does not fit is denied (``batch.counts`` 0).  Requests whose pages are not left
         are denied in either case.
 
+        ``min_new``: tokens that a request has at least, if any; past 16 rows a key-value head the kernel of few rows is left out.
         A captured call keeps ``max_new`` (1: the decode step's kernel alone); without it, it is made for up to ``rows`` tokens a request,
         whatever this step's are."""
         new, this_step = self._whole(new, "new"), False
